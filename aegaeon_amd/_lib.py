@@ -54,6 +54,11 @@ HOST_UNCACHED = 1
 HOST_COHERENT = 2
 PROBE_READ = 1
 PROBE_WRITE = 2
+FORMAT_MXFP4 = 1
+FORMAT_MXFP8 = 2
+DTYPE_BFLOAT16 = 1
+DTYPE_FLOAT16 = 2
+DTYPE_FLOAT32 = 3
 #: bit 62 of a fence word: the move behind it (or one before it on the same
 #: stream) failed
 FENCE_FAILED = 1 << 62
@@ -85,6 +90,12 @@ EXPORTED_SYMBOLS = (
     "aegkv_stream_create_masked",
     "aegkv_stream_destroy",
     "aegkv_stream_release",
+    "aegkv_quant_page_bytes",
+    "aegkv_batch_plan",
+    "aegkv_quant_write",
+    "aegkv_quant_read",
+    "aegkv_quant_attend_workspace",
+    "aegkv_quant_attend",
 )
 
 _P = ctypes.c_void_p
@@ -134,6 +145,26 @@ _SIGNATURES = {
     "aegkv_stream_create_masked": (_INT, [_PP, ctypes.POINTER(ctypes.c_uint32), ctypes.c_int32]),
     "aegkv_stream_destroy": (_INT, [_P]),
     "aegkv_stream_release": (_INT, [_P]),
+    "aegkv_quant_page_bytes": (_INT, [_INT, _I32, _I32, _I32, _I64P]),
+    "aegkv_batch_plan": (
+        _INT,
+        [_I64, _I64P, _I64P, _I64P, _I64P, _I64, _I32, _I32, _I32, _I64, _I64, _I64, _I64, _I64,
+         _INT, _P, _I64P],
+    ),
+    "aegkv_quant_write": (
+        _INT,
+        [_P, _P, _INT, _I32, _P, _P, _P, _I64, _I64, _P, _I64, _I64, _I64, _INT, _P],
+    ),
+    "aegkv_quant_read": (
+        _INT,
+        [_P, _P, _INT, _I32, _P, _P, _INT, _P, _I64, _I64, _P, _I64, _I64, _I64, _INT, _P],
+    ),
+    "aegkv_quant_attend_workspace": (_INT, [_P, _I32, _I64P]),
+    "aegkv_quant_attend": (
+        _INT,
+        [_P, _P, _INT, _I32, _P, _P, _P, _I64, _I64, _P, _I64, _I64, _I64, _INT,
+         ctypes.c_double, _P, _I64, _P],
+    ),
 }
 
 _lib = None

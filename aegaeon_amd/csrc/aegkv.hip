@@ -27,6 +27,7 @@
 
 #include <hip/hip_runtime.h>
 #include "aegkv.h"
+#include "batch_plan_build.h"
 #include "copy_walk.h"
 #include "errors.h"
 #include "staged_runs.h"
@@ -40,6 +41,7 @@
 #include <deque>
 #include <map>
 #include <mutex>
+#include <utility>
 #include <vector>
 
 // ---------------------------------------------------------------- errors --
@@ -2818,3 +2820,7 @@ int aegkv_host_free(void* ptr) {
 }
 
 }  // extern "C"
+
+// ================================================ quantised cache ==
+
+#include "quant_calls.h"

@@ -1,0 +1,89 @@
+// The plan of one batch over a quantised paged cache: what aegkv_batch_plan
+// lays out in a caller's buffer (plan.cpp) and the kernels of quant_cache.h
+// read from its copy on the device. Internal to the library.
+#ifndef AEGKV_BATCH_PLAN_H
+#define AEGKV_BATCH_PLAN_H
+
+#include <cstdint>
+
+namespace aegkv_batch {
+
+constexpr uint64_t kMagic = 0x314e414c50425141ull;
+
+// Tokens are written and read in spans of 16 (a span lies in one block) and
+// attended over in tiles of 32.
+constexpr int kSpan = 16;
+constexpr int kTile = 32;
+
+// Row r of a sequence's queries under one KV head is new token r / group,
+// query head kv_head * group + r % group. Attention takes rows by kind:
+//   kFew, kMore: up to 16 (32) rows of a sequence, one workgroup's four waves
+//                share out the tiles of an item and join at its end;
+//   kMany:       blocks of kManyRows rows, the waves share out the rows.
+enum Kind { kFew = 0, kMore = 1, kMany = 2, kKinds = 3 };
+constexpr int kManyRows = 32;
+constexpr int kKindRows[kKinds] = {16, 32, kManyRows};
+
+struct Seq {
+  int32_t len;         // positions in the cache, the new ones included
+  int32_t fresh;       // new tokens: positions len - fresh .. len - 1
+  int32_t table;       // first entry of its block table
+  int32_t token;       // row of its first new token
+  int32_t new_span;    // spans of new tokens before this sequence
+  int32_t read_span;   // spans of all tokens before this sequence
+  int64_t read_token;  // tokens before this sequence
+};
+static_assert(sizeof(Seq) == 32, "Seq layout");
+
+// One workgroup's attention: rows [row, row + rows) of a sequence under one
+// KV head over visited tiles [tile, tile_end). Visited tile v is the cache's
+// tile v below `first_tiles` (the first tokens that stay visible), else v -
+// first_tiles + window_tile.
+struct Item {
+  int32_t seq, kv_head, row, rows;
+  int32_t tile, tile_end, first_tiles, window_tile;
+  int32_t slot;        // where its part of the sum goes; -1: it is the whole
+  int32_t pad[3];
+};
+static_assert(sizeof(Item) == 48, "Item layout");
+
+// Rows whose tiles were shared out to `parts` items with consecutive slots.
+struct Merge {
+  int32_t seq, kv_head, row, rows;
+  int32_t slot, parts, kind, pad;
+};
+static_assert(sizeof(Merge) == 32, "Merge layout");
+
+// What a plan has room for; fixed when it is made. Offsets into the buffer
+// follow from it, so that a captured launch stays right across updates.
+struct Room {
+  int64_t bytes;
+  int64_t seqs, columns, tokens;   // sequences, table entries, new tokens
+  int64_t new_spans, read_spans;
+  int64_t items[kKinds];           // 0: no such kernel is launched
+  int64_t slots[kKinds];
+  int64_t merges;
+  int64_t at_seqs, at_table, at_items[kKinds], at_merges;
+};
+
+struct Header {
+  uint64_t magic;
+  Room room;
+  int64_t num_blocks;
+  int32_t block_size, kv_heads, heads, group;
+  int32_t window, sinks;           // window 0: none
+  int32_t num_seqs, num_tokens;
+  int32_t new_spans, read_spans;
+  int32_t items[kKinds], slots[kKinds];
+  int32_t merges;
+  int32_t complete;                // every position of every sequence has its block
+  int64_t read_tokens;
+};
+
+inline const Seq* seqs(const void* p, const Room& r) {
+  return reinterpret_cast<const Seq*>(static_cast<const char*>(p) + r.at_seqs);
+}
+
+}  // namespace aegkv_batch
+
+#endif  // AEGKV_BATCH_PLAN_H

@@ -1,13 +1,17 @@
-// Native swap planning: the transfer entries of many block tables at once.
+// Native planning: the transfer entries of many block tables at once, and the
+// plan of a batch over a quantised cache (batch_plan_build.h).
 //
-// Host-only C++ (no device code). Follows, per column, the rules of
+// Host-only C++ (no device code). Transfer entries follow, per column, the rules of
 // BlockTable.transfer_entries (aegaeon/block_manager.py:446-478) over
 // CacheGroupConfig.num_skipped_blocks / kernel_block_extent (:196-266) and
 // cache_transfer.kernel_block_extent_for_attention_page (cache_transfer.py:
 // 48-94). Contract in include/aegkv.h.
 
 #include "aegkv.h"
+#include "batch_plan_build.h"
 #include "errors.h"
+
+#include <exception>
 
 #define plan_fail aegkv_set_error
 
@@ -117,6 +121,66 @@ int aegkv_transfer_entries(int32_t num_groups, const int32_t* group_kind,
   }
   *num_rows = rows;
   return 0;
+}
+
+int aegkv_batch_plan(int64_t num_seqs, const int64_t* column_offsets, const int64_t* block_ids,
+                     const int64_t* seq_lens, const int64_t* new_lens, int64_t num_blocks,
+                     int32_t block_size, int32_t kv_heads, int32_t heads, int64_t window,
+                     int64_t sinks, int64_t max_seqs, int64_t max_columns, int64_t max_tokens,
+                     int update, void* plan, int64_t* plan_bytes) {
+  using namespace aegkv_batch;
+  aegkv_clear_error();
+  if (!plan_bytes) return plan_fail(AEGKV_EINVAL, "plan_bytes must not be null");
+  const int64_t held = *plan_bytes;
+  if (num_seqs < 0 || num_seqs > INT32_MAX / 2)
+    return plan_fail(AEGKV_EINVAL, "%lld sequences", ll(num_seqs));
+  if (num_seqs > 0 && (!column_offsets || !seq_lens || !new_lens))
+    return plan_fail(AEGKV_EINVAL, "sequence arrays must not be null");
+  if (num_seqs > 0 && column_offsets[num_seqs] > 0 && !block_ids)
+    return plan_fail(AEGKV_EINVAL, "block ids must not be null");
+  if (max_seqs < 0 || max_columns < 0 || max_tokens < 0 || max_seqs > INT32_MAX / 2 ||
+      max_columns > kMostTokens / 16 || max_tokens > kMostTokens / 16)
+    return plan_fail(AEGKV_EINVAL, "room for %lld sequences, %lld columns and %lld new tokens",
+                     ll(max_seqs), ll(max_columns), ll(max_tokens));
+  const Batch b{num_seqs, column_offsets, block_ids, seq_lens, new_lens};
+  try {
+    Header h;
+    int rc = describe(h, num_blocks, block_size, kv_heads, heads, window, sinks);
+    if (rc) return rc;
+    rc = check(h, b);
+    if (rc) return rc;
+    std::vector<Rows> rows[kKinds];
+    rows_of(h, b, rows);
+    if (update) {
+      Header was;
+      if (!plan || held < static_cast<int64_t>(sizeof was))
+        return plan_fail(AEGKV_EINVAL, "an update needs the plan");
+      std::memcpy(&was, plan, sizeof was);
+      if (was.magic != kMagic || was.room.bytes != held)
+        return plan_fail(AEGKV_EINVAL, "this is no plan of %lld bytes", ll(held));
+      if (was.num_blocks != h.num_blocks || was.block_size != h.block_size ||
+          was.kv_heads != h.kv_heads || was.heads != h.heads || was.window != h.window ||
+          was.sinks != h.sinks)
+        return plan_fail(AEGKV_EINVAL, "an update keeps the blocks, heads, window and sinks");
+      h.room = was.room;
+    } else {
+      make_room(h, b, rows, max_seqs, max_columns, max_tokens);
+      *plan_bytes = h.room.bytes;
+      if (!plan) return 0;
+      if (held < h.room.bytes)
+        return plan_fail(AEGKV_ENOMEM, "the plan takes %lld bytes, not %lld", ll(h.room.bytes),
+                         ll(held));
+    }
+    // built aside, so that a refused update leaves the plan as it was
+    std::vector<char> aside(static_cast<size_t>(h.room.bytes));
+    rc = fill(h, b, rows, aside.data());
+    if (rc) return rc;
+    std::memcpy(aside.data(), &h, sizeof h);
+    std::memcpy(plan, aside.data(), aside.size());
+    return 0;
+  } catch (const std::exception& e) {
+    return plan_fail(AEGKV_ENOMEM, "no memory for the plan: %s", e.what());
+  }
 }
 
 }  // extern "C"

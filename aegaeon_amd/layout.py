@@ -77,6 +77,17 @@ def kv_tensor_specs(num_layers: int, num_blocks: int, block_size: int, kv_heads:
     return specs
 
 
+def quant_kv_tensor_specs(num_layers: int, num_blocks: int, block_size: int, kv_heads: int,
+                          head_dim: int, fmt: str = "mxfp4") -> List[KVCacheTensorSpec]:
+    """kv_tensor_specs of a cache held in 4 or 8 bits (ops.QuantCache): one K
+    and one V tensor of num_blocks pages per layer, in the same order."""
+    from . import ops
+
+    size = num_blocks * ops.quant_page_bytes(fmt, block_size, kv_heads, head_dim)
+    return [KVCacheTensorSpec(size, (f"layers.{layer}.{kv}",))
+            for layer in range(num_layers) for kv in ("k", "v")]
+
+
 @dataclass
 class CompositeCache:
     """Device backing tensors plus their composite layout (vllm_cache.py:43-51)."""

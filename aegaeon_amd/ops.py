@@ -957,3 +957,307 @@ def fence_host_wait(host_words: HostFenceWords, index: int, value: int,
                               f"the move it counts (value {value}) or one before it on its "
                               "stream moved nothing")
     return rc == 1
+
+
+# ---- quantised caches ---------------------------------------------------------
+
+_FORMATS = {"mxfp4": _lib.FORMAT_MXFP4, "mxfp8": _lib.FORMAT_MXFP8}
+_DTYPES = {torch.bfloat16: _lib.DTYPE_BFLOAT16, torch.float16: _lib.DTYPE_FLOAT16,
+           torch.float32: _lib.DTYPE_FLOAT32}
+
+
+def quant_page_bytes(fmt: str, block_size: int, kv_heads: int, head_dim: int) -> int:
+    """Bytes of one block of K (or of V) in a quantised cache
+    (aegkv_quant_page_bytes): "mxfp4" holds a value in 4 bits, "mxfp8" in 8,
+    both with one scale byte for 32 values of a head."""
+    if fmt not in _FORMATS:
+        raise ValueError(f"unknown cache format {fmt!r}")
+    n = ctypes.c_int64()
+    _lib.check(_lib.load().aegkv_quant_page_bytes(_FORMATS[fmt], int(block_size), int(kv_heads),
+                                                  int(head_dim), ctypes.byref(n)))
+    return int(n.value)
+
+
+class QuantCache:
+    """K and V of one layer in a quantised format, as pages of a paged cache.
+
+    k_pages and v_pages are device tensors of num_blocks pages each, of any
+    element type (a composite cache's backing tensors over
+    layout.quant_kv_tensor_specs serve as they are), which swaps, copies and
+    migrations move like any other segment. A page holds block_size tokens (16,
+    32, 64 or 128) of kv_heads heads, 64, 128 or 256 values wide; its layout is
+    described in include/aegkv.h.
+    """
+
+    def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, *, kv_heads: int,
+                 head_dim: int, block_size: int, fmt: str = "mxfp4"):
+        self.page_bytes = quant_page_bytes(fmt, block_size, kv_heads, head_dim)
+        for t, what in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+            _require_device(t, what)
+            if _tensor_bytes(t) == 0 or _tensor_bytes(t) % self.page_bytes:
+                raise ValueError(f"{what} of {_tensor_bytes(t)} bytes are no whole pages of "
+                                 f"{self.page_bytes}")
+        if k_pages.device != v_pages.device or _tensor_bytes(k_pages) != _tensor_bytes(v_pages):
+            raise ValueError("k_pages and v_pages must be equally large and on one device")
+        self.k_pages, self.v_pages = k_pages, v_pages
+        self.kv_heads, self.head_dim = int(kv_heads), int(head_dim)
+        self.block_size, self.fmt = int(block_size), fmt
+        self.num_blocks = _tensor_bytes(k_pages) // self.page_bytes
+        self.device = k_pages.device
+        self._args = (_FORMATS[fmt], self.head_dim, k_pages.data_ptr(), v_pages.data_ptr())
+
+
+class CacheBatch:
+    """A batch over a quantised cache: which blocks its sequences hold, and how
+    attention over them is shared out (aegkv_batch_plan). One batch serves all
+    layers of a model step.
+
+    block_tables: a list of block ids for each sequence, or a 2-D array with a row
+    each; column c holds the positions [c * block_size, (c + 1) * block_size), -1
+    marks a released column (as BlockTable.group_blocks does), and columns behind
+    the sequence's last are ignored. seq_lens counts all tokens of a
+    sequence, new_lens those at its end that are new: the ones quant_write
+    writes and quant_attend takes as queries. A query at position p sees the
+    positions j <= p with p - j < window (0: all) or j < sinks.
+
+    Everything is checked here, once (ValueError). update() puts another batch in
+    its place, also for calls captured into a graph, if it fits the room
+    that max_seqs, max_columns (of all block tables) and max_tokens (new ones) asked
+    for and its sequences have as many rows (new tokens times heads / kv_heads) as
+    the first batch's: up to 16, up to 32, or more.
+    """
+
+    def __init__(self, block_tables, seq_lens, new_lens, *, num_blocks: int, block_size: int,
+                 kv_heads: int, heads: int | None = None, window: int = 0, sinks: int = 0,
+                 max_seqs: int = 0, max_columns: int = 0, max_tokens: int = 0,
+                 device: torch.device | None = None, stream: torch.cuda.Stream | None = None):
+        self.num_blocks, self.block_size = int(num_blocks), int(block_size)
+        self.kv_heads = int(kv_heads)
+        self.heads = self.kv_heads if heads is None else int(heads)
+        self.window, self.sinks = int(window), int(sinks)
+        self._room = (int(max_seqs), int(max_columns), int(max_tokens))
+        self._host = None
+        self._make(block_tables, seq_lens, new_lens, update=0)
+        self.device = torch.device(device if device is not None else "cuda")
+        if self.device.type != "cuda":
+            raise ValueError(f"a batch lives on a device (HIP), not on {self.device}")
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self._workspace: dict = {}
+        self._used: dict = {}     # raw stream -> event behind its last call over this batch
+        with torch.cuda.device(self.device):
+            st = stream if stream is not None else torch.cuda.current_stream()
+            if torch.cuda.is_current_stream_capturing():
+                raise ValueError("a batch cannot be made while a stream is captured")
+            with torch.cuda.stream(st):
+                self._plan = torch.empty(self._host.size, dtype=torch.uint8, device=self.device)
+                self._upload(st)
+
+    def _make(self, block_tables, seq_lens, new_lens, update: int) -> None:
+        if isinstance(block_tables, (torch.Tensor, np.ndarray)):
+            if block_tables.ndim != 2:
+                raise ValueError("block tables are a list a sequence or a 2-D array")
+            offsets = np.arange(len(block_tables) + 1, dtype=np.int64) * block_tables.shape[1]
+            ids = _i64(block_tables)
+        else:
+            rows = [_i64(t) for t in block_tables]
+            offsets = np.zeros(len(rows) + 1, np.int64)
+            np.cumsum([r.size for r in rows], out=offsets[1:])
+            ids = np.concatenate(rows) if rows else np.zeros(0, np.int64)
+        lens, new = _i64(seq_lens), _i64(new_lens)
+        if not offsets.size - 1 == lens.size == new.size:
+            raise ValueError(f"{offsets.size - 1} block tables, {lens.size} lengths and "
+                             f"{new.size} new lengths")
+        lib = _lib.load()
+        args = (lens.size, _p64(offsets), _p64(ids), _p64(lens), _p64(new), self.num_blocks,
+                self.block_size, self.kv_heads, self.heads, self.window, self.sinks, *self._room,
+                update)
+        n = ctypes.c_int64(self._host.size if update else 0)
+        host = self._host
+        if not update:
+            _lib.check(lib.aegkv_batch_plan(*args, None, ctypes.byref(n)))
+            host = np.zeros(n.value, np.uint8)
+        _lib.check(lib.aegkv_batch_plan(*args, host.ctypes.data, ctypes.byref(n)))
+        self._host = host
+        self._host_ptr = host.ctypes.data
+        self.num_seqs, self.num_tokens = int(lens.size), int(new.sum())
+        self.read_tokens = int(lens.sum())
+
+    def _upload(self, st: torch.cuda.Stream) -> None:
+        pinned = torch.empty(self._host.size, dtype=torch.uint8, pin_memory=True)
+        pinned.numpy()[:] = self._host
+        self._plan.copy_(pinned, non_blocking=True)
+        self._uploaded = torch.cuda.Event()
+        self._uploaded.record(st)
+        self._stream = st.cuda_stream
+
+    def update(self, block_tables, seq_lens, new_lens, *,
+               stream: torch.cuda.Stream | None = None) -> None:
+        """Put another batch over the same cache in this one's place. The change
+        is enqueued on `stream` (default: the current one) behind every call
+        made over this batch; a graph that holds such calls is replayed on that
+        stream, or ordered before and behind it by the caller."""
+        with torch.cuda.device(self.device):
+            st = stream if stream is not None else torch.cuda.current_stream()
+            with torch.cuda.stream(st):
+                if torch.cuda.is_current_stream_capturing():
+                    raise ValueError("a batch is updated outside the capture; the graph's calls "
+                                     "find what it holds when they are replayed")
+                self._make(block_tables, seq_lens, new_lens, update=1)
+                if st.cuda_stream != self._stream:
+                    st.wait_event(self._uploaded)
+                for event in self._used.values():
+                    st.wait_event(event)
+                self._used.clear()
+                self._upload(st)
+
+    def _enter(self, raw: int, stream: torch.cuda.Stream | None):
+        """Order a call on the raw stream behind the upload. The stream, where
+        the call is to be noted by _leave."""
+        if raw == self._stream:
+            return None
+        st = stream if stream is not None else torch.cuda.current_stream(self.device)
+        with torch.cuda.stream(st):
+            if torch.cuda.is_current_stream_capturing():
+                return None     # capture begins behind a synchronize
+        st.wait_event(self._uploaded)
+        return st
+
+    def _leave(self, st: torch.cuda.Stream | None) -> None:
+        if st is None:
+            return
+        event = self._used.get(st.cuda_stream)
+        if event is None:
+            event = self._used[st.cuda_stream] = torch.cuda.Event()
+        event.record(st)
+        self._plan.record_stream(st)
+
+
+def _quant_call(cache: QuantCache, batch: CacheBatch):
+    if (batch.block_size, batch.kv_heads) != (cache.block_size, cache.kv_heads):
+        raise ValueError(f"a batch of {batch.block_size}-token blocks and {batch.kv_heads} KV heads "
+                         f"over a cache of {cache.block_size} and {cache.kv_heads}")
+    if batch.num_blocks > cache.num_blocks:
+        raise ValueError(f"a batch over {batch.num_blocks} blocks, a cache of {cache.num_blocks}")
+    if batch.device != cache.device:
+        raise ValueError(f"a batch on {batch.device}, a cache on {cache.device}")
+
+
+def _rows_arg(t: torch.Tensor, what: str, heads: int, cache: QuantCache, dtypes):
+    """(pointer, token stride, head stride) of a [tokens, heads, head_dim] tensor."""
+    if t.device != cache.device:
+        raise ValueError(f"{what} on {t.device}, the cache on {cache.device}")
+    if t.dim() != 3 or t.size(1) != heads or t.size(2) != cache.head_dim:
+        raise ValueError(f"{what} must be [tokens, {heads}, {cache.head_dim}], not "
+                         f"{list(t.shape)}")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{what} of {t.dtype} is not supported")
+    if t.numel() and t.stride(2) != 1:
+        raise ValueError(f"{what}: the last axis must be contiguous")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what} requires a gradient, which these operators do not give")
+    return t.data_ptr(), t.stride(0), t.stride(1)
+
+
+def _on_stream(cache: QuantCache, batch: CacheBatch, stream, fn) -> None:
+    def call():
+        raw = _stream_ptr(cache.device, stream)
+        st = batch._enter(raw, stream)
+        _lib.check(fn(raw))
+        batch._leave(st)
+
+    _call_on(cache.device, call)
+
+
+def _empty_on(stream, *args, **kwargs) -> torch.Tensor:
+    """A tensor of `stream`'s (default: the current one's) memory pool."""
+    if stream is None:
+        return torch.empty(*args, **kwargs)
+    with torch.cuda.stream(stream):
+        return torch.empty(*args, **kwargs)
+
+
+def quant_write(cache: QuantCache, batch: CacheBatch, k: torch.Tensor, v: torch.Tensor, *,
+                stream: torch.cuda.Stream | None = None) -> None:
+    """Write the batch's new tokens into the cache (aegkv_quant_write).
+
+    k, v: [tokens, kv_heads, head_dim] of bfloat16, float16 or float32, with any
+    strides on the first two axes (slices of a fused projection, say); row i is
+    the batch's i-th new token, and rows behind the last are not read. Every 32
+    values share the smallest power-of-two scale under which the largest fits the format,
+    and each takes its nearest code, ties to even. A group with a NaN or an
+    infinity reads back as NaN.
+    """
+    _quant_call(cache, batch)
+    kp = _rows_arg(k, "k", cache.kv_heads, cache, _DTYPES)
+    vp = _rows_arg(v, "v", cache.kv_heads, cache, _DTYPES)
+    if k.dtype != v.dtype or k.size(0) != v.size(0):
+        raise ValueError(f"k and v differ: {k.size(0)} tokens of {k.dtype}, {v.size(0)} of "
+                         f"{v.dtype}")
+    lib = _lib.load()
+    _on_stream(cache, batch, stream, lambda raw: lib.aegkv_quant_write(
+        batch._host_ptr, batch._plan.data_ptr(), *cache._args, *kp, *vp, k.size(0),
+        _DTYPES[k.dtype], raw))
+
+
+def quant_read(cache: QuantCache, batch: CacheBatch, *, tokens: str = "all",
+               dtype: torch.dtype = torch.bfloat16,
+               out: tuple[torch.Tensor, torch.Tensor] | None = None,
+               stream: torch.cuda.Stream | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """K and V of the batch's tokens as values of `dtype` (aegkv_quant_read):
+    [tokens, kv_heads, head_dim] each, all tokens of the sequences one after
+    another ("all"), or the new ones ("new"). `out`: two tensors to read into (their
+    type counts); rows behind the last token are left as they were."""
+    _quant_call(cache, batch)
+    if tokens not in ("all", "new"):
+        raise ValueError(f"tokens are 'all' or 'new', not {tokens!r}")
+    n = batch.read_tokens if tokens == "all" else batch.num_tokens
+    if out is None:
+        if dtype not in _DTYPES:
+            raise ValueError(f"reading as {dtype} is not supported")
+        shape = (n, cache.kv_heads, cache.head_dim)
+        out = tuple(_empty_on(stream, shape, dtype=dtype, device=cache.device) for _ in range(2))
+    k, v = out
+    kp = _rows_arg(k, "k", cache.kv_heads, cache, _DTYPES)
+    vp = _rows_arg(v, "v", cache.kv_heads, cache, _DTYPES)
+    if k.dtype != v.dtype or k.size(0) != v.size(0):
+        raise ValueError(f"k and v differ: {k.size(0)} tokens of {k.dtype}, {v.size(0)} of "
+                         f"{v.dtype}")
+    lib = _lib.load()
+    _on_stream(cache, batch, stream, lambda raw: lib.aegkv_quant_read(
+        batch._host_ptr, batch._plan.data_ptr(), *cache._args, 1 if tokens == "new" else 0,
+        *kp, *vp, k.size(0), _DTYPES[k.dtype], raw))
+    return k, v
+
+
+def quant_attend(cache: QuantCache, batch: CacheBatch, q: torch.Tensor, *,
+                 scale: float | None = None, out: torch.Tensor | None = None,
+                 stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """Attention of the batch's new tokens over the cache (aegkv_quant_attend),
+    for single tokens, chunks and whole prompts alike, also side by side.
+
+    q: [tokens, heads, head_dim] of bfloat16 or float16, row i the query of the
+    batch's i-th new token, whose K and V are in the cache already (quant_write).
+    scale: of the scores, head_dim ** -0.5 by default. `out` (q itself is fine)
+    takes the result; rows behind the batch's last token are left as they were.
+    """
+    _quant_call(cache, batch)
+    qp = _rows_arg(q, "q", batch.heads, cache, (torch.bfloat16, torch.float16))
+    if out is None:
+        out = _empty_on(stream, q.shape, dtype=q.dtype, device=q.device)
+    op = _rows_arg(out, "out", batch.heads, cache, (q.dtype,))
+    if out.size(0) != q.size(0):
+        raise ValueError(f"{q.size(0)} queries, {out.size(0)} rows of out")
+    lib = _lib.load()
+    d = cache.head_dim
+    size = batch._workspace.get(d)
+    if size is None:
+        n = ctypes.c_int64()
+        _lib.check(lib.aegkv_quant_attend_workspace(batch._host_ptr, d, ctypes.byref(n)))
+        size = batch._workspace[d] = int(n.value)
+    work = _empty_on(stream, size, dtype=torch.uint8, device=q.device) if size else None
+    _on_stream(cache, batch, stream, lambda raw: lib.aegkv_quant_attend(
+        batch._host_ptr, batch._plan.data_ptr(), *cache._args, *qp, *op, q.size(0),
+        _DTYPES[q.dtype], d ** -0.5 if scale is None else float(scale),
+        work.data_ptr() if size else None, size, raw))
+    return out

@@ -22,7 +22,8 @@
  *   - The caller keeps every buffer alive until the stream has passed the
  *     enqueued work (record an event after the call and wait on it).
  *   - Calls are not for stream capture (hipGraph), except
- *     aegkv_copy_blocks_noalloc: their descriptors are copied from a host
+ *     aegkv_copy_blocks_noalloc and the calls over quantised caches: the
+ *     others' descriptors are copied from a host
  *     ring whose slots later calls reuse, and a replayed copy would read
  *     whatever the slot holds then. On a capturing stream they return
  *     AEGKV_EINVAL with nothing enqueued (aegkv_load_slices in STAGED mode,
@@ -503,6 +504,119 @@ int aegkv_guard_merge(uint64_t* guard, const uint64_t* source_guard, hipStream_t
 int aegkv_fence_publish(uint64_t* host_word, uint64_t value, const uint64_t* guard,
                         hipStream_t stream);
 int aegkv_fence_host_wait(const uint64_t* host_word, uint64_t value, int64_t timeout_us);
+
+/*
+ * Quantised caches: K and V of one layer held in 4 or 8 bits a value, written
+ * token by token, read back, and attended over. No counterpart in the
+ * reference, whose caches hold the model's own type. To every other call here
+ * such a cache is two more segments of whole pages, with 3.76 (1.94) times
+ * fewer bytes than a 16-bit one of 128-wide heads to swap, copy or migrate.
+ *
+ * Formats: 32 consecutive values of a head share a scale 2^(b - 127), b one
+ * byte (255: the group is no number), and are held as
+ *   AEGKV_FORMAT_MXFP4  sign and 0, 0.5, 1, 1.5, 2, 3, 4 or 6 (E2M1), two a
+ *                       byte, the earlier value in the low half;
+ *   AEGKV_FORMAT_MXFP8  8-bit floats (E4M3, largest 448).
+ * Page of one block: kv_heads chunks, one a head. A chunk is block_size rows
+ * of a token's codes (head_dim / 2 or head_dim bytes), then head_dim / 32
+ * planes of block_size scale bytes. block_size is 16, 32, 64 or 128 tokens,
+ * head_dim 64, 128 or 256. Pages are 16-byte aligned and as long as
+ * aegkv_quant_page_bytes says; K and V are separate tensors of num_blocks pages.
+ */
+#define AEGKV_FORMAT_MXFP4 1
+#define AEGKV_FORMAT_MXFP8 2
+#define AEGKV_DTYPE_BFLOAT16 1
+#define AEGKV_DTYPE_FLOAT16 2
+#define AEGKV_DTYPE_FLOAT32 3
+int aegkv_quant_page_bytes(int format, int32_t block_size, int32_t kv_heads, int32_t head_dim,
+                           int64_t* bytes);
+
+/*
+ * The plan of a batch (host-only; no GPU): its sequences, their blocks, and how
+ * attention over them is cut into workgroups. All layers of a model step share
+ * one plan. Sequence s holds seq_lens[s] tokens of which the last new_lens[s] are new:
+ * they are what aegkv_quant_write writes and what queries. Its blocks are
+ * block_ids[column_offsets[s] .. column_offsets[s + 1]), column c holding the
+ * positions [c * block_size, (c + 1) * block_size); -1 marks a released column,
+ * which no query may see and no new token lie in.
+ * A query at position p sees the positions j <= p with p - j < window (0: no
+ * window) or j < sinks.
+ *
+ * Everything is checked here, once, so that the calls over the plan read only
+ * blocks below num_blocks: AEGKV_ERANGE for ids and columns, AEGKV_EDUP if a
+ * token's place is written twice, AEGKV_EINVAL otherwise.
+ *
+ * `plan` takes *plan_bytes bytes, which a call with a null plan sets; the
+ * caller copies them to the device (16-byte aligned) before the calls that take both.
+ * max_seqs, max_columns and max_tokens (new ones) ask for room beyond this
+ * batch's own. With update != 0, plan is an earlier plan of *plan_bytes bytes
+ * over the same blocks, heads, window and sinks, which is rewritten in place if
+ * the batch fits its room (AEGKV_ENOMEM otherwise, and the plan is unchanged):
+ * the caller copies it to the same device memory again, ordered behind the
+ * calls that use what it held, and calls captured into a graph then work on the
+ * new batch when they are replayed. A plan with room takes sequences with as
+ * many rows (new tokens times query heads of a KV head) as the batch it was
+ * made for had: up to 16, up to 32, more.
+ */
+int aegkv_batch_plan(int64_t num_seqs, const int64_t* column_offsets, const int64_t* block_ids,
+                     const int64_t* seq_lens, const int64_t* new_lens, int64_t num_blocks,
+                     int32_t block_size, int32_t kv_heads, int32_t heads, int64_t window,
+                     int64_t sinks, int64_t max_seqs, int64_t max_columns, int64_t max_tokens,
+                     int update, void* plan, int64_t* plan_bytes);
+
+/*
+ * Write the batch's new tokens into the cache. k and v: [num_tokens][kv_heads]
+ * [head_dim] values of `dtype`, strides in elements (none negative; the last
+ * axis is contiguous), row i the batch's i-th new token; rows behind the last
+ * are not read. Each group takes the smallest scale (b from 16 to 254) under
+ * which its largest magnitude is at most the format's largest value, and each
+ * value its nearest code, ties to the even one. A group that holds a NaN or an
+ * infinity is written as no number. Only the tokens' own bytes change.
+ *
+ * These calls launch kernels only: they allocate nothing, use no ring, and may
+ * be captured. Captured over a plan with room, a call has to be given arrays
+ * that hold all the plan has room for.
+ */
+int aegkv_quant_write(const void* plan, const void* device_plan, int format, int32_t head_dim,
+                      void* k_pages, void* v_pages, const void* k, int64_t k_token_stride,
+                      int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                      int64_t v_head_stride, int64_t num_tokens, int dtype, hipStream_t stream);
+
+/*
+ * Read tokens back as values of `dtype` (each rounded once; no number: NaN): the
+ * batch's new tokens (new_tokens != 0), or all tokens of its sequences, one
+ * sequence after another (AEGKV_ERANGE if one has a released column). Rows of k
+ * and v must not overlap; rows behind the last token are left as they were.
+ */
+int aegkv_quant_read(const void* plan, const void* device_plan, int format, int32_t head_dim,
+                     const void* k_pages, const void* v_pages, int new_tokens, void* k,
+                     int64_t k_token_stride, int64_t k_head_stride, void* v,
+                     int64_t v_token_stride, int64_t v_head_stride, int64_t num_tokens, int dtype,
+                     hipStream_t stream);
+
+/*
+ * Attention of the batch's new tokens over the cache: out[i] = sum over the
+ * positions j that query i sees of softmax_j(scale * q[i] . K[j]) V[j], query
+ * head h over KV head h / (heads / kv_heads). q and out: [num_tokens][heads]
+ * [head_dim] of bfloat16 or float16; rows behind the batch's last token are left as
+ * they were. out may be q itself. The cache's values are taken in the queries' type
+ * (bfloat16 holds them all but those of 2^128; float16 rounds what is below
+ * 2^-14, and beyond its range a value is an infinity). Scores, softmax and sums
+ * are held in 32 bits; probabilities enter the second product in the queries' type.
+ * What a query does not see changes nothing, NaN included.
+ *
+ * workspace: aegkv_quant_attend_workspace bytes of device memory, 16-byte aligned,
+ * of this call alone until it has run (calls on one stream may share one, and
+ * so may a graph's; calls that may overlap may not). Nothing in it has to be
+ * set. The result does not depend on other calls: no atomics are used.
+ */
+int aegkv_quant_attend_workspace(const void* plan, int32_t head_dim, int64_t* bytes);
+int aegkv_quant_attend(const void* plan, const void* device_plan, int format, int32_t head_dim,
+                       const void* k_pages, const void* v_pages, const void* q,
+                       int64_t q_token_stride, int64_t q_head_stride, void* out,
+                       int64_t out_token_stride, int64_t out_head_stride, int64_t num_tokens,
+                       int dtype, double scale, void* workspace, int64_t workspace_bytes,
+                       hipStream_t stream);
 
 #ifdef __cplusplus
 }
