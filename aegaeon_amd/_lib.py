@@ -234,6 +234,12 @@ class _GeneralPath:
     def pack_ids32(values, limit):
         return None
 
+    @staticmethod
+    def quant_write(*args):
+        return None
+
+    quant_read = quant_attend = quant_write
+
 
 _hostargs = None
 
@@ -258,6 +264,11 @@ def hostargs():
             module = _GeneralPath
         _hostargs = module
     return _hostargs
+
+
+def address(name: str) -> int:
+    """Address of one of the library's entry points."""
+    return ctypes.cast(getattr(load(), name), ctypes.c_void_p).value
 
 
 def check(status: int) -> None:

@@ -29,6 +29,10 @@ HIPCC_FLAGS = [
     "-shared",
     # packed FP32 instructions stay disabled in every HIP build here
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+    # matrix results in ordinary registers: in accumulation registers, which
+    # arithmetic has to copy out of and back, attention's inner loop was 1.7
+    # times as long
+    "-mllvm", "-amdgpu-mfma-vgpr-form=1",
     "-Wall",
     "-Wno-unused-function",
 ]

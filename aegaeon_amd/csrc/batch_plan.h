@@ -43,14 +43,14 @@ struct Item {
   int32_t seq, kv_head, row, rows;
   int32_t tile, tile_end, first_tiles, window_tile;
   int32_t slot;        // where its part of the sum goes; -1: it is the whole
-  int32_t pad[3];
+  int32_t base, token, table;   // the sequence's first new position, token row, table
 };
 static_assert(sizeof(Item) == 48, "Item layout");
 
 // Rows whose tiles were shared out to `parts` items with consecutive slots.
 struct Merge {
   int32_t seq, kv_head, row, rows;
-  int32_t slot, parts, kind, pad;
+  int32_t slot, parts, kind, token;
 };
 static_assert(sizeof(Merge) == 32, "Merge layout");
 

@@ -213,14 +213,15 @@ inline int fill(Header& h, const Batch& b, const std::vector<Rows>* rows, char* 
             return aegkv_set_error(AEGKV_ENOMEM, "the plan has no room for %lld parts of sums",
                                    ll(slots + parts));
           merge[merges++] = Merge{r.seq, head, r.row, r.rows, static_cast<int32_t>(slots),
-                                  static_cast<int32_t>(parts), kind, 0};
+                                  static_cast<int32_t>(parts), kind, seq[r.seq].token};
         }
         for (int64_t p = 0; p < parts; ++p) {
           Item& it = item[items++];
           it = Item{r.seq, head, r.row, r.rows,
                     static_cast<int32_t>(r.tiles * p / parts),
                     static_cast<int32_t>(r.tiles * (p + 1) / parts),
-                    r.first_tiles, r.window_tile, -1, {0, 0, 0}};
+                    r.first_tiles, r.window_tile, -1,
+                    seq[r.seq].len - seq[r.seq].fresh, seq[r.seq].token, seq[r.seq].table};
           if (parts > 1) it.slot = static_cast<int32_t>(slots++);
         }
       }

@@ -1,5 +1,5 @@
 // aegaeon_amd._hostargs: the argument tables of a move, read from Python
-// objects in one pass.
+// objects in one pass, and the calls over a quantised cache.
 //
 // A copy over 72 backing tensors asks each for its device, layout, size and
 // address. Asked from Python one attribute at a time that is 50 us, several
@@ -7,8 +7,16 @@
 // None for anything but the plain case (a list of dense device tensors, a
 // list of Python integers), and the caller then takes the general path, which
 // names what is wrong or converts other kinds of sequences.
+//
+// A decode step makes two calls a layer over a quantised cache. Their tensors
+// checked and their C arguments made in Python, they took the host 7.4 us
+// (write) and 14 (attend), 3 to 6 of which are the launches; here 4.0 and 8.1.
+// These functions too take the plain case only: None, with nothing enqueued,
+// for anything else.
 
 #include <torch/csrc/autograd/python_variable.h>
+#include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 
 #include <cstdint>
 #include <cstring>
@@ -129,6 +137,177 @@ PyObject* pack_ids32(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return out.release();
 }
 
+// What QuantCache and CacheBatch keep for these calls, packed by _lib.
+struct CacheArgs {
+  int64_t write, read, attend;   // addresses of the C entry points
+  int64_t format, head_dim, k_pages, v_pages;
+  int64_t kv_heads, block_size, num_blocks, device;
+};
+struct BatchArgs {
+  int64_t host_plan, device_plan, stream;
+  int64_t kv_heads, heads, block_size, num_blocks, device;
+  int64_t num_tokens, read_tokens;
+  int64_t workspace[3];          // bytes for heads 64, 128 and 256 wide
+};
+
+typedef int (*WriteFn)(const void*, const void*, int, int32_t, void*, void*, const void*, int64_t,
+                       int64_t, const void*, int64_t, int64_t, int64_t, int, void*);
+typedef int (*ReadFn)(const void*, const void*, int, int32_t, const void*, const void*, int, void*,
+                      int64_t, int64_t, void*, int64_t, int64_t, int64_t, int, void*);
+typedef int (*AttendFn)(const void*, const void*, int, int32_t, const void*, const void*,
+                        const void*, int64_t, int64_t, void*, int64_t, int64_t, int64_t, int,
+                        double, void*, int64_t, void*);
+
+template <typename P>
+P* at_address(int64_t a) {
+  return reinterpret_cast<P*>(static_cast<intptr_t>(a));
+}
+
+// AEGKV_DTYPE_* of a type, 0 for others
+int dtype_code(at::ScalarType t) {
+  return t == at::kBFloat16 ? 1 : t == at::kHalf ? 2 : t == at::kFloat ? 3 : 0;
+}
+
+// The arguments of one call: cache, batch, raw stream, current device.
+struct QuantArgs {
+  CacheArgs c;
+  BatchArgs b;
+  void* stream;
+
+  bool take(PyObject* cache, PyObject* batch, PyObject* raw, PyObject* current) {
+    if (!PyBytes_CheckExact(cache) || !PyBytes_CheckExact(batch) || !PyLong_CheckExact(raw) ||
+        !PyLong_CheckExact(current) || PyBytes_GET_SIZE(cache) != sizeof c ||
+        PyBytes_GET_SIZE(batch) != sizeof b)
+      return false;
+    std::memcpy(&c, PyBytes_AS_STRING(cache), sizeof c);
+    std::memcpy(&b, PyBytes_AS_STRING(batch), sizeof b);
+    const int64_t s = PyLong_AsLongLong(raw);
+    stream = at_address<void>(s);
+    return s == b.stream && PyLong_AsLongLong(current) == c.device && b.device == c.device &&
+           b.kv_heads == c.kv_heads && b.block_size == c.block_size &&
+           b.num_blocks <= c.num_blocks && !PyErr_Occurred();
+  }
+
+  // A [tokens, heads, head_dim] tensor of the cache's device.
+  const at::Tensor* rows(PyObject* o, int64_t heads) const {
+    if (!THPVariable_CheckExact(o)) return nullptr;
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (!t.defined() || !t.is_cuda() || t.get_device() != c.device ||
+        t.layout() != at::kStrided || t.dim() != 3 || t.size(1) != heads ||
+        t.size(2) != c.head_dim || !dtype_code(t.scalar_type()) || t.stride(2) != 1 ||
+        t.size(0) == 0 || (t.requires_grad() && c10::GradMode::is_enabled()))
+      return nullptr;
+    return &t;
+  }
+};
+
+bool alike(const at::Tensor& a, const at::Tensor& b) {
+  return a.scalar_type() == b.scalar_type() && a.size(0) == b.size(0);
+}
+
+// quant_write(cache, batch, k, v, stream, device) -> True, or None
+PyObject* quant_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  QuantArgs q;
+  if (nargs != 6 || !q.take(args[0], args[1], args[4], args[5])) Py_RETURN_NONE;
+  try {
+    const at::Tensor* k = q.rows(args[2], q.c.kv_heads);
+    const at::Tensor* v = q.rows(args[3], q.c.kv_heads);
+    if (!k || !v || !alike(*k, *v)) Py_RETURN_NONE;
+    if (at_address<std::remove_pointer_t<WriteFn>>(q.c.write)(
+            at_address<void>(q.b.host_plan), at_address<void>(q.b.device_plan),
+            static_cast<int>(q.c.format), static_cast<int32_t>(q.c.head_dim),
+            at_address<void>(q.c.k_pages), at_address<void>(q.c.v_pages), k->data_ptr(),
+            k->stride(0), k->stride(1), v->data_ptr(), v->stride(0), v->stride(1), k->size(0),
+            dtype_code(k->scalar_type()), q.stream) != 0)
+      Py_RETURN_NONE;
+    Py_RETURN_TRUE;
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+}
+
+// quant_read(cache, batch, new tokens, out or dtype code, stream, device) -> (k, v), or None
+PyObject* quant_read(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  QuantArgs q;
+  if (nargs != 6 || !q.take(args[0], args[1], args[4], args[5])) Py_RETURN_NONE;
+  try {
+    const bool fresh = args[2] == Py_True;
+    Ref made(nullptr);
+    PyObject* out = args[3];
+    if (PyLong_CheckExact(out)) {
+      const long code = PyLong_AsLong(out);
+      const int64_t tokens = fresh ? q.b.num_tokens : q.b.read_tokens;
+      if (tokens <= 0 || code < 1 || code > 3) Py_RETURN_NONE;
+      const auto options =
+          at::TensorOptions()
+              .dtype(code == 1 ? at::kBFloat16 : code == 2 ? at::kHalf : at::kFloat)
+              .device(at::kCUDA, static_cast<c10::DeviceIndex>(q.c.device));
+      at::Tensor k = at::empty({tokens, q.c.kv_heads, q.c.head_dim}, options);
+      at::Tensor v = at::empty({tokens, q.c.kv_heads, q.c.head_dim}, options);
+      made.p = PyTuple_New(2);
+      if (!made.p) return nullptr;
+      PyTuple_SET_ITEM(made.p, 0, THPVariable_Wrap(k));
+      PyTuple_SET_ITEM(made.p, 1, THPVariable_Wrap(v));
+      out = made.p;
+    }
+    if (!PyTuple_CheckExact(out) || PyTuple_GET_SIZE(out) != 2) Py_RETURN_NONE;
+    const at::Tensor* k = q.rows(PyTuple_GET_ITEM(out, 0), q.c.kv_heads);
+    const at::Tensor* v = q.rows(PyTuple_GET_ITEM(out, 1), q.c.kv_heads);
+    if (!k || !v || !alike(*k, *v)) Py_RETURN_NONE;
+    if (at_address<std::remove_pointer_t<ReadFn>>(q.c.read)(
+            at_address<void>(q.b.host_plan), at_address<void>(q.b.device_plan),
+            static_cast<int>(q.c.format), static_cast<int32_t>(q.c.head_dim),
+            at_address<void>(q.c.k_pages), at_address<void>(q.c.v_pages), fresh, k->data_ptr(),
+            k->stride(0), k->stride(1), v->data_ptr(), v->stride(0), v->stride(1), k->size(0),
+            dtype_code(k->scalar_type()), q.stream) != 0)
+      Py_RETURN_NONE;
+    if (made.p) return made.release();
+    Py_INCREF(out);
+    return out;
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+}
+
+// quant_attend(cache, batch, q, out or None, scale or None, stream, device) -> out, or None
+PyObject* quant_attend(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  QuantArgs q;
+  if (nargs != 7 || !q.take(args[0], args[1], args[5], args[6])) Py_RETURN_NONE;
+  try {
+    const at::Tensor* query = q.rows(args[2], q.b.heads);
+    if (!query || query->scalar_type() == at::kFloat) Py_RETURN_NONE;
+    double scale = q.c.head_dim == 64 ? 0.125 : q.c.head_dim == 256 ? 0.0625 : 0.08838834764831845;
+    if (args[4] != Py_None) {
+      if (!PyFloat_CheckExact(args[4])) Py_RETURN_NONE;
+      scale = PyFloat_AS_DOUBLE(args[4]);
+    }
+    at::Tensor made;
+    const at::Tensor* out = &made;
+    if (args[3] == Py_None) {
+      made = at::empty(query->sizes(), query->options().requires_grad(false));
+    } else {
+      out = q.rows(args[3], q.b.heads);
+      if (!out || !alike(*query, *out)) Py_RETURN_NONE;
+    }
+    const int64_t bytes = q.b.workspace[q.c.head_dim == 64 ? 0 : q.c.head_dim == 128 ? 1 : 2];
+    at::Tensor work;   // goes back to the stream's pool, behind the call
+    if (bytes) work = at::empty({bytes}, query->options().dtype(at::kByte).requires_grad(false));
+    if (at_address<std::remove_pointer_t<AttendFn>>(q.c.attend)(
+            at_address<void>(q.b.host_plan), at_address<void>(q.b.device_plan),
+            static_cast<int>(q.c.format), static_cast<int32_t>(q.c.head_dim),
+            at_address<void>(q.c.k_pages), at_address<void>(q.c.v_pages), query->data_ptr(),
+            query->stride(0), query->stride(1), out->data_ptr(), out->stride(0), out->stride(1),
+            query->size(0), dtype_code(query->scalar_type()), scale,
+            bytes ? work.data_ptr() : nullptr, bytes, q.stream) != 0)
+      Py_RETURN_NONE;
+    if (args[3] == Py_None) return THPVariable_Wrap(made);
+    Py_INCREF(args[3]);
+    return args[3];
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+}
+
 template <typename F>
 PyCFunction as_method(F* f) {
   return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f));
@@ -138,6 +317,9 @@ PyMethodDef methods[] = {
     {"segment_table", as_method(segment_table), METH_FASTCALL, nullptr},
     {"pack_ids32", as_method(pack_ids32), METH_FASTCALL, nullptr},
     {"pack_ids", pack_ids, METH_O, nullptr},
+    {"quant_write", as_method(quant_write), METH_FASTCALL, nullptr},
+    {"quant_read", as_method(quant_read), METH_FASTCALL, nullptr},
+    {"quant_attend", as_method(quant_attend), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_hostargs", nullptr, -1, methods,

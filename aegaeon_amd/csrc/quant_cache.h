@@ -338,51 +338,135 @@ struct AttendArgs {
 // each half: what its matrix operands are made of, without any exchange. The
 // order of the tokens and values along a product's inner axis is free, so it
 // is the one in which they were loaded.
-template <int FMT, int D>
-struct CacheTile {
-  static constexpr int kKWords = Chunk<FMT, D>::kCode / 16;
-  static constexpr int kVBytes = Chunk<FMT, D>::kCode / 16;
-  static constexpr int kVWords = (kVBytes + 3) / 4;
-  static constexpr int kKScales = D == 256 ? 2 : 1;
-  uint32_t k[2][kKWords];
-  uint32_t ks[2][kKScales];
-  uint32_t v[2][4][kVWords];
-  uint32_t vs[2];       // four tokens' scale bytes
 
-  __device__ __forceinline__ void load(const QuantPages& p, int64_t head_offset,
-                                       int block_shift, const int32_t* table, int32_t tile, int m,
-                                       int g) {
-    using C = Chunk<FMT, D>;
-    const int32_t block_size = 1 << block_shift;
+// Where a half of 16 tokens lies: the same for the whole wave, so that a load is
+// a scalar address and a lane's own 32-bit offset.
+struct Half {
+  const char* k;        // codes of its first token
+  const char* v;
+  const char* k_scales;
+  const char* v_scales;
+};
+
+template <int FMT, int D>
+__device__ __forceinline__ Half find_half(const QuantPages& p, int64_t head_offset,
+                                          int block_shift, const int32_t* table,
+                                          int32_t position) {
+  using C = Chunk<FMT, D>;
+  const int32_t column = position >> block_shift;
+  const int32_t inside = position & ((1 << block_shift) - 1);
+  const int64_t at = int64_t(table[column]) * p.page_bytes + head_offset;
+  const int64_t codes = at + int64_t(inside) * C::kCode;
+  const int64_t scales = at + (int64_t(C::kCode) << block_shift) + inside;
+  return Half{p.k + codes, p.v + codes, p.k + scales, p.v + scales};
+}
+
+template <int BYTES>
+__device__ __forceinline__ void load_bytes(uint32_t* to, const char* base, uint32_t offset) {
+  const char* p = base + offset;
+  if constexpr (BYTES == 1) {
+    to[0] = *reinterpret_cast<const uint8_t*>(p);
+  } else if constexpr (BYTES == 2) {
+    to[0] = *reinterpret_cast<const uint16_t*>(p);
+  } else {
+    __builtin_memcpy(to, __builtin_assume_aligned(p, BYTES < 16 ? BYTES : 16), BYTES);
+  }
+}
+
+// A lane's part of 16 tokens of K, and the scales of its groups.
+template <int FMT, int D>
+struct KPart {
+  static constexpr int kWords = Chunk<FMT, D>::kCode / 16;
+  static constexpr int kScales = D == 256 ? 2 : 1;
+  uint32_t code[kWords], scale[kScales];
+
+  __device__ __forceinline__ void load(const Half& h, int block_shift, uint32_t m, uint32_t g) {
+    load_bytes<kWords * 4>(code, h.k, m * Chunk<FMT, D>::kCode + g * (kWords * 4));
+#pragma unroll
+    for (uint32_t i = 0; i < kScales; ++i)
+      load_bytes<1>(&scale[i], h.k_scales, ((D == 64 ? g / 2 : g * kScales + i) << block_shift) + m);
+  }
+
+  // The matrix operand of step S: the lane's values 8 S .. 8 S + 7.
+  template <typename T, int S>
+  __device__ __forceinline__ typename Operand<T>::v8 operand() const {
+    const float s = scale_of(scale[kScales == 2 ? S / 4 : 0]);
+    const uint32_t* w = &code[S * Format<FMT>::kBits / 4];
+    const uint32_t f[4] = {decode_pair<FMT, T, 0>(w, s), decode_pair<FMT, T, 1>(w, s),
+                           decode_pair<FMT, T, 2>(w, s), decode_pair<FMT, T, 3>(w, s)};
+    typename Operand<T>::v8 k;
+    __builtin_memcpy(&k, f, 16);
+    return k;
+  }
+};
+
+// A lane's part of 32 tokens of V: BYTES of each of its eight tokens, from byte
+// `from` of the lane's on.
+template <int FMT, int D, int BYTES>
+struct VPart {
+  static constexpr int kWords = (BYTES + 3) / 4;
+  static constexpr int kPairs = BYTES * 4 / Format<FMT>::kBits;   // pairs of values
+  uint32_t code[2][4][kWords], scale[2];    // scale: a byte for each of four tokens
+
+  __device__ __forceinline__ void load(const Half* h, int block_shift, uint32_t m, uint32_t g,
+                                       uint32_t from) {
+    constexpr uint32_t kCode = Chunk<FMT, D>::kCode;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const int32_t position = tile * kTile + half * 16;
-      const int32_t column = position >> block_shift;
-      const int32_t inside = position - (column << block_shift);
-      const int64_t at = int64_t(table[column]) * p.page_bytes + head_offset;
-      const char* kc = p.k + at + inside * C::kCode;
-      const char* vc = p.v + at + inside * C::kCode;
-      const char* ksc = p.k + at + block_size * C::kCode + inside;
-      const char* vsc = p.v + at + block_size * C::kCode + inside;
-      constexpr int kKBytes = kKWords * 4;
-      __builtin_memcpy(k[half],
-                       __builtin_assume_aligned(kc + m * C::kCode + g * kKBytes,
-                                                kKBytes < 16 ? kKBytes : 16), kKBytes);
 #pragma unroll
-      for (int i = 0; i < kKScales; ++i)
-        ks[half][i] = static_cast<uint8_t>(
-            ksc[(D == 64 ? g / 2 : g * kKScales + i) * block_size + m]);
+      for (uint32_t i = 0; i < 4; ++i)
+        load_bytes<BYTES>(code[half][i], h[half].v + i * kCode,
+                          4 * g * kCode + m * (kCode / 16) + from);
+      load_bytes<4>(&scale[half], h[half].v_scales, ((m * D / 512) << block_shift) + 4 * g);
+    }
+  }
+
+  // What no row of [low, high] sees may hold anything: its product with a
+  // probability of 0 has to be 0. Returns the seen tokens (bit 4 half + i) that are
+  // no number; they count as 0 too and are noted apart.
+  __device__ __forceinline__ uint32_t clear_unseen(int32_t begin, int32_t g, int32_t low,
+                                                   int32_t high, int32_t window, int32_t sinks) {
+    uint32_t odd = 0;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const char* t = vc + (4 * g + i) * C::kCode + m * kVBytes;
-        if constexpr (kVBytes == 2) {
-          v[half][i][0] = *reinterpret_cast<const uint16_t*>(t);
-        } else {
-          __builtin_memcpy(v[half][i], __builtin_assume_aligned(t, kVBytes), kVBytes);
-        }
+        const int32_t j = begin + 16 * half + 4 * g + i;
+        const bool any = (j <= high) & ((low - j < window) | (j < sinks));
+        const uint32_t byte = (scale[half] >> (8 * i)) & 255u;
+        const bool number = byte != kNoNumber;
+        odd |= any & !number ? 1u << (4 * half + i) : 0u;
+        const uint32_t keep = any & number ? ~0u : 0u;
+        scale[half] = (scale[half] & ~(255u << (8 * i))) | ((keep ? byte : 127u) << (8 * i));
+#pragma unroll
+        for (int w = 0; w < kWords; ++w) code[half][i][w] &= keep;
       }
-      vs[half] = *reinterpret_cast<const uint32_t*>(vsc + (m * D / 512) * block_size + 4 * g);
     }
+    return odd;
+  }
+
+  __device__ __forceinline__ void scales(float (*s)[4]) const {
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[half][i] = scale_of((scale[half] >> (8 * i)) & 255u);
+  }
+
+  // The operands of values 2 B and 2 B + 1: eight tokens side by side each.
+  template <typename T, int B>
+  __device__ __forceinline__ void operands(const float (*s)[4], typename Operand<T>::v8* even,
+                                           typename Operand<T>::v8* odd) const {
+    uint32_t e[4], o[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int half = t / 2, i = 2 * (t % 2);
+      const uint32_t c0 = decode_pair<FMT, T, B>(code[half][i], s[half][i]);
+      const uint32_t c1 = decode_pair<FMT, T, B>(code[half][i + 1], s[half][i + 1]);
+      e[t] = __builtin_amdgcn_perm(c1, c0, 0x05040100u);
+      o[t] = __builtin_amdgcn_perm(c1, c0, 0x07060302u);
+    }
+    __builtin_memcpy(even, e, 16);
+    __builtin_memcpy(odd, o, 16);
   }
 };
 
@@ -415,49 +499,148 @@ __device__ __forceinline__ bool seen(const AttendArgs& a, int32_t p, int32_t j) 
   return (j <= p) & ((p - j < a.window) | (j < a.sinks));
 }
 
+// Rows that see a V that is no number are none in its group of values; the
+// others, in whose product it had to count as 0, stay as they are. Sets in
+// `poison` bit (D / 128 or 1) r + i where the lane's row of row tile r is none
+// in the i-th group of the lane's values [D/4 g, D/4 (g + 1)). `odd`: bits of the
+// tokens 4g + i (16 + 4g + i) of the tile, held by the operand's lanes, lane m in
+// the group of values [D/16 m, ..).
+template <int D, int R>
+__device__ __forceinline__ void note_odd(const AttendArgs& a, uint32_t odd, int32_t begin,
+                                         const int32_t* position, int g, uint32_t& poison) {
+  constexpr int kEach = D == 256 ? 2 : 1;
+#pragma unroll 1
+  for (int t = 0; t < kTile; ++t) {
+    const int bit = 4 * (t / 16) + t % 4;
+    const int32_t j = begin + t;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int group = D == 64 ? g / 2 : g * kEach + i;
+      const int from = (t % 16) / 4 * 16 + group * 512 / D;
+      const bool none = (__shfl(static_cast<int>(odd), from) >> bit) & 1;
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        poison |= none & seen(a, position[r], j) ? 1u << (kEach * r + i) : 0u;
+    }
+  }
+}
+
+// Which of the tiles that rows [low, high] visit comes v-th.
+__device__ __forceinline__ int32_t tile_at(const Item& it, int32_t v) {
+  return v < it.first_tiles ? v : v - it.first_tiles + it.window_tile;
+}
+
+// Whether every row of [low, high] sees every token of the tile at `begin`.
+__device__ __forceinline__ bool seen_whole(const AttendArgs& a, int32_t low, int32_t high,
+                                           int32_t begin) {
+  return (begin + kTile - 1 <= low) & ((high - begin < a.window) | (begin + kTile <= a.sinks));
+}
+
+// Query rows of a 16-row tile as a matrix operand: lane's row, its values [D/4 g, ..).
+template <typename T, int D>
+__device__ __forceinline__ void load_query(const AttendArgs& a, const Item& it, int32_t row,
+                                           bool there, int g, typename Operand<T>::v8* q) {
+  const int32_t token = row / a.group;
+  const T* from = reinterpret_cast<const T*>(a.q.base) + (int64_t(it.token) + token) * a.q.token +
+                  (int64_t(it.kv_head) * a.group + (row - token * a.group)) * a.q.head +
+                  g * (D / 4);
+#pragma unroll
+  for (int s = 0; s < D / 32; ++s) {
+    uint32_t w[4] = {0, 0, 0, 0};
+    if (there) {
+      if (a.q.whole_words) {
+        const v4u x = *(const gv4u*)(from + s * 8);
+        __builtin_memcpy(w, &x, 16);
+      } else {
+        T t[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[j] = from[s * 8 + j];
+        __builtin_memcpy(w, t, 16);
+      }
+    }
+    __builtin_memcpy(&q[s], w, 16);
+  }
+}
+
+// Scores of a row tile (lane's row, eight of its tokens) into probabilities
+// against the largest score so far, with the sums made before faded to it.
+template <typename T, int N>
+__device__ __forceinline__ typename Operand<T>::v8 softmax_step(f32x4* x, float c, float& top,
+                                                               float& sum, f32x4 (&o)[N]) {
+  float most = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
+                     fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+  most = fmaxf(top, row_max(most));
+  if (__any(most > top)) {
+    const float fade = top == most ? 1.f : __builtin_amdgcn_exp2f((top - most) * c);
+    sum *= fade;
+#pragma unroll
+    for (int d = 0; d < N; ++d) o[d] *= fade;
+    top = most;
+  }
+  const float lift = Operand<T>::kLift - (most == -INFINITY ? 0.f : most * c);
+  typename Operand<T>::v8 p;
+  float total = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i / 4][i % 4], c, lift));
+    total += e;
+    p[i] = static_cast<T>(e);
+  }
+  sum += total;
+  return p;
+}
+
 constexpr int kAttendLanes = 256, kAttendWaves = 4;
 
 template <int FMT, int D, typename T, int R>
 __global__ __launch_bounds__(kAttendLanes) void quant_attend_kernel(AttendArgs a) {
   typedef typename Operand<T>::v8 v8;
-  using Tile = CacheTile<FMT, D>;
   constexpr int kSteps = D / 32;    // matrix steps along the head
   constexpr int kOut = D / 16;      // output tiles of 16 values
   constexpr int kPad = D + 4;
+  constexpr int kEach = D == 256 ? 2 : 1;   // groups of the lane's values of the result
   __shared__ float joined[kAttendWaves][16][kPad];
   __shared__ float stats[2][kAttendWaves][16 * R];
 
-  const Header& h = header(a.plan);
-  if (static_cast<int32_t>(blockIdx.x) >= h.items[a.kind]) return;
   const Item it = reinterpret_cast<const Item*>(a.plan + a.at_items)[blockIdx.x];
-  const Seq seq = reinterpret_cast<const Seq*>(a.plan + a.at_seqs)[it.seq];
-  const int32_t* table = reinterpret_cast<const int32_t*>(a.plan + a.at_table) + seq.table;
+  if (static_cast<int32_t>(blockIdx.x) >= header(a.plan).items[a.kind]) return;
+  const int32_t* table = reinterpret_cast<const int32_t*>(a.plan + a.at_table) + it.table;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int lane = threadIdx.x % 64, m = lane % 16, g = lane / 16;
   const int64_t head_offset = it.kv_head * Chunk<FMT, D>::bytes(1 << a.block_shift);
 
-  // queries: row m of each row tile, its values [D/4 g, D/4 (g + 1))
+  struct Tile {
+    KPart<FMT, D> k[2];
+    VPart<FMT, D, Chunk<FMT, D>::kCode / 16> v;
+  };
+  const auto load = [&](Tile* t, int32_t v) {
+    const int32_t position = tile_at(it, v) * kTile;
+    const Half h[2] = {
+        find_half<FMT, D>(a.pages, head_offset, a.block_shift, table, position),
+        find_half<FMT, D>(a.pages, head_offset, a.block_shift, table, position + 16)};
+    t->k[0].load(h[0], a.block_shift, m, g);
+    t->k[1].load(h[1], a.block_shift, m, g);
+    t->v.load(h, a.block_shift, m, g, 0);
+  };
+  Tile cur;
+  int32_t at = it.tile + wave;
+  if (at < it.tile_end) load(&cur, at);
+
   v8 q[R][kSteps];
   int32_t position[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int32_t row = it.row + 16 * r + m;
     const bool there = 16 * r + m < it.rows;
-    const int32_t token = row / a.group;
-    position[r] = seq.len - seq.fresh + (there ? token : 0);
-    const T* from = reinterpret_cast<const T*>(a.q.base) + (int64_t(seq.token) + token) * a.q.token +
-                    (int64_t(it.kv_head) * a.group + (row - token * a.group)) * a.q.head + g * (D / 4);
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) q[r][s][j] = there ? from[s * 8 + j] : T(0.f);
-    }
+    position[r] = it.base + (there ? row / a.group : 0);
+    load_query<T, D>(a, it, row, there, g, q[r]);
   }
-  const int32_t base = seq.len - seq.fresh;
-  const int32_t low = base + it.row / a.group, high = base + (it.row + it.rows - 1) / a.group;
+  const int32_t low = it.base + it.row / a.group;
+  const int32_t high = it.base + (it.row + it.rows - 1) / a.group;
 
   f32x4 o[R][kOut];
   float top[R], sum[R];
+  uint32_t poison = 0;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     top[r] = -INFINITY;
@@ -466,18 +649,10 @@ __global__ __launch_bounds__(kAttendLanes) void quant_attend_kernel(AttendArgs a
     for (int d = 0; d < kOut; ++d) o[r][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  auto tile_at = [&](int32_t v) {
-    return v < it.first_tiles ? v : v - it.first_tiles + it.window_tile;
-  };
-  Tile cur;
-  int32_t at = it.tile + wave;
-  if (at < it.tile_end)
-    cur.load(a.pages, head_offset, a.block_shift, table, tile_at(at), m, g);
   for (; at < it.tile_end; at += kAttendWaves) {
-    const int32_t tile = tile_at(at);
+    const int32_t begin = tile_at(it, at) * kTile;
     Tile next = cur;
-    if (at + kAttendWaves < it.tile_end)
-      next.load(a.pages, head_offset, a.block_shift, table, tile_at(at + kAttendWaves), m, g);
+    if (at + kAttendWaves < it.tile_end) load(&next, at + kAttendWaves);
 
     // scores: lane holds row m, tokens 4g + i of both halves
     f32x4 x[R][2];
@@ -485,132 +660,47 @@ __global__ __launch_bounds__(kAttendLanes) void quant_attend_kernel(AttendArgs a
     for (int half = 0; half < 2; ++half) {
 #pragma unroll
       for (int r = 0; r < R; ++r) x[r][half] = f32x4{0.f, 0.f, 0.f, 0.f};
+      each_constant<0, kSteps>([&](auto s) {
+        const v8 k = cur.k[half].template operand<T, decltype(s)::value>();
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const float scale = scale_of(cur.ks[half][Tile::kKScales == 2 ? s / 4 : 0]);
-        const uint32_t* w = &cur.k[half][s * Format<FMT>::kBits / 4];
-        uint32_t f[4];
-        f[0] = decode_pair<FMT, T, 0>(w, scale);
-        f[1] = decode_pair<FMT, T, 1>(w, scale);
-        f[2] = decode_pair<FMT, T, 2>(w, scale);
-        f[3] = decode_pair<FMT, T, 3>(w, scale);
-        v8 kf;
-        __builtin_memcpy(&kf, f, 16);
-#pragma unroll
-        for (int r = 0; r < R; ++r) x[r][half] = Operand<T>::mma(kf, q[r][s], x[r][half]);
-      }
+        for (int r = 0; r < R; ++r)
+          x[r][half] = Operand<T>::mma(k, q[r][decltype(s)::value], x[r][half]);
+      });
     }
 
-    // Tokens that some row does not see; in other tiles every row sees every
-    // token. All by selection: with branches around the changed elements the
-    // compiler lost one of the changes (the first element's, its operands being
-    // copied out of the matrix registers in several places).
-    const int32_t begin = tile * kTile;
-    const bool whole = (begin + kTile - 1 <= low) &
-                       ((high - begin < a.window) | (begin + kTile <= a.sinks));
-    uint32_t odd = 0;   // seen tokens (bit 4 half + i) whose V is no number
-    if (!whole) {
+    // Tokens that some row does not see. All by selection: with branches around
+    // the changed elements the compiler lost one of the changes (the first
+    // element's, its operands being copied out of the matrix registers in
+    // several places).
+    if (!seen_whole(a, low, high, begin)) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+      for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int32_t j = begin + 16 * half + 4 * g + i;
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int r = 0; r < R; ++r)
-            x[r][half][i] = seen(a, position[r], j) ? x[r][half][i] : -INFINITY;
-          // what no row sees may hold anything: its product with a
-          // probability of 0 has to be 0
-          const bool any = (j <= high) & ((low - j < a.window) | (j < a.sinks));
-          const uint32_t byte = (cur.vs[half] >> (8 * i)) & 255u;
-          const bool number = byte != kNoNumber;
-          odd |= any & !number ? 1u << (4 * half + i) : 0u;
-          const uint32_t keep = any & number ? ~0u : 0u;
-          cur.vs[half] = (cur.vs[half] & ~(255u << (8 * i))) | ((keep ? byte : 127u) << (8 * i));
-#pragma unroll
-          for (int w = 0; w < Tile::kVWords; ++w) cur.v[half][i][w] &= keep;
-        }
-      }
+            x[r][half][i] = seen(a, position[r], begin + 16 * half + 4 * g + i) ? x[r][half][i]
+                                                                                : -INFINITY;
+      const uint32_t odd = cur.v.clear_unseen(begin, g, low, high, a.window, a.sinks);
+      if (__any(odd != 0)) note_odd<D, R>(a, odd, begin, position, g, poison);
     }
 
     v8 p[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      float most = fmaxf(fmaxf(fmaxf(x[r][0][0], x[r][0][1]), fmaxf(x[r][0][2], x[r][0][3])),
-                         fmaxf(fmaxf(x[r][1][0], x[r][1][1]), fmaxf(x[r][1][2], x[r][1][3])));
-      most = fmaxf(top[r], row_max(most));
-      if (__any(most > top[r])) {
-        const float fade = top[r] == most ? 1.f : __builtin_amdgcn_exp2f((top[r] - most) * a.c);
-        sum[r] *= fade;
-#pragma unroll
-        for (int d = 0; d < kOut; ++d) o[r][d] *= fade;
-        top[r] = most;
-      }
-      const float lift = Operand<T>::kLift - (most == -INFINITY ? 0.f : most * a.c);
-      float e[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r][i / 4][i % 4], a.c, lift));
-        sum[r] += e[i];
-        p[r][i] = static_cast<T>(e[i]);
-      }
-    }
+    for (int r = 0; r < R; ++r) p[r] = softmax_step<T>(x[r], a.c, top[r], sum[r], o[r]);
 
-    // values: pairs of tokens side by side, one operand per value of the lane
-    float vscale[2][4];
-#pragma unroll
-    for (int half = 0; half < 2; ++half)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) vscale[half][i] = scale_of((cur.vs[half] >> (8 * i)) & 255u);
-    auto values = [&](auto pair) {
-      constexpr int B = decltype(pair)::value;
-      uint32_t even[4], oddv[4];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int half = t / 2, i = 2 * (t % 2);
-        const uint32_t c0 = decode_pair<FMT, T, B>(cur.v[half][i], vscale[half][i]);
-        const uint32_t c1 = decode_pair<FMT, T, B>(cur.v[half][i + 1], vscale[half][i + 1]);
-        even[t] = __builtin_amdgcn_perm(c1, c0, 0x05040100u);
-        oddv[t] = __builtin_amdgcn_perm(c1, c0, 0x07060302u);
-      }
-      v8 f0, f1;
-      __builtin_memcpy(&f0, even, 16);
-      __builtin_memcpy(&f1, oddv, 16);
+    float scale[2][4];
+    cur.v.scales(scale);
+    each_constant<0, kOut / 2>([&](auto b) {
+      constexpr int B = decltype(b)::value;
+      v8 even, odd;
+      cur.v.template operands<T, B>(scale, &even, &odd);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        o[r][2 * B] = Operand<T>::mma(f0, p[r], o[r][2 * B]);
-        o[r][2 * B + 1] = Operand<T>::mma(f1, p[r], o[r][2 * B + 1]);
+        o[r][2 * B] = Operand<T>::mma(even, p[r], o[r][2 * B]);
+        o[r][2 * B + 1] = Operand<T>::mma(odd, p[r], o[r][2 * B + 1]);
       }
-    };
-    each_constant<0, kOut / 2>(values);
-
-    // Rows that see a V that is no number are none there; the others, in whose
-    // product it had to count as 0, stay as they are. Lane l of the operand
-    // knows the groups of values [D/16 m, ..), of the result [D/4 g, ..).
-    if (__any(odd != 0)) {
-      for (int t = 0; t < kTile; ++t) {
-        const int owner_g = (t % 16) / 4, bit = 4 * (t / 16) + t % 4;
-        const int32_t j = begin + t;
-#pragma unroll
-        for (int grp = 0; grp < D / 32; ++grp) {
-          // a lane of the operand that holds this token and group
-          const int from = owner_g * 16 + grp * 512 / D;
-          const bool none = (__shfl(static_cast<int>(odd), from) >> bit) & 1;
-          if (!none) continue;
-#pragma unroll
-          for (int r = 0; r < R; ++r) {
-            const bool sees = seen(a, position[r], j);
-#pragma unroll
-            for (int d = 0; d < kOut; ++d)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int value = (D / 16) * (4 * g + i) + d;
-                o[r][d][i] = sees & (value / 32 == grp) ? __uint_as_float(0x7FC00000u)
-                                                        : o[r][d][i];
-              }
-          }
-        }
-      }
-    }
+    });
     cur = next;
   }
 
@@ -634,7 +724,9 @@ __global__ __launch_bounds__(kAttendLanes) void quant_attend_kernel(AttendArgs a
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int d = 0; d < kOut; ++d)
-        joined[wave][m][(D / 16) * (4 * g + i) + d] = o[r][d][i] * fade;
+        joined[wave][m][(D / 16) * (4 * g + i) + d] =
+            (poison >> (kEach * r + (kEach == 2 ? i / 2 : 0))) & 1 ? __uint_as_float(0x7FC00000u)
+                                                                   : o[r][d][i] * fade;
     __syncthreads();
     const int row = threadIdx.x / 16, part = threadIdx.x % 16;
     if (16 * r + row < it.rows) {
@@ -655,13 +747,13 @@ __global__ __launch_bounds__(kAttendLanes) void quant_attend_kernel(AttendArgs a
       }
       if (it.slot < 0) {
         const int32_t n = it.row + 16 * r + row, token = n / a.group;
-        T* to = reinterpret_cast<T*>(a.out.base) + (int64_t(seq.token) + token) * a.out.token +
+        T* to = reinterpret_cast<T*>(a.out.base) + (int64_t(it.token) + token) * a.out.token +
                 (int64_t(it.kv_head) * a.group + (n - token * a.group)) * a.out.head;
         const float inv = 1.f / total;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) to[part * (D / 16) + i] = static_cast<T>(y[i] * inv);
       } else {
-        float* to = a.work + it.slot * a.slot_floats + (16 * r + row) * (D + 2);
+        float* to = a.work + it.slot * a.slot_floats + (16 * r + row) * (D + 4);
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) to[part * (D / 16) + i] = y[i];
         if (part == 0) {
@@ -674,44 +766,82 @@ __global__ __launch_bounds__(kAttendLanes) void quant_attend_kernel(AttendArgs a
   }
 }
 
-// Rows whose tiles several items shared: one workgroup a row, 256 / D parts
-// side by side.
+// Rows whose tiles several items shared: their parts, scaled to the largest
+// score of all, over the sum of their sums. A workgroup's lanes are groups of D / 4,
+// four values a lane. Up to kSides parts (rows of prompts) each group takes rows
+// of its own; more (few rows over a long axis) are shared out to the groups.
+constexpr int kMergeRows = 16;   // workgroups of one merge
+
 template <int D, typename T>
 __global__ __launch_bounds__(256) void quant_merge_kernel(AttendArgs a) {
-  constexpr int kSide = 256 / D;
-  __shared__ float side[kSide][D];
-  __shared__ float side_sum[kSide];
-  const Header& h = header(a.plan);
-  if (static_cast<int32_t>(blockIdx.x) >= h.merges) return;
+  constexpr int kLanes = D / 4, kSides = 256 / kLanes;
+  __shared__ f32x4 side[kSides][kLanes];
+  __shared__ float side_sum[kSides], side_top[4];
   const Merge mg = reinterpret_cast<const Merge*>(a.plan + a.at_merges)[blockIdx.x];
-  const int row = blockIdx.y;
-  if (row >= mg.rows) return;
-  const Seq seq = reinterpret_cast<const Seq*>(a.plan + a.at_seqs)[mg.seq];
+  if (static_cast<int32_t>(blockIdx.x) >= header(a.plan).merges) return;
   const int64_t each = a.kind_slot_floats[mg.kind];
-  const float* from = a.work_base + a.kind_work[mg.kind] + mg.slot * each + row * (D + 2);
-  float most = -INFINITY;
-  for (int p = 0; p < mg.parts; ++p) most = fmaxf(most, from[p * each + D]);
-  const int d = threadIdx.x % D, s = threadIdx.x / D;
-  float y = 0.f, total = 0.f;
-  for (int p = s; p < mg.parts; p += kSide) {
-    const float t = from[p * each + D];
-    const float fade = t == most ? 1.f : __builtin_amdgcn_exp2f((t - most) * a.c);
-    y += fade * from[p * each + d];
-    total += fade * from[p * each + D + 1];
-  }
-  side[s][d] = y;
-  if (d == 0) side_sum[s] = total;
-  __syncthreads();
-  if (s != 0) return;
+  const float* parts = a.work_base + a.kind_work[mg.kind] + mg.slot * each;
+  const int at = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  const auto store = [&](int32_t row, f32x4 y, float total) {
+    const int32_t n = mg.row + row, token = n / a.group;
+    T* to = reinterpret_cast<T*>(a.out.base) + (int64_t(mg.token) + token) * a.out.token +
+            (int64_t(mg.kv_head) * a.group + (n - token * a.group)) * a.out.head + 4 * at;
 #pragma unroll
-  for (int i = 1; i < kSide; ++i) {
-    y += side[i][d];
-    total += side_sum[i];
+    for (int i = 0; i < 4; ++i) to[i] = static_cast<T>(y[i] / total);
+  };
+  if (mg.parts <= kSides) {
+    for (int32_t row = blockIdx.y * kSides + group; row < mg.rows; row += kMergeRows * kSides) {
+      const float* from = parts + row * (D + 4);
+      float t[kSides], most = -INFINITY;
+#pragma unroll
+      for (int p = 0; p < kSides; ++p) {
+        t[p] = p < mg.parts ? from[p * each + D] : -INFINITY;
+        most = fmaxf(most, t[p]);
+      }
+      f32x4 y = {0.f, 0.f, 0.f, 0.f};
+      float total = 0.f;
+#pragma unroll
+      for (int p = 0; p < kSides; ++p) {
+        if (p >= mg.parts) continue;
+        const float fade = t[p] == most ? 1.f : __builtin_amdgcn_exp2f((t[p] - most) * a.c);
+        y += *reinterpret_cast<const f32x4*>(from + p * each + 4 * at) * fade;
+        total += from[p * each + D + 1] * fade;
+      }
+      store(row, y, total);
+    }
+    return;
   }
-  const int32_t n = mg.row + row, token = n / a.group;
-  T* to = reinterpret_cast<T*>(a.out.base) + (int64_t(seq.token) + token) * a.out.token +
-          (int64_t(mg.kv_head) * a.group + (n - token * a.group)) * a.out.head;
-  to[d] = static_cast<T>(y / total);
+  for (int32_t row = blockIdx.y; row < mg.rows; row += kMergeRows) {
+    const float* from = parts + row * (D + 4);
+    float most = -INFINITY;
+    for (int p = threadIdx.x; p < mg.parts; p += 256) most = fmaxf(most, from[p * each + D]);
+#pragma unroll
+    for (int far = 32; far; far /= 2) most = fmaxf(most, __shfl_xor(most, far));
+    if (threadIdx.x % 64 == 0) side_top[threadIdx.x / 64] = most;
+    __syncthreads();
+    most = fmaxf(fmaxf(side_top[0], side_top[1]), fmaxf(side_top[2], side_top[3]));
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+    float total = 0.f;
+#pragma unroll 4
+    for (int p = group; p < mg.parts; p += kSides) {
+      const float t = from[p * each + D];
+      const float fade = t == most ? 1.f : __builtin_amdgcn_exp2f((t - most) * a.c);
+      y += *reinterpret_cast<const f32x4*>(from + p * each + 4 * at) * fade;
+      total += from[p * each + D + 1] * fade;
+    }
+    side[group][at] = y;
+    if (at == 0) side_sum[group] = total;
+    __syncthreads();
+    if (group == 0) {
+#pragma unroll
+      for (int i = 1; i < kSides; ++i) {
+        y += side[i][at];
+        total += side_sum[i];
+      }
+      store(row, y, total);
+    }
+    __syncthreads();
+  }
 }
 
 }  // namespace

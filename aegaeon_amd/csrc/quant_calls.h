@@ -181,7 +181,7 @@ int64_t parts_floats(const Header& h, int32_t head_dim, int64_t* at, int64_t* ea
   int64_t floats = 0;
   for (int kind = 0; kind < kKinds; ++kind) {
     at[kind] = floats;
-    each[kind] = int64_t(kKindRows[kind]) * (head_dim + 2);
+    each[kind] = int64_t(kKindRows[kind]) * (head_dim + 4);   // row, its top and sum
     floats += h.room.slots[kind] * each[kind];
   }
   return floats;
@@ -324,10 +324,8 @@ int aegkv_quant_attend(const void* plan, const void* device_plan, int format, in
     constexpr int kFormat = decltype(fmt)::value, kDim = decltype(d)::value;
     const auto launch = [&](auto t) {
       typedef decltype(t) T;
-      int merged_rows = 0;
       for (int kind = 0; kind < kKinds; ++kind) {
         if (!h.room.items[kind]) continue;
-        if (h.room.slots[kind]) merged_rows = kKindRows[kind];
         a.kind = kind;
         a.at_items = h.room.at_items[kind];
         a.work = a.work_base + a.kind_work[kind];
@@ -341,7 +339,7 @@ int aegkv_quant_attend(const void* plan, const void* device_plan, int format, in
         if (rc) return rc;
       }
       if (h.room.merges) {
-        const dim3 grid(static_cast<uint32_t>(h.room.merges), merged_rows);
+        const dim3 grid(static_cast<uint32_t>(h.room.merges), kMergeRows);
         quant_merge_kernel<kDim, T><<<grid, 256, 0, stream>>>(a);
         return launched("quant_merge_kernel launch");
       }

@@ -11,6 +11,7 @@ libaegkv.so; there is no Python or CPU fallback.
 from __future__ import annotations
 
 import ctypes
+import struct
 import sys
 import threading
 import weakref
@@ -1005,6 +1006,10 @@ class QuantCache:
         self.num_blocks = _tensor_bytes(k_pages) // self.page_bytes
         self.device = k_pages.device
         self._args = (_FORMATS[fmt], self.head_dim, k_pages.data_ptr(), v_pages.data_ptr())
+        # CacheArgs of csrc/hostargs.cpp
+        self._packed = struct.pack(
+            "11q", *(_lib.address(f"aegkv_quant_{op}") for op in ("write", "read", "attend")),
+            *self._args, self.kv_heads, self.block_size, self.num_blocks, self.device.index)
 
 
 class CacheBatch:
@@ -1043,7 +1048,12 @@ class CacheBatch:
             raise ValueError(f"a batch lives on a device (HIP), not on {self.device}")
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
-        self._workspace: dict = {}
+        self._workspace = {}    # bytes by head width
+        for d in (64, 128, 256):
+            n = ctypes.c_int64()
+            _lib.check(_lib.load().aegkv_quant_attend_workspace(self._host_ptr, d,
+                                                                ctypes.byref(n)))
+            self._workspace[d] = int(n.value)
         self._used: dict = {}     # raw stream -> event behind its last call over this batch
         with torch.cuda.device(self.device):
             st = stream if stream is not None else torch.cuda.current_stream()
@@ -1090,6 +1100,11 @@ class CacheBatch:
         self._uploaded = torch.cuda.Event()
         self._uploaded.record(st)
         self._stream = st.cuda_stream
+        # BatchArgs of csrc/hostargs.cpp
+        self._packed = struct.pack(
+            "13q", self._host_ptr, self._plan.data_ptr(), self._stream, self.kv_heads, self.heads,
+            self.block_size, self.num_blocks, self.device.index, self.num_tokens,
+            self.read_tokens, *self._workspace.values())
 
     def update(self, block_tables, seq_lens, new_lens, *,
                stream: torch.cuda.Stream | None = None) -> None:
@@ -1143,6 +1158,11 @@ def _quant_call(cache: QuantCache, batch: CacheBatch):
         raise ValueError(f"a batch on {batch.device}, a cache on {cache.device}")
 
 
+def _here(cache: QuantCache) -> tuple:
+    """(raw current stream of the cache's device, current device)."""
+    return torch._C._cuda_getCurrentRawStream(cache.device.index), torch._C._cuda_getDevice()
+
+
 def _rows_arg(t: torch.Tensor, what: str, heads: int, cache: QuantCache, dtypes):
     """(pointer, token stride, head stride) of a [tokens, heads, head_dim] tensor."""
     if t.device != cache.device:
@@ -1188,6 +1208,9 @@ def quant_write(cache: QuantCache, batch: CacheBatch, k: torch.Tensor, v: torch.
     and each takes its nearest code, ties to even. A group with a NaN or an
     infinity reads back as NaN.
     """
+    if stream is None and _lib.hostargs().quant_write(
+            cache._packed, batch._packed, k, v, *_here(cache)) is not None:
+        return
     _quant_call(cache, batch)
     kp = _rows_arg(k, "k", cache.kv_heads, cache, _DTYPES)
     vp = _rows_arg(v, "v", cache.kv_heads, cache, _DTYPES)
@@ -1208,9 +1231,15 @@ def quant_read(cache: QuantCache, batch: CacheBatch, *, tokens: str = "all",
     [tokens, kv_heads, head_dim] each, all tokens of the sequences one after
     another ("all"), or the new ones ("new"). `out`: two tensors to read into (their
     type counts); rows behind the last token are left as they were."""
-    _quant_call(cache, batch)
     if tokens not in ("all", "new"):
         raise ValueError(f"tokens are 'all' or 'new', not {tokens!r}")
+    if stream is None:
+        done = _lib.hostargs().quant_read(cache._packed, batch._packed, tokens == "new",
+                                          _DTYPES.get(dtype) if out is None else out,
+                                          *_here(cache))
+        if done is not None:
+            return done
+    _quant_call(cache, batch)
     n = batch.read_tokens if tokens == "all" else batch.num_tokens
     if out is None:
         if dtype not in _DTYPES:
@@ -1241,6 +1270,11 @@ def quant_attend(cache: QuantCache, batch: CacheBatch, q: torch.Tensor, *,
     scale: of the scores, head_dim ** -0.5 by default. `out` (q itself is fine)
     takes the result; rows behind the batch's last token are left as they were.
     """
+    if stream is None:
+        done = _lib.hostargs().quant_attend(cache._packed, batch._packed, q, out, scale,
+                                            *_here(cache))
+        if done is not None:
+            return done
     _quant_call(cache, batch)
     qp = _rows_arg(q, "q", batch.heads, cache, (torch.bfloat16, torch.float16))
     if out is None:
@@ -1250,11 +1284,7 @@ def quant_attend(cache: QuantCache, batch: CacheBatch, q: torch.Tensor, *,
         raise ValueError(f"{q.size(0)} queries, {out.size(0)} rows of out")
     lib = _lib.load()
     d = cache.head_dim
-    size = batch._workspace.get(d)
-    if size is None:
-        n = ctypes.c_int64()
-        _lib.check(lib.aegkv_quant_attend_workspace(batch._host_ptr, d, ctypes.byref(n)))
-        size = batch._workspace[d] = int(n.value)
+    size = batch._workspace[d]
     work = _empty_on(stream, size, dtype=torch.uint8, device=q.device) if size else None
     _on_stream(cache, batch, stream, lambda raw: lib.aegkv_quant_attend(
         batch._host_ptr, batch._plan.data_ptr(), *cache._args, *qp, *op, q.size(0),
