@@ -21,7 +21,7 @@ constexpr int kTile = 32;
 //                share out the tiles of an item and join at its end;
 //   kMany:       blocks of kManyRows rows, the waves share out the rows.
 enum Kind { kFew = 0, kMore = 1, kMany = 2, kKinds = 3 };
-constexpr int kManyRows = 32;
+constexpr int kManyRows = 128;
 constexpr int kKindRows[kKinds] = {16, 32, kManyRows};
 
 struct Seq {

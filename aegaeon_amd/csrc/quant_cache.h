@@ -502,27 +502,29 @@ __device__ __forceinline__ bool seen(const AttendArgs& a, int32_t p, int32_t j) 
 // Rows that see a V that is no number are none in its group of values; the
 // others, in whose product it had to count as 0, stay as they are. Sets in
 // `poison` bit (D / 128 or 1) r + i where the lane's row of row tile r is none
-// in the i-th group of the lane's values [D/4 g, D/4 (g + 1)). `odd`: bits of the
-// tokens 4g + i (16 + 4g + i) of the tile, held by the operand's lanes, lane m in
-// the group of values [D/16 m, ..).
-template <int D, int R>
-__device__ __forceinline__ void note_odd(const AttendArgs& a, uint32_t odd, int32_t begin,
+// in the i-th group of the lane's values [D/4 g, D/4 (g + 1)). none(group, t):
+// whether the tile's token t is no number there.
+template <int D, int R, typename F>
+__device__ __forceinline__ void note_odd(const AttendArgs& a, const F& none, int32_t begin,
                                          const int32_t* position, int g, uint32_t& poison) {
   constexpr int kEach = D == 256 ? 2 : 1;
 #pragma unroll 1
   for (int t = 0; t < kTile; ++t) {
-    const int bit = 4 * (t / 16) + t % 4;
-    const int32_t j = begin + t;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int group = D == 64 ? g / 2 : g * kEach + i;
-      const int from = (t % 16) / 4 * 16 + group * 512 / D;
-      const bool none = (__shfl(static_cast<int>(odd), from) >> bit) & 1;
+      const bool is_none = none(D == 64 ? g / 2 : g * kEach + i, t);
 #pragma unroll
       for (int r = 0; r < R; ++r)
-        poison |= none & seen(a, position[r], j) ? 1u << (kEach * r + i) : 0u;
+        poison |= is_none & seen(a, position[r], begin + t) ? 1u << (kEach * r + i) : 0u;
     }
   }
+}
+
+// A value of the result, or none.
+template <int D>
+__device__ __forceinline__ float unless_poisoned(float x, uint32_t poison, int r, int i) {
+  constexpr int kEach = D == 256 ? 2 : 1;
+  return (poison >> (kEach * r + (kEach == 2 ? i / 2 : 0))) & 1 ? __uint_as_float(0x7FC00000u) : x;
 }
 
 // Which of the tiles that rows [low, high] visit comes v-th.
@@ -598,7 +600,6 @@ __global__ __launch_bounds__(kAttendLanes) void quant_attend_kernel(AttendArgs a
   constexpr int kSteps = D / 32;    // matrix steps along the head
   constexpr int kOut = D / 16;      // output tiles of 16 values
   constexpr int kPad = D + 4;
-  constexpr int kEach = D == 256 ? 2 : 1;   // groups of the lane's values of the result
   __shared__ float joined[kAttendWaves][16][kPad];
   __shared__ float stats[2][kAttendWaves][16 * R];
 
@@ -682,7 +683,14 @@ __global__ __launch_bounds__(kAttendLanes) void quant_attend_kernel(AttendArgs a
             x[r][half][i] = seen(a, position[r], begin + 16 * half + 4 * g + i) ? x[r][half][i]
                                                                                 : -INFINITY;
       const uint32_t odd = cur.v.clear_unseen(begin, g, low, high, a.window, a.sinks);
-      if (__any(odd != 0)) note_odd<D, R>(a, odd, begin, position, g, poison);
+      if (__any(odd != 0)) {
+        // lane m of the operand holds the group of values [D/16 m, ..)
+        const auto none = [&](int group, int t) {
+          const int from = (t % 16) / 4 * 16 + group * 512 / D;
+          return ((__shfl(static_cast<int>(odd), from) >> (4 * (t / 16) + t % 4)) & 1) != 0;
+        };
+        note_odd<D, R>(a, none, begin, position, g, poison);
+      }
     }
 
     v8 p[R];
@@ -725,8 +733,7 @@ __global__ __launch_bounds__(kAttendLanes) void quant_attend_kernel(AttendArgs a
 #pragma unroll
       for (int d = 0; d < kOut; ++d)
         joined[wave][m][(D / 16) * (4 * g + i) + d] =
-            (poison >> (kEach * r + (kEach == 2 ? i / 2 : 0))) & 1 ? __uint_as_float(0x7FC00000u)
-                                                                   : o[r][d][i] * fade;
+            unless_poisoned<D>(o[r][d][i] * fade, poison, r, i);
     __syncthreads();
     const int row = threadIdx.x / 16, part = threadIdx.x % 16;
     if (16 * r + row < it.rows) {
@@ -763,6 +770,199 @@ __global__ __launch_bounds__(kAttendLanes) void quant_attend_kernel(AttendArgs a
       }
     }
     __syncthreads();
+  }
+}
+
+// Prompts: 128 rows a workgroup, 32 a wave. The cache's tokens become matrix
+// operands once for all of them: a stage of 64 tokens, each wave making a quarter
+// of K's operands and of V's, is laid in shared memory lane by lane as the matrix
+// instructions take them, so that reads and writes are whole and without
+// conflicts. Two stages: while one is multiplied, the next one's bytes are on their
+// way in registers, and one barrier a stage is enough.
+constexpr int kStageTiles = 2, kWaveRows = 32;
+static_assert(kManyRows == kAttendWaves * kWaveRows, "rows of a workgroup");
+
+template <int D>
+struct Stage {
+  v4u k[2 * kStageTiles][D / 32][64];
+  v4u v[kStageTiles][D / 16][64];
+  uint8_t odd[kStageTiles][D / 32][4];   // of four tokens in each half: no numbers
+};
+
+template <int FMT, int D, typename T>
+__global__ __launch_bounds__(kAttendLanes, D == 256 ? 1 : 2) void quant_prompt_kernel(
+    AttendArgs a) {
+  typedef typename Operand<T>::v8 v8;
+  constexpr int R = kWaveRows / 16, kSteps = D / 32, kOut = D / 16;
+  __shared__ Stage<D> stages[2];
+
+  const Item it = reinterpret_cast<const Item*>(a.plan + a.at_items)[blockIdx.x];
+  if (static_cast<int32_t>(blockIdx.x) >= header(a.plan).items[a.kind]) return;
+  const int32_t* table = reinterpret_cast<const int32_t*>(a.plan + a.at_table) + it.table;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int lane = threadIdx.x % 64, m = lane % 16, g = lane / 16;
+  const int64_t head_offset = it.kv_head * Chunk<FMT, D>::bytes(1 << a.block_shift);
+  const int32_t low = it.base + it.row / a.group;
+  const int32_t high = it.base + (it.row + it.rows - 1) / a.group;
+
+  // this wave's share of a stage: half a tile of K, half the values of a tile of V
+  constexpr int kVBytes = Chunk<FMT, D>::kCode / 32;
+  const int own_tile = wave / 2, own_half = wave % 2;
+  KPart<FMT, D> k;
+  VPart<FMT, D, kVBytes> v;
+  const auto load = [&](int32_t at) {
+    if (at + own_tile >= it.tile_end) return;
+    const int32_t position = tile_at(it, at + own_tile) * kTile;
+    const Half h[2] = {
+        find_half<FMT, D>(a.pages, head_offset, a.block_shift, table, position),
+        find_half<FMT, D>(a.pages, head_offset, a.block_shift, table, position + 16)};
+    k.load(own_half ? h[1] : h[0], a.block_shift, m, g);
+    v.load(h, a.block_shift, m, g, own_half * kVBytes);
+  };
+  const auto lay = [&](Stage<D>& to, int32_t at) {
+    if (at + own_tile >= it.tile_end) return;
+    each_constant<0, kSteps>([&](auto s) {
+      const v8 f = k.template operand<T, decltype(s)::value>();
+      __builtin_memcpy(&to.k[wave][decltype(s)::value][lane], &f, 16);
+    });
+    const int32_t begin = tile_at(it, at + own_tile) * kTile;
+    if (!seen_whole(a, low, high, begin)) {
+      const uint32_t odd = v.clear_unseen(begin, g, low, high, a.window, a.sinks);
+      if (own_half == 0 && m % (512 / D) == 0) to.odd[own_tile][m * D / 512][g] = odd;
+    }
+    float scale[2][4];
+    v.scales(scale);
+    each_constant<0, decltype(v)::kPairs>([&](auto b) {
+      v8 even, odd;
+      v.template operands<T, decltype(b)::value>(scale, &even, &odd);
+      const int first = 2 * (own_half * decltype(v)::kPairs + decltype(b)::value);
+      __builtin_memcpy(&to.v[own_tile][first][lane], &even, 16);
+      __builtin_memcpy(&to.v[own_tile][first + 1][lane], &odd, 16);
+    });
+  };
+  load(it.tile);
+
+  const int32_t row0 = it.row + wave * kWaveRows;
+  const int32_t rows = min(max(it.rows - wave * kWaveRows, 0), kWaveRows);
+  const int32_t wave_low = it.base + row0 / a.group;
+  const int32_t wave_high = rows ? it.base + (row0 + rows - 1) / a.group : -1;
+  v8 q[R][kSteps];
+  int32_t position[R];
+  f32x4 o[R][kOut];
+  float top[R], sum[R];
+  uint32_t poison = 0;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const bool there = 16 * r + m < rows;
+    position[r] = there ? it.base + (row0 + 16 * r + m) / a.group : wave_low;
+    load_query<T, D>(a, it, row0 + 16 * r + m, there, g, q[r]);
+    top[r] = -INFINITY;
+    sum[r] = 0.f;
+#pragma unroll
+    for (int d = 0; d < kOut; ++d) o[r][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  const auto multiply = [&](const Stage<D>& from, int32_t at, int tile) {
+    if (at + tile >= it.tile_end) return;
+    const int32_t begin = tile_at(it, at + tile) * kTile;
+    // tiles that none of the wave's rows sees
+    if ((begin > wave_high) |
+        ((wave_low - (begin + kTile - 1) >= a.window) & (begin >= a.sinks)))
+      return;
+    f32x4 x[R][2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) x[r][half] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        v8 f;
+        __builtin_memcpy(&f, &from.k[2 * tile + half][s][lane], 16);
+#pragma unroll
+        for (int r = 0; r < R; ++r) x[r][half] = Operand<T>::mma(f, q[r][s], x[r][half]);
+      }
+    }
+    if (!seen_whole(a, wave_low, wave_high, begin)) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+            x[r][half][i] = seen(a, position[r], begin + 16 * half + 4 * g + i) ? x[r][half][i]
+                                                                                : -INFINITY;
+    }
+    if (!seen_whole(a, low, high, begin)) {   // then its no numbers were cleared
+      uint32_t odd = 0;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        uint32_t w;
+        __builtin_memcpy(&w, from.odd[tile][i], 4);
+        odd |= w;
+      }
+      if (odd) {
+        const auto none = [&](int group, int t) {
+          return ((from.odd[tile][group][(t % 16) / 4] >> (4 * (t / 16) + t % 4)) & 1) != 0;
+        };
+        note_odd<D, R>(a, none, begin, position, g, poison);
+      }
+    }
+    v8 p[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) p[r] = softmax_step<T>(x[r], a.c, top[r], sum[r], o[r]);
+#pragma unroll
+    for (int d = 0; d < kOut; ++d) {
+      v8 f;
+      __builtin_memcpy(&f, &from.v[tile][d][lane], 16);
+#pragma unroll
+      for (int r = 0; r < R; ++r) o[r][d] = Operand<T>::mma(f, p[r], o[r][d]);
+    }
+  };
+
+  int turn = 0;
+  for (int32_t at = it.tile; at < it.tile_end; at += kStageTiles, turn ^= 1) {
+    lay(stages[turn], at);
+    load(at + kStageTiles);
+    __syncthreads();
+#pragma unroll
+    for (int tile = 0; tile < kStageTiles; ++tile) multiply(stages[turn], at, tile);
+  }
+
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float total = row_sum(sum[r]);
+    const int32_t n = row0 + 16 * r + m;
+    if (16 * r + m >= rows) continue;
+    float* part = a.work + it.slot * a.slot_floats + (n - it.row) * (D + 4);
+    const int32_t token = n / a.group;
+    T* to = reinterpret_cast<T*>(a.out.base) + (int64_t(it.token) + token) * a.out.token +
+            (int64_t(it.kv_head) * a.group + (n - token * a.group)) * a.out.head;
+    const float inv = it.slot < 0 ? 1.f / total : 1.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float y[kOut];
+#pragma unroll
+      for (int d = 0; d < kOut; ++d) y[d] = unless_poisoned<D>(o[r][d][i] * inv, poison, r, i);
+      const int first = kOut * (4 * g + i);
+      if (it.slot >= 0) {
+#pragma unroll
+        for (int d = 0; d < kOut; d += 4) __builtin_memcpy(part + first + d, y + d, 16);
+      } else {
+        T t[kOut];
+#pragma unroll
+        for (int d = 0; d < kOut; ++d) t[d] = static_cast<T>(y[d]);
+        if (a.out.whole_words) {
+          __builtin_memcpy(__builtin_assume_aligned(to + first, kOut < 8 ? 8 : 16), t, sizeof t);
+        } else {
+#pragma unroll
+          for (int d = 0; d < kOut; ++d) to[first + d] = t[d];
+        }
+      }
+    }
+    if (it.slot >= 0 && g == 0) {
+      part[D] = top[r];
+      part[D + 1] = total;
+    }
   }
 }
 

@@ -333,8 +333,10 @@ int aegkv_quant_attend(const void* plan, const void* device_plan, int format, in
         const dim3 grid(static_cast<uint32_t>(h.room.items[kind]));
         if (kind == kFew)
           quant_attend_kernel<kFormat, kDim, T, 1><<<grid, kAttendLanes, 0, stream>>>(a);
-        else
+        else if (kind == kMore)
           quant_attend_kernel<kFormat, kDim, T, 2><<<grid, kAttendLanes, 0, stream>>>(a);
+        else
+          quant_prompt_kernel<kFormat, kDim, T><<<grid, kAttendLanes, 0, stream>>>(a);
         const int rc = launched("quant_attend_kernel launch");
         if (rc) return rc;
       }
