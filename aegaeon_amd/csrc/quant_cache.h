@@ -275,8 +275,7 @@ struct Operand;
 template <>
 struct Operand<__bf16> {
   typedef bf16x8 v8;
-  // probabilities lie in [0, 2^kLift]
-  static constexpr float kLift = 0.f;
+  static constexpr float kLift = 0.f, kLimit = 65536.f;
   static __device__ __forceinline__ f32x4 mma(v8 a, v8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
@@ -292,9 +291,10 @@ struct Operand<__bf16> {
 template <>
 struct Operand<_Float16> {
   typedef f16x8 v8;
-  // float16 keeps 2^-24 at the least: lifted, small probabilities of long
-  // contexts are not lost beside the largest one (the sum is lifted alike)
-  static constexpr float kLift = 14.f;
+  // float16 keeps 2^-24 at the least and 2^16 at the most: lifted, small
+  // probabilities of long contexts are not lost beside the largest one (the sum
+  // is lifted alike), and a row may still grow 2^8-fold
+  static constexpr float kLift = 7.f, kLimit = 32768.f;
   static __device__ __forceinline__ f32x4 mma(v8 a, v8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
@@ -564,38 +564,62 @@ __device__ __forceinline__ void load_query(const AttendArgs& a, const Item& it, 
   }
 }
 
-// Scores of a row tile (lane's row, eight of its tokens) into probabilities
-// against the largest score so far, with the sums made before faded to it.
+// A row's running sums are taken against a score that need not be its largest,
+// only near it: 2^kLift stands for `top`, and what grows past kLimit, in the sum
+// of a lane's eight tokens, has the row's scores looked through for their largest
+// and the sums made before fade to it. The types' relative precision is the
+// same over the whole range between; looked through for every tile, with the
+// lanes' exchange, it took a third of the arithmetic.
+struct RowState {
+  float top = -INFINITY;
+  float lift = 1e30f;    // kLift - top * c; as large while there is no top
+  float sum = 0.f;
+};
+
+// Scores of a row tile (lane's row, eight of its tokens) into probabilities.
 template <typename T, int N>
-__device__ __forceinline__ typename Operand<T>::v8 softmax_step(f32x4* x, float c, float& top,
-                                                               float& sum, f32x4 (&o)[N]) {
-  float most = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
-                     fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
-  most = fmaxf(top, row_max(most));
-  if (__any(most > top)) {
-    const float fade = top == most ? 1.f : __builtin_amdgcn_exp2f((top - most) * c);
-    sum *= fade;
+__device__ __forceinline__ typename Operand<T>::v8 softmax_step(const f32x4* x, float c,
+                                                               RowState& s, f32x4 (&o)[N]) {
+  float e[8], total;
+  const auto exponents = [&]() {
+    total = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i / 4][i % 4], c, s.lift));
+      total += e[i];
+    }
+  };
+  exponents();
+  if (__any(total > Operand<T>::kLimit)) {
+    float most = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
+                       fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+    most = fmaxf(s.top, row_max(most));
+    const float fade = s.top == most ? 1.f : __builtin_amdgcn_exp2f((s.top - most) * c);
+    s.sum *= fade;
 #pragma unroll
     for (int d = 0; d < N; ++d) o[d] *= fade;
-    top = most;
+    s.top = most;
+    if (most != -INFINITY) s.lift = Operand<T>::kLift - most * c;
+    exponents();
   }
-  const float lift = Operand<T>::kLift - (most == -INFINITY ? 0.f : most * c);
+  s.sum += total;
   typename Operand<T>::v8 p;
-  float total = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i / 4][i % 4], c, lift));
-    total += e;
-    p[i] = static_cast<T>(e);
-  }
-  sum += total;
+  for (int i = 0; i < 8; ++i) p[i] = static_cast<T>(e[i]);
   return p;
 }
 
 constexpr int kAttendLanes = 256, kAttendWaves = 4;
 
+// Waves a SIMD has to hold: what the registers allow where 16 rows' sums and two
+// tiles of codes take few of them.
+template <int FMT, int D, int R>
+constexpr int kAttendPerSimd =
+    R == 1 && D * Format<FMT>::kBits <= 512 ? 4 : D <= 128 && R == 1 ? 3 : D <= 128 ? 2 : 1;
+
 template <int FMT, int D, typename T, int R>
-__global__ __launch_bounds__(kAttendLanes) void quant_attend_kernel(AttendArgs a) {
+__global__ __launch_bounds__(kAttendLanes, (kAttendPerSimd<FMT, D, R>)) void quant_attend_kernel(
+    AttendArgs a) {
   typedef typename Operand<T>::v8 v8;
   constexpr int kSteps = D / 32;    // matrix steps along the head
   constexpr int kOut = D / 16;      // output tiles of 16 values
@@ -640,12 +664,10 @@ __global__ __launch_bounds__(kAttendLanes) void quant_attend_kernel(AttendArgs a
   const int32_t high = it.base + (it.row + it.rows - 1) / a.group;
 
   f32x4 o[R][kOut];
-  float top[R], sum[R];
+  RowState state[R];
   uint32_t poison = 0;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    top[r] = -INFINITY;
-    sum[r] = 0.f;
 #pragma unroll
     for (int d = 0; d < kOut; ++d) o[r][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -695,7 +717,7 @@ __global__ __launch_bounds__(kAttendLanes) void quant_attend_kernel(AttendArgs a
 
     v8 p[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) p[r] = softmax_step<T>(x[r], a.c, top[r], sum[r], o[r]);
+    for (int r = 0; r < R; ++r) p[r] = softmax_step<T>(x[r], a.c, state[r], o[r]);
 
     float scale[2][4];
     cur.v.scales(scale);
@@ -715,9 +737,9 @@ __global__ __launch_bounds__(kAttendLanes) void quant_attend_kernel(AttendArgs a
   // join the waves: each scales its part to the largest score of all
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const float s = row_sum(sum[r]);
+    const float s = row_sum(state[r].sum);
     if (g == 0) {
-      stats[0][wave][16 * r + m] = top[r];
+      stats[0][wave][16 * r + m] = state[r].top;
       stats[1][wave][16 * r + m] = s;
     }
   }
@@ -727,7 +749,8 @@ __global__ __launch_bounds__(kAttendLanes) void quant_attend_kernel(AttendArgs a
     float most = stats[0][0][16 * r + m];
 #pragma unroll
     for (int w = 1; w < kAttendWaves; ++w) most = fmaxf(most, stats[0][w][16 * r + m]);
-    const float fade = top[r] == most ? 1.f : __builtin_amdgcn_exp2f((top[r] - most) * a.c);
+    const float top = state[r].top;
+    const float fade = top == most ? 1.f : __builtin_amdgcn_exp2f((top - most) * a.c);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -849,15 +872,13 @@ __global__ __launch_bounds__(kAttendLanes, D == 256 ? 1 : 2) void quant_prompt_k
   v8 q[R][kSteps];
   int32_t position[R];
   f32x4 o[R][kOut];
-  float top[R], sum[R];
+  RowState state[R];
   uint32_t poison = 0;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const bool there = 16 * r + m < rows;
     position[r] = there ? it.base + (row0 + 16 * r + m) / a.group : wave_low;
     load_query<T, D>(a, it, row0 + 16 * r + m, there, g, q[r]);
-    top[r] = -INFINITY;
-    sum[r] = 0.f;
 #pragma unroll
     for (int d = 0; d < kOut; ++d) o[r][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -909,7 +930,7 @@ __global__ __launch_bounds__(kAttendLanes, D == 256 ? 1 : 2) void quant_prompt_k
     }
     v8 p[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) p[r] = softmax_step<T>(x[r], a.c, top[r], sum[r], o[r]);
+    for (int r = 0; r < R; ++r) p[r] = softmax_step<T>(x[r], a.c, state[r], o[r]);
 #pragma unroll
     for (int d = 0; d < kOut; ++d) {
       v8 f;
@@ -930,7 +951,7 @@ __global__ __launch_bounds__(kAttendLanes, D == 256 ? 1 : 2) void quant_prompt_k
 
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const float total = row_sum(sum[r]);
+    const float total = row_sum(state[r].sum);
     const int32_t n = row0 + 16 * r + m;
     if (16 * r + m >= rows) continue;
     float* part = a.work + it.slot * a.slot_floats + (n - it.row) * (D + 4);
@@ -960,7 +981,7 @@ __global__ __launch_bounds__(kAttendLanes, D == 256 ? 1 : 2) void quant_prompt_k
       }
     }
     if (it.slot >= 0 && g == 0) {
-      part[D] = top[r];
+      part[D] = state[r].top;
       part[D + 1] = total;
     }
   }
