@@ -17,28 +17,36 @@ constexpr int kTile = 32;
 
 // Row r of a sequence's queries under one KV head is new token r / group,
 // query head kv_head * group + r % group. Attention takes rows by kind:
-//   kFew, kMore: up to 16 (32) rows of a sequence, one workgroup's four waves
-//                share out the tiles of an item and join at its end;
-//   kMany:       blocks of kManyRows rows, the waves share out the rows.
-enum Kind { kFew = 0, kMore = 1, kMany = 2, kKinds = 3 };
+//   kFew, kMore: up to 16 (32) rows of a sequence; the four waves of a workgroup
+//                take an item's tiles in turn and join at its end;
+//   kMany:       blocks of kManyRows rows, shared out to the waves;
+//   kWide:       as kFew, with the waves of a whole CU in one workgroup: few
+//                short sequences, whose tiles need no second launch to be joined.
+enum Kind { kFew = 0, kMore = 1, kMany = 2, kWide = 3, kKinds = 4 };
 constexpr int kManyRows = 128;
-constexpr int kKindRows[kKinds] = {16, 32, kManyRows};
+constexpr int kKindRows[kKinds] = {16, 32, kManyRows, 16};
 
 struct Seq {
   int32_t len;         // positions in the cache, the new ones included
   int32_t fresh;       // new tokens: positions len - fresh .. len - 1
   int32_t table;       // first entry of its block table
   int32_t token;       // row of its first new token
-  int32_t new_span;    // spans of new tokens before this sequence
   int32_t read_span;   // spans of all tokens before this sequence
+  int32_t pad;
   int64_t read_token;  // tokens before this sequence
 };
 static_assert(sizeof(Seq) == 32, "Seq layout");
 
-// One workgroup's attention: rows [row, row + rows) of a sequence under one
-// KV head over visited tiles [tile, tile_end). Visited tile v is the cache's
-// tile v below `first_tiles` (the first tokens that stay visible), else v -
-// first_tiles + window_tile.
+// Up to 16 new tokens of a sequence inside one block.
+struct NewSpan {
+  int32_t block, inside, count;
+  int32_t token;       // row of the first
+};
+static_assert(sizeof(NewSpan) == 16, "NewSpan layout");
+
+// One workgroup's work: rows [row, row + rows) of a sequence under one KV head over visited tiles
+// [tile, tile_end). Visited tile v is the cache's tile v below `first_tiles` (the
+// first tokens that stay visible), else v - first_tiles + window_tile.
 struct Item {
   int32_t seq, kv_head, row, rows;
   int32_t tile, tile_end, first_tiles, window_tile;
@@ -47,12 +55,16 @@ struct Item {
 };
 static_assert(sizeof(Item) == 48, "Item layout");
 
-// Rows whose tiles were shared out to `parts` items with consecutive slots.
+// Rows whose tiles were cut into `parts` items with consecutive slots, as one
+// workgroup joins them: up to kMergeRows rows of up to as many parts, or one row.
+// Row i of them is row `row` + i of the sequence and `first` + i of the items.
+constexpr int kMergeRows = 8;
 struct Merge {
   int32_t seq, kv_head, row, rows;
   int32_t slot, parts, kind, token;
+  int32_t first, pad[3];
 };
-static_assert(sizeof(Merge) == 32, "Merge layout");
+static_assert(sizeof(Merge) == 48, "Merge layout");
 
 // What a plan has room for; fixed when it is made. Offsets into the buffer
 // follow from it, so that a captured launch stays right across updates.
@@ -60,10 +72,10 @@ struct Room {
   int64_t bytes;
   int64_t seqs, columns, tokens;   // sequences, table entries, new tokens
   int64_t new_spans, read_spans;
-  int64_t items[kKinds];           // 0: no such kernel is launched
+  int64_t items[kKinds];           // a workgroup each; 0: no such kernel is launched
   int64_t slots[kKinds];
   int64_t merges;
-  int64_t at_seqs, at_table, at_items[kKinds], at_merges;
+  int64_t at_seqs, at_table, at_new_spans, at_items[kKinds], at_merges;
 };
 
 struct Header {

@@ -8,6 +8,8 @@
 
 #include <algorithm>
 #include <cstring>
+#include <functional>
+#include <queue>
 #include <vector>
 
 namespace aegkv_batch {
@@ -15,10 +17,15 @@ namespace aegkv_batch {
 // Positions are 32-bit in the kernels, with room for a tile behind the last.
 constexpr int64_t kMostTokens = (int64_t(1) << 31) - 1024;
 
-// Workgroups that one attention launch is cut into where the rows alone make
-// fewer, and the fewest tiles a cut is worth.
-constexpr int64_t kTarget[kKinds] = {1024, 1024, 1024};
-constexpr int64_t kLeastTiles[kKinds] = {16, 16, 16};
+// How many workgroups of a kind the chip holds at once (at 128-wide heads).
+constexpr int64_t kHeld[kKinds] = {768, 512, 512, 256};
+// What a workgroup takes before and behind its tiles, and what joining cut rows
+// takes, in the time of a tile.
+constexpr int64_t kEnds[kKinds] = {8, 8, 8, 8}, kJoin[kKinds] = {8, 8, 8, 0};
+// The most items that rows are cut into, beyond one for each.
+constexpr int64_t kCuts[kKinds] = {3072, 2048, 2048, 0};
+// kWide takes up to a workgroup a CU, of sequences up to this many tiles.
+constexpr int64_t kWideGroups = 256, kWideTiles = 128;
 
 struct Batch {
   int64_t num_seqs;
@@ -43,15 +50,15 @@ struct Rows {
   int32_t first_tiles, window_tile, tiles;
 };
 
-inline int kind_of(int64_t rows) {
-  return rows <= kKindRows[kFew] ? kFew : rows <= kKindRows[kMore] ? kMore : kMany;
+inline int kind_of(int64_t rows, bool wide) {
+  return rows <= kKindRows[kFew] ? (wide ? kWide : kFew) : rows <= kKindRows[kMore] ? kMore : kMany;
 }
 
-inline void rows_of(const Header& h, const Batch& b, std::vector<Rows>* out) {
+inline void rows_of(const Header& h, const Batch& b, bool wide, std::vector<Rows>* out) {
   for (int64_t s = 0; s < b.num_seqs; ++s) {
     const int64_t rows = b.fresh[s] * h.group;
     if (!rows) continue;
-    const int kind = kind_of(rows);
+    const int kind = kind_of(rows, wide);
     for (int64_t row = 0; row < rows; row += kKindRows[kind]) {
       const int64_t n = std::min<int64_t>(kKindRows[kind], rows - row);
       const int64_t base = b.lens[s] - b.fresh[s];
@@ -70,23 +77,65 @@ inline void rows_of(const Header& h, const Batch& b, std::vector<Rows>* out) {
   }
 }
 
-inline int64_t cut(const std::vector<Rows>& rows, int64_t kv_heads, int64_t tiles_each) {
+// The time when every row block's tiles are cut into equal parts of at most
+// `each`, and the next of the workgroups that the chip holds takes the longest one left. The KV
+// heads are alike: one of them, on its share of the chip, stands for all.
+inline int64_t time_of(const std::vector<Rows>& rows, int64_t kv_heads, int kind, int64_t each) {
+  std::vector<int64_t> sizes;
+  bool cut = false;
+  for (const Rows& r : rows) {
+    const int64_t parts = up(r.tiles, each);
+    cut |= parts > 1;
+    sizes.insert(sizes.end(), static_cast<size_t>(parts), up(r.tiles, parts) + kEnds[kind]);
+  }
+  std::sort(sizes.begin(), sizes.end(), std::greater<int64_t>());
+  const int64_t copies = std::max<int64_t>(1, kv_heads / kHeld[kind]);
+  const size_t held = static_cast<size_t>(std::max<int64_t>(1, kHeld[kind] / kv_heads));
+  std::priority_queue<int64_t, std::vector<int64_t>, std::greater<int64_t>> busy;
+  int64_t end = 0;
+  for (int64_t t : sizes) {
+    int64_t from = 0;
+    if (busy.size() >= held) {
+      from = busy.top();
+      busy.pop();
+    }
+    busy.push(from + t * copies);
+    end = std::max(end, from + t * copies);
+  }
+  return end + (cut ? kJoin[kind] : 0);
+}
+
+inline int64_t items_of(const std::vector<Rows>& rows, int64_t kv_heads, int64_t each) {
   int64_t n = 0;
-  for (const Rows& r : rows) n += up(r.tiles, tiles_each);
+  for (const Rows& r : rows) n += up(r.tiles, each);
   return n * kv_heads;
 }
 
-// Tiles per item: about kTarget items, none below kLeastTiles, at most `most`.
-inline int64_t tiles_per_item(const std::vector<Rows>& rows, int64_t kv_heads, int kind,
-                              int64_t most) {
+// Tiles of an item at most: of cuts into 1/1 .. 1/8 of what a workgroup would
+// take of equal shares, and none at all, the one whose time is least.
+inline int64_t share_out(const std::vector<Rows>& rows, int64_t kv_heads, int kind,
+                         int64_t most_items) {
   int64_t total = 0, longest = 1;
   for (const Rows& r : rows) {
     total += r.tiles * kv_heads;
     longest = std::max<int64_t>(longest, r.tiles);
   }
-  int64_t each = std::max(kLeastTiles[kind], up(total, kTarget[kind]));
-  while (each < longest && cut(rows, kv_heads, each) > most) each = up(each * 5, 4);
-  return each;
+  const int64_t count = static_cast<int64_t>(rows.size()) * kv_heads;
+  if (kind == kWide || count >= 8 * kHeld[kind]) return longest;
+  int64_t best = longest, least = time_of(rows, kv_heads, kind, longest);
+  for (int64_t eighths = 8; eighths >= 1; --eighths) {
+    const int64_t each = std::max<int64_t>(4, up(total * eighths, 8 * kHeld[kind]));
+    if (each >= longest) continue;
+    const int64_t items = items_of(rows, kv_heads, each);
+    if (items > most_items || items > count + kCuts[kind]) break;
+    const int64_t t = time_of(rows, kv_heads, kind, each);
+    if (t < least) {
+      least = t;
+      best = each;
+    }
+    if (each == 4) break;
+  }
+  return best;
 }
 
 inline int check(const Header& h, const Batch& b) {
@@ -158,6 +207,7 @@ inline int fill(Header& h, const Batch& b, const std::vector<Rows>* rows, char* 
   auto* seq = reinterpret_cast<Seq*>(base + room.at_seqs);
   auto* table = reinterpret_cast<int32_t*>(base + room.at_table);
   auto* merge = reinterpret_cast<Merge*>(base + room.at_merges);
+  auto* span = reinterpret_cast<NewSpan*>(base + room.at_new_spans);
   int64_t columns = 0, tokens = 0, new_spans = 0, read_spans = 0, read_tokens = 0;
   h.complete = 1;
   for (int64_t s = 0; s < b.num_seqs; ++s) columns += up(b.lens[s], h.block_size) + 1;
@@ -173,7 +223,6 @@ inline int fill(Header& h, const Batch& b, const std::vector<Rows>* rows, char* 
     seq[s].fresh = static_cast<int32_t>(fresh);
     seq[s].table = static_cast<int32_t>(columns);
     seq[s].token = static_cast<int32_t>(tokens);
-    seq[s].new_span = static_cast<int32_t>(new_spans);
     seq[s].read_span = static_cast<int32_t>(read_spans);
     seq[s].read_token = read_tokens;
     for (int64_t c = 0; c < need; ++c) {
@@ -184,7 +233,17 @@ inline int fill(Header& h, const Batch& b, const std::vector<Rows>* rows, char* 
     table[columns + need] = 0;   // the tile behind the last block may look here
     columns += need + 1;
     tokens += fresh;
-    if (fresh) new_spans += up(len, kSpan) - (len - fresh) / kSpan;
+    for (int64_t at = len - fresh; at < len;) {
+      const int64_t end = std::min(len, (at / kSpan + 1) * kSpan);
+      if (new_spans >= room.new_spans)
+        return aegkv_set_error(AEGKV_ENOMEM, "the new tokens do not fit the plan's %lld spans",
+                               ll(room.new_spans));
+      span[new_spans++] = NewSpan{table[seq[s].table + at / h.block_size],
+                                  static_cast<int32_t>(at % h.block_size),
+                                  static_cast<int32_t>(end - at),
+                                  static_cast<int32_t>(seq[s].token + at - (len - fresh))};
+      at = end;
+    }
     read_spans += up(len, kSpan);
     read_tokens += len;
   }
@@ -193,36 +252,46 @@ inline int fill(Header& h, const Batch& b, const std::vector<Rows>* rows, char* 
   h.new_spans = static_cast<int32_t>(new_spans);
   h.read_spans = static_cast<int32_t>(read_spans);
   h.read_tokens = read_tokens;
-  if (new_spans > room.new_spans || read_spans > room.read_spans)
-    return aegkv_set_error(AEGKV_ENOMEM, "%lld new and %lld read spans do not fit the plan",
-                           ll(new_spans), ll(read_spans));
+  if (read_spans > room.read_spans)
+    return aegkv_set_error(AEGKV_ENOMEM, "%lld spans to read do not fit the plan", ll(read_spans));
   int64_t merges = 0;
   for (int kind = 0; kind < kKinds; ++kind) {
-    int64_t items = 0, slots = 0;
-    const int64_t each = tiles_per_item(rows[kind], h.kv_heads, kind, room.items[kind]);
-    if (cut(rows[kind], h.kv_heads, each) > room.items[kind])
+    const std::vector<Rows>& all = rows[kind];
+    if (static_cast<int64_t>(all.size()) * h.kv_heads > room.items[kind])
       return aegkv_set_error(AEGKV_ENOMEM, "the plan has no room for sequences of this many new "
                              "tokens (%s rows under a KV head)",
-                             kind == kFew ? "up to 16" : kind == kMore ? "17 to 32" : "over 32");
+                             kind == kMany ? "over 32" : kind == kMore ? "17 to 32" : "up to 16");
+    const int64_t each = share_out(all, h.kv_heads, kind, room.items[kind]);
+    // the longest go first, so that the last to end are short
+    std::vector<size_t> order(all.size());
+    for (size_t i = 0; i < order.size(); ++i) order[i] = i;
+    const auto size = [&](size_t i) { return up(all[i].tiles, up(all[i].tiles, each)); };
+    std::stable_sort(order.begin(), order.end(),
+                     [&](size_t x, size_t y) { return size(x) > size(y); });
     auto* item = reinterpret_cast<Item*>(base + room.at_items[kind]);
-    for (const Rows& r : rows[kind]) {
+    int64_t items = 0, slots = 0;
+    for (size_t i : order) {
+      const Rows& r = all[i];
       const int64_t parts = up(r.tiles, each);
       for (int32_t head = 0; head < h.kv_heads; ++head) {
-        if (parts > 1) {
-          if (merges >= room.merges || slots + parts > room.slots[kind])
+        const int64_t slot = slots;
+        for (int64_t p = 0; p < parts; ++p)
+          item[items++] = Item{r.seq, head, r.row, r.rows,
+                               static_cast<int32_t>(r.tiles * p / parts),
+                               static_cast<int32_t>(r.tiles * (p + 1) / parts), r.first_tiles,
+                               r.window_tile, parts > 1 ? static_cast<int32_t>(slots++) : -1,
+                               seq[r.seq].len - seq[r.seq].fresh, seq[r.seq].token,
+                               seq[r.seq].table};
+        if (parts == 1) continue;
+        const int32_t rows_each = parts <= kMergeRows ? kMergeRows : 1;
+        for (int32_t first = 0; first < r.rows; first += rows_each) {
+          if (merges >= room.merges || slots > room.slots[kind])
             return aegkv_set_error(AEGKV_ENOMEM, "the plan has no room for %lld parts of sums",
-                                   ll(slots + parts));
-          merge[merges++] = Merge{r.seq, head, r.row, r.rows, static_cast<int32_t>(slots),
-                                  static_cast<int32_t>(parts), kind, seq[r.seq].token};
-        }
-        for (int64_t p = 0; p < parts; ++p) {
-          Item& it = item[items++];
-          it = Item{r.seq, head, r.row, r.rows,
-                    static_cast<int32_t>(r.tiles * p / parts),
-                    static_cast<int32_t>(r.tiles * (p + 1) / parts),
-                    r.first_tiles, r.window_tile, -1,
-                    seq[r.seq].len - seq[r.seq].fresh, seq[r.seq].token, seq[r.seq].table};
-          if (parts > 1) it.slot = static_cast<int32_t>(slots++);
+                                   ll(slots));
+          merge[merges++] = Merge{r.seq, head, r.row + first,
+                                  std::min(rows_each, r.rows - first),
+                                  static_cast<int32_t>(slot), static_cast<int32_t>(parts), kind,
+                                  seq[r.seq].token, first, {0, 0, 0}};
         }
       }
     }
@@ -261,27 +330,46 @@ inline void make_room(Header& h, const Batch& b, const std::vector<Rows>* rows, 
   };
   r.at_seqs = take(r.seqs * static_cast<int64_t>(sizeof(Seq)));
   r.at_table = take(r.columns * 4);
+  r.at_new_spans = take(r.new_spans * static_cast<int64_t>(sizeof(NewSpan)));
   for (int kind = 0; kind < kKinds; ++kind) {
-    if (exact) {
-      const int64_t each = tiles_per_item(rows[kind], h.kv_heads, kind, INT64_MAX);
-      r.items[kind] = cut(rows[kind], h.kv_heads, each);
-      r.slots[kind] = 0;
+    const int64_t count = static_cast<int64_t>(rows[kind].size()) * h.kv_heads;
+    r.items[kind] = r.slots[kind] = 0;
+    if (count && exact) {
+      const int64_t each = share_out(rows[kind], h.kv_heads, kind, INT32_MAX);
+      r.items[kind] = items_of(rows[kind], h.kv_heads, each);
       for (const Rows& x : rows[kind]) {
-        if (x.tiles <= each) continue;
-        r.merges += h.kv_heads;
-        r.slots[kind] += up(x.tiles, each) * h.kv_heads;
+        const int64_t parts = up(x.tiles, each);
+        if (parts == 1) continue;
+        r.slots[kind] += parts * h.kv_heads;
+        r.merges += up(x.rows, parts <= kMergeRows ? kMergeRows : 1) * h.kv_heads;
       }
-    } else if (rows[kind].empty()) {
-      r.items[kind] = r.slots[kind] = 0;
-    } else {
-      const int64_t blocks = kind == kMany ? r.tokens * h.group / kManyRows + r.seqs : r.seqs;
-      r.items[kind] = r.slots[kind] = kTarget[kind] + blocks * h.kv_heads;
-      r.merges += blocks * h.kv_heads;
+    } else if (count) {
+      const int64_t most = (kind == kMany ? r.tokens * h.group / kManyRows + r.seqs : r.seqs) *
+                           h.kv_heads;
+      r.items[kind] = most + kCuts[kind];
+      if (kind != kWide) {
+        // row by row where one has more than kMergeRows parts
+        const int64_t many = std::min(most, r.items[kind] / (kMergeRows + 1));
+        r.slots[kind] = r.items[kind];
+        r.merges += most * up(kKindRows[kind], kMergeRows) + many * kKindRows[kind];
+      }
     }
     r.at_items[kind] = take(r.items[kind] * static_cast<int64_t>(sizeof(Item)));
   }
   r.at_merges = take(r.merges * static_cast<int64_t>(sizeof(Merge)));
   r.bytes = at;
+}
+
+// Whether the rows of few new tokens go to kWide: fixed when the plan is made.
+inline bool wide(const Header& h, const Batch& b, int64_t max_seqs, int64_t max_columns) {
+  int64_t seqs = 0, longest = max_columns * h.block_size;
+  for (int64_t s = 0; s < b.num_seqs; ++s) {
+    if (b.fresh[s] * h.group > kKindRows[kWide] || !b.fresh[s]) continue;
+    ++seqs;
+    longest = std::max(longest, b.lens[s]);
+  }
+  const int64_t tiles = up(longest, kTile);
+  return std::max(seqs, max_seqs) * h.kv_heads <= kWideGroups && tiles <= kWideTiles;
 }
 
 inline int describe(Header& h, int64_t num_blocks, int32_t block_size, int32_t kv_heads,

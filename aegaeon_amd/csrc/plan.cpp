@@ -150,7 +150,6 @@ int aegkv_batch_plan(int64_t num_seqs, const int64_t* column_offsets, const int6
     rc = check(h, b);
     if (rc) return rc;
     std::vector<Rows> rows[kKinds];
-    rows_of(h, b, rows);
     if (update) {
       Header was;
       if (!plan || held < static_cast<int64_t>(sizeof was))
@@ -163,7 +162,9 @@ int aegkv_batch_plan(int64_t num_seqs, const int64_t* column_offsets, const int6
           was.sinks != h.sinks)
         return plan_fail(AEGKV_EINVAL, "an update keeps the blocks, heads, window and sinks");
       h.room = was.room;
+      rows_of(h, b, h.room.items[kWide] > 0, rows);
     } else {
+      rows_of(h, b, wide(h, b, max_seqs, max_columns), rows);
       make_room(h, b, rows, max_seqs, max_columns, max_tokens);
       *plan_bytes = h.room.bytes;
       if (!plan) return 0;

@@ -62,15 +62,31 @@ struct Values {
   bool whole_words;
 };
 
-__device__ __forceinline__ const Header& header(const char* plan) {
-  return *reinterpret_cast<const Header*>(plan);
+// The plan does not change while a kernel runs. Read as constant memory, what is
+// the same for a wave comes by scalar loads; as ordinary memory, once a kernel
+// stores anything, by vector loads in one queue with the cache's, and waiting
+// for a block id meant waiting for every tile on its way.
+#define AEGKV_CONSTANT __attribute__((address_space(4)))
+
+template <typename T>
+__device__ __forceinline__ const AEGKV_CONSTANT T* in_plan(const char* plan, int64_t offset) {
+  return (const AEGKV_CONSTANT T*)(reinterpret_cast<uintptr_t>(plan) +
+                                   static_cast<uintptr_t>(offset));
+}
+
+// The same address, to read from anew: what few steps need is not held in scalar
+// registers (a hundred, and spilled ones cost vector instructions) in between.
+template <typename P>
+__device__ __forceinline__ P anew(P p) {
+  asm volatile("" : "+s"(p));
+  return p;
 }
 
 // ------------------------------------------------------------ write, read --
 
 struct SpanArgs {
   const char* plan;
-  int64_t at_seqs, at_table;
+  int64_t at_seqs, at_table, at_new_spans;
   char* pages[2];       // K, V
   Values values[2];
   int64_t page_bytes;
@@ -86,27 +102,29 @@ struct Span {
 };
 
 __device__ __forceinline__ bool find_span(const SpanArgs& a, int32_t i, Span* s) {
-  const Header& h = header(a.plan);
-  if (i >= (a.fresh ? h.new_spans : h.read_spans)) return false;
-  const Seq* seq = reinterpret_cast<const Seq*>(a.plan + a.at_seqs);
-  // the last sequence that begins at or before span i; sequences without
-  // spans begin where the next one does
-  int32_t lo = 0, hi = h.num_seqs - 1;
+  const auto* h = in_plan<Header>(a.plan, 0);
+  if (a.fresh) {
+    const auto* n = in_plan<NewSpan>(a.plan, a.at_new_spans) + i;
+    *s = Span{n->block, n->inside, n->count, n->token};
+    return i < h->new_spans;
+  }
+  if (i >= h->read_spans) return false;
+  const auto* seq = in_plan<Seq>(a.plan, a.at_seqs);
+  // the last sequence that begins at or before span i; empty sequences begin
+  // where the next one does
+  int32_t lo = 0, hi = h->num_seqs - 1;
   while (lo < hi) {
     const int32_t mid = (lo + hi + 1) >> 1;
-    if ((a.fresh ? seq[mid].new_span : seq[mid].read_span) <= i) lo = mid;
+    if (seq[mid].read_span <= i) lo = mid;
     else hi = mid - 1;
   }
-  const Seq q = seq[lo];
-  const int32_t from = a.fresh ? q.len - q.fresh : 0;
-  const int32_t nth = i - (a.fresh ? q.new_span : q.read_span);
-  const int32_t grid = (from / kSpan + nth) * kSpan;
-  const int32_t begin = max(grid, from), end = min(grid + kSpan, q.len);
+  const auto* q = seq + lo;
+  const int32_t begin = (i - q->read_span) * kSpan;
   const int32_t column = begin / a.block_size;
-  s->block = reinterpret_cast<const int32_t*>(a.plan + a.at_table)[q.table + column];
+  s->block = in_plan<int32_t>(a.plan, a.at_table)[q->table + column];
   s->inside = begin - column * a.block_size;
-  s->count = end - begin;
-  s->token = (a.fresh ? int64_t(q.token) : q.read_token) + (begin - from);
+  s->count = min(kSpan, q->len - begin);
+  s->token = q->read_token + begin;
   return true;
 }
 
@@ -317,20 +335,33 @@ __device__ __forceinline__ uint32_t decode_pair(const uint32_t* w, float s) {
     return Operand<T>::template fp8<PAIR % 2>(w[PAIR / 2], s);
 }
 
-struct AttendArgs {
-  const char* plan;
-  int64_t at_seqs, at_table, at_items, at_merges;
+// What every step of attention needs.
+struct Scope {
   QuantPages pages;
+  float c;              // scale * log2(e)
+  int32_t block_shift, window, sinks;
+};
+
+struct AttendArgs {
+  Scope scope;
+  const char* plan;
+  int64_t at_table, at_items, at_merges;
   Values q, out;
   float* work;          // parts of this kind's items, by slot
   int64_t slot_floats;
   int64_t kind_work[kKinds];   // merge: where each kind's parts begin
   float* work_base;
   int64_t kind_slot_floats[kKinds];
-  float c;              // scale * log2(e)
-  int32_t block_shift, group, window, sinks;
-  int32_t kind;
+  int32_t group, kind;
 };
+
+typedef const AEGKV_CONSTANT AttendArgs* ColdArgs;
+typedef const AEGKV_CONSTANT Item* ItemPtr;
+
+// A kernel's only argument, read where it is needed.
+__device__ __forceinline__ ColdArgs cold_args() {
+  return anew((ColdArgs)__builtin_amdgcn_kernarg_segment_ptr());
+}
 
 // A wave's tile of 32 tokens as it lies in the cache. Lane l (m = l % 16, g = l
 // / 16) holds of K, for both halves of 16 tokens, token m's values [D/4 g, D/4 (g
@@ -350,12 +381,10 @@ struct Half {
 
 template <int FMT, int D>
 __device__ __forceinline__ Half find_half(const QuantPages& p, int64_t head_offset,
-                                          int block_shift, const int32_t* table,
-                                          int32_t position) {
+                                          int block_shift, int32_t block, int32_t position) {
   using C = Chunk<FMT, D>;
-  const int32_t column = position >> block_shift;
   const int32_t inside = position & ((1 << block_shift) - 1);
-  const int64_t at = int64_t(table[column]) * p.page_bytes + head_offset;
+  const int64_t at = int64_t(block) * p.page_bytes + head_offset;
   const int64_t codes = at + int64_t(inside) * C::kCode;
   const int64_t scales = at + (int64_t(C::kCode) << block_shift) + inside;
   return Half{p.k + codes, p.v + codes, p.k + scales, p.v + scales};
@@ -495,7 +524,7 @@ __device__ __forceinline__ void each_constant(const F& f) {
 }
 
 // Whether a query at position p sees position j (window: INT32_MAX for none).
-__device__ __forceinline__ bool seen(const AttendArgs& a, int32_t p, int32_t j) {
+__device__ __forceinline__ bool seen(const Scope& a, int32_t p, int32_t j) {
   return (j <= p) & ((p - j < a.window) | (j < a.sinks));
 }
 
@@ -505,7 +534,7 @@ __device__ __forceinline__ bool seen(const AttendArgs& a, int32_t p, int32_t j) 
 // in the i-th group of the lane's values [D/4 g, D/4 (g + 1)). none(group, t):
 // whether the tile's token t is no number there.
 template <int D, int R, typename F>
-__device__ __forceinline__ void note_odd(const AttendArgs& a, const F& none, int32_t begin,
+__device__ __forceinline__ void note_odd(const Scope& a, const F& none, int32_t begin,
                                          const int32_t* position, int g, uint32_t& poison) {
   constexpr int kEach = D == 256 ? 2 : 1;
 #pragma unroll 1
@@ -528,29 +557,34 @@ __device__ __forceinline__ float unless_poisoned(float x, uint32_t poison, int r
 }
 
 // Which of the tiles that rows [low, high] visit comes v-th.
-__device__ __forceinline__ int32_t tile_at(const Item& it, int32_t v) {
-  return v < it.first_tiles ? v : v - it.first_tiles + it.window_tile;
-}
+struct Tiles {
+  int32_t first_tiles, skipped, end;
+  __device__ __forceinline__ int32_t at(int32_t v) const {
+    return v < first_tiles ? v : v + skipped;
+  }
+};
 
 // Whether every row of [low, high] sees every token of the tile at `begin`.
-__device__ __forceinline__ bool seen_whole(const AttendArgs& a, int32_t low, int32_t high,
+__device__ __forceinline__ bool seen_whole(const Scope& a, int32_t low, int32_t high,
                                            int32_t begin) {
   return (begin + kTile - 1 <= low) & ((high - begin < a.window) | (begin + kTile <= a.sinks));
 }
 
 // Query rows of a 16-row tile as a matrix operand: lane's row, its values [D/4 g, ..).
 template <typename T, int D>
-__device__ __forceinline__ void load_query(const AttendArgs& a, const Item& it, int32_t row,
-                                           bool there, int g, typename Operand<T>::v8* q) {
-  const int32_t token = row / a.group;
-  const T* from = reinterpret_cast<const T*>(a.q.base) + (int64_t(it.token) + token) * a.q.token +
-                  (int64_t(it.kv_head) * a.group + (row - token * a.group)) * a.q.head +
+__device__ __forceinline__ void load_query(ColdArgs args, ItemPtr it, int32_t row, bool there,
+                                           int g, typename Operand<T>::v8* q) {
+  const int32_t group = args->group, token = row / group;
+  const bool whole_words = args->q.whole_words;
+  const T* from = reinterpret_cast<const T*>(args->q.base) +
+                  (int64_t(it->token) + token) * args->q.token +
+                  (int64_t(it->kv_head) * group + (row - token * group)) * args->q.head +
                   g * (D / 4);
 #pragma unroll
   for (int s = 0; s < D / 32; ++s) {
     uint32_t w[4] = {0, 0, 0, 0};
     if (there) {
-      if (a.q.whole_words) {
+      if (whole_words) {
         const v4u x = *(const gv4u*)(from + s * 8);
         __builtin_memcpy(w, &x, 16);
       } else {
@@ -614,54 +648,91 @@ constexpr int kAttendLanes = 256, kAttendWaves = 4;
 // Waves a SIMD has to hold: what the registers allow where 16 rows' sums and two
 // tiles of codes take few of them.
 template <int FMT, int D, int R>
-constexpr int kAttendPerSimd =
-    R == 1 && D * Format<FMT>::kBits <= 512 ? 4 : D <= 128 && R == 1 ? 3 : D <= 128 ? 2 : 1;
+constexpr int kAttendPerSimd = D <= 128 && R == 1 ? 3 : D <= 128 ? 2 : 1;
+// Tiles on their way. Two, at three waves a SIMD, where the registers hold them:
+// with one, at four waves, 48 sequences of 40 heads took 110 us instead of 100.
+template <int FMT, int D, int R, int WAVES>
+constexpr int kTilesAhead = R == 1 && WAVES == 4 && D <= 128 ? 2 : 1;
+template <int FMT, int D>
+constexpr int kWideWaves = D * Format<FMT>::kBits <= 512 ? 16 : 8;
 
-template <int FMT, int D, typename T, int R>
-__global__ __launch_bounds__(kAttendLanes, (kAttendPerSimd<FMT, D, R>)) void quant_attend_kernel(
-    AttendArgs a) {
+// Where a row's result begins.
+template <typename T, typename P>
+__device__ __forceinline__ T* result_row(ColdArgs args, P it, int32_t row) {
+  const int32_t group = args->group, token = row / group;
+  return reinterpret_cast<T*>(args->out.base) + (int64_t(it->token) + token) * args->out.token +
+         (int64_t(it->kv_head) * group + (row - token * group)) * args->out.head;
+}
+
+// Where a workgroup's waves join: four of them at a time.
+template <int D, int R, int WAVES>
+struct Joined {
+  float part[4][16][D + 4];
+  float top[WAVES][16 * R], sum[WAVES][16 * R];
+};
+
+template <int FMT, int D, typename T, int R, int WAVES>
+__device__ __forceinline__ void attend_item(const Scope& a, ItemPtr it,
+                                            Joined<D, R, WAVES>& share) {
   typedef typename Operand<T>::v8 v8;
   constexpr int kSteps = D / 32;    // matrix steps along the head
   constexpr int kOut = D / 16;      // output tiles of 16 values
-  constexpr int kPad = D + 4;
-  __shared__ float joined[kAttendWaves][16][kPad];
-  __shared__ float stats[2][kAttendWaves][16 * R];
-
-  const Item it = reinterpret_cast<const Item*>(a.plan + a.at_items)[blockIdx.x];
-  if (static_cast<int32_t>(blockIdx.x) >= header(a.plan).items[a.kind]) return;
-  const int32_t* table = reinterpret_cast<const int32_t*>(a.plan + a.at_table) + it.table;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int lane = threadIdx.x % 64, m = lane % 16, g = lane / 16;
-  const int64_t head_offset = it.kv_head * Chunk<FMT, D>::bytes(1 << a.block_shift);
+  const ColdArgs args = cold_args();
+  const auto* table = in_plan<int32_t>(args->plan, args->at_table) + it->table;
+  const Tiles tiles = {it->first_tiles, it->window_tile - it->first_tiles, it->tile_end};
+  const int64_t head_offset = it->kv_head * Chunk<FMT, D>::bytes(1 << a.block_shift);
 
+  // kAhead tiles are on their way while one is worked on: a tile's K is asked for
+  // as soon as the registers it goes to are operands, its V as soon as theirs are,
+  // and the blocks that it lies in one step earlier still.
   struct Tile {
     KPart<FMT, D> k[2];
     VPart<FMT, D, Chunk<FMT, D>::kCode / 16> v;
   };
-  const auto load = [&](Tile* t, int32_t v) {
-    const int32_t position = tile_at(it, v) * kTile;
-    const Half h[2] = {
-        find_half<FMT, D>(a.pages, head_offset, a.block_shift, table, position),
-        find_half<FMT, D>(a.pages, head_offset, a.block_shift, table, position + 16)};
-    t->k[0].load(h[0], a.block_shift, m, g);
-    t->k[1].load(h[1], a.block_shift, m, g);
-    t->v.load(h, a.block_shift, m, g, 0);
+  struct Blocks {
+    int32_t position, block[2];
   };
-  Tile cur;
-  int32_t at = it.tile + wave;
-  if (at < it.tile_end) load(&cur, at);
+  const auto find = [&](int32_t v) {
+    Blocks b;
+    b.position = tiles.at(min(v, tiles.end - 1)) * kTile;
+    b.block[0] = table[b.position >> a.block_shift];
+    b.block[1] = table[(b.position + 16) >> a.block_shift];
+    return b;
+  };
+  const auto load_k = [&](Tile& t, const Blocks& b, Half* h) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      h[i] = find_half<FMT, D>(a.pages, head_offset, a.block_shift, b.block[i],
+                               b.position + 16 * i);
+      t.k[i].load(h[i], a.block_shift, m, g);
+    }
+  };
+  constexpr int kAhead = kTilesAhead<FMT, D, R, WAVES>;
+  Tile held[kAhead];
+  int32_t at = it->tile + wave;
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    if (at + i * WAVES < tiles.end) {
+      Half h[2];
+      load_k(held[i], find(at + i * WAVES), h);
+      held[i].v.load(h, a.block_shift, m, g, 0);
+    }
+  }
+  Blocks ahead = find(at + kAhead * WAVES);
 
   v8 q[R][kSteps];
   int32_t position[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int32_t row = it.row + 16 * r + m;
-    const bool there = 16 * r + m < it.rows;
-    position[r] = it.base + (there ? row / a.group : 0);
-    load_query<T, D>(a, it, row, there, g, q[r]);
+    const int32_t row = it->row + 16 * r + m;
+    const bool there = 16 * r + m < it->rows;
+    position[r] = it->base + (there ? row / args->group : 0);
+    load_query<T, D>(args, it, row, there, g, q[r]);
   }
-  const int32_t low = it.base + it.row / a.group;
-  const int32_t high = it.base + (it.row + it.rows - 1) / a.group;
+  const int32_t low = it->base + it->row / args->group;
+  const int32_t high = it->base + (it->row + it->rows - 1) / args->group;
 
   f32x4 o[R][kOut];
   RowState state[R];
@@ -672,10 +743,9 @@ __global__ __launch_bounds__(kAttendLanes, (kAttendPerSimd<FMT, D, R>)) void qua
     for (int d = 0; d < kOut; ++d) o[r][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  for (; at < it.tile_end; at += kAttendWaves) {
-    const int32_t begin = tile_at(it, at) * kTile;
-    Tile next = cur;
-    if (at + kAttendWaves < it.tile_end) load(&next, at + kAttendWaves);
+  const auto step = [&](Tile& t) {
+    const int32_t begin = tiles.at(at) * kTile;
+    const bool more = at + kAhead * WAVES < tiles.end;
 
     // scores: lane holds row m, tokens 4g + i of both halves
     f32x4 x[R][2];
@@ -684,12 +754,15 @@ __global__ __launch_bounds__(kAttendLanes, (kAttendPerSimd<FMT, D, R>)) void qua
 #pragma unroll
       for (int r = 0; r < R; ++r) x[r][half] = f32x4{0.f, 0.f, 0.f, 0.f};
       each_constant<0, kSteps>([&](auto s) {
-        const v8 k = cur.k[half].template operand<T, decltype(s)::value>();
+        const v8 k = t.k[half].template operand<T, decltype(s)::value>();
 #pragma unroll
         for (int r = 0; r < R; ++r)
           x[r][half] = Operand<T>::mma(k, q[r][decltype(s)::value], x[r][half]);
       });
     }
+    Half h[2];
+    if (more) load_k(t, ahead, h);
+    ahead = find(at + (kAhead + 1) * WAVES);
 
     // Tokens that some row does not see. All by selection: with branches around
     // the changed elements the compiler lost one of the changes (the first
@@ -704,12 +777,12 @@ __global__ __launch_bounds__(kAttendLanes, (kAttendPerSimd<FMT, D, R>)) void qua
           for (int r = 0; r < R; ++r)
             x[r][half][i] = seen(a, position[r], begin + 16 * half + 4 * g + i) ? x[r][half][i]
                                                                                 : -INFINITY;
-      const uint32_t odd = cur.v.clear_unseen(begin, g, low, high, a.window, a.sinks);
+      const uint32_t odd = t.v.clear_unseen(begin, g, low, high, a.window, a.sinks);
       if (__any(odd != 0)) {
         // lane m of the operand holds the group of values [D/16 m, ..)
-        const auto none = [&](int group, int t) {
-          const int from = (t % 16) / 4 * 16 + group * 512 / D;
-          return ((__shfl(static_cast<int>(odd), from) >> (4 * (t / 16) + t % 4)) & 1) != 0;
+        const auto none = [&](int group, int i) {
+          const int from = (i % 16) / 4 * 16 + group * 512 / D;
+          return ((__shfl(static_cast<int>(odd), from) >> (4 * (i / 16) + i % 4)) & 1) != 0;
         };
         note_odd<D, R>(a, none, begin, position, g, poison);
       }
@@ -720,80 +793,105 @@ __global__ __launch_bounds__(kAttendLanes, (kAttendPerSimd<FMT, D, R>)) void qua
     for (int r = 0; r < R; ++r) p[r] = softmax_step<T>(x[r], a.c, state[r], o[r]);
 
     float scale[2][4];
-    cur.v.scales(scale);
+    t.v.scales(scale);
     each_constant<0, kOut / 2>([&](auto b) {
       constexpr int B = decltype(b)::value;
-      v8 even, odd;
-      cur.v.template operands<T, B>(scale, &even, &odd);
+      v8 first, second;
+      t.v.template operands<T, B>(scale, &first, &second);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        o[r][2 * B] = Operand<T>::mma(even, p[r], o[r][2 * B]);
-        o[r][2 * B + 1] = Operand<T>::mma(odd, p[r], o[r][2 * B + 1]);
+        o[r][2 * B] = Operand<T>::mma(first, p[r], o[r][2 * B]);
+        o[r][2 * B + 1] = Operand<T>::mma(second, p[r], o[r][2 * B + 1]);
       }
     });
-    cur = next;
+    if (more) t.v.load(h, a.block_shift, m, g, 0);
+    at += WAVES;
+  };
+  while (at < tiles.end) {
+    step(held[0]);
+    if constexpr (kAhead == 2) {
+      if (at >= tiles.end) break;
+      step(held[1]);
+    }
   }
 
-  // join the waves: each scales its part to the largest score of all
+  // join the waves, four at a time: each scales its part to the largest of
+  // their scores
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const float s = row_sum(state[r].sum);
     if (g == 0) {
-      stats[0][wave][16 * r + m] = state[r].top;
-      stats[1][wave][16 * r + m] = s;
+      share.top[wave][16 * r + m] = state[r].top;
+      share.sum[wave][16 * r + m] = s;
     }
   }
   __syncthreads();
+  const ColdArgs end_args = cold_args();
+  const ItemPtr ended = anew(it);
+  constexpr int kRowLanes = WAVES * 4, kEach = D / kRowLanes;   // of a row, values of each
+  const int row = threadIdx.x / kRowLanes, part = threadIdx.x % kRowLanes;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    float most = stats[0][0][16 * r + m];
+    float most = share.top[0][16 * r + m];
 #pragma unroll
-    for (int w = 1; w < kAttendWaves; ++w) most = fmaxf(most, stats[0][w][16 * r + m]);
+    for (int w = 1; w < WAVES; ++w) most = fmaxf(most, share.top[w][16 * r + m]);
     const float top = state[r].top;
     const float fade = top == most ? 1.f : __builtin_amdgcn_exp2f((top - most) * a.c);
+    float y[kEach] = {};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int four = 0; four < WAVES; four += 4) {
+      if (wave / 4 == four / 4) {
 #pragma unroll
-      for (int d = 0; d < kOut; ++d)
-        joined[wave][m][(D / 16) * (4 * g + i) + d] =
-            unless_poisoned<D>(o[r][d][i] * fade, poison, r, i);
-    __syncthreads();
-    const int row = threadIdx.x / 16, part = threadIdx.x % 16;
-    if (16 * r + row < it.rows) {
-      float all = stats[0][0][16 * r + row], total = 0.f;
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int w = 1; w < kAttendWaves; ++w) all = fmaxf(all, stats[0][w][16 * r + row]);
-#pragma unroll
-      for (int w = 0; w < kAttendWaves; ++w) {
-        const float t = stats[0][w][16 * r + row];
-        total += stats[1][w][16 * r + row] * (t == all ? 1.f : __builtin_amdgcn_exp2f((t - all) * a.c));
+          for (int d = 0; d < kOut; ++d)
+            share.part[wave % 4][m][(D / 16) * (4 * g + i) + d] =
+                unless_poisoned<D>(o[r][d][i] * fade, poison, r, i);
       }
-      float y[D / 16];
+      __syncthreads();
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        y[i] = 0.f;
+      for (int i = 0; i < kEach; ++i) {
 #pragma unroll
-        for (int w = 0; w < kAttendWaves; ++w) y[i] += joined[w][row][part * (D / 16) + i];
+        for (int w = 0; w < 4; ++w) y[i] += share.part[w][row][part * kEach + i];
       }
-      if (it.slot < 0) {
-        const int32_t n = it.row + 16 * r + row, token = n / a.group;
-        T* to = reinterpret_cast<T*>(a.out.base) + (int64_t(it.token) + token) * a.out.token +
-                (int64_t(it.kv_head) * a.group + (n - token * a.group)) * a.out.head;
+      __syncthreads();
+    }
+    if (16 * r + row < ended->rows) {
+      float all = share.top[0][16 * r + row], total = 0.f;
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) all = fmaxf(all, share.top[w][16 * r + row]);
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        const float t = share.top[w][16 * r + row];
+        total += share.sum[w][16 * r + row] *
+                 (t == all ? 1.f : __builtin_amdgcn_exp2f((t - all) * a.c));
+      }
+      if (ended->slot < 0) {
+        T* to = result_row<T>(end_args, ended, ended->row + 16 * r + row);
         const float inv = 1.f / total;
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) to[part * (D / 16) + i] = static_cast<T>(y[i] * inv);
+        for (int i = 0; i < kEach; ++i) to[part * kEach + i] = static_cast<T>(y[i] * inv);
       } else {
-        float* to = a.work + it.slot * a.slot_floats + (16 * r + row) * (D + 4);
+        float* to = end_args->work + ended->slot * end_args->slot_floats + (16 * r + row) * (D + 4);
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) to[part * (D / 16) + i] = y[i];
+        for (int i = 0; i < kEach; ++i) to[part * kEach + i] = y[i];
         if (part == 0) {
           to[D] = all;
           to[D + 1] = total;
         }
       }
     }
-    __syncthreads();
   }
+}
+
+template <int FMT, int D, typename T, int R, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, (WAVES > 4 ? WAVES / 4 : kAttendPerSimd<FMT, D, R>)) void
+quant_attend_kernel(AttendArgs args) {
+  __shared__ Joined<D, R, WAVES> joined;
+  const Scope scope = args.scope;
+  const ItemPtr it = in_plan<Item>(args.plan, args.at_items) + blockIdx.x;
+  if (static_cast<int32_t>(blockIdx.x) >= in_plan<Header>(args.plan, 0)->items[args.kind]) return;
+  attend_item<FMT, D, T, R, WAVES>(scope, it, joined);
 }
 
 // Prompts: 128 rows a workgroup, 32 a wave. The cache's tokens become matrix
@@ -813,20 +911,19 @@ struct Stage {
 };
 
 template <int FMT, int D, typename T>
-__global__ __launch_bounds__(kAttendLanes, D == 256 ? 1 : 2) void quant_prompt_kernel(
-    AttendArgs a) {
+__device__ __forceinline__ void attend_prompt_item(const Scope& a, ItemPtr it,
+                                                   Stage<D> (&stages)[2]) {
   typedef typename Operand<T>::v8 v8;
   constexpr int R = kWaveRows / 16, kSteps = D / 32, kOut = D / 16;
-  __shared__ Stage<D> stages[2];
-
-  const Item it = reinterpret_cast<const Item*>(a.plan + a.at_items)[blockIdx.x];
-  if (static_cast<int32_t>(blockIdx.x) >= header(a.plan).items[a.kind]) return;
-  const int32_t* table = reinterpret_cast<const int32_t*>(a.plan + a.at_table) + it.table;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int lane = threadIdx.x % 64, m = lane % 16, g = lane / 16;
-  const int64_t head_offset = it.kv_head * Chunk<FMT, D>::bytes(1 << a.block_shift);
-  const int32_t low = it.base + it.row / a.group;
-  const int32_t high = it.base + (it.row + it.rows - 1) / a.group;
+  const ColdArgs args = cold_args();
+  const auto* table = in_plan<int32_t>(args->plan, args->at_table) + it->table;
+  const Tiles tiles = {it->first_tiles, it->window_tile - it->first_tiles, it->tile_end};
+  const int32_t group = args->group;
+  const int64_t head_offset = it->kv_head * Chunk<FMT, D>::bytes(1 << a.block_shift);
+  const int32_t low = it->base + it->row / group;
+  const int32_t high = it->base + (it->row + it->rows - 1) / group;
 
   // this wave's share of a stage: half a tile of K, half the values of a tile of V
   constexpr int kVBytes = Chunk<FMT, D>::kCode / 32;
@@ -834,21 +931,22 @@ __global__ __launch_bounds__(kAttendLanes, D == 256 ? 1 : 2) void quant_prompt_k
   KPart<FMT, D> k;
   VPart<FMT, D, kVBytes> v;
   const auto load = [&](int32_t at) {
-    if (at + own_tile >= it.tile_end) return;
-    const int32_t position = tile_at(it, at + own_tile) * kTile;
-    const Half h[2] = {
-        find_half<FMT, D>(a.pages, head_offset, a.block_shift, table, position),
-        find_half<FMT, D>(a.pages, head_offset, a.block_shift, table, position + 16)};
+    if (at + own_tile >= tiles.end) return;
+    const int32_t position = tiles.at(at + own_tile) * kTile;
+    const Half h[2] = {find_half<FMT, D>(a.pages, head_offset, a.block_shift,
+                                         table[position >> a.block_shift], position),
+                       find_half<FMT, D>(a.pages, head_offset, a.block_shift,
+                                         table[(position + 16) >> a.block_shift], position + 16)};
     k.load(own_half ? h[1] : h[0], a.block_shift, m, g);
     v.load(h, a.block_shift, m, g, own_half * kVBytes);
   };
   const auto lay = [&](Stage<D>& to, int32_t at) {
-    if (at + own_tile >= it.tile_end) return;
+    if (at + own_tile >= tiles.end) return;
     each_constant<0, kSteps>([&](auto s) {
       const v8 f = k.template operand<T, decltype(s)::value>();
       __builtin_memcpy(&to.k[wave][decltype(s)::value][lane], &f, 16);
     });
-    const int32_t begin = tile_at(it, at + own_tile) * kTile;
+    const int32_t begin = tiles.at(at + own_tile) * kTile;
     if (!seen_whole(a, low, high, begin)) {
       const uint32_t odd = v.clear_unseen(begin, g, low, high, a.window, a.sinks);
       if (own_half == 0 && m % (512 / D) == 0) to.odd[own_tile][m * D / 512][g] = odd;
@@ -863,12 +961,12 @@ __global__ __launch_bounds__(kAttendLanes, D == 256 ? 1 : 2) void quant_prompt_k
       __builtin_memcpy(&to.v[own_tile][first + 1][lane], &odd, 16);
     });
   };
-  load(it.tile);
+  load(it->tile);
 
-  const int32_t row0 = it.row + wave * kWaveRows;
-  const int32_t rows = min(max(it.rows - wave * kWaveRows, 0), kWaveRows);
-  const int32_t wave_low = it.base + row0 / a.group;
-  const int32_t wave_high = rows ? it.base + (row0 + rows - 1) / a.group : -1;
+  const int32_t row0 = it->row + wave * kWaveRows;
+  const int32_t rows = min(max(it->rows - wave * kWaveRows, 0), kWaveRows);
+  const int32_t wave_low = it->base + row0 / group;
+  const int32_t wave_high = rows ? it->base + (row0 + rows - 1) / group : -1;
   v8 q[R][kSteps];
   int32_t position[R];
   f32x4 o[R][kOut];
@@ -877,15 +975,15 @@ __global__ __launch_bounds__(kAttendLanes, D == 256 ? 1 : 2) void quant_prompt_k
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const bool there = 16 * r + m < rows;
-    position[r] = there ? it.base + (row0 + 16 * r + m) / a.group : wave_low;
-    load_query<T, D>(a, it, row0 + 16 * r + m, there, g, q[r]);
+    position[r] = there ? it->base + (row0 + 16 * r + m) / group : wave_low;
+    load_query<T, D>(args, it, row0 + 16 * r + m, there, g, q[r]);
 #pragma unroll
     for (int d = 0; d < kOut; ++d) o[r][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
   const auto multiply = [&](const Stage<D>& from, int32_t at, int tile) {
-    if (at + tile >= it.tile_end) return;
-    const int32_t begin = tile_at(it, at + tile) * kTile;
+    if (at + tile >= tiles.end) return;
+    const int32_t begin = tiles.at(at + tile) * kTile;
     // tiles that none of the wave's rows sees
     if ((begin > wave_high) |
         ((wave_low - (begin + kTile - 1) >= a.window) & (begin >= a.sinks)))
@@ -941,7 +1039,7 @@ __global__ __launch_bounds__(kAttendLanes, D == 256 ? 1 : 2) void quant_prompt_k
   };
 
   int turn = 0;
-  for (int32_t at = it.tile; at < it.tile_end; at += kStageTiles, turn ^= 1) {
+  for (int32_t at = it->tile; at < tiles.end; at += kStageTiles, turn ^= 1) {
     lay(stages[turn], at);
     load(at + kStageTiles);
     __syncthreads();
@@ -949,30 +1047,31 @@ __global__ __launch_bounds__(kAttendLanes, D == 256 ? 1 : 2) void quant_prompt_k
     for (int tile = 0; tile < kStageTiles; ++tile) multiply(stages[turn], at, tile);
   }
 
+  const ColdArgs end_args = cold_args();
+  const ItemPtr ended = anew(it);
+  const int32_t slot = ended->slot;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const float total = row_sum(state[r].sum);
     const int32_t n = row0 + 16 * r + m;
     if (16 * r + m >= rows) continue;
-    float* part = a.work + it.slot * a.slot_floats + (n - it.row) * (D + 4);
-    const int32_t token = n / a.group;
-    T* to = reinterpret_cast<T*>(a.out.base) + (int64_t(it.token) + token) * a.out.token +
-            (int64_t(it.kv_head) * a.group + (n - token * a.group)) * a.out.head;
-    const float inv = it.slot < 0 ? 1.f / total : 1.f;
+    float* part = end_args->work + slot * end_args->slot_floats + (n - ended->row) * (D + 4);
+    T* to = result_row<T>(end_args, ended, n);
+    const float inv = slot < 0 ? 1.f / total : 1.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float y[kOut];
 #pragma unroll
       for (int d = 0; d < kOut; ++d) y[d] = unless_poisoned<D>(o[r][d][i] * inv, poison, r, i);
       const int first = kOut * (4 * g + i);
-      if (it.slot >= 0) {
+      if (slot >= 0) {
 #pragma unroll
         for (int d = 0; d < kOut; d += 4) __builtin_memcpy(part + first + d, y + d, 16);
       } else {
         T t[kOut];
 #pragma unroll
         for (int d = 0; d < kOut; ++d) t[d] = static_cast<T>(y[d]);
-        if (a.out.whole_words) {
+        if (end_args->out.whole_words) {
           __builtin_memcpy(__builtin_assume_aligned(to + first, kOut < 8 ? 8 : 16), t, sizeof t);
         } else {
 #pragma unroll
@@ -980,51 +1079,60 @@ __global__ __launch_bounds__(kAttendLanes, D == 256 ? 1 : 2) void quant_prompt_k
         }
       }
     }
-    if (it.slot >= 0 && g == 0) {
+    if (slot >= 0 && g == 0) {
       part[D] = state[r].top;
       part[D + 1] = total;
     }
   }
 }
 
+template <int FMT, int D, typename T>
+__global__ __launch_bounds__(kAttendLanes, D == 256 ? 1 : 2) void quant_prompt_kernel(
+    AttendArgs args) {
+  __shared__ Stage<D> stages[2];
+  const Scope scope = args.scope;
+  const ItemPtr it = in_plan<Item>(args.plan, args.at_items) + blockIdx.x;
+  if (static_cast<int32_t>(blockIdx.x) >= in_plan<Header>(args.plan, 0)->items[args.kind]) return;
+  attend_prompt_item<FMT, D, T>(scope, it, stages);
+}
+
 // Rows whose tiles several items shared: their parts, scaled to the largest
 // score of all, over the sum of their sums. A workgroup's lanes are groups of D / 4,
-// four values a lane. Up to kSides parts (rows of prompts) each group takes rows
-// of its own; more (few rows over a long axis) are shared out to the groups.
-constexpr int kMergeRows = 16;   // workgroups of one merge
-
+// four values a lane. Of up to kMergeRows parts each group takes rows of its own;
+// more (few rows over a long axis) are shared out to the groups, one row a workgroup.
 template <int D, typename T>
 __global__ __launch_bounds__(256) void quant_merge_kernel(AttendArgs a) {
   constexpr int kLanes = D / 4, kSides = 256 / kLanes;
   __shared__ f32x4 side[kSides][kLanes];
   __shared__ float side_sum[kSides], side_top[4];
-  const Merge mg = reinterpret_cast<const Merge*>(a.plan + a.at_merges)[blockIdx.x];
-  if (static_cast<int32_t>(blockIdx.x) >= header(a.plan).merges) return;
-  const int64_t each = a.kind_slot_floats[mg.kind];
-  const float* parts = a.work_base + a.kind_work[mg.kind] + mg.slot * each;
+  const auto* mg = in_plan<Merge>(a.plan, a.at_merges) + blockIdx.x;
+  if (static_cast<int32_t>(blockIdx.x) >= in_plan<Header>(a.plan, 0)->merges) return;
+  const int64_t each = a.kind_slot_floats[mg->kind];
+  const int32_t parts = mg->parts;
+  const float* rows = a.work_base + a.kind_work[mg->kind] + mg->slot * each +
+                      mg->first * (D + 4);
   const int at = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   const auto store = [&](int32_t row, f32x4 y, float total) {
-    const int32_t n = mg.row + row, token = n / a.group;
-    T* to = reinterpret_cast<T*>(a.out.base) + (int64_t(mg.token) + token) * a.out.token +
-            (int64_t(mg.kv_head) * a.group + (n - token * a.group)) * a.out.head + 4 * at;
+    T* to = result_row<T>((ColdArgs)__builtin_amdgcn_kernarg_segment_ptr(), mg, mg->row + row) +
+            4 * at;
 #pragma unroll
     for (int i = 0; i < 4; ++i) to[i] = static_cast<T>(y[i] / total);
   };
-  if (mg.parts <= kSides) {
-    for (int32_t row = blockIdx.y * kSides + group; row < mg.rows; row += kMergeRows * kSides) {
-      const float* from = parts + row * (D + 4);
-      float t[kSides], most = -INFINITY;
+  if (parts <= kMergeRows) {
+    for (int32_t row = group; row < mg->rows; row += kSides) {
+      const float* from = rows + row * (D + 4);
+      float t[kMergeRows], most = -INFINITY;
 #pragma unroll
-      for (int p = 0; p < kSides; ++p) {
-        t[p] = p < mg.parts ? from[p * each + D] : -INFINITY;
+      for (int p = 0; p < kMergeRows; ++p) {
+        t[p] = p < parts ? from[p * each + D] : -INFINITY;
         most = fmaxf(most, t[p]);
       }
       f32x4 y = {0.f, 0.f, 0.f, 0.f};
       float total = 0.f;
 #pragma unroll
-      for (int p = 0; p < kSides; ++p) {
-        if (p >= mg.parts) continue;
-        const float fade = t[p] == most ? 1.f : __builtin_amdgcn_exp2f((t[p] - most) * a.c);
+      for (int p = 0; p < kMergeRows; ++p) {
+        if (p >= parts) continue;
+        const float fade = t[p] == most ? 1.f : __builtin_amdgcn_exp2f((t[p] - most) * a.scope.c);
         y += *reinterpret_cast<const f32x4*>(from + p * each + 4 * at) * fade;
         total += from[p * each + D + 1] * fade;
       }
@@ -1032,37 +1140,32 @@ __global__ __launch_bounds__(256) void quant_merge_kernel(AttendArgs a) {
     }
     return;
   }
-  for (int32_t row = blockIdx.y; row < mg.rows; row += kMergeRows) {
-    const float* from = parts + row * (D + 4);
-    float most = -INFINITY;
-    for (int p = threadIdx.x; p < mg.parts; p += 256) most = fmaxf(most, from[p * each + D]);
+  float most = -INFINITY;
+  for (int p = threadIdx.x; p < parts; p += 256) most = fmaxf(most, rows[p * each + D]);
 #pragma unroll
-    for (int far = 32; far; far /= 2) most = fmaxf(most, __shfl_xor(most, far));
-    if (threadIdx.x % 64 == 0) side_top[threadIdx.x / 64] = most;
-    __syncthreads();
-    most = fmaxf(fmaxf(side_top[0], side_top[1]), fmaxf(side_top[2], side_top[3]));
-    f32x4 y = {0.f, 0.f, 0.f, 0.f};
-    float total = 0.f;
+  for (int far = 32; far; far /= 2) most = fmaxf(most, __shfl_xor(most, far));
+  if (threadIdx.x % 64 == 0) side_top[threadIdx.x / 64] = most;
+  __syncthreads();
+  most = fmaxf(fmaxf(side_top[0], side_top[1]), fmaxf(side_top[2], side_top[3]));
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+  float total = 0.f;
 #pragma unroll 4
-    for (int p = group; p < mg.parts; p += kSides) {
-      const float t = from[p * each + D];
-      const float fade = t == most ? 1.f : __builtin_amdgcn_exp2f((t - most) * a.c);
-      y += *reinterpret_cast<const f32x4*>(from + p * each + 4 * at) * fade;
-      total += from[p * each + D + 1] * fade;
-    }
-    side[group][at] = y;
-    if (at == 0) side_sum[group] = total;
-    __syncthreads();
-    if (group == 0) {
-#pragma unroll
-      for (int i = 1; i < kSides; ++i) {
-        y += side[i][at];
-        total += side_sum[i];
-      }
-      store(row, y, total);
-    }
-    __syncthreads();
+  for (int p = group; p < parts; p += kSides) {
+    const float t = rows[p * each + D];
+    const float fade = t == most ? 1.f : __builtin_amdgcn_exp2f((t - most) * a.scope.c);
+    y += *reinterpret_cast<const f32x4*>(rows + p * each + 4 * at) * fade;
+    total += rows[p * each + D + 1] * fade;
   }
+  side[group][at] = y;
+  if (at == 0) side_sum[group] = total;
+  __syncthreads();
+  if (group != 0) return;
+#pragma unroll
+  for (int i = 1; i < kSides; ++i) {
+    y += side[i][at];
+    total += side_sum[i];
+  }
+  store(0, y, total);
 }
 
 }  // namespace

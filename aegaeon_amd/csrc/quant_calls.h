@@ -163,6 +163,7 @@ int span_args(const QuantCall& c, bool fresh, SpanArgs* a, dim3* grid) {
   a->plan = c.plan;
   a->at_seqs = h.room.at_seqs;
   a->at_table = h.room.at_table;
+  a->at_new_spans = h.room.at_new_spans;
   a->pages[0] = const_cast<char*>(c.k);
   a->pages[1] = const_cast<char*>(c.v);
   a->page_bytes = c.page_bytes;
@@ -307,18 +308,17 @@ int aegkv_quant_attend(const void* plan, const void* device_plan, int format, in
     if (rc) return rc;
   }
   a.plan = c.plan;
-  a.at_seqs = h.room.at_seqs;
   a.at_table = h.room.at_table;
   a.at_merges = h.room.at_merges;
-  a.pages = QuantPages{c.k, c.v, c.page_bytes};
+  a.scope.pages = QuantPages{c.k, c.v, c.page_bytes};
   a.work_base = static_cast<float*>(workspace);
-  a.c = static_cast<float>(factor);
-  a.block_shift = __builtin_ctz(h.block_size);
+  a.scope.c = static_cast<float>(factor);
+  a.scope.block_shift = __builtin_ctz(h.block_size);
   a.group = h.group;
-  a.window = h.window ? h.window : INT32_MAX;
-  a.sinks = h.sinks;
+  a.scope.window = h.window ? h.window : INT32_MAX;
+  a.scope.sinks = h.sinks;
   rc = check_grid(h.room.merges, 256);
-  for (int kind = 0; kind < kKinds && !rc; ++kind) rc = check_grid(h.room.items[kind], kAttendLanes);
+  for (int kind = 0; kind < kKinds && !rc; ++kind) rc = check_grid(h.room.items[kind], 1024);
   if (rc) return rc;
   return by_shape(format, head_dim, [&](auto fmt, auto d) {
     constexpr int kFormat = decltype(fmt)::value, kDim = decltype(d)::value;
@@ -331,17 +331,20 @@ int aegkv_quant_attend(const void* plan, const void* device_plan, int format, in
         a.work = a.work_base + a.kind_work[kind];
         a.slot_floats = a.kind_slot_floats[kind];
         const dim3 grid(static_cast<uint32_t>(h.room.items[kind]));
+        constexpr int kWaves = kWideWaves<kFormat, kDim>;
         if (kind == kFew)
-          quant_attend_kernel<kFormat, kDim, T, 1><<<grid, kAttendLanes, 0, stream>>>(a);
+          quant_attend_kernel<kFormat, kDim, T, 1, 4><<<grid, 256, 0, stream>>>(a);
         else if (kind == kMore)
-          quant_attend_kernel<kFormat, kDim, T, 2><<<grid, kAttendLanes, 0, stream>>>(a);
+          quant_attend_kernel<kFormat, kDim, T, 2, 4><<<grid, 256, 0, stream>>>(a);
+        else if (kind == kWide)
+          quant_attend_kernel<kFormat, kDim, T, 1, kWaves><<<grid, kWaves * 64, 0, stream>>>(a);
         else
           quant_prompt_kernel<kFormat, kDim, T><<<grid, kAttendLanes, 0, stream>>>(a);
         const int rc = launched("quant_attend_kernel launch");
         if (rc) return rc;
       }
       if (h.room.merges) {
-        const dim3 grid(static_cast<uint32_t>(h.room.merges), kMergeRows);
+        const dim3 grid(static_cast<uint32_t>(h.room.merges));
         quant_merge_kernel<kDim, T><<<grid, 256, 0, stream>>>(a);
         return launched("quant_merge_kernel launch");
       }
