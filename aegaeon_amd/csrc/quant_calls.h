@@ -152,8 +152,8 @@ int check_grid(int64_t workgroups, int lanes) {
   return 0;
 }
 
-// Spans of 16 tokens of a row group a workgroup: kSpanRows rows, all heads of a
-// decode step's single tokens, a few of whole spans.
+// Rows (a token of a head) that a workgroup of a write or read takes about: all
+// heads of a decode step's single tokens, a few of whole spans.
 constexpr int64_t kSpanRows = 64;
 
 int span_args(const QuantCall& c, bool fresh, SpanArgs* a, dim3* grid) {
@@ -172,9 +172,9 @@ int span_args(const QuantCall& c, bool fresh, SpanArgs* a, dim3* grid) {
   a->fresh = fresh;
   a->heads_each = static_cast<int32_t>(
       std::min<int64_t>(h.kv_heads, std::max<int64_t>(1, kSpanRows * spans / std::max<int64_t>(1, tokens))));
-  *grid = dim3(static_cast<uint32_t>(spans),
-               static_cast<uint32_t>((h.kv_heads + a->heads_each - 1) / a->heads_each), 2);
-  return check_grid(spans, kSpanLanes);
+  a->head_groups = (h.kv_heads + a->heads_each - 1) / a->heads_each;
+  *grid = dim3(static_cast<uint32_t>(spans * a->head_groups), 2);
+  return check_grid(spans * a->head_groups, kSpanLanes);
 }
 
 // Workspace of attention: each kind's parts one after another.
