@@ -448,30 +448,43 @@ __device__ __forceinline__ Half find_half(const QuantPages& p, int64_t head_offs
   return Half{p.k + codes, p.v + codes, p.k + scales, p.v + scales};
 }
 
-template <int BYTES>
+// STREAM: what no other workgroup reads goes past the caches.
+template <int BYTES, bool STREAM>
 __device__ __forceinline__ void load_bytes(uint32_t* to, const char* base, uint32_t offset) {
   const char* p = base + offset;
+  const auto one = [](const auto* at) {
+    return STREAM ? __builtin_nontemporal_load(at) : *at;
+  };
   if constexpr (BYTES == 1) {
-    to[0] = *reinterpret_cast<const uint8_t*>(p);
+    to[0] = one(reinterpret_cast<const uint8_t*>(p));
   } else if constexpr (BYTES == 2) {
-    to[0] = *reinterpret_cast<const uint16_t*>(p);
+    to[0] = one(reinterpret_cast<const uint16_t*>(p));
+  } else if constexpr (BYTES == 4) {
+    to[0] = one(reinterpret_cast<const uint32_t*>(p));
+  } else if constexpr (BYTES == 8) {
+    const v2u x = one(reinterpret_cast<const v2u*>(p));
+    __builtin_memcpy(to, &x, 8);
   } else {
-    __builtin_memcpy(to, __builtin_assume_aligned(p, BYTES < 16 ? BYTES : 16), BYTES);
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i) {
+      const v4u x = one(reinterpret_cast<const v4u*>(p) + i);
+      __builtin_memcpy(to + 4 * i, &x, 16);
+    }
   }
 }
 
 // A lane's part of 16 tokens of K, and the scales of its groups.
-template <int FMT, int D>
+template <int FMT, int D, bool STREAM>
 struct KPart {
   static constexpr int kWords = Chunk<FMT, D>::kCode / 16;
   static constexpr int kScales = D == 256 ? 2 : 1;
   uint32_t code[kWords], scale[kScales];
 
   __device__ __forceinline__ void load(const Half& h, int block_shift, uint32_t m, uint32_t g) {
-    load_bytes<kWords * 4>(code, h.k, m * Chunk<FMT, D>::kCode + g * (kWords * 4));
+    load_bytes<kWords * 4, STREAM>(code, h.k, m * Chunk<FMT, D>::kCode + g * (kWords * 4));
 #pragma unroll
     for (uint32_t i = 0; i < kScales; ++i)
-      load_bytes<1>(&scale[i], h.k_scales, ((D == 64 ? g / 2 : g * kScales + i) << block_shift) + m);
+      load_bytes<1, STREAM>(&scale[i], h.k_scales, ((D == 64 ? g / 2 : g * kScales + i) << block_shift) + m);
   }
 
   // The matrix operand of step S: the lane's values 8 S .. 8 S + 7.
@@ -489,7 +502,7 @@ struct KPart {
 
 // A lane's part of 32 tokens of V: BYTES of each of its eight tokens, from byte
 // `from` of the lane's on.
-template <int FMT, int D, int BYTES>
+template <int FMT, int D, int BYTES, bool STREAM>
 struct VPart {
   static constexpr int kWords = (BYTES + 3) / 4;
   static constexpr int kPairs = BYTES * 4 / Format<FMT>::kBits;   // pairs of values
@@ -502,9 +515,9 @@ struct VPart {
     for (int half = 0; half < 2; ++half) {
 #pragma unroll
       for (uint32_t i = 0; i < 4; ++i)
-        load_bytes<BYTES>(code[half][i], h[half].v + i * kCode,
+        load_bytes<BYTES, STREAM>(code[half][i], h[half].v + i * kCode,
                           4 * g * kCode + m * (kCode / 16) + from);
-      load_bytes<4>(&scale[half], h[half].v_scales, ((m * D / 512) << block_shift) + 4 * g);
+      load_bytes<4, STREAM>(&scale[half], h[half].v_scales, ((m * D / 512) << block_shift) + 4 * g);
     }
   }
 
@@ -746,8 +759,8 @@ __device__ __forceinline__ void attend_item(const Scope& a, ItemPtr it,
   // as soon as the registers it goes to are operands, its V as soon as theirs are,
   // and the blocks that it lies in one step earlier still.
   struct Tile {
-    KPart<FMT, D> k[2];
-    VPart<FMT, D, Chunk<FMT, D>::kCode / 16> v;
+    KPart<FMT, D, true> k[2];
+    VPart<FMT, D, Chunk<FMT, D>::kCode / 16, true> v;
   };
   struct Blocks {
     int32_t position, block[2];
@@ -986,8 +999,8 @@ __device__ __forceinline__ void attend_prompt_item(const Scope& a, ItemPtr it,
   // this wave's share of a stage: half a tile of K, half the values of a tile of V
   constexpr int kVBytes = Chunk<FMT, D>::kCode / 32;
   const int own_tile = wave / 2, own_half = wave % 2;
-  KPart<FMT, D> k;
-  VPart<FMT, D, kVBytes> v;
+  KPart<FMT, D, false> k;
+  VPart<FMT, D, kVBytes, false> v;
   const auto load = [&](int32_t at) {
     if (at + own_tile >= tiles.end) return;
     const int32_t position = tiles.at(at + own_tile) * kTile;
