@@ -1060,18 +1060,27 @@ __device__ __forceinline__ void attend_prompt_item(const Scope& a, ItemPtr it,
         ((wave_low - (begin + kTile - 1) >= a.window) & (begin >= a.sinks)))
       return;
     f32x4 x[R][2];
+    // The operands are read from shared memory together, V's before the softmax:
+    // two at a time where they are used, four prompts took 231 us instead of 226.
+    v8 kf[2][kSteps];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
+    for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-      for (int r = 0; r < R; ++r) x[r][half] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int half = 0; half < 2; ++half)
+        __builtin_memcpy(&kf[half][s], &from.k[2 * tile + half][s][lane], 16);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        v8 f;
-        __builtin_memcpy(&f, &from.k[2 * tile + half][s][lane], 16);
+    for (int r = 0; r < R; ++r) x[r][0] = x[r][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int r = 0; r < R; ++r) x[r][half] = Operand<T>::mma(f, q[r][s], x[r][half]);
-      }
-    }
+    for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int r = 0; r < R; ++r) x[r][half] = Operand<T>::mma(kf[half][s], q[r][s], x[r][half]);
+    v8 vf[kOut];
+#pragma unroll
+    for (int d = 0; d < kOut; ++d) __builtin_memcpy(&vf[d], &from.v[tile][d][lane], 16);
+    __builtin_amdgcn_sched_barrier(0);
     if (!seen_whole(a, wave_low, wave_high, begin)) {
 #pragma unroll
       for (int half = 0; half < 2; ++half)
@@ -1101,12 +1110,9 @@ __device__ __forceinline__ void attend_prompt_item(const Scope& a, ItemPtr it,
 #pragma unroll
     for (int r = 0; r < R; ++r) p[r] = softmax_step<T>(x[r], a.c, state[r], o[r]);
 #pragma unroll
-    for (int d = 0; d < kOut; ++d) {
-      v8 f;
-      __builtin_memcpy(&f, &from.v[tile][d][lane], 16);
+    for (int d = 0; d < kOut; ++d)
 #pragma unroll
-      for (int r = 0; r < R; ++r) o[r][d] = Operand<T>::mma(f, p[r], o[r][d]);
-    }
+      for (int r = 0; r < R; ++r) o[r][d] = Operand<T>::mma(vf[d], p[r], o[r][d]);
   };
 
   int turn = 0;
