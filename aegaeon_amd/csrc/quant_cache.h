@@ -110,7 +110,8 @@ __device__ __forceinline__ bool find_span(const SpanArgs& a, int32_t i, Span* s)
     *s = Span{n->block, n->inside, n->count, n->token};
     return i < h->new_spans;
   }
-  if (i >= h->read_spans) return false;
+  // a captured read may find, after an update, a batch with released columns
+  if (i >= h->read_spans || !h->complete) return false;
   const auto* seq = in_plan<Seq>(a.plan, a.at_seqs);
   // the last sequence that begins at or before span i; empty sequences begin
   // where the next one does
@@ -535,8 +536,8 @@ struct VPart {
         const bool any = (j <= high) & ((low - j < window) | (j < sinks));
         const uint32_t byte = (scale[half] >> (8 * i)) & 255u;
         const bool number = byte != kNoNumber;
-        odd |= any & !number ? 1u << (4 * half + i) : 0u;
-        const uint32_t keep = any & number ? ~0u : 0u;
+        odd |= (any & !number) ? 1u << (4 * half + i) : 0u;
+        const uint32_t keep = (any & number) ? ~0u : 0u;
         scale[half] = (scale[half] & ~(255u << (8 * i))) | ((keep ? byte : 127u) << (8 * i));
 #pragma unroll
         for (int w = 0; w < kWords; ++w) code[half][i][w] &= keep;
@@ -578,13 +579,6 @@ __device__ __forceinline__ float row_max(float x) {
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-__device__ __forceinline__ float row_sum(float x) {
-  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-  auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
 // f(0), .., f(N - 1) with constants
 template <int I, int N, typename F>
 __device__ __forceinline__ void each_constant(const F& f) {
@@ -615,7 +609,7 @@ __device__ __forceinline__ void note_odd(const Scope& a, const F& none, int32_t 
       const bool is_none = none(D == 64 ? g / 2 : g * kEach + i, t);
 #pragma unroll
       for (int r = 0; r < R; ++r)
-        poison |= is_none & seen(a, position[r], begin + t) ? 1u << (kEach * r + i) : 0u;
+        poison |= (is_none & seen(a, position[r], begin + t)) ? 1u << (kEach * r + i) : 0u;
     }
   }
 }
@@ -670,32 +664,35 @@ __device__ __forceinline__ void load_query(ColdArgs args, ItemPtr it, int32_t ro
 }
 
 // A row's running sums are taken against a score that need not be its largest,
-// only near it: 2^kLift stands for `top`, and what grows past kLimit, in the sum
-// of a lane's eight tokens, has the row's scores looked through for their largest
-// and the sums made before fade to it. The types' relative precision is the
-// same over the whole range between; looked through for every tile, with the
-// lanes' exchange, it took a third of the arithmetic.
+// only near it: 2^kLift stands for `top`, and a probability past kLimit has the
+// row's scores looked through for their largest and the sums made before fade
+// to it. The types' relative precision is the same over the whole range
+// between; looked through for every tile, with the lanes' exchange, it took a
+// third of the arithmetic.
+// The sum is that of the rounded probabilities, the ones that V is multiplied
+// with, as one more product, with ones: what rounding adds to both cancels
+// in part (against 64 bits 0.0021 instead of 0.0023 in bfloat16), every lane of a
+// row has it, and a matrix instruction does the work of seven additions.
 struct RowState {
   float top = -INFINITY;
   float lift = 1e30f;    // kLift - top * c; as large while there is no top
-  float sum = 0.f;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};   // four times the same
 };
 
 // Scores of a row tile (lane's row, eight of its tokens) into probabilities.
 template <typename T, int N>
 __device__ __forceinline__ typename Operand<T>::v8 softmax_step(const f32x4* x, float c,
                                                                RowState& s, f32x4 (&o)[N]) {
-  float e[8], total;
+  float e[8], largest;
   const auto exponents = [&]() {
-    total = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 8; ++i)
       e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i / 4][i % 4], c, s.lift));
-      total += e[i];
-    }
+    largest = fmaxf(fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])),
+                    fmaxf(fmaxf(e[4], e[5]), fmaxf(e[6], e[7])));
   };
   exponents();
-  if (__any(total > Operand<T>::kLimit)) {
+  if (__any(largest > Operand<T>::kLimit)) {
     float most = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
                        fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
     most = fmaxf(s.top, row_max(most));
@@ -707,10 +704,13 @@ __device__ __forceinline__ typename Operand<T>::v8 softmax_step(const f32x4* x, 
     if (most != -INFINITY) s.lift = Operand<T>::kLift - most * c;
     exponents();
   }
-  s.sum += total;
-  typename Operand<T>::v8 p;
+  typename Operand<T>::v8 p, ones;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) p[i] = static_cast<T>(e[i]);
+  for (int i = 0; i < 8; ++i) {
+    p[i] = static_cast<T>(e[i]);
+    ones[i] = T(1.f);
+  }
+  s.sum = Operand<T>::mma(ones, p, s.sum);
   return p;
 }
 
@@ -890,7 +890,7 @@ __device__ __forceinline__ void attend_item(const Scope& a, ItemPtr it,
   // their scores
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const float s = row_sum(state[r].sum);
+    const float s = state[r].sum[0];
     if (g == 0) {
       share.top[wave][16 * r + m] = state[r].top;
       share.sum[wave][16 * r + m] = s;
@@ -1129,7 +1129,7 @@ __device__ __forceinline__ void attend_prompt_item(const Scope& a, ItemPtr it,
   const int32_t slot = ended->slot;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const float total = row_sum(state[r].sum);
+    const float total = state[r].sum[0];
     const int32_t n = row0 + 16 * r + m;
     if (16 * r + m >= rows) continue;
     float* part = end_args->work + slot * end_args->slot_floats + (n - ended->row) * (D + 4);

@@ -1054,7 +1054,7 @@ class CacheBatch:
             _lib.check(_lib.load().aegkv_quant_attend_workspace(self._host_ptr, d,
                                                                 ctypes.byref(n)))
             self._workspace[d] = int(n.value)
-        self._used: dict = {}     # raw stream -> event behind its last call over this batch
+        self._used: dict = {}     # raw stream -> stream of calls made elsewhere than at home
         with torch.cuda.device(self.device):
             st = stream if stream is not None else torch.cuda.current_stream()
             if torch.cuda.is_current_stream_capturing():
@@ -1099,7 +1099,7 @@ class CacheBatch:
         self._plan.copy_(pinned, non_blocking=True)
         self._uploaded = torch.cuda.Event()
         self._uploaded.record(st)
-        self._stream = st.cuda_stream
+        self._home, self._stream = st, st.cuda_stream
         # BatchArgs of csrc/hostargs.cpp
         self._packed = struct.pack(
             "13q", self._host_ptr, self._plan.data_ptr(), self._stream, self.kv_heads, self.heads,
@@ -1119,10 +1119,9 @@ class CacheBatch:
                     raise ValueError("a batch is updated outside the capture; the graph's calls "
                                      "find what it holds when they are replayed")
                 self._make(block_tables, seq_lens, new_lens, update=1)
-                if st.cuda_stream != self._stream:
-                    st.wait_event(self._uploaded)
-                for event in self._used.values():
-                    st.wait_event(event)
+                for other in (self._home, *self._used.values()):
+                    if _alive(other) and other.cuda_stream != st.cuda_stream:
+                        st.wait_event(other.record_event())
                 self._used.clear()
                 self._upload(st)
 
@@ -1135,17 +1134,36 @@ class CacheBatch:
         with torch.cuda.stream(st):
             if torch.cuda.is_current_stream_capturing():
                 return None     # capture begins behind a synchronize
-        st.wait_event(self._uploaded)
+        if _alive(self._home):  # a closed stream was waited for
+            st.wait_event(self._uploaded)
         return st
 
     def _leave(self, st: torch.cuda.Stream | None) -> None:
-        if st is None:
+        if st is not None:
+            self._used[st.cuda_stream] = st
+
+    def __del__(self, _finalizing=sys.is_finalizing):
+        # the plan's memory goes back to its home stream's pool: behind the calls
+        # on other streams that read it. (Not Tensor.record_stream, which records
+        # an event on them when the memory goes, when they may be closed.)
+        if _finalizing() or not getattr(self, "_used", None):
             return
-        event = self._used.get(st.cuda_stream)
-        if event is None:
-            event = self._used[st.cuda_stream] = torch.cuda.Event()
-        event.record(st)
-        self._plan.record_stream(st)
+        try:
+            for st in self._used.values():
+                if not _alive(st):
+                    continue
+                if _alive(self._home):
+                    self._home.wait_event(st.record_event())
+                else:
+                    st.synchronize()
+        except Exception:
+            pass
+
+
+def _alive(stream: torch.cuda.Stream) -> bool:
+    """Whether a stream may still be handed to the runtime (a closed dedicated
+    stream, whose work was waited for, may not)."""
+    return not getattr(stream, "closed", False)
 
 
 def _quant_call(cache: QuantCache, batch: CacheBatch):

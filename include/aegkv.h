@@ -586,7 +586,9 @@ int aegkv_quant_write(const void* plan, const void* device_plan, int format, int
  * Read tokens back as values of `dtype` (each rounded once; no number: NaN): the
  * batch's new tokens (new_tokens != 0), or all tokens of its sequences, one
  * sequence after another (AEGKV_ERANGE if one has a released column). Rows of k
- * and v must not overlap; rows behind the last token are left as they were.
+ * and v must not overlap; rows behind the last token are left as they were. A
+ * captured read of all tokens, replayed after an update to a batch with a
+ * released column, leaves k and v as they were.
  */
 int aegkv_quant_read(const void* plan, const void* device_plan, int format, int32_t head_dim,
                      const void* k_pages, const void* v_pages, int new_tokens, void* k,

@@ -444,6 +444,75 @@ def test_capture_has_to_hold_all_that_a_replay_may_reach(gpu):
     batch.update([[i] for i in range(4)], [1] * 4, [1] * 4)
 
 
+def test_a_captured_read_of_released_columns_reads_nothing(gpu):
+    cache, k, _ = make(gpu, "mxfp8", 12, 16, 2, 64)
+    batch = batch_for(gpu, [[3, 4, 5]], [40], [1], cache, window=8, max_columns=4)
+    out = tuple(torch.zeros(64, 2, 64, dtype=F16, device=gpu) for _ in range(2))
+    ops.quant_read(cache, batch, out=out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.quant_read(cache, batch, out=out)
+    for table, whole in (([6, 7, 8], True), ([-1, -1, 8], False), ([1, 2, 3], True)):
+        batch.update([table], [40], [1])
+        out[0].fill_(9)
+        g.replay()
+        if whole:
+            want = k.get(*ref.places(table, 16, range(40))).to(F16)
+            assert torch.equal(out[0][:40].cpu(), want) and (out[0][40:] == 9).all()
+        else:
+            assert (out[0] == 9).all()
+
+
+def test_dedicated_streams(gpu):
+    lens = [300]
+    tables = tables_for(lens, 16, 20)
+    cache, k, v = make(gpu, "mxfp4", 20, 16, 2, 128, seed=1)
+    q = torch.randn(1, 8, 128, generator=torch.Generator().manual_seed(3)).to(BF16).to(gpu)
+    batch = batch_for(gpu, tables, lens, [1], cache, heads=8)
+    own = ops.DedicatedStream(gpu)
+    own.stream.wait_stream(torch.cuda.current_stream())
+    out = ops.quant_attend(cache, batch, q, stream=own.stream)
+    got, _ = ops.quant_read(cache, batch, dtype=F32, stream=own.stream)
+    own.stream.synchronize()
+    check_attend(out, k, v, tables, lens, [1], q, 16, BF16)
+    assert torch.equal(got.cpu(), k.get(*ref.places(tables[0], 16, range(300))).float())
+    own.close()
+    batch.update(tables, lens, [1])             # behind calls on a stream that is gone
+    assert torch.equal(ops.quant_attend(cache, batch, q), out)
+    home = ops.DedicatedStream(gpu)
+    home.stream.wait_stream(torch.cuda.current_stream())
+    batch = batch_for(gpu, tables, lens, [1], cache, heads=8, stream=home.stream)
+    home.close()
+    assert torch.equal(ops.quant_attend(cache, batch, q), out)
+    batch.update(tables, lens, [1])
+    assert torch.equal(ops.quant_attend(cache, batch, q), out)
+    del batch
+    torch.cuda.synchronize()
+
+
+def test_the_general_path_gives_the_same(gpu, monkeypatch):
+    """Without the native argument readers."""
+    from aegaeon_amd import _lib
+
+    lens, new = [70, 33], [3, 1]
+    tables = tables_for(lens, 32, 8)
+    outs = []
+    for general in (False, True):
+        if general:
+            monkeypatch.setattr(_lib, "_hostargs", _lib._GeneralPath)
+        cache, _, _ = make(gpu, "mxfp8", 8, 32, 2, 64, seed=4)
+        batch = batch_for(gpu, tables, lens, new, cache, heads=6)
+        gen = torch.Generator().manual_seed(3)
+        x, y = torch.randn(2, 4, 2, 64, generator=gen).to(F16).to(gpu)
+        q = torch.randn(4, 6, 64, generator=gen).to(F16).to(gpu)
+        ops.quant_write(cache, batch, x, y)
+        outs.append((cache.k_pages, cache.v_pages, ops.quant_attend(cache, batch, q),
+                     ops.quant_attend(cache, batch, q, scale=1), *ops.quant_read(cache, batch),
+                     *ops.quant_read(cache, batch, tokens="new", dtype=F32)))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
 def test_streams_other_than_the_batch_s_own(gpu):
     """Calls on several streams over one batch, updates between them, and the
     batch dropped while they run."""
