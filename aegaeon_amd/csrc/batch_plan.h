@@ -19,12 +19,10 @@ constexpr int kTile = 32;
 // query head kv_head * group + r % group. Attention takes rows by kind:
 //   kFew, kMore: up to 16 (32) rows of a sequence; the four waves of a workgroup
 //                take an item's tiles in turn and join at its end;
-//   kMany:       blocks of kManyRows rows, shared out to the waves;
-//   kWide:       as kFew, with the waves of a whole CU in one workgroup: few
-//                short sequences, whose tiles need no second launch to be joined.
-enum Kind { kFew = 0, kMore = 1, kMany = 2, kWide = 3, kKinds = 4 };
+//   kMany:       blocks of kManyRows rows, shared out to the waves.
+enum Kind { kFew = 0, kMore = 1, kMany = 2, kKinds = 3 };
 constexpr int kManyRows = 128;
-constexpr int kKindRows[kKinds] = {16, 32, kManyRows, 16};
+constexpr int kKindRows[kKinds] = {16, 32, kManyRows};
 
 struct Seq {
   int32_t len;         // positions in the cache, the new ones included

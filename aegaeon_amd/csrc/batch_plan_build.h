@@ -17,15 +17,21 @@ namespace aegkv_batch {
 // Positions are 32-bit in the kernels, with room for a tile behind the last.
 constexpr int64_t kMostTokens = (int64_t(1) << 31) - 1024;
 
+// Cutting rows over workgroups. Whole rows, the longest first, where the chip is
+// evenly full of them (48 sequences of 40 heads: 119 us cut at every 1/1024 of the
+// tiles, 104 whole); else the cut whose estimated time is least. Equal shares of the
+// flattened tiles, a workgroup going from one sequence's end to the next one's
+// beginning, were slower than items of unequal size with one workgroup each (64
+// requests: 72-80 us, 64), and so was one workgroup of 16 waves a head for few short
+// sequences (1,025 tokens: 12.6 us, 10.3 cut and joined; 4,096: 25, 10.4).
+//
 // How many workgroups of a kind the chip holds at once (at 128-wide heads).
-constexpr int64_t kHeld[kKinds] = {768, 512, 512, 256};
+constexpr int64_t kHeld[kKinds] = {768, 512, 512};
 // What a workgroup takes before and behind its tiles, and what joining cut rows
 // takes, in the time of a tile.
-constexpr int64_t kEnds[kKinds] = {8, 8, 8, 8}, kJoin[kKinds] = {8, 8, 8, 0};
+constexpr int64_t kEnds[kKinds] = {8, 8, 8}, kJoin[kKinds] = {8, 8, 8};
 // The most items that rows are cut into, beyond one for each.
-constexpr int64_t kCuts[kKinds] = {3072, 2048, 2048, 0};
-// kWide takes up to a workgroup a CU, of sequences up to this many tiles.
-constexpr int64_t kWideGroups = 256, kWideTiles = 128;
+constexpr int64_t kCuts[kKinds] = {3072, 2048, 2048};
 
 struct Batch {
   int64_t num_seqs;
@@ -50,15 +56,15 @@ struct Rows {
   int32_t first_tiles, window_tile, tiles;
 };
 
-inline int kind_of(int64_t rows, bool wide) {
-  return rows <= kKindRows[kFew] ? (wide ? kWide : kFew) : rows <= kKindRows[kMore] ? kMore : kMany;
+inline int kind_of(int64_t rows) {
+  return rows <= kKindRows[kFew] ? kFew : rows <= kKindRows[kMore] ? kMore : kMany;
 }
 
-inline void rows_of(const Header& h, const Batch& b, bool wide, std::vector<Rows>* out) {
+inline void rows_of(const Header& h, const Batch& b, std::vector<Rows>* out) {
   for (int64_t s = 0; s < b.num_seqs; ++s) {
     const int64_t rows = b.fresh[s] * h.group;
     if (!rows) continue;
-    const int kind = kind_of(rows, wide);
+    const int kind = kind_of(rows);
     for (int64_t row = 0; row < rows; row += kKindRows[kind]) {
       const int64_t n = std::min<int64_t>(kKindRows[kind], rows - row);
       const int64_t base = b.lens[s] - b.fresh[s];
@@ -121,7 +127,7 @@ inline int64_t share_out(const std::vector<Rows>& rows, int64_t kv_heads, int ki
     longest = std::max<int64_t>(longest, r.tiles);
   }
   const int64_t count = static_cast<int64_t>(rows.size()) * kv_heads;
-  if (kind == kWide || count >= 8 * kHeld[kind]) return longest;
+  if (count >= 8 * kHeld[kind]) return longest;
   int64_t best = longest, least = time_of(rows, kv_heads, kind, longest);
   for (int64_t eighths = 8; eighths >= 1; --eighths) {
     const int64_t each = std::max<int64_t>(4, up(total * eighths, 8 * kHeld[kind]));
@@ -347,29 +353,15 @@ inline void make_room(Header& h, const Batch& b, const std::vector<Rows>* rows, 
       const int64_t most = (kind == kMany ? r.tokens * h.group / kManyRows + r.seqs : r.seqs) *
                            h.kv_heads;
       r.items[kind] = most + kCuts[kind];
-      if (kind != kWide) {
-        // row by row where one has more than kMergeRows parts
-        const int64_t many = std::min(most, r.items[kind] / (kMergeRows + 1));
-        r.slots[kind] = r.items[kind];
-        r.merges += most * up(kKindRows[kind], kMergeRows) + many * kKindRows[kind];
-      }
+      // row by row where one has more than kMergeRows parts
+      const int64_t many = std::min(most, r.items[kind] / (kMergeRows + 1));
+      r.slots[kind] = r.items[kind];
+      r.merges += most * up(kKindRows[kind], kMergeRows) + many * kKindRows[kind];
     }
     r.at_items[kind] = take(r.items[kind] * static_cast<int64_t>(sizeof(Item)));
   }
   r.at_merges = take(r.merges * static_cast<int64_t>(sizeof(Merge)));
   r.bytes = at;
-}
-
-// Whether the rows of few new tokens go to kWide: fixed when the plan is made.
-inline bool wide(const Header& h, const Batch& b, int64_t max_seqs, int64_t max_columns) {
-  int64_t seqs = 0, longest = max_columns * h.block_size;
-  for (int64_t s = 0; s < b.num_seqs; ++s) {
-    if (b.fresh[s] * h.group > kKindRows[kWide] || !b.fresh[s]) continue;
-    ++seqs;
-    longest = std::max(longest, b.lens[s]);
-  }
-  const int64_t tiles = up(longest, kTile);
-  return std::max(seqs, max_seqs) * h.kv_heads <= kWideGroups && tiles <= kWideTiles;
 }
 
 inline int describe(Header& h, int64_t num_blocks, int32_t block_size, int32_t kv_heads,

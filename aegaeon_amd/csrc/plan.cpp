@@ -162,9 +162,9 @@ int aegkv_batch_plan(int64_t num_seqs, const int64_t* column_offsets, const int6
           was.sinks != h.sinks)
         return plan_fail(AEGKV_EINVAL, "an update keeps the blocks, heads, window and sinks");
       h.room = was.room;
-      rows_of(h, b, h.room.items[kWide] > 0, rows);
+      rows_of(h, b, rows);
     } else {
-      rows_of(h, b, wide(h, b, max_seqs, max_columns), rows);
+      rows_of(h, b, rows);
       make_room(h, b, rows, max_seqs, max_columns, max_tokens);
       *plan_bytes = h.room.bytes;
       if (!plan) return 0;

@@ -268,6 +268,11 @@ struct SpanWalk {
   }
 };
 
+// Write: e = least power with max |x| <= largest * 2^e over a group of 32, codes
+// rne(x 2^-e). Bound by HBM: 12,300 prompt tokens of 40 heads, 128 wide, bfloat16
+// to mxfp4 (251 MB read, 66 written) take 62 us, 5.1 TB/s. Values come past the
+// caches (85 us when they went through), the heads of a span are neighbouring
+// workgroups; codes and scales stay in the L2, where attention looks for them next.
 template <int FMT, int D, typename T>
 __global__ __launch_bounds__(kSpanLanes) void quant_write_kernel(SpanArgs a) {
   using C = Chunk<FMT, D>;
@@ -306,6 +311,8 @@ __global__ __launch_bounds__(kSpanLanes) void quant_write_kernel(SpanArgs a) {
   }
 }
 
+// Read: x = code * 2^(byte - 127), rounded once. Bound by HBM: the same tokens
+// back take 50 us (6.3 TB/s), 24 contexts of 8 heads (552 MB) 99 us (5.6 TB/s).
 template <int FMT, int D, typename T>
 __global__ __launch_bounds__(kSpanLanes) void quant_read_kernel(SpanArgs a) {
   using C = Chunk<FMT, D>;
@@ -718,14 +725,12 @@ constexpr int kAttendLanes = 256, kAttendWaves = 4;
 
 // Waves a SIMD has to hold: what the registers allow where 16 rows' sums and two
 // tiles of codes take few of them.
-template <int FMT, int D, int R>
+template <int D, int R>
 constexpr int kAttendPerSimd = D <= 128 && R == 1 ? 3 : D <= 128 ? 2 : 1;
 // Tiles on their way. Two, at three waves a SIMD, where the registers hold them:
 // with one, at four waves, 48 sequences of 40 heads took 110 us instead of 100.
-template <int FMT, int D, int R, int WAVES>
-constexpr int kTilesAhead = R == 1 && WAVES == 4 && D <= 128 ? 2 : 1;
-template <int FMT, int D>
-constexpr int kWideWaves = D * Format<FMT>::kBits <= 512 ? 16 : 8;
+template <int D, int R>
+constexpr int kTilesAhead = R == 1 && D <= 128 ? 2 : 1;
 
 // Where a row's result begins.
 template <typename T, typename P>
@@ -735,16 +740,27 @@ __device__ __forceinline__ T* result_row(ColdArgs args, P it, int32_t row) {
          (int64_t(it->kv_head) * group + (row - token * group)) * args->out.head;
 }
 
-// Where a workgroup's waves join: four of them at a time.
-template <int D, int R, int WAVES>
+// Single tokens and short runs: S^T = K Q^T and O^T = V^T P^T over tiles of 32
+// tokens, one pass, with each row's reference score and sum kept as the tiles go by.
+// With the tokens along the matrix rows of the first product, its result is the
+// second one's operand as it lies in the registers, and a row's state is its
+// lane's. Codes become operands in registers (64 conversions and 32 permutes a
+// tile of 128-wide heads in mxfp4); the rows of all query heads of a KV head share them.
+// Bound by HBM: 64 requests of 8 KV heads (278 MB) take 54 us and their parts 5 to
+// join, 4.8 TB/s in all; 48 of 40 heads (536 MB, none cut) 95 us, 5.7 TB/s. What is
+// missing to the copy rate of 6.5 is the ends of items (read, join) and the
+// scattered kilobyte a block and head.
+
+// Where a workgroup's waves join, a row tile at a time.
+template <int D, int R>
 struct Joined {
-  float part[4][16][D + 4];
-  float top[WAVES][16 * R], sum[WAVES][16 * R];
+  float part[kAttendWaves][16][D + 4];
+  float top[kAttendWaves][16 * R], sum[kAttendWaves][16 * R];
 };
 
-template <int FMT, int D, typename T, int R, int WAVES>
+template <int FMT, int D, typename T, int R>
 __device__ __forceinline__ void attend_item(const Scope& a, ItemPtr it,
-                                            Joined<D, R, WAVES>& share) {
+                                            Joined<D, R>& share) {
   typedef typename Operand<T>::v8 v8;
   constexpr int kSteps = D / 32;    // matrix steps along the head
   constexpr int kOut = D / 16;      // output tiles of 16 values
@@ -780,18 +796,18 @@ __device__ __forceinline__ void attend_item(const Scope& a, ItemPtr it,
       t.k[i].load(h[i], a.block_shift, m, g);
     }
   };
-  constexpr int kAhead = kTilesAhead<FMT, D, R, WAVES>;
+  constexpr int kAhead = kTilesAhead<D, R>;
   Tile held[kAhead];
   int32_t at = it->tile + wave;
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) {
-    if (at + i * WAVES < tiles.end) {
+    if (at + i * kAttendWaves < tiles.end) {
       Half h[2];
-      load_k(held[i], find(at + i * WAVES), h);
+      load_k(held[i], find(at + i * kAttendWaves), h);
       held[i].v.load(h, a.block_shift, m, g, 0);
     }
   }
-  Blocks ahead = find(at + kAhead * WAVES);
+  Blocks ahead = find(at + kAhead * kAttendWaves);
 
   v8 q[R][kSteps];
   int32_t position[R];
@@ -816,7 +832,7 @@ __device__ __forceinline__ void attend_item(const Scope& a, ItemPtr it,
 
   const auto step = [&](Tile& t) {
     const int32_t begin = tiles.at(at) * kTile;
-    const bool more = at + kAhead * WAVES < tiles.end;
+    const bool more = at + kAhead * kAttendWaves < tiles.end;
 
     // scores: lane holds row m, tokens 4g + i of both halves
     f32x4 x[R][2];
@@ -833,7 +849,7 @@ __device__ __forceinline__ void attend_item(const Scope& a, ItemPtr it,
     }
     Half h[2];
     if (more) load_k(t, ahead, h);
-    ahead = find(at + (kAhead + 1) * WAVES);
+    ahead = find(at + (kAhead + 1) * kAttendWaves);
 
     // Tokens that some row does not see. All by selection: with branches around
     // the changed elements the compiler lost one of the changes (the first
@@ -876,7 +892,7 @@ __device__ __forceinline__ void attend_item(const Scope& a, ItemPtr it,
       }
     });
     if (more) t.v.load(h, a.block_shift, m, g, 0);
-    at += WAVES;
+    at += kAttendWaves;
   };
   while (at < tiles.end) {
     step(held[0]);
@@ -886,8 +902,7 @@ __device__ __forceinline__ void attend_item(const Scope& a, ItemPtr it,
     }
   }
 
-  // join the waves, four at a time: each scales its part to the largest of
-  // their scores
+  // join the waves: each scales its part to the largest of their scores
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const float s = state[r].sum[0];
@@ -899,40 +914,35 @@ __device__ __forceinline__ void attend_item(const Scope& a, ItemPtr it,
   __syncthreads();
   const ColdArgs end_args = cold_args();
   const ItemPtr ended = anew(it);
-  constexpr int kRowLanes = WAVES * 4, kEach = D / kRowLanes;   // of a row, values of each
+  constexpr int kRowLanes = 16, kEach = D / kRowLanes;   // of a row, values of each
   const int row = threadIdx.x / kRowLanes, part = threadIdx.x % kRowLanes;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     float most = share.top[0][16 * r + m];
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) most = fmaxf(most, share.top[w][16 * r + m]);
+    for (int w = 1; w < kAttendWaves; ++w) most = fmaxf(most, share.top[w][16 * r + m]);
     const float top = state[r].top;
     const float fade = top == most ? 1.f : __builtin_amdgcn_exp2f((top - most) * a.c);
     float y[kEach] = {};
 #pragma unroll
-    for (int four = 0; four < WAVES; four += 4) {
-      if (wave / 4 == four / 4) {
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+      for (int d = 0; d < kOut; ++d)
+        share.part[wave][m][(D / 16) * (4 * g + i) + d] =
+            unless_poisoned<D>(o[r][d][i] * fade, poison, r, i);
+    __syncthreads();
 #pragma unroll
-          for (int d = 0; d < kOut; ++d)
-            share.part[wave % 4][m][(D / 16) * (4 * g + i) + d] =
-                unless_poisoned<D>(o[r][d][i] * fade, poison, r, i);
-      }
-      __syncthreads();
+    for (int i = 0; i < kEach; ++i) {
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) y[i] += share.part[w][row][part * kEach + i];
-      }
-      __syncthreads();
+      for (int w = 0; w < kAttendWaves; ++w) y[i] += share.part[w][row][part * kEach + i];
     }
+    if (r + 1 < R) __syncthreads();   // before the next row tile's parts
     if (16 * r + row < ended->rows) {
       float all = share.top[0][16 * r + row], total = 0.f;
 #pragma unroll
-      for (int w = 1; w < WAVES; ++w) all = fmaxf(all, share.top[w][16 * r + row]);
+      for (int w = 1; w < kAttendWaves; ++w) all = fmaxf(all, share.top[w][16 * r + row]);
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) {
+      for (int w = 0; w < kAttendWaves; ++w) {
         const float t = share.top[w][16 * r + row];
         total += share.sum[w][16 * r + row] *
                  (t == all ? 1.f : __builtin_amdgcn_exp2f((t - all) * a.c));
@@ -955,22 +965,27 @@ __device__ __forceinline__ void attend_item(const Scope& a, ItemPtr it,
   }
 }
 
-template <int FMT, int D, typename T, int R, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, (WAVES > 4 ? WAVES / 4 : kAttendPerSimd<FMT, D, R>)) void
-quant_attend_kernel(AttendArgs args) {
-  __shared__ Joined<D, R, WAVES> joined;
+template <int FMT, int D, typename T, int R>
+__global__ __launch_bounds__(kAttendLanes, (kAttendPerSimd<D, R>)) void quant_attend_kernel(
+    AttendArgs args) {
+  __shared__ Joined<D, R> joined;
   const Scope scope = args.scope;
   const ItemPtr it = in_plan<Item>(args.plan, args.at_items) + blockIdx.x;
   if (static_cast<int32_t>(blockIdx.x) >= in_plan<Header>(args.plan, 0)->items[args.kind]) return;
-  attend_item<FMT, D, T, R, WAVES>(scope, it, joined);
+  attend_item<FMT, D, T, R>(scope, it, joined);
 }
 
-// Prompts: 128 rows a workgroup, 32 a wave. The cache's tokens become matrix
+// Prompts, as the above: 128 rows a workgroup, 32 a wave. The cache's tokens become matrix
 // operands once for all of them: a stage of 64 tokens, each wave making a quarter
 // of K's operands and of V's, is laid in shared memory lane by lane as the matrix
 // instructions take them, so that reads and writes are whole and without
 // conflicts. Two stages: while one is multiplied, the next one's bytes are on their
-// way in registers, and one barrier a stage is enough.
+// way in registers, and one barrier a stage is enough. Four prompts of 1,000 to
+// 4,096 tokens, 32 heads over 8 (158 GFLOP) take 218-230 us, 690-725 TFLOP/s; converted
+// by every wave for itself, 321. Bound by the issue of two waves a SIMD: 29 % of
+// the cycles multiply, 38 % are vector instructions (an exponential, 16
+// cycles, for each score); reading operands earlier, waiting for loads elsewhere,
+// wave priorities and 3 instead of 2 tiles on their way changed less than 3 %.
 constexpr int kStageTiles = 2, kWaveRows = 32;
 static_assert(kManyRows == kAttendWaves * kWaveRows, "rows of a workgroup");
 
@@ -1177,6 +1192,8 @@ __global__ __launch_bounds__(kAttendLanes, D == 256 ? 1 : 2) void quant_prompt_k
 // score of all, over the sum of their sums. A workgroup's lanes are groups of D / 4,
 // four values a lane. Of up to kMergeRows parts each group takes rows of its own;
 // more (few rows over a long axis) are shared out to the groups, one row a workgroup.
+// 5 us, most of it the launch and two dependent reads; when one lane a value
+// walked all parts, 128 parts of 56 rows took 54.
 template <int D, typename T>
 __global__ __launch_bounds__(256) void quant_merge_kernel(AttendArgs a) {
   constexpr int kLanes = D / 4, kSides = 256 / kLanes;

@@ -318,7 +318,7 @@ int aegkv_quant_attend(const void* plan, const void* device_plan, int format, in
   a.scope.window = h.window ? h.window : INT32_MAX;
   a.scope.sinks = h.sinks;
   rc = check_grid(h.room.merges, 256);
-  for (int kind = 0; kind < kKinds && !rc; ++kind) rc = check_grid(h.room.items[kind], 1024);
+  for (int kind = 0; kind < kKinds && !rc; ++kind) rc = check_grid(h.room.items[kind], kAttendLanes);
   if (rc) return rc;
   return by_shape(format, head_dim, [&](auto fmt, auto d) {
     constexpr int kFormat = decltype(fmt)::value, kDim = decltype(d)::value;
@@ -331,13 +331,10 @@ int aegkv_quant_attend(const void* plan, const void* device_plan, int format, in
         a.work = a.work_base + a.kind_work[kind];
         a.slot_floats = a.kind_slot_floats[kind];
         const dim3 grid(static_cast<uint32_t>(h.room.items[kind]));
-        constexpr int kWaves = kWideWaves<kFormat, kDim>;
         if (kind == kFew)
-          quant_attend_kernel<kFormat, kDim, T, 1, 4><<<grid, 256, 0, stream>>>(a);
+          quant_attend_kernel<kFormat, kDim, T, 1><<<grid, kAttendLanes, 0, stream>>>(a);
         else if (kind == kMore)
-          quant_attend_kernel<kFormat, kDim, T, 2, 4><<<grid, 256, 0, stream>>>(a);
-        else if (kind == kWide)
-          quant_attend_kernel<kFormat, kDim, T, 1, kWaves><<<grid, kWaves * 64, 0, stream>>>(a);
+          quant_attend_kernel<kFormat, kDim, T, 2><<<grid, kAttendLanes, 0, stream>>>(a);
         else
           quant_prompt_kernel<kFormat, kDim, T><<<grid, kAttendLanes, 0, stream>>>(a);
         const int rc = launched("quant_attend_kernel launch");
