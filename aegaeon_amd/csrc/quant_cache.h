@@ -985,7 +985,7 @@ __global__ __launch_bounds__(kAttendLanes, (kAttendPerSimd<D, R>)) void quant_at
 // by every wave for itself, 321. Bound by the issue of two waves a SIMD: 29 % of
 // the cycles multiply, 38 % are vector instructions (an exponential, 16
 // cycles, for each score); reading operands earlier, waiting for loads elsewhere,
-// wave priorities and 3 instead of 2 tiles on their way changed less than 3 %.
+// loads without conditions and wave priorities changed less than 3 %.
 constexpr int kStageTiles = 2, kWaveRows = 32;
 static_assert(kManyRows == kAttendWaves * kWaveRows, "rows of a workgroup");
 
