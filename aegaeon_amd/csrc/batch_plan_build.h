@@ -31,7 +31,7 @@ constexpr int64_t kHeld[kKinds] = {768, 512, 512};
 // takes, in the time of a tile.
 constexpr int64_t kEnds[kKinds] = {8, 8, 8}, kJoin[kKinds] = {8, 8, 8};
 // The most items that rows are cut into, beyond one for each.
-constexpr int64_t kCuts[kKinds] = {3072, 2048, 2048};
+constexpr int64_t kCuts[kKinds] = {4096, 2048, 2048};
 
 struct Batch {
   int64_t num_seqs;
@@ -127,7 +127,7 @@ inline int64_t share_out(const std::vector<Rows>& rows, int64_t kv_heads, int ki
     longest = std::max<int64_t>(longest, r.tiles);
   }
   const int64_t count = static_cast<int64_t>(rows.size()) * kv_heads;
-  if (count >= 8 * kHeld[kind]) return longest;
+  if (count >= 8 * kHeld[kind] && longest * kHeld[kind] <= total) return longest;
   int64_t best = longest, least = time_of(rows, kv_heads, kind, longest);
   for (int64_t eighths = 8; eighths >= 1; --eighths) {
     const int64_t each = std::max<int64_t>(4, up(total * eighths, 8 * kHeld[kind]));

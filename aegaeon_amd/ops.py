@@ -5,7 +5,9 @@
 and runs on the current stream like ops/swap.cu:21-32. `swap_segments` is the
 composite-page data plane of Worker.swap_blocks (aegaeon/worker.py:2265-2329)
 and `copy_blocks` the in-HBM block copy. Every call is one C-ABI call into
-libaegkv.so; there is no Python or CPU fallback.
+libaegkv.so; there is no Python or CPU fallback. `QuantCache`, `CacheBatch` and
+`quant_write`, `quant_read`, `quant_attend` hold a cache in 4 or 8 bits, which the
+moves take like any other; the reference has none.
 """
 
 from __future__ import annotations

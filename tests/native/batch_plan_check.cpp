@@ -181,7 +181,33 @@ static void check_plan(const Made& m, const std::vector<char>& buf, int bs, int 
   REQUIRE(rows_found == want_rows * kv);
 }
 
+// One long sequence among many short ones is cut, however many those are.
+static void check_long_among_short() {
+  Made m;
+  for (int s = 0; s < 3000; ++s) {
+    const int64_t len = s == 1234 ? 100000 : 40;
+    for (int64_t c = 0; c < (len + 15) / 16; ++c) m.ids.push_back(static_cast<int64_t>(m.ids.size()));
+    m.offsets.push_back(static_cast<int64_t>(m.ids.size()));
+    m.lens.push_back(len);
+    m.fresh.push_back(1);
+  }
+  const int64_t room[3] = {0, 0, 0};
+  std::vector<char> buf;
+  REQUIRE(plan_of(m, 1 << 20, 16, 4, 16, 0, 0, room, &buf, 0) == 0);
+  check_plan(m, buf, 16, 4, 16, 0, 0);
+  Header h;
+  std::memcpy(&h, buf.data(), sizeof h);
+  int32_t longest = 0;
+  for (int i = 0; i < h.items[kFew]; ++i) {
+    Item it;
+    std::memcpy(&it, buf.data() + h.room.at_items[kFew] + i * sizeof(Item), sizeof it);
+    longest = std::max(longest, it.tile_end - it.tile);
+  }
+  REQUIRE(longest <= 400);   // of 3125 tiles
+}
+
 int main() {
+  check_long_among_short();
   int updates = 0;
   for (int round = 0; round < 400; ++round) {
     const int sizes[] = {16, 32, 64, 128};

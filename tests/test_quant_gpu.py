@@ -594,6 +594,38 @@ def test_a_cache_is_written_attended_moved_and_attended_again(gpu):
     pool.free()
 
 
+def test_partial_pages_of_kernel_blocks(gpu):
+    """Manager pages of two kernel blocks: the batch names kernel blocks, the
+    swap moves the live ones of a page."""
+    from aegaeon_amd.cache_groups import CacheGroupRuntimeConfig
+
+    group = CacheGroupRuntimeConfig("attention", 32, 16)
+    pages, heads, d, length = 10, 2, 128, 75        # pages of 32: two whole, one by 11 tokens
+    cache, k, v = make(gpu, "mxfp4", 2 * pages, 16, heads, d, seed=6)
+    page = 2 * cache.page_bytes
+    backing = [cache.k_pages.view(pages, page), cache.v_pages.view(pages, page)]
+    pool = ops.PinnedHostPool(6 * 2 * page)
+    layout = ops.SegmentLayout(backing, [page] * 2, [0, page], [1, 1], pages, [2], pool.tensor,
+                               2 * page, 0)
+    table, back = [7, 2, 5], [1, 9, 4]
+    q = torch.randn(1, 6, d, generator=torch.Generator().manual_seed(1)).to(BF16).to(gpu)
+
+    def attend(ids):
+        batch = batch_for(gpu, [group.to_kernel_block_ids(ids)], [length], [1], cache, heads=6)
+        return ops.quant_attend(cache, batch, q)
+
+    before = attend(table)
+    check_attend(before, k, v, [group.to_kernel_block_ids(table)], [length], [1], q, 16, BF16)
+    extents = ([0] * 3, [0] * 3, [2, 2, 1])
+    layout.swap(table, [3, 0, 4], *extents, False)
+    for t in backing:
+        t[table] = -1
+    layout.swap([3, 0, 4], back, *extents, True)
+    assert torch.equal(attend(back), before)
+    torch.cuda.synchronize()
+    pool.free()
+
+
 def test_refusals_on_the_device(gpu):
     cache, _, _ = make(gpu, "mxfp4", 8, 16, 2, 128)
     batch = batch_for(gpu, [[0, 1]], [20], [2], cache, heads=4)
