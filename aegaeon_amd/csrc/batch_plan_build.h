@@ -84,8 +84,9 @@ inline void rows_of(const Header& h, const Batch& b, std::vector<Rows>* out) {
 }
 
 // The time when every row block's tiles are cut into equal parts of at most
-// `each`, and the next of the workgroups that the chip holds takes the longest one left. The KV
-// heads are alike: one of them, on its share of the chip, stands for all.
+// `each`, and the next of the workgroups that the chip holds takes the longest
+// one left. The KV heads are alike: one of them, on its share of the chip,
+// stands for all.
 inline int64_t time_of(const std::vector<Rows>& rows, int64_t kv_heads, int kind, int64_t each) {
   std::vector<int64_t> sizes;
   bool cut = false;

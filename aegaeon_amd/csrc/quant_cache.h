@@ -138,7 +138,8 @@ __device__ __forceinline__ void load8(const T* p, bool whole_words, float* x) {
   if (whole_words) {
     v4u w[sizeof(T) / 2];
 #pragma unroll
-    for (unsigned i = 0; i < sizeof(T) / 2; ++i) w[i] = __builtin_nontemporal_load((const gv4u*)p + i);
+    for (unsigned i = 0; i < sizeof(T) / 2; ++i)
+      w[i] = __builtin_nontemporal_load((const gv4u*)p + i);
     __builtin_memcpy(t, w, sizeof t);
   } else {
 #pragma unroll
@@ -492,7 +493,8 @@ struct KPart {
     load_bytes<kWords * 4, STREAM>(code, h.k, m * Chunk<FMT, D>::kCode + g * (kWords * 4));
 #pragma unroll
     for (uint32_t i = 0; i < kScales; ++i)
-      load_bytes<1, STREAM>(&scale[i], h.k_scales, ((D == 64 ? g / 2 : g * kScales + i) << block_shift) + m);
+      load_bytes<1, STREAM>(&scale[i], h.k_scales,
+                            ((D == 64 ? g / 2 : g * kScales + i) << block_shift) + m);
   }
 
   // The matrix operand of step S: the lane's values 8 S .. 8 S + 7.
@@ -759,8 +761,7 @@ struct Joined {
 };
 
 template <int FMT, int D, typename T, int R>
-__device__ __forceinline__ void attend_item(const Scope& a, ItemPtr it,
-                                            Joined<D, R>& share) {
+__device__ __forceinline__ void attend_item(const Scope& a, ItemPtr it, Joined<D, R>& share) {
   typedef typename Operand<T>::v8 v8;
   constexpr int kSteps = D / 32;    // matrix steps along the head
   constexpr int kOut = D / 16;      // output tiles of 16 values

@@ -99,7 +99,8 @@ int check_values(const void* base, int64_t tokens, int32_t heads, int32_t head_d
       return fail(AEGKV_EOVERLAP, "%s: rows of %d values overlap at strides %lld and %lld", what,
                   head_dim, ll(token_stride), ll(head_stride));
   }
-  out->whole_words = aligned16(base) && (token_stride * es) % 16 == 0 && (head_stride * es) % 16 == 0;
+  out->whole_words =
+      aligned16(base) && (token_stride * es) % 16 == 0 && (head_stride * es) % 16 == 0;
   return check_device_range(base, static_cast<int64_t>(last) * es, what);
 }
 
@@ -170,8 +171,9 @@ int span_args(const QuantCall& c, bool fresh, SpanArgs* a, dim3* grid) {
   a->kv_heads = h.kv_heads;
   a->block_size = h.block_size;
   a->fresh = fresh;
-  a->heads_each = static_cast<int32_t>(
-      std::min<int64_t>(h.kv_heads, std::max<int64_t>(1, kSpanRows * spans / std::max<int64_t>(1, tokens))));
+  const int64_t heads = kSpanRows * spans / std::max<int64_t>(1, tokens);
+  a->heads_each =
+      static_cast<int32_t>(std::min<int64_t>(h.kv_heads, std::max<int64_t>(1, heads)));
   a->head_groups = (h.kv_heads + a->heads_each - 1) / a->heads_each;
   *grid = dim3(static_cast<uint32_t>(spans * a->head_groups), 2);
   return check_grid(spans * a->head_groups, kSpanLanes);
@@ -318,7 +320,8 @@ int aegkv_quant_attend(const void* plan, const void* device_plan, int format, in
   a.scope.window = h.window ? h.window : INT32_MAX;
   a.scope.sinks = h.sinks;
   rc = check_grid(h.room.merges, 256);
-  for (int kind = 0; kind < kKinds && !rc; ++kind) rc = check_grid(h.room.items[kind], kAttendLanes);
+  for (int kind = 0; kind < kKinds && !rc; ++kind)
+    rc = check_grid(h.room.items[kind], kAttendLanes);
   if (rc) return rc;
   return by_shape(format, head_dim, [&](auto fmt, auto d) {
     constexpr int kFormat = decltype(fmt)::value, kDim = decltype(d)::value;

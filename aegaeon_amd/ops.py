@@ -1170,8 +1170,8 @@ def _alive(stream: torch.cuda.Stream) -> bool:
 
 def _quant_call(cache: QuantCache, batch: CacheBatch):
     if (batch.block_size, batch.kv_heads) != (cache.block_size, cache.kv_heads):
-        raise ValueError(f"a batch of {batch.block_size}-token blocks and {batch.kv_heads} KV heads "
-                         f"over a cache of {cache.block_size} and {cache.kv_heads}")
+        raise ValueError(f"a batch of {batch.block_size}-token blocks and {batch.kv_heads} KV "
+                         f"heads over a cache of {cache.block_size} and {cache.kv_heads}")
     if batch.num_blocks > cache.num_blocks:
         raise ValueError(f"a batch over {batch.num_blocks} blocks, a cache of {cache.num_blocks}")
     if batch.device != cache.device:

@@ -186,7 +186,8 @@ static void check_long_among_short() {
   Made m;
   for (int s = 0; s < 3000; ++s) {
     const int64_t len = s == 1234 ? 100000 : 40;
-    for (int64_t c = 0; c < (len + 15) / 16; ++c) m.ids.push_back(static_cast<int64_t>(m.ids.size()));
+    for (int64_t c = 0; c < (len + 15) / 16; ++c)
+      m.ids.push_back(static_cast<int64_t>(m.ids.size()));
     m.offsets.push_back(static_cast<int64_t>(m.ids.size()));
     m.lens.push_back(len);
     m.fresh.push_back(1);
