@@ -57,7 +57,7 @@ struct Rows {
 };
 
 inline int kind_of(int64_t rows) {
-  return rows <= kKindRows[kFew] ? kFew : rows <= kKindRows[kMore] ? kMore : kMany;
+  return rows <= kKindRows[kFew] ? kFew : rows <= kMostMore ? kMore : kMany;
 }
 
 inline void rows_of(const Header& h, const Batch& b, std::vector<Rows>* out) {
@@ -267,7 +267,7 @@ inline int fill(Header& h, const Batch& b, const std::vector<Rows>* rows, char* 
     if (static_cast<int64_t>(all.size()) * h.kv_heads > room.items[kind])
       return aegkv_set_error(AEGKV_ENOMEM, "the plan has no room for sequences of this many new "
                              "tokens (%s rows under a KV head)",
-                             kind == kMany ? "over 32" : kind == kMore ? "17 to 32" : "up to 16");
+                             kind == kMany ? "over 64" : kind == kMore ? "17 to 64" : "up to 16");
     const int64_t each = share_out(all, h.kv_heads, kind, room.items[kind]);
     // the longest go first, so that the last to end are short
     std::vector<size_t> order(all.size());
@@ -351,7 +351,9 @@ inline void make_room(Header& h, const Batch& b, const std::vector<Rows>* rows, 
         r.merges += up(x.rows, parts <= kMergeRows ? kMergeRows : 1) * h.kv_heads;
       }
     } else if (count) {
-      const int64_t most = (kind == kMany ? r.tokens * h.group / kManyRows + r.seqs : r.seqs) *
+      const int64_t most = (kind == kMany   ? r.tokens * h.group / kManyRows + r.seqs
+                            : kind == kMore ? r.seqs * (kMostMore / kKindRows[kMore])
+                                            : r.seqs) *
                            h.kv_heads;
       r.items[kind] = most + kCuts[kind];
       // row by row where one has more than kMergeRows parts

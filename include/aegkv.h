@@ -556,7 +556,7 @@ int aegkv_quant_page_bytes(int format, int32_t block_size, int32_t kv_heads, int
  * calls that use what it held, and calls captured into a graph then work on the
  * new batch when they are replayed. A plan with room takes sequences with as
  * many rows (new tokens times query heads of a KV head) as the batch it was
- * made for had: up to 16, up to 32, more.
+ * made for had: up to 16, up to 64, more.
  */
 int aegkv_batch_plan(int64_t num_seqs, const int64_t* column_offsets, const int64_t* block_ids,
                      const int64_t* seq_lens, const int64_t* new_lens, int64_t num_blocks,
