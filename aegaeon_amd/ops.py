@@ -1057,12 +1057,14 @@ class CacheBatch:
                                                                 ctypes.byref(n)))
             self._workspace[d] = int(n.value)
         self._used: dict = {}     # raw stream -> stream of calls made elsewhere than at home
+        self._home = None
         with torch.cuda.device(self.device):
             st = stream if stream is not None else torch.cuda.current_stream()
             if torch.cuda.is_current_stream_capturing():
                 raise ValueError("a batch cannot be made while a stream is captured")
             with torch.cuda.stream(st):
                 self._plan = torch.empty(self._host.size, dtype=torch.uint8, device=self.device)
+                self._pool = st     # whose memory pool the plan goes back to
                 self._upload(st)
 
     def _make(self, block_tables, seq_lens, new_lens, update: int) -> None:
@@ -1145,27 +1147,43 @@ class CacheBatch:
             self._used[st.cuda_stream] = st
 
     def __del__(self, _finalizing=sys.is_finalizing):
-        # the plan's memory goes back to its home stream's pool: behind the calls
-        # on other streams that read it. (Not Tensor.record_stream, which records
+        # The plan's memory goes back to the pool of the stream it was made on,
+        # wherever updates have moved the batch since: that stream waits for the
+        # calls on all others that read it. (Not Tensor.record_stream, which records
         # an event on them when the memory goes, when they may be closed.)
-        if _finalizing() or not getattr(self, "_used", None):
+        if _finalizing() or getattr(self, "_home", None) is None:
             return
         try:
-            for st in self._used.values():
-                if not _alive(st):
-                    continue
-                if _alive(self._home):
-                    self._home.wait_event(st.record_event())
+            pool = self._pool
+            raw = pool.cuda_stream if _alive(pool) else None
+            others = [st for st in (self._home, *self._used.values())
+                      if _alive(st) and st.cuda_stream != raw]
+            if not others:
+                return
+            if any(_capturing(st) for st in (*others, *((pool,) if raw is not None else ()))):
+                _kept.append(self._plan)    # no stream may wait for a captured one
+                return
+            for st in others:
+                if raw is not None:
+                    pool.wait_event(st.record_event())
                 else:
                     st.synchronize()
         except Exception:
-            pass
+            _kept.append(self._plan)
+
+
+_kept: list = []    # plans that no stream could be ordered behind: never reused
 
 
 def _alive(stream: torch.cuda.Stream) -> bool:
     """Whether a stream may still be handed to the runtime (a closed dedicated
     stream, whose work was waited for, may not)."""
     return not getattr(stream, "closed", False)
+
+
+def _capturing(stream: torch.cuda.Stream) -> bool:
+    with torch.cuda.stream(stream):
+        return torch.cuda.is_current_stream_capturing()
 
 
 def _quant_call(cache: QuantCache, batch: CacheBatch):

@@ -151,6 +151,58 @@ def test_python_refuses_what_it_cannot_take(aegkv_lib):
         ops.QuantCache(page, page, kv_heads=1, head_dim=128, block_size=16)
 
 
+class Recorded:
+    """A stream that notes what it is asked for."""
+
+    def __init__(self, raw, closed=False):
+        self.cuda_stream, self.closed = raw, closed
+        self.waits, self.synchronized = [], 0
+
+    def record_event(self):
+        return self
+
+    def wait_event(self, event):
+        self.waits.append(event)
+
+    def synchronize(self):
+        self.synchronized += 1
+
+
+def dropped(monkeypatch, pool, home, used=(), capturing=()):
+    """Drop a batch made on `pool`, updated to `home`, with calls on `used`."""
+    monkeypatch.setattr(ops, "_capturing", lambda st: st in capturing, raising=False)
+    monkeypatch.setattr(ops, "_kept", [], raising=False)
+    batch = ops.CacheBatch.__new__(ops.CacheBatch)
+    batch._plan, batch._pool, batch._home = object(), pool, home
+    batch._used = {st.cuda_stream: st for st in used}
+    plan = batch._plan
+    del batch
+    return plan in ops._kept
+
+
+def test_a_plan_s_memory_goes_back_behind_all_that_read_it(monkeypatch):
+    """The memory is the pool's of the stream a batch was made on, also when an
+    update has made another one its home."""
+    a, b, c = (Recorded(i) for i in range(3))
+    assert not dropped(monkeypatch, a, a) and not a.waits
+    assert not dropped(monkeypatch, a, b) and a.waits == [b]
+    a.waits.clear()
+    assert not dropped(monkeypatch, a, b, [c, a]) and a.waits == [b, c] and not b.waits
+    a.waits.clear()
+    assert not dropped(monkeypatch, a, a, [c]) and a.waits == [c]
+    gone = Recorded(7, closed=True)         # its work was waited for
+    assert not dropped(monkeypatch, gone, b, [c])
+    assert b.synchronized == 1 and c.synchronized == 1
+    a.waits.clear()
+    assert not dropped(monkeypatch, a, gone, [c]) and a.waits == [c]
+    # what cannot be ordered is not given back
+    a.waits.clear()
+    assert dropped(monkeypatch, a, b, capturing=[b]) and not a.waits
+    assert dropped(monkeypatch, a, b, capturing=[a]) and not a.waits
+    b.record_event = lambda: 1 / 0
+    assert dropped(monkeypatch, a, b)
+
+
 @pytest.mark.parametrize("fmt", ["mxfp4", "mxfp8"])
 def test_the_reference_s_own_rounding(fmt):
     """Every code is read as it was written; the largest value of a group is

@@ -543,6 +543,33 @@ def test_streams_other_than_the_batch_s_own(gpu):
         check_attend(out, k, v, at, n, [1, 1], q, 16, BF16)
 
 
+def test_a_dropped_batch_s_memory_waits_for_the_stream_it_moved_to(gpu):
+    """The stream that a batch was made on, whose allocations may take the plan's
+    memory next, is behind the calls on the stream it was updated to."""
+    lens = [300]
+    tables = tables_for(lens, 16, 20)
+    cache, k, v = make(gpu, "mxfp4", 20, 16, 2, 128, seed=1)
+    q = torch.randn(1, 8, 128, generator=torch.Generator().manual_seed(3)).to(BF16).to(gpu)
+    made, moved = torch.cuda.Stream(), torch.cuda.Stream()
+    for calls_elsewhere in (False, True):
+        torch.cuda.synchronize()
+        batch = batch_for(gpu, tables, lens, [1], cache, heads=8, stream=made)
+        batch.update(tables, lens, [1], stream=moved)
+        with torch.cuda.stream(moved):
+            if calls_elsewhere:
+                outs = [ops.quant_attend(cache, batch, q, stream=torch.cuda.default_stream())]
+            torch.cuda._sleep(1 << 29)      # a good fraction of a second
+            out = ops.quant_attend(cache, batch, q)
+        del batch
+        behind = made.record_event()
+        assert not behind.query()
+        behind.synchronize()
+        assert moved.query()
+        check_attend(out, k, v, tables, lens, [1], q, 16, BF16)
+        if calls_elsewhere:
+            assert torch.equal(outs[0], out)
+
+
 def test_a_cache_is_written_attended_moved_and_attended_again(gpu):
     """One model step after another as a serving engine makes them: two layers
     over a composite cache, a prompt, decode steps, a swap to the host and back to other
