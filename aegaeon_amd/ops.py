@@ -1058,6 +1058,7 @@ class CacheBatch:
             self._workspace[d] = int(n.value)
         self._used: dict = {}     # raw stream -> stream of calls made elsewhere than at home
         self._home = None
+        _require_stream(self.device, stream)
         with torch.cuda.device(self.device):
             st = stream if stream is not None else torch.cuda.current_stream()
             if torch.cuda.is_current_stream_capturing():
@@ -1116,6 +1117,7 @@ class CacheBatch:
         is enqueued on `stream` (default: the current one) behind every call
         made over this batch; a graph that holds such calls is replayed on that
         stream, or ordered before and behind it by the caller."""
+        _require_stream(self.device, stream)
         with torch.cuda.device(self.device):
             st = stream if stream is not None else torch.cuda.current_stream()
             with torch.cuda.stream(st):
@@ -1181,12 +1183,17 @@ def _alive(stream: torch.cuda.Stream) -> bool:
     return not getattr(stream, "closed", False)
 
 
+def _require_stream(device: torch.device, stream: torch.cuda.Stream | None) -> None:
+    if stream is not None and stream.device != device:
+        raise ValueError(f"a stream of {stream.device} for work on {device}")
+
+
 def _capturing(stream: torch.cuda.Stream) -> bool:
     with torch.cuda.stream(stream):
         return torch.cuda.is_current_stream_capturing()
 
 
-def _quant_call(cache: QuantCache, batch: CacheBatch):
+def _quant_call(cache: QuantCache, batch: CacheBatch, stream: torch.cuda.Stream | None):
     if (batch.block_size, batch.kv_heads) != (cache.block_size, cache.kv_heads):
         raise ValueError(f"a batch of {batch.block_size}-token blocks and {batch.kv_heads} KV "
                          f"heads over a cache of {cache.block_size} and {cache.kv_heads}")
@@ -1194,6 +1201,7 @@ def _quant_call(cache: QuantCache, batch: CacheBatch):
         raise ValueError(f"a batch over {batch.num_blocks} blocks, a cache of {cache.num_blocks}")
     if batch.device != cache.device:
         raise ValueError(f"a batch on {batch.device}, a cache on {cache.device}")
+    _require_stream(cache.device, stream)
 
 
 def _here(cache: QuantCache) -> tuple:
@@ -1249,7 +1257,7 @@ def quant_write(cache: QuantCache, batch: CacheBatch, k: torch.Tensor, v: torch.
     if stream is None and _lib.hostargs().quant_write(
             cache._packed, batch._packed, k, v, *_here(cache)) is not None:
         return
-    _quant_call(cache, batch)
+    _quant_call(cache, batch, stream)
     kp = _rows_arg(k, "k", cache.kv_heads, cache, _DTYPES)
     vp = _rows_arg(v, "v", cache.kv_heads, cache, _DTYPES)
     if k.dtype != v.dtype or k.size(0) != v.size(0):
@@ -1277,7 +1285,7 @@ def quant_read(cache: QuantCache, batch: CacheBatch, *, tokens: str = "all",
                                           *_here(cache))
         if done is not None:
             return done
-    _quant_call(cache, batch)
+    _quant_call(cache, batch, stream)
     n = batch.read_tokens if tokens == "all" else batch.num_tokens
     if out is None:
         if dtype not in _DTYPES:
@@ -1313,7 +1321,7 @@ def quant_attend(cache: QuantCache, batch: CacheBatch, q: torch.Tensor, *,
                                             *_here(cache))
         if done is not None:
             return done
-    _quant_call(cache, batch)
+    _quant_call(cache, batch, stream)
     qp = _rows_arg(q, "q", batch.heads, cache, (torch.bfloat16, torch.float16))
     if out is None:
         out = _empty_on(stream, q.shape, dtype=q.dtype, device=q.device)

@@ -4,6 +4,7 @@
 import ctypes
 import shutil
 import subprocess
+import types
 from pathlib import Path
 
 import numpy as np
@@ -201,6 +202,26 @@ def test_a_plan_s_memory_goes_back_behind_all_that_read_it(monkeypatch):
     assert dropped(monkeypatch, a, b, capturing=[a]) and not a.waits
     b.record_event = lambda: 1 / 0
     assert dropped(monkeypatch, a, b)
+
+
+def test_streams_of_another_device_are_refused(aegkv_lib):
+    stream = types.SimpleNamespace(device=torch.device("cuda", 1))
+    args = ([[0]], [1], [1])
+    with pytest.raises(ValueError, match="cuda:1 for work on cuda:0"):
+        ops.CacheBatch(*args, num_blocks=4, block_size=16, kv_heads=1, device="cuda:0",
+                       stream=stream)
+    batch = ops.CacheBatch.__new__(ops.CacheBatch)
+    batch.device = torch.device("cuda", 0)
+    with pytest.raises(ValueError, match="cuda:1 for work on cuda:0"):
+        batch.update(*args, stream=stream)
+    like = types.SimpleNamespace(block_size=16, kv_heads=1, num_blocks=4, device=batch.device,
+                                 heads=1, head_dim=128, read_tokens=1, num_tokens=1)
+    x = torch.zeros(1, 1, 128)
+    for call in (lambda: ops.quant_write(like, like, x, x, stream=stream),
+                 lambda: ops.quant_read(like, like, stream=stream),
+                 lambda: ops.quant_attend(like, like, x, stream=stream)):
+        with pytest.raises(ValueError, match="cuda:1 for work on cuda:0"):
+            call()
 
 
 @pytest.mark.parametrize("fmt", ["mxfp4", "mxfp8"])
