@@ -1061,7 +1061,7 @@ class CacheBatch:
         _require_stream(self.device, stream)
         with torch.cuda.device(self.device):
             st = stream if stream is not None else torch.cuda.current_stream()
-            if torch.cuda.is_current_stream_capturing():
+            if torch.cuda.is_current_stream_capturing() or stream is not None and _capturing(st):
                 raise ValueError("a batch cannot be made while a stream is captured")
             with torch.cuda.stream(st):
                 self._plan = torch.empty(self._host.size, dtype=torch.uint8, device=self.device)
@@ -1120,14 +1120,15 @@ class CacheBatch:
         _require_stream(self.device, stream)
         with torch.cuda.device(self.device):
             st = stream if stream is not None else torch.cuda.current_stream()
+            others = [other for other in (self._home, *self._used.values())
+                      if _alive(other) and other.cuda_stream != st.cuda_stream]
+            if torch.cuda.is_current_stream_capturing() or any(map(_capturing, (st, *others))):
+                raise ValueError("a batch is updated outside the capture; the graph's calls "
+                                 "find what it holds when they are replayed")
             with torch.cuda.stream(st):
-                if torch.cuda.is_current_stream_capturing():
-                    raise ValueError("a batch is updated outside the capture; the graph's calls "
-                                     "find what it holds when they are replayed")
+                for other in others:
+                    st.wait_event(other.record_event())
                 self._make(block_tables, seq_lens, new_lens, update=1)
-                for other in (self._home, *self._used.values()):
-                    if _alive(other) and other.cuda_stream != st.cuda_stream:
-                        st.wait_event(other.record_event())
                 self._used.clear()
                 self._upload(st)
 

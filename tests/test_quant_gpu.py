@@ -570,6 +570,38 @@ def test_a_dropped_batch_s_memory_waits_for_the_stream_it_moved_to(gpu):
             assert torch.equal(outs[0], out)
 
 
+def test_an_update_during_a_capture_of_the_batch_s_stream_is_refused(gpu):
+    """On any stream: it would wait for the captured calls, and so join them."""
+    lens = [300]
+    tables = tables_for(lens, 16, 20)
+    cache, k, v = make(gpu, "mxfp4", 20, 16, 2, 128, seed=1)
+    q = torch.randn(1, 8, 128, generator=torch.Generator().manual_seed(3)).to(BF16).to(gpu)
+    home, other = torch.cuda.Stream(), torch.cuda.Stream()
+    batch = batch_for(gpu, tables, lens, [1], cache, heads=8, max_columns=20, stream=home)
+    want = ops.quant_attend(cache, batch, q)
+    out = torch.zeros_like(want)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=home):
+        ops.quant_attend(cache, batch, q, out=out)
+        with torch.cuda.stream(other):
+            with pytest.raises(ValueError, match="outside the capture"):
+                batch.update(tables, lens, [1])
+        with pytest.raises(ValueError, match="outside the capture"):
+            batch.update(tables, lens, [1], stream=other)
+        with torch.cuda.stream(other):
+            with pytest.raises(ValueError, match="while a stream is captured"):
+                batch_for(gpu, tables, lens, [1], cache, stream=home)
+    for _ in range(3):
+        out.zero_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    batch.update(tables, [200], [1], stream=other)
+    check_attend(ops.quant_attend(cache, batch, q), k, v, tables, [200], [1], q, 16, BF16)
+
+
 def test_a_cache_is_written_attended_moved_and_attended_again(gpu):
     """One model step after another as a serving engine makes them: two layers
     over a composite cache, a prompt, decode steps, a swap to the host and back to other
