@@ -1066,7 +1066,7 @@ class CacheBatch:
             with torch.cuda.stream(st):
                 self._plan = torch.empty(self._host.size, dtype=torch.uint8, device=self.device)
                 self._pool = st     # whose memory pool the plan goes back to
-                self._upload(st)
+                self._upload(st, self._pinned())
 
     def _make(self, block_tables, seq_lens, new_lens, update: int) -> None:
         if isinstance(block_tables, (torch.Tensor, np.ndarray)):
@@ -1098,12 +1098,20 @@ class CacheBatch:
         self.num_seqs, self.num_tokens = int(lens.size), int(new.sum())
         self.read_tokens = int(lens.sum())
 
-    def _upload(self, st: torch.cuda.Stream) -> None:
-        pinned = torch.empty(self._host.size, dtype=torch.uint8, pin_memory=True)
-        pinned.numpy()[:] = self._host
-        self._plan.copy_(pinned, non_blocking=True)
-        self._uploaded = torch.cuda.Event()
-        self._uploaded.record(st)
+    def _pinned(self) -> torch.Tensor:
+        return torch.empty(self._host.size, dtype=torch.uint8, pin_memory=True)
+
+    def _upload(self, st: torch.cuda.Stream, pinned: torch.Tensor) -> None:
+        try:
+            pinned.numpy()[:] = self._host
+            self._plan.copy_(pinned, non_blocking=True)
+            self._uploaded = torch.cuda.Event()
+            self._uploaded.record(st)
+        except BaseException:
+            # calls go by the host's plan, kernels by the device's: now that they may
+            # differ, nothing is taken over this batch any more ("no plan")
+            self._host[:8] = 0
+            raise
         self._home, self._stream = st, st.cuda_stream
         # BatchArgs of csrc/hostargs.cpp
         self._packed = struct.pack(
@@ -1128,9 +1136,10 @@ class CacheBatch:
             with torch.cuda.stream(st):
                 for other in others:
                     st.wait_event(other.record_event())
+                pinned = self._pinned()
                 self._make(block_tables, seq_lens, new_lens, update=1)
+                self._upload(st, pinned)
                 self._used.clear()
-                self._upload(st)
 
     def _enter(self, raw: int, stream: torch.cuda.Stream | None):
         """Order a call on the raw stream behind the upload. The stream, where

@@ -570,6 +570,46 @@ def test_a_dropped_batch_s_memory_waits_for_the_stream_it_moved_to(gpu):
             assert torch.equal(outs[0], out)
 
 
+def test_an_update_that_fails_leaves_no_batch_by_halves(gpu, monkeypatch):
+    """Calls go by the host's plan and kernels by the device's."""
+    tables = tables_for([300, 40], 16, 30)
+    cache, k, v = make(gpu, "mxfp4", 30, 16, 2, 128, seed=1)
+    q = torch.randn(2, 8, 128, generator=torch.Generator().manual_seed(3)).to(BF16).to(gpu)
+    batch = batch_for(gpu, tables, [300, 40], [1, 1], cache, heads=8, max_tokens=20)
+    before = ops.quant_attend(cache, batch, q)
+    host = batch._host.copy()
+    empty = torch.empty
+
+    def no_pinned_memory(*args, **kw):
+        if kw.get("pin_memory"):
+            raise RuntimeError("none left")
+        return empty(*args, **kw)
+
+    with monkeypatch.context() as m:
+        m.setattr(torch, "empty", no_pinned_memory)
+        with pytest.raises(RuntimeError, match="none left"):
+            batch.update(tables, [100, 20], [1, 1])
+    assert (batch._host == host).all()
+    assert torch.equal(ops.quant_attend(cache, batch, q), before)
+
+    class NoCopy:
+        data_ptr = batch._plan.data_ptr
+
+        def copy_(self, *args, **kw):
+            raise RuntimeError("no copy")
+
+    plan, batch._plan = batch._plan, NoCopy()
+    with pytest.raises(RuntimeError, match="no copy"):
+        batch.update(tables, [100, 20], [1, 1])
+    batch._plan = plan
+    x = torch.zeros(2, 2, 128, dtype=BF16, device=gpu)
+    for call in (lambda: ops.quant_attend(cache, batch, q), lambda: ops.quant_read(cache, batch),
+                 lambda: ops.quant_write(cache, batch, x, x),
+                 lambda: batch.update(tables, [300, 40], [1, 1])):
+        with pytest.raises(ValueError, match="no plan"):
+            call()
+
+
 def test_an_update_during_a_capture_of_the_batch_s_stream_is_refused(gpu):
     """On any stream: it would wait for the captured calls, and so join them."""
     lens = [300]
