@@ -4,6 +4,9 @@
 #define AEGKV_QUANT_CALLS_H
 
 #include "quant_cache.h"
+#include "value_places.h"
+
+#include <initializer_list>
 
 namespace {
 
@@ -114,6 +117,35 @@ int check_count(int64_t given, int64_t now, int64_t room, bool capturing, const 
   return 0;
 }
 
+// The first `tokens` rows of checked values.
+Place rows_place(const Values& v, int64_t tokens, int32_t heads, int32_t head_dim, int dtype) {
+  const int64_t es = element_bytes(dtype);
+  return place(v.base, tokens, heads, head_dim * es, v.token * es, v.head * es);
+}
+
+// What a call writes shares no byte with what it reads beside it: workgroups run
+// in no order.
+struct Named {
+  Place at;
+  const char* what;
+};
+
+int check_apart(const Named& w, std::initializer_list<Named> others) {
+  for (const Named& o : others)
+    if (overlap(w.at, o.at)) return fail(AEGKV_EOVERLAP, "%s and %s overlap", w.what, o.what);
+  return 0;
+}
+
+Named k_cache(const QuantCall& c) {
+  return Named{place(c.k, c.h.num_blocks * c.page_bytes), "the K cache"};
+}
+Named v_cache(const QuantCall& c) {
+  return Named{place(c.v, c.h.num_blocks * c.page_bytes), "the V cache"};
+}
+Named plan_place(const QuantCall& c) {
+  return Named{place(c.plan, c.h.room.bytes), "the plan's device copy"};
+}
+
 template <typename F>
 int by_type(int dtype, const F& f) {
   switch (dtype) {
@@ -214,9 +246,9 @@ int aegkv_quant_write(const void* plan, const void* device_plan, int format, int
   QuantCall c;
   int rc = open_call(plan, device_plan, format, head_dim, k_pages, v_pages, stream, &c);
   if (rc) return rc;
-  const int64_t cache = c.h.num_blocks * c.page_bytes;
-  if (c.k < c.v + cache && c.v < c.k + cache)
-    return fail(AEGKV_EOVERLAP, "the K and V caches overlap");
+  rc = check_apart(k_cache(c), {v_cache(c), plan_place(c)});
+  if (!rc) rc = check_apart(v_cache(c), {plan_place(c)});
+  if (rc) return rc;
   rc = check_count(num_tokens, c.h.num_tokens, c.h.room.tokens, c.capturing, "k and v");
   SpanArgs a;
   dim3 grid;
@@ -224,6 +256,10 @@ int aegkv_quant_write(const void* plan, const void* device_plan, int format, int
                              k_head_stride, false, "k", &a.values[0]);
   if (!rc) rc = check_values(v, num_tokens, c.h.kv_heads, head_dim, dtype, v_token_stride,
                              v_head_stride, false, "v", &a.values[1]);
+  const int64_t reached = c.capturing ? c.h.room.tokens : c.h.num_tokens;
+  for (int i = 0; i < 2 && !rc; ++i)
+    rc = check_apart(Named{rows_place(a.values[i], reached, c.h.kv_heads, head_dim, dtype),
+                           i ? "v" : "k"}, {k_cache(c), v_cache(c)});
   if (!rc) rc = span_args(c, true, &a, &grid);
   if (rc || grid.x == 0) return rc;
   return by_shape(format, head_dim, [&](auto fmt, auto d) {
@@ -256,6 +292,15 @@ int aegkv_quant_read(const void* plan, const void* device_plan, int format, int3
                              k_head_stride, true, "k", &a.values[0]);
   if (!rc) rc = check_values(v, num_tokens, h.kv_heads, head_dim, dtype, v_token_stride,
                              v_head_stride, true, "v", &a.values[1]);
+  if (!rc) {
+    const int64_t reached = new_tokens ? (c.capturing ? h.room.tokens : h.num_tokens)
+                                       : (c.capturing ? h.room.read_spans * kSpan : h.read_tokens);
+    const Place to[2] = {rows_place(a.values[0], reached, h.kv_heads, head_dim, dtype),
+                         rows_place(a.values[1], reached, h.kv_heads, head_dim, dtype)};
+    rc = check_apart(Named{to[0], "k"}, {Named{to[1], "v"}, k_cache(c), v_cache(c),
+                                         plan_place(c)});
+    if (!rc) rc = check_apart(Named{to[1], "v"}, {k_cache(c), v_cache(c), plan_place(c)});
+  }
   if (!rc) rc = span_args(c, new_tokens != 0, &a, &grid);
   if (rc || grid.x == 0) return rc;
   return by_shape(format, head_dim, [&](auto fmt, auto d) {
@@ -309,6 +354,17 @@ int aegkv_quant_attend(const void* plan, const void* device_plan, int format, in
     rc = check_device_range(workspace, 4 * floats, "the workspace");
     if (rc) return rc;
   }
+  const int64_t reached = c.capturing ? h.room.tokens : h.num_tokens;
+  const Place from = rows_place(a.q, reached, h.heads, head_dim, dtype);
+  const Place to = rows_place(a.out, reached, h.heads, head_dim, dtype);
+  const Place parts = place(workspace, 4 * floats);
+  // in place every row is read by the workgroup that writes it, or before all that do
+  if (!same(from, to)) rc = check_apart(Named{to, "out"}, {Named{from, "q"}});
+  if (!rc) rc = check_apart(Named{to, "out"}, {k_cache(c), v_cache(c), plan_place(c)});
+  if (!rc) rc = check_apart(Named{parts, "the workspace"},
+                            {Named{to, "out"}, Named{from, "q"}, k_cache(c), v_cache(c),
+                             plan_place(c)});
+  if (rc) return rc;
   a.plan = c.plan;
   a.at_table = h.room.at_table;
   a.at_merges = h.room.at_merges;

@@ -1323,8 +1323,8 @@ def quant_attend(cache: QuantCache, batch: CacheBatch, q: torch.Tensor, *,
 
     q: [tokens, heads, head_dim] of bfloat16 or float16, row i the query of the
     batch's i-th new token, whose K and V are in the cache already (quant_write).
-    scale: of the scores, head_dim ** -0.5 by default. `out` (q itself is fine)
-    takes the result; rows behind the batch's last token are left as they were.
+    scale: of the scores, head_dim ** -0.5 by default. `out` (q itself is fine, other
+    overlaps are refused) takes the result; rows behind the batch's last token are left as they were.
     """
     if stream is None:
         done = _lib.hostargs().quant_attend(cache._packed, batch._packed, q, out, scale,

@@ -573,6 +573,12 @@ int aegkv_batch_plan(int64_t num_seqs, const int64_t* column_offsets, const int6
  * value its nearest code, ties to the even one. A group that holds a NaN or an
  * infinity is written as no number. Only the tokens' own bytes change.
  *
+ * Of what these three calls write, nothing may share a byte with another of their
+ * arguments (AEGKV_EOVERLAP; but for out = q of attention): the K and V caches,
+ * k and v of a read, values and caches, workspace and plan. Rows of values that are
+ * alike but for their beginning (slices of one buffer) are looked at one by one,
+ * others from their first byte to their last.
+ *
  * These calls launch kernels only: they allocate nothing, use no ring, and may
  * be captured. Captured over a plan with room, a call has to be given arrays
  * that hold all the plan has room for.
@@ -601,7 +607,7 @@ int aegkv_quant_read(const void* plan, const void* device_plan, int format, int3
  * positions j that query i sees of softmax_j(scale * q[i] . K[j]) V[j], query
  * head h over KV head h / (heads / kv_heads). q and out: [num_tokens][heads]
  * [head_dim] of bfloat16 or float16; rows behind the batch's last token are left as
- * they were. out may be q itself. The cache's values are taken in the queries' type
+ * they were. out may be q itself (the same place and strides). The cache's values are taken in the queries' type
  * (bfloat16 holds them all but those of 2^128; float16 rounds what is below
  * 2^-14, and beyond its range a value is an infinity). Scores, softmax and sums
  * are held in 32 bits; probabilities enter the second product in the queries' type.

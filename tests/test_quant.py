@@ -268,3 +268,19 @@ def test_plans_of_random_batches_under_sanitizers(tmp_path):
     run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
     assert run.returncode == 0, run.stdout + run.stderr
     assert "clean" in run.stdout
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="g++ is not installed")
+def test_places_that_overlap_under_sanitizers(tmp_path):
+    """tests/native/value_places_check.cpp: rows of values share a byte exactly
+    where they are said to."""
+    exe = tmp_path / "value_places_check"
+    cmd = ["g++", "-std=c++17", "-O1", "-g", "-fno-omit-frame-pointer", "-Wall",
+           "-fsanitize=address,undefined", "-fno-sanitize-recover=all",
+           f"-I{REPO / 'aegaeon_amd' / 'csrc'}",
+           str(REPO / "tests" / "native" / "value_places_check.cpp"), "-o", str(exe)]
+    res = subprocess.run(cmd, capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0, res.stderr
+    run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stdout + run.stderr
+    assert "clean" in run.stdout

@@ -764,3 +764,52 @@ def test_refusals_on_the_device(gpu):
     with pytest.raises(ValueError, match="pages"):
         ops.QuantCache(cache.k_pages[:, :-16].contiguous(), cache.v_pages, kv_heads=2,
                        head_dim=128, block_size=16)
+
+
+def test_what_a_call_writes_shares_no_byte_with_its_other_arguments(gpu):
+    """Shifted views and the like are refused; slices of one buffer that only
+    interleave are not, and rows behind the batch's last token do not count."""
+    lens, new = [40, 20], [2, 1]
+    tables = tables_for(lens, 16, 8)
+    cache, k, v = make(gpu, "mxfp4", 8, 16, 2, 128, seed=1)
+    batch = batch_for(gpu, tables, lens, new, cache, heads=4)
+    buf = torch.randn(7, 4, 256, generator=torch.Generator().manual_seed(3)).to(BF16).to(gpu)
+    q = buf[:3, :, :128]
+    kept = buf.clone()
+    pages = cache.k_pages.view(-1)[:6 * 2 * 128 * 2 * 2].view(BF16).view(-1, 4, 128)
+
+    def bad(match, fn):
+        with pytest.raises(ValueError, match=match):
+            fn()
+
+    bad("out and q overlap", lambda: ops.quant_attend(cache, batch, q, out=buf[1:4, :, :128]))
+    bad("out and q overlap", lambda: ops.quant_attend(cache, batch, q, out=buf[:3, :, 64:192]))
+    bad("out and q overlap", lambda: ops.quant_attend(
+        cache, batch, q, out=buf.view(-1)[:3 * 512].view(3, 4, 128)))
+    bad("out and the K cache", lambda: ops.quant_attend(cache, batch, q, out=pages[:3]))
+    bad("k and v overlap", lambda: ops.quant_read(cache, batch, tokens="new", out=(
+        buf[:3, :2, :128], buf[:3, :2, :128])))
+    bad("k and v overlap", lambda: ops.quant_read(cache, batch, tokens="new", out=(
+        buf[:3, :2, :128], buf[:3, 1:3, :128])))
+    bad("v and the K cache", lambda: ops.quant_read(cache, batch, tokens="new", out=(
+        buf[:3, :2, :128], pages[:3, :2])))
+    bad("k and the K cache", lambda: ops.quant_write(cache, batch, pages[:3, :2],
+                                                     buf[:3, :2, :128]))
+    bad("K cache and the V cache", lambda: ops.quant_write(
+        ops.QuantCache(cache.k_pages, cache.k_pages, kv_heads=2, head_dim=128, block_size=16),
+        batch, buf[:3, :2, :128], buf[:3, 2:, :128]))
+    roomy = batch_for(gpu, tables, lens, new, cache, heads=4, max_seqs=64)
+    inside = roomy._plan[:3 * 4 * 256].view(BF16).view(3, 4, 128)
+    bad("out and the plan", lambda: ops.quant_attend(cache, roomy, q, out=inside))
+    assert torch.equal(buf, kept) and torch.equal(cache.k_pages.cpu(), k.raw)
+    # one buffer's halves, and its rows behind the batch's last
+    want = ops.quant_attend(cache, batch, q)
+    check_attend(want, k, v, tables, lens, new, q, 16, BF16)
+    beside = buf[:3, :, 128:]
+    assert torch.equal(ops.quant_attend(cache, batch, q, out=beside), want)
+    assert torch.equal(q, kept[:3, :, :128])
+    behind = buf[3:, :, :128]
+    assert torch.equal(ops.quant_attend(cache, batch, buf[:4, :, :128], out=behind)[:3], want)
+    got = ops.quant_read(cache, batch, tokens="new", out=(buf[:3, :2, :128], buf[:3, 2:, :128]))
+    assert all(torch.equal(a, b) for a, b in zip(
+        got, ops.quant_read(cache, batch, tokens="new")))
