@@ -813,3 +813,35 @@ def test_what_a_call_writes_shares_no_byte_with_its_other_arguments(gpu):
     got = ops.quant_read(cache, batch, tokens="new", out=(buf[:3, :2, :128], buf[:3, 2:, :128]))
     assert all(torch.equal(a, b) for a, b in zip(
         got, ops.quant_read(cache, batch, tokens="new")))
+
+
+@pytest.mark.parametrize("fmt,d,bs", SHAPES)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("new", [1, 12, 60])
+def test_no_numbers_that_a_write_stored(gpu, fmt, d, bs, dtype, new):
+    """A NaN or an infinity in a token's K makes every row that sees it none, one in V
+    the 32 values of its group: also in old tokens, whose tiles every row sees,
+    and as quant_write stores them (codes of 0 under the byte 255)."""
+    n, heads = 300, 3
+    tables = tables_for([n], bs, 24)
+    cache, k_ref, v_ref = make(gpu, fmt, 24, bs, heads, d, seed=2)
+    gen = torch.Generator().manual_seed(5)
+    k, v = (torch.randn(n, heads, d, generator=gen) for _ in range(2))
+    k[37, 0, d - 1] = math.nan          # all of head 0's queries
+    v[5, 1, 3] = math.inf               # the first group of head 1's
+    v[n - 1, 2, d - 1] = -math.inf      # the last group of head 2's last query
+    whole = batch_for(gpu, tables, [n], [n], cache)
+    ops.quant_write(cache, whole, k.to(dtype).to(gpu), v.to(dtype).to(gpu))
+    place = ref.places(tables[0], bs, range(n))
+    k_ref.put(*place, *ref.quantise(fmt, k.to(dtype)))
+    v_ref.put(*place, *ref.quantise(fmt, v.to(dtype)))
+    batch = batch_for(gpu, tables, [n], [new], cache, heads=2 * heads)
+    q = torch.randn(new, 2 * heads, d, generator=gen).to(dtype).to(gpu)
+    out = ops.quant_attend(cache, batch, q)
+    check_attend(out, k_ref, v_ref, tables, [n], [new], q, bs, dtype)
+    none = out.isnan().cpu()
+    want = torch.zeros_like(none)
+    want[:, :2] = True
+    want[:, 2:4, :32] = True
+    want[-1, 4:, -32:] = True
+    assert torch.equal(none, want)
