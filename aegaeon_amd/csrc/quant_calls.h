@@ -173,7 +173,10 @@ int by_shape(int format, int head_dim, const F& f) {
                                       : width(Constant<AEGKV_FORMAT_MXFP8>{});
 }
 
-int launched(const char* what) {
+template <typename K, typename A>
+int launch(K kernel, dim3 grid, int lanes, hipStream_t stream, const A& args, const char* what) {
+  (void)hipGetLastError();  // clear a stale error: the check below is for this launch
+  kernel<<<grid, lanes, 0, stream>>>(args);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? 0 : hip_fail(e, what);
 }
@@ -264,9 +267,8 @@ int aegkv_quant_write(const void* plan, const void* device_plan, int format, int
   if (rc || grid.x == 0) return rc;
   return by_shape(format, head_dim, [&](auto fmt, auto d) {
     return by_type(dtype, [&](auto t) {
-      quant_write_kernel<decltype(fmt)::value, decltype(d)::value, decltype(t)>
-          <<<grid, kSpanLanes, 0, stream>>>(a);
-      return launched("quant_write_kernel launch");
+      return launch(quant_write_kernel<decltype(fmt)::value, decltype(d)::value, decltype(t)>, grid,
+                    kSpanLanes, stream, a, "quant_write_kernel launch");
     });
   });
 }
@@ -305,9 +307,8 @@ int aegkv_quant_read(const void* plan, const void* device_plan, int format, int3
   if (rc || grid.x == 0) return rc;
   return by_shape(format, head_dim, [&](auto fmt, auto d) {
     return by_type(dtype, [&](auto t) {
-      quant_read_kernel<decltype(fmt)::value, decltype(d)::value, decltype(t)>
-          <<<grid, kSpanLanes, 0, stream>>>(a);
-      return launched("quant_read_kernel launch");
+      return launch(quant_read_kernel<decltype(fmt)::value, decltype(d)::value, decltype(t)>, grid,
+                    kSpanLanes, stream, a, "quant_read_kernel launch");
     });
   });
 }
@@ -381,7 +382,7 @@ int aegkv_quant_attend(const void* plan, const void* device_plan, int format, in
   if (rc) return rc;
   return by_shape(format, head_dim, [&](auto fmt, auto d) {
     constexpr int kFormat = decltype(fmt)::value, kDim = decltype(d)::value;
-    const auto launch = [&](auto t) {
+    const auto attend = [&](auto t) {
       typedef decltype(t) T;
       for (int kind = 0; kind < kKinds; ++kind) {
         if (!h.room.items[kind]) continue;
@@ -390,23 +391,18 @@ int aegkv_quant_attend(const void* plan, const void* device_plan, int format, in
         a.work = a.work_base + a.kind_work[kind];
         a.slot_floats = a.kind_slot_floats[kind];
         const dim3 grid(static_cast<uint32_t>(h.room.items[kind]));
-        if (kind == kFew)
-          quant_attend_kernel<kFormat, kDim, T, 1><<<grid, kAttendLanes, 0, stream>>>(a);
-        else if (kind == kMore)
-          quant_attend_kernel<kFormat, kDim, T, 2><<<grid, kAttendLanes, 0, stream>>>(a);
-        else
-          quant_prompt_kernel<kFormat, kDim, T><<<grid, kAttendLanes, 0, stream>>>(a);
-        const int rc = launched("quant_attend_kernel launch");
+        const auto kernel = kind == kFew    ? quant_attend_kernel<kFormat, kDim, T, 1>
+                            : kind == kMore ? quant_attend_kernel<kFormat, kDim, T, 2>
+                                            : quant_prompt_kernel<kFormat, kDim, T>;
+        const int rc = launch(kernel, grid, kAttendLanes, stream, a, "quant_attend_kernel launch");
         if (rc) return rc;
       }
-      if (h.room.merges) {
-        const dim3 grid(static_cast<uint32_t>(h.room.merges));
-        quant_merge_kernel<kDim, T><<<grid, 256, 0, stream>>>(a);
-        return launched("quant_merge_kernel launch");
-      }
+      if (h.room.merges)
+        return launch(quant_merge_kernel<kDim, T>, dim3(static_cast<uint32_t>(h.room.merges)), 256,
+                      stream, a, "quant_merge_kernel launch");
       return 0;
     };
-    return dtype == AEGKV_DTYPE_BFLOAT16 ? launch(__bf16{}) : launch(_Float16{});
+    return dtype == AEGKV_DTYPE_BFLOAT16 ? attend(__bf16{}) : attend(_Float16{});
   });
 }
 

@@ -1,6 +1,7 @@
 """Quantised caches on the GPU: written pages, tokens read back and attention
 against the 64-bit definition (quant_reference.py)."""
 
+import ctypes
 import math
 import random
 
@@ -845,3 +846,35 @@ def test_no_numbers_that_a_write_stored(gpu, fmt, d, bs, dtype, new):
     want[:, 2:4, :32] = True
     want[-1, 4:, -32:] = True
     assert torch.equal(none, want)
+
+
+def test_an_error_that_other_code_left_is_not_a_call_s_own(gpu):
+    """HIP keeps a thread's last error until someone asks: a call over a quantised
+    cache neither fails for it nor runs a second time (in place that would take
+    results for queries)."""
+    lens, new = [400, 90], [1, 30]
+    tables = tables_for(lens, 16, 40)
+    cache, k, v = make(gpu, "mxfp4", 40, 16, 2, 128, seed=1)
+    batch = batch_for(gpu, tables, lens, new, cache, heads=8)
+    gen = torch.Generator().manual_seed(3)
+    q = torch.randn(31, 8, 128, generator=gen).to(BF16).to(gpu)
+    x = torch.randn(31, 2, 128, generator=gen).to(BF16).to(gpu)
+    hip = ctypes.CDLL("libamdhip64.so.7")
+
+    def leave_an_error():
+        assert hip.hipSetDevice(4096) != 0      # no such device: nothing else happens
+        assert hip.hipPeekAtLastError() != 0
+
+    for stream in (None, torch.cuda.current_stream()):
+        want = ops.quant_attend(cache, batch, q)
+        same = q.clone()
+        torch.cuda.synchronize()
+        leave_an_error()
+        ops.quant_attend(cache, batch, same, out=same, stream=stream)
+        assert torch.equal(same, want)
+        leave_an_error()
+        ops.quant_write(cache, batch, x, x, stream=stream)
+        leave_an_error()
+        ops.quant_read(cache, batch, stream=stream)
+        ops.quant_write(cache, batch, x, x)
+        assert hip.hipGetLastError() == 0
