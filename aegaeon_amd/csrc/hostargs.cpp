@@ -12,7 +12,9 @@
 // checked and their C arguments made in Python, they took the host 7.4 us
 // (write) and 14 (attend), 3 to 6 of which are the launches; here 4.0 and 8.1.
 // These functions too take the plain case only: None, with nothing enqueued,
-// for anything else.
+// for anything else. What the library itself answers is the answer: its status, if
+// it refused the call or failed in it, as a number. (A call made a second time
+// could take what the first one wrote for its input.)
 
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
@@ -205,7 +207,7 @@ bool alike(const at::Tensor& a, const at::Tensor& b) {
   return a.scalar_type() == b.scalar_type() && a.size(0) == b.size(0);
 }
 
-// quant_write(cache, batch, k, v, stream, device) -> True, or None
+// quant_write(cache, batch, k, v, stream, device) -> True, a status, or None
 PyObject* quant_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   QuantArgs q;
   if (nargs != 6 || !q.take(args[0], args[1], args[4], args[5])) Py_RETURN_NONE;
@@ -213,20 +215,21 @@ PyObject* quant_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const at::Tensor* k = q.rows(args[2], q.c.kv_heads);
     const at::Tensor* v = q.rows(args[3], q.c.kv_heads);
     if (!k || !v || !alike(*k, *v)) Py_RETURN_NONE;
-    if (at_address<std::remove_pointer_t<WriteFn>>(q.c.write)(
+    const int status = at_address<std::remove_pointer_t<WriteFn>>(q.c.write)(
             at_address<void>(q.b.host_plan), at_address<void>(q.b.device_plan),
             static_cast<int>(q.c.format), static_cast<int32_t>(q.c.head_dim),
             at_address<void>(q.c.k_pages), at_address<void>(q.c.v_pages), k->data_ptr(),
             k->stride(0), k->stride(1), v->data_ptr(), v->stride(0), v->stride(1), k->size(0),
-            dtype_code(k->scalar_type()), q.stream) != 0)
-      Py_RETURN_NONE;
+            dtype_code(k->scalar_type()), q.stream);
+    if (status) return PyLong_FromLong(status);
     Py_RETURN_TRUE;
   } catch (...) {
     Py_RETURN_NONE;
   }
 }
 
-// quant_read(cache, batch, new tokens, out or dtype code, stream, device) -> (k, v), or None
+// quant_read(cache, batch, new tokens, out or dtype code, stream, device) -> (k, v), a
+// status, or None
 PyObject* quant_read(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   QuantArgs q;
   if (nargs != 6 || !q.take(args[0], args[1], args[4], args[5])) Py_RETURN_NONE;
@@ -246,21 +249,24 @@ PyObject* quant_read(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       at::Tensor v = at::empty({tokens, q.c.kv_heads, q.c.head_dim}, options);
       made.p = PyTuple_New(2);
       if (!made.p) return nullptr;
-      PyTuple_SET_ITEM(made.p, 0, THPVariable_Wrap(k));
-      PyTuple_SET_ITEM(made.p, 1, THPVariable_Wrap(v));
+      for (int i = 0; i < 2; ++i) {
+        PyObject* wrapped = THPVariable_Wrap(i ? v : k);
+        if (!wrapped) return nullptr;
+        PyTuple_SET_ITEM(made.p, i, wrapped);
+      }
       out = made.p;
     }
     if (!PyTuple_CheckExact(out) || PyTuple_GET_SIZE(out) != 2) Py_RETURN_NONE;
     const at::Tensor* k = q.rows(PyTuple_GET_ITEM(out, 0), q.c.kv_heads);
     const at::Tensor* v = q.rows(PyTuple_GET_ITEM(out, 1), q.c.kv_heads);
     if (!k || !v || !alike(*k, *v)) Py_RETURN_NONE;
-    if (at_address<std::remove_pointer_t<ReadFn>>(q.c.read)(
+    const int status = at_address<std::remove_pointer_t<ReadFn>>(q.c.read)(
             at_address<void>(q.b.host_plan), at_address<void>(q.b.device_plan),
             static_cast<int>(q.c.format), static_cast<int32_t>(q.c.head_dim),
             at_address<void>(q.c.k_pages), at_address<void>(q.c.v_pages), fresh, k->data_ptr(),
             k->stride(0), k->stride(1), v->data_ptr(), v->stride(0), v->stride(1), k->size(0),
-            dtype_code(k->scalar_type()), q.stream) != 0)
-      Py_RETURN_NONE;
+            dtype_code(k->scalar_type()), q.stream);
+    if (status) return PyLong_FromLong(status);
     if (made.p) return made.release();
     Py_INCREF(out);
     return out;
@@ -269,7 +275,8 @@ PyObject* quant_read(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   }
 }
 
-// quant_attend(cache, batch, q, out or None, scale or None, stream, device) -> out, or None
+// quant_attend(cache, batch, q, out or None, scale or None, stream, device) -> out, a
+// status, or None
 PyObject* quant_attend(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   QuantArgs q;
   if (nargs != 7 || !q.take(args[0], args[1], args[5], args[6])) Py_RETURN_NONE;
@@ -281,28 +288,28 @@ PyObject* quant_attend(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       if (!PyFloat_CheckExact(args[4])) Py_RETURN_NONE;
       scale = PyFloat_AS_DOUBLE(args[4]);
     }
-    at::Tensor made;
-    const at::Tensor* out = &made;
+    Ref result(nullptr);
     if (args[3] == Py_None) {
-      made = at::empty(query->sizes(), query->options().requires_grad(false));
+      result.p = THPVariable_Wrap(
+          at::empty(query->sizes(), query->options().requires_grad(false)));
+      if (!result.p) return nullptr;
     } else {
-      out = q.rows(args[3], q.b.heads);
-      if (!out || !alike(*query, *out)) Py_RETURN_NONE;
+      Py_INCREF(args[3]);
+      result.p = args[3];
     }
+    const at::Tensor* out = q.rows(result.p, q.b.heads);
+    if (!out || !alike(*query, *out)) Py_RETURN_NONE;
     const int64_t bytes = q.b.workspace[q.c.head_dim == 64 ? 0 : q.c.head_dim == 128 ? 1 : 2];
     at::Tensor work;   // goes back to the stream's pool, behind the call
     if (bytes) work = at::empty({bytes}, query->options().dtype(at::kByte).requires_grad(false));
-    if (at_address<std::remove_pointer_t<AttendFn>>(q.c.attend)(
+    const int status = at_address<std::remove_pointer_t<AttendFn>>(q.c.attend)(
             at_address<void>(q.b.host_plan), at_address<void>(q.b.device_plan),
             static_cast<int>(q.c.format), static_cast<int32_t>(q.c.head_dim),
             at_address<void>(q.c.k_pages), at_address<void>(q.c.v_pages), query->data_ptr(),
             query->stride(0), query->stride(1), out->data_ptr(), out->stride(0), out->stride(1),
             query->size(0), dtype_code(query->scalar_type()), scale,
-            bytes ? work.data_ptr() : nullptr, bytes, q.stream) != 0)
-      Py_RETURN_NONE;
-    if (args[3] == Py_None) return THPVariable_Wrap(made);
-    Py_INCREF(args[3]);
-    return args[3];
+            bytes ? work.data_ptr() : nullptr, bytes, q.stream);
+    return status ? PyLong_FromLong(status) : result.release();
   } catch (...) {
     Py_RETURN_NONE;
   }

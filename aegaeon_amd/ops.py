@@ -1219,6 +1219,13 @@ def _here(cache: QuantCache) -> tuple:
     return torch._C._cuda_getCurrentRawStream(cache.device.index), torch._C._cuda_getDevice()
 
 
+def _answer(done):
+    """What a native call gave: its result, or the status of the library."""
+    if type(done) is int:
+        _lib.check(done)
+    return done
+
+
 def _rows_arg(t: torch.Tensor, what: str, heads: int, cache: QuantCache, dtypes):
     """(pointer, token stride, head stride) of a [tokens, heads, head_dim] tensor."""
     if t.device != cache.device:
@@ -1264,9 +1271,11 @@ def quant_write(cache: QuantCache, batch: CacheBatch, k: torch.Tensor, v: torch.
     and each takes its nearest code, ties to even. A group with a NaN or an
     infinity reads back as NaN.
     """
-    if stream is None and _lib.hostargs().quant_write(
-            cache._packed, batch._packed, k, v, *_here(cache)) is not None:
-        return
+    if stream is None:
+        done = _lib.hostargs().quant_write(cache._packed, batch._packed, k, v, *_here(cache))
+        if done is not None:
+            _answer(done)
+            return
     _quant_call(cache, batch, stream)
     kp = _rows_arg(k, "k", cache.kv_heads, cache, _DTYPES)
     vp = _rows_arg(v, "v", cache.kv_heads, cache, _DTYPES)
@@ -1294,7 +1303,7 @@ def quant_read(cache: QuantCache, batch: CacheBatch, *, tokens: str = "all",
                                           _DTYPES.get(dtype) if out is None else out,
                                           *_here(cache))
         if done is not None:
-            return done
+            return _answer(done)
     _quant_call(cache, batch, stream)
     n = batch.read_tokens if tokens == "all" else batch.num_tokens
     if out is None:
@@ -1330,7 +1339,7 @@ def quant_attend(cache: QuantCache, batch: CacheBatch, q: torch.Tensor, *,
         done = _lib.hostargs().quant_attend(cache._packed, batch._packed, q, out, scale,
                                             *_here(cache))
         if done is not None:
-            return done
+            return _answer(done)
     _quant_call(cache, batch, stream)
     qp = _rows_arg(q, "q", batch.heads, cache, (torch.bfloat16, torch.float16))
     if out is None:

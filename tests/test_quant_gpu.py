@@ -878,3 +878,38 @@ def test_an_error_that_other_code_left_is_not_a_call_s_own(gpu):
         ops.quant_read(cache, batch, stream=stream)
         ops.quant_write(cache, batch, x, x)
         assert hip.hipGetLastError() == 0
+
+
+def test_a_call_that_fails_is_not_made_again(gpu):
+    """The native path takes what it cannot read to the general one; a call that the
+    library itself refused or could not finish is an error at once."""
+    import struct
+
+    from aegaeon_amd import _lib
+
+    cache, _, _ = make(gpu, "mxfp4", 8, 16, 2, 128)
+    batch = batch_for(gpu, [[0, 1]], [20], [2], cache, heads=4)
+    x = torch.zeros(2, 2, 128, dtype=BF16, device=gpu)
+    q = torch.zeros(2, 4, 128, dtype=BF16, device=gpu)
+    calls = []
+
+    @ctypes.CFUNCTYPE(ctypes.c_int)
+    def fails():
+        calls.append(1)
+        return 98       # hipErrorInvalidDeviceFunction, as a launch would return it
+
+    at = ctypes.cast(fails, ctypes.c_void_p).value
+    was = cache._packed
+    cache._packed = struct.pack("3q", at, at, at) + was[24:]
+    for call in (lambda: ops.quant_write(cache, batch, x, x),
+                 lambda: ops.quant_read(cache, batch),
+                 lambda: ops.quant_read(cache, batch, tokens="new", out=(x, x.clone())),
+                 lambda: ops.quant_attend(cache, batch, q)):
+        calls.clear()
+        with pytest.raises(_lib.AegkvError):
+            call()
+        assert len(calls) == 1
+    cache._packed = was
+    with pytest.raises(ValueError, match="tokens"):
+        ops.quant_write(cache, batch, x[:1], x[:1])
+    ops.quant_attend(cache, batch, q)
