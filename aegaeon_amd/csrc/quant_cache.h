@@ -678,13 +678,17 @@ __device__ __forceinline__ void load_query(ColdArgs args, ItemPtr it, int32_t ro
 // to it. The types' relative precision is the same over the whole range
 // between; looked through for every tile, with the lanes' exchange, it took a
 // third of the arithmetic.
+// Added to a product of a score of thousands, `lift` is off by as much as it was rounded
+// by: nothing beside what rounds such a score, until (past 2^28) it is more than the
+// exponents have room for. Rows whose lift passes kLimit take each tile the long
+// way, against their largest score itself. So do rows that have no score yet.
 // The sum is that of the rounded probabilities, the ones that V is multiplied
 // with, as one more product, with ones: what rounding adds to both cancels
 // in part (against 64 bits 0.0021 instead of 0.0023 in bfloat16), every lane of a
 // row has it, and a matrix instruction does the work of seven additions.
 struct RowState {
   float top = -INFINITY;
-  float lift = 1e30f;    // kLift - top * c; as large while there is no top
+  float lift = 1e30f;    // kLift - top * c; past kLimit while there is no top
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};   // four times the same
 };
 
@@ -692,15 +696,16 @@ struct RowState {
 template <typename T, int N>
 __device__ __forceinline__ typename Operand<T>::v8 softmax_step(const f32x4* x, float c,
                                                                RowState& s, f32x4 (&o)[N]) {
-  float e[8], largest;
-  const auto exponents = [&]() {
+  float e[8];
+  const auto exponents = [&](float from, float lift) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i / 4][i % 4], c, s.lift));
-    largest = fmaxf(fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])),
-                    fmaxf(fmaxf(e[4], e[5]), fmaxf(e[6], e[7])));
+      e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i / 4][i % 4] - from, c, lift));
   };
-  exponents();
+  exponents(0.f, s.lift);
+  const float largest =
+      fmaxf(fmaxf(fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])),
+                  fmaxf(fmaxf(e[4], e[5]), fmaxf(e[6], e[7]))), fabsf(s.lift));
   if (__any(largest > Operand<T>::kLimit)) {
     float most = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
                        fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
@@ -711,7 +716,8 @@ __device__ __forceinline__ typename Operand<T>::v8 softmax_step(const f32x4* x, 
     for (int d = 0; d < N; ++d) o[d] *= fade;
     s.top = most;
     if (most != -INFINITY) s.lift = Operand<T>::kLift - most * c;
-    exponents();
+    const bool far = (fabsf(s.lift) > Operand<T>::kLimit) & (most != -INFINITY);
+    exponents(far ? most : 0.f, far ? Operand<T>::kLift : s.lift);
   }
   typename Operand<T>::v8 p, ones;
 #pragma unroll

@@ -913,3 +913,40 @@ def test_a_call_that_fails_is_not_made_again(gpu):
     with pytest.raises(ValueError, match="tokens"):
         ops.quant_write(cache, batch, x[:1], x[:1])
     ops.quant_attend(cache, batch, q)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("new", [1, 20, 90])
+def test_scores_of_any_size(gpu, dtype, new):
+    """Scores as large as 32 bits hold, of either sign: their differences count.
+    One value of a query times one of a key, so that every score is exact; the
+    tokens with the largest one share the result."""
+    d, n, heads = 64, 400, 2
+    tables = tables_for([n], 16, 30)
+    big = 2.0 ** 100 if dtype == BF16 else 2.0 ** 13
+    for sign in (1, -1):
+        k_ref = ref.Pages("mxfp8", 30, 16, heads, d)
+        v_ref = ref.Pages("mxfp8", 30, 16, heads, d)
+        gen = torch.Generator().manual_seed(5)
+        k = torch.zeros(n, heads, d)
+        k[:, :, 0] = sign * big * (1 + torch.randint(0, 8, (n, heads), generator=gen) / 8)
+        v = torch.randn(n, heads, d, generator=gen)
+        place = ref.places(tables[0], 16, range(n))
+        k_ref.put(*place, *ref.quantise("mxfp8", k))
+        v_ref.put(*place, *ref.quantise("mxfp8", v))
+        assert torch.equal(k_ref.get(*place), k.double())       # no key was rounded
+        cache = ops.QuantCache(k_ref.raw.to(gpu), v_ref.raw.to(gpu), kv_heads=heads, head_dim=d,
+                               block_size=16, fmt="mxfp8")
+        batch = batch_for(gpu, tables, [n], [new], cache, heads=4)
+        for size in ((1, 2.0 ** 20) if dtype == BF16 else (1, 2.0 ** 15)):
+            q = torch.zeros(new, 4, d)
+            q[:, :, 0] = size
+            q = q.to(dtype)
+            out = ops.quant_attend(cache, batch, q.to(gpu), scale=1.0).cpu().double()
+            see = ref.visible(n, new, 0, 0)
+            want, weight, _ = ref.attend(k_ref.get(*place), v_ref.get(*place), q, see, 1.0)
+            # scores are exact and differ by 2^9 and more, where they do: beside what
+            # rounds probabilities and result, only sums of up to n terms in 32 bits
+            u = torch.finfo(dtype).eps / 2
+            tol = u * want.abs() + weight * (u + (n + 8) * 2.0 ** -24) * 1.01
+            assert ((out - want).abs() <= tol).all(), (sign, size, float((out - want).abs().max()))
