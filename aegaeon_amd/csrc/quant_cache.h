@@ -354,13 +354,17 @@ __global__ __launch_bounds__(kSpanLanes) void quant_read_kernel(SpanArgs a) {
 // --------------------------------------------------------------- attention --
 
 // Matrix operands in the queries' type. The cache's values are exact in
-// bfloat16 and, between 2^-24 and its largest value, in float16.
+// bfloat16 and, between 2^-24 and its largest value, in float16. Groups whose scale
+// byte is kFar or more may hold values beyond that (4 or 256 times the scale), or no
+// number.
 template <typename T>
 struct Operand;
 template <>
 struct Operand<__bf16> {
   typedef bf16x8 v8;
   static constexpr float kLift = 0.f, kLimit = 65536.f;
+  template <int FMT>
+  static constexpr uint32_t kFar = Format<FMT>::kBits == 4 ? 253 : 247;   // 2^128
   static __device__ __forceinline__ f32x4 mma(v8 a, v8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
@@ -380,6 +384,8 @@ struct Operand<_Float16> {
   // probabilities of long contexts are not lost beside the largest one (the sum
   // is lifted alike), and a row may still grow 2^8-fold
   static constexpr float kLift = 7.f, kLimit = 32768.f;
+  template <int FMT>
+  static constexpr uint32_t kFar = Format<FMT>::kBits == 4 ? 141 : 135;   // 2^16
   static __device__ __forceinline__ f32x4 mma(v8 a, v8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
@@ -531,11 +537,26 @@ struct VPart {
     }
   }
 
+  // Whether a group may hold what is no operand of the queries' type: some scale
+  // byte reaches kFar (a byte's low bits carry into its top one, which is set).
+  template <typename T>
+  __device__ __forceinline__ bool far() const {
+    constexpr uint32_t kFar = Operand<T>::template kFar<FMT>;
+    static_assert(kFar >= 128, "the byte's top bit is set");
+    uint32_t found = 0;
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+      found |= ((scale[half] & 0x7F7F7F7Fu) + (256 - kFar) * 0x01010101u) & scale[half];
+    return (found & 0x80808080u) != 0;
+  }
+
   // What no row of [low, high] sees may hold anything: its product with a
-  // probability of 0 has to be 0. Returns the seen tokens (bit 4 half + i) that are
-  // no number; they count as 0 too and are noted apart.
-  __device__ __forceinline__ uint32_t clear_unseen(int32_t begin, int32_t g, int32_t low,
-                                                   int32_t high, int32_t window, int32_t sinks) {
+  // probability of 0 has to be 0. Returns the seen tokens (bit 4 half + i) whose
+  // values here are no operands of the queries' type, or are no numbers; they count
+  // as 0 too, for the rows that do not see them, and add_far adds them for the others.
+  template <typename T>
+  __device__ __forceinline__ uint32_t clear(int32_t begin, int32_t g, int32_t low, int32_t high,
+                                            int32_t window, int32_t sinks) {
     uint32_t odd = 0;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -544,7 +565,12 @@ struct VPart {
         const int32_t j = begin + 16 * half + 4 * g + i;
         const bool any = (j <= high) & ((low - j < window) | (j < sinks));
         const uint32_t byte = (scale[half] >> (8 * i)) & 255u;
-        const bool number = byte != kNoNumber;
+        bool number = byte < Operand<T>::template kFar<FMT>;
+        if constexpr (Format<FMT>::kBits == 8) {   // E4M3 has codes that are none
+#pragma unroll
+          for (int w = 0; w < kWords; ++w)
+            number &= (((code[half][i][w] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) == 0;
+        }
         odd |= (any & !number) ? 1u << (4 * half + i) : 0u;
         const uint32_t keep = (any & number) ? ~0u : 0u;
         scale[half] = (scale[half] & ~(255u << (8 * i))) | ((keep ? byte : 127u) << (8 * i));
@@ -602,32 +628,72 @@ __device__ __forceinline__ bool seen(const Scope& a, int32_t p, int32_t j) {
   return (j <= p) & ((p - j < a.window) | (j < a.sinks));
 }
 
-// Rows that see a V that is no number are none in its group of values; the
-// others, in whose product it had to count as 0, stay as they are. Sets in
-// `poison` bit (D / 128 or 1) r + i where the lane's row of row tile r is none
-// in the i-th group of the lane's values [D/4 g, D/4 (g + 1)). none(group, t):
-// whether the tile's token t is no number there.
-template <int D, int R, typename F>
-__device__ __forceinline__ void note_odd(const Scope& a, const F& none, int32_t begin,
-                                         const int32_t* position, int g, uint32_t& poison) {
-  constexpr int kEach = D == 256 ? 2 : 1;
-#pragma unroll 1
-  for (int t = 0; t < kTile; ++t) {
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const bool is_none = none(D == 64 ? g / 2 : g * kEach + i, t);
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-        poison |= (is_none & seen(a, position[r], begin + t)) ? 1u << (kEach * r + i) : 0u;
-    }
-  }
+// The tokens of `odd` (a lane's bits, as VPart::clear gives them): bit m for token t of the
+// tile where lane m of its four tokens' has it.
+__device__ __forceinline__ uint32_t lanes_of(uint32_t odd, int t) {
+  const uint64_t all = __ballot((odd >> (4 * (t / 16) + t % 4)) & 1);
+  return static_cast<uint32_t>(all >> (16 * (t % 16 / 4))) & 0xFFFFu;
 }
 
-// A value of the result, or none.
-template <int D>
-__device__ __forceinline__ float unless_poisoned(float x, uint32_t poison, int r, int i) {
-  constexpr int kEach = D == 256 ? 2 : 1;
-  return (poison >> (kEach * r + (kEach == 2 ? i / 2 : 0))) & 1 ? __uint_as_float(0x7FC00000u) : x;
+// Adds to the rows of R row tiles that see them, in 32 bits, the tokens that
+// were cleared from V's operands: values [FIRST, FIRST + COUNT) of the runs [D/16 m, D/16
+// (m + 1)) with m in who(t), which is the same for the whole wave. Read anew from
+// the cache, a token at a time: they are rare. By selection, as above where scores
+// are hidden.
+template <int FMT, int D, typename T, int R, int FIRST, int COUNT, typename W>
+__device__ __forceinline__ void add_far(const Scope& a, const W& who,
+                                        const AEGKV_CONSTANT int32_t* table, int64_t head_offset,
+                                        int32_t begin, const int32_t* position, int m, int g,
+                                        const typename Operand<T>::v8* p, f32x4 (*o)[D / 16]) {
+  constexpr int kBits = Format<FMT>::kBits, kRun = Chunk<FMT, D>::kCode / 16;
+  constexpr int kEach = COUNT < 8 ? COUNT : 8;
+#pragma unroll 1
+  for (int t = 0; t < kTile; ++t) {
+    const uint32_t lanes = who(t);
+    if (!lanes) continue;
+    // nothing of this is held in registers while there are no such tokens
+    int first = 4 * g, row = m;
+    asm volatile("" : "+v"(first), "+v"(row));
+    const int32_t j = begin + t;
+    const Half h = find_half<FMT, D>(a.pages, head_offset, a.block_shift,
+                                     table[j >> a.block_shift], j);
+    float weight[R];
+    bool sees[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      uint32_t w[4];
+      __builtin_memcpy(w, &p[r], 16);
+      const int word = 2 * (t / 16) + t % 4 / 2;
+      const uint32_t pair = static_cast<uint32_t>(
+          __shfl(static_cast<int>(word < 2 ? (word ? w[1] : w[0]) : (word == 2 ? w[2] : w[3])),
+                 16 * (t % 16 / 4) + row));
+      weight[r] = static_cast<float>(
+          __builtin_bit_cast(T, static_cast<uint16_t>(t % 2 ? pair >> 16 : pair)));
+      sees[r] = seen(a, position[r], j);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t run = first + i;
+      const bool here = (lanes >> run) & 1;
+#pragma unroll
+      for (int at = 0; at < COUNT; at += kEach) {
+        Codes<FMT> c = {};
+        __builtin_memcpy(c.w, h.v + run * kRun + (FIRST + at) * kBits / 8, kEach * kBits / 8);
+        c.byte = static_cast<uint8_t>(h.v_scales[(run * D / 512) << a.block_shift]);
+        float x[8];
+        c.decode(x);
+        __builtin_amdgcn_sched_barrier(0);   // one run at a time: few registers
+#pragma unroll
+        for (int d = 0; d < kEach; ++d)
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const float was = o[r][FIRST + at + d][i];
+            o[r][FIRST + at + d][i] =
+                (here & sees[r]) ? __builtin_fmaf(weight[r], x[d], was) : was;
+          }
+      }
+    }
+  }
 }
 
 // Which of the tiles that rows [low, high] visit comes v-th.
@@ -830,7 +896,6 @@ __device__ __forceinline__ void attend_item(const Scope& a, ItemPtr it, Joined<D
 
   f32x4 o[R][kOut];
   RowState state[R];
-  uint32_t poison = 0;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
 #pragma unroll
@@ -862,7 +927,8 @@ __device__ __forceinline__ void attend_item(const Scope& a, ItemPtr it, Joined<D
     // the changed elements the compiler lost one of the changes (the first
     // element's, its operands being copied out of the matrix registers in
     // several places).
-    if (!seen_whole(a, low, high, begin)) {
+    uint32_t odd = 0;
+    if (!seen_whole(a, low, high, begin) || __any(t.v.template far<T>())) {
 #pragma unroll
       for (int half = 0; half < 2; ++half)
 #pragma unroll
@@ -871,15 +937,7 @@ __device__ __forceinline__ void attend_item(const Scope& a, ItemPtr it, Joined<D
           for (int r = 0; r < R; ++r)
             x[r][half][i] = seen(a, position[r], begin + 16 * half + 4 * g + i) ? x[r][half][i]
                                                                                 : -INFINITY;
-      const uint32_t odd = t.v.clear_unseen(begin, g, low, high, a.window, a.sinks);
-      if (__any(odd != 0)) {
-        // lane m of the operand holds the group of values [D/16 m, ..)
-        const auto none = [&](int group, int i) {
-          const int from = (i % 16) / 4 * 16 + group * 512 / D;
-          return ((__shfl(static_cast<int>(odd), from) >> (4 * (i / 16) + i % 4)) & 1) != 0;
-        };
-        note_odd<D, R>(a, none, begin, position, g, poison);
-      }
+      odd = t.v.template clear<T>(begin, g, low, high, a.window, a.sinks);
     }
 
     v8 p[R];
@@ -898,14 +956,18 @@ __device__ __forceinline__ void attend_item(const Scope& a, ItemPtr it, Joined<D
         o[r][2 * B + 1] = Operand<T>::mma(second, p[r], o[r][2 * B + 1]);
       }
     });
+    if (__any(odd != 0))
+      add_far<FMT, D, T, R, 0, kOut>(a, [&](int i) { return lanes_of(odd, i); }, table,
+                                     head_offset, begin, position, m, g, p, o);
     if (more) t.v.load(h, a.block_shift, m, g, 0);
     at += kAttendWaves;
   };
   while (at < tiles.end) {
     step(held[0]);
     if constexpr (kAhead == 2) {
-      if (at >= tiles.end) break;
-      step(held[1]);
+      // not by leaving the loop: then the compiler held twenty registers more
+      // and spilled some (64 decodes: 71 us instead of 58)
+      if (at < tiles.end) step(held[1]);
     }
   }
 
@@ -935,8 +997,7 @@ __device__ __forceinline__ void attend_item(const Scope& a, ItemPtr it, Joined<D
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int d = 0; d < kOut; ++d)
-        share.part[wave][m][(D / 16) * (4 * g + i) + d] =
-            unless_poisoned<D>(o[r][d][i] * fade, poison, r, i);
+        share.part[wave][m][(D / 16) * (4 * g + i) + d] = o[r][d][i] * fade;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
@@ -994,13 +1055,17 @@ __global__ __launch_bounds__(kAttendLanes, (kAttendPerSimd<D, R>)) void quant_at
 // cycles, for each score); reading operands earlier, waiting for loads elsewhere,
 // loads without conditions and wave priorities changed less than 3 %.
 constexpr int kStageTiles = 2, kWaveRows = 32;
+static_assert(kAttendWaves == 4 && kStageTiles == 2, "a wave makes half a tile's operands");
 static_assert(kManyRows == kAttendWaves * kWaveRows, "rows of a workgroup");
 
 template <int D>
 struct Stage {
   v4u k[2 * kStageTiles][D / 32][64];
   v4u v[kStageTiles][D / 16][64];
-  uint8_t odd[kStageTiles][D / 32][4];   // of four tokens in each half: no numbers
+  // tokens that V's operands lack, for each half of a lane's values: whether
+  // there are any (by the wave that made them), and then the lanes that cleared them (lanes_of)
+  v4u far;
+  uint16_t far_lanes[kStageTiles][2][kTile];
 };
 
 template <int FMT, int D, typename T>
@@ -1034,15 +1099,29 @@ __device__ __forceinline__ void attend_prompt_item(const Scope& a, ItemPtr it,
     v.load(h, a.block_shift, m, g, own_half * kVBytes);
   };
   const auto lay = [&](Stage<D>& to, int32_t at) {
-    if (at + own_tile >= tiles.end) return;
+    uint32_t* const own_far = reinterpret_cast<uint32_t*>(&to.far) + wave;
+    if (at + own_tile >= tiles.end) {
+      if (lane == 0) *own_far = 0;
+      return;
+    }
     each_constant<0, kSteps>([&](auto s) {
       const v8 f = k.template operand<T, decltype(s)::value>();
       __builtin_memcpy(&to.k[wave][decltype(s)::value][lane], &f, 16);
     });
     const int32_t begin = tiles.at(at + own_tile) * kTile;
-    if (!seen_whole(a, low, high, begin)) {
-      const uint32_t odd = v.clear_unseen(begin, g, low, high, a.window, a.sinks);
-      if (own_half == 0 && m % (512 / D) == 0) to.odd[own_tile][m * D / 512][g] = odd;
+    uint32_t odd = 0;
+    if (!seen_whole(a, low, high, begin) || __any(v.template far<T>()))
+      odd = v.template clear<T>(begin, g, low, high, a.window, a.sinks);
+    const bool far = __any(odd != 0);
+    if (lane == 0) *own_far = far;
+    if (far) {
+      uint32_t lanes = 0;
+#pragma unroll 1
+      for (int t = 0; t < kTile; ++t) {
+        const uint32_t found = lanes_of(odd, t);
+        lanes = lane == t ? found : lanes;
+      }
+      if (lane < kTile) to.far_lanes[own_tile][own_half][lane] = static_cast<uint16_t>(lanes);
     }
     float scale[2][4];
     v.scales(scale);
@@ -1064,7 +1143,6 @@ __device__ __forceinline__ void attend_prompt_item(const Scope& a, ItemPtr it,
   int32_t position[R];
   f32x4 o[R][kOut];
   RowState state[R];
-  uint32_t poison = 0;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const bool there = 16 * r + m < rows;
@@ -1074,7 +1152,7 @@ __device__ __forceinline__ void attend_prompt_item(const Scope& a, ItemPtr it,
     for (int d = 0; d < kOut; ++d) o[r][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  const auto multiply = [&](const Stage<D>& from, int32_t at, int tile) {
+  const auto multiply = [&](const Stage<D>& from, int32_t at, int tile, uint32_t any_far) {
     if (at + tile >= tiles.end) return;
     const int32_t begin = tiles.at(at + tile) * kTile;
     // tiles that none of the wave's rows sees
@@ -1113,21 +1191,6 @@ __device__ __forceinline__ void attend_prompt_item(const Scope& a, ItemPtr it,
             x[r][half][i] = seen(a, position[r], begin + 16 * half + 4 * g + i) ? x[r][half][i]
                                                                                 : -INFINITY;
     }
-    if (!seen_whole(a, low, high, begin)) {   // then its no numbers were cleared
-      uint32_t odd = 0;
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        uint32_t w;
-        __builtin_memcpy(&w, from.odd[tile][i], 4);
-        odd |= w;
-      }
-      if (odd) {
-        const auto none = [&](int group, int t) {
-          return ((from.odd[tile][group][(t % 16) / 4] >> (4 * (t / 16) + t % 4)) & 1) != 0;
-        };
-        note_odd<D, R>(a, none, begin, position, g, poison);
-      }
-    }
     v8 p[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) p[r] = softmax_step<T>(x[r], a.c, state[r], o[r]);
@@ -1135,6 +1198,17 @@ __device__ __forceinline__ void attend_prompt_item(const Scope& a, ItemPtr it,
     for (int d = 0; d < kOut; ++d)
 #pragma unroll
       for (int r = 0; r < R; ++r) o[r][d] = Operand<T>::mma(vf[d], p[r], o[r][d]);
+    if (!__builtin_amdgcn_readfirstlane(any_far)) return;
+    const auto add = [&](auto half) {
+      constexpr int kHalf = decltype(half)::value;
+      if (!__builtin_amdgcn_readfirstlane(uint32_t{from.far[2 * tile + kHalf]})) return;
+      add_far<FMT, D, T, R, kHalf * kOut / 2, kOut / 2>(
+          a, [&](int t) {
+            return __builtin_amdgcn_readfirstlane(uint32_t{from.far_lanes[tile][kHalf][t]});
+          }, table, head_offset, begin, position, m, g, p, o);
+    };
+    add(std::integral_constant<int, 0>{});
+    add(std::integral_constant<int, 1>{});
   };
 
   int turn = 0;
@@ -1142,8 +1216,10 @@ __device__ __forceinline__ void attend_prompt_item(const Scope& a, ItemPtr it,
     lay(stages[turn], at);
     load(at + kStageTiles);
     __syncthreads();
+    const v4u far = stages[turn].far;
+    const uint32_t any_far = far[0] | far[1] | far[2] | far[3];
 #pragma unroll
-    for (int tile = 0; tile < kStageTiles; ++tile) multiply(stages[turn], at, tile);
+    for (int tile = 0; tile < kStageTiles; ++tile) multiply(stages[turn], at, tile, any_far);
   }
 
   const ColdArgs end_args = cold_args();
@@ -1161,7 +1237,7 @@ __device__ __forceinline__ void attend_prompt_item(const Scope& a, ItemPtr it,
     for (int i = 0; i < 4; ++i) {
       float y[kOut];
 #pragma unroll
-      for (int d = 0; d < kOut; ++d) y[d] = unless_poisoned<D>(o[r][d][i] * inv, poison, r, i);
+      for (int d = 0; d < kOut; ++d) y[d] = o[r][d][i] * inv;
       const int first = kOut * (4 * g + i);
       if (slot >= 0) {
 #pragma unroll

@@ -607,10 +607,12 @@ int aegkv_quant_read(const void* plan, const void* device_plan, int format, int3
  * positions j that query i sees of softmax_j(scale * q[i] . K[j]) V[j], query
  * head h over KV head h / (heads / kv_heads). q and out: [num_tokens][heads]
  * [head_dim] of bfloat16 or float16; rows behind the batch's last token are left as
- * they were. out may be q itself (the same place and strides). The cache's values are taken in the queries' type
- * (bfloat16 holds them all but those of 2^128; float16 rounds what is below
- * 2^-14, and beyond its range a value is an infinity). Scores, softmax and sums
- * are held in 32 bits; probabilities enter the second product in the queries' type.
+ * they were. out may be q itself (the same place and strides). K and V are taken in
+ * the queries' type, in which float16 rounds what is below 2^-14. Beyond its range
+ * (65504; bfloat16: 2^128) a value of K is an infinity; one of V is added in 32 bits.
+ * Scores, softmax and sums are held in 32 bits, and probabilities enter the second
+ * product in the queries' type, up to 2^16 times a row's reference: sums over values
+ * of 2^100 and more may overflow.
  * What a query does not see changes nothing, NaN included.
  *
  * workspace: aegkv_quant_attend_workspace bytes of device memory, 16-byte aligned,

@@ -950,3 +950,67 @@ def test_scores_of_any_size(gpu, dtype, new):
             u = torch.finfo(dtype).eps / 2
             tol = u * want.abs() + weight * (u + (n + 8) * 2.0 ** -24) * 1.01
             assert ((out - want).abs() <= tol).all(), (sign, size, float((out - want).abs().max()))
+
+
+@pytest.mark.parametrize("fmt,d,bs", SHAPES)
+@pytest.mark.parametrize("new", [1, 12, 60])
+@pytest.mark.parametrize("group,window,sinks", [(1, 0, 0), (4, 0, 0), (4, 50, 5)])
+def test_values_beyond_the_queries_type(gpu, fmt, d, bs, new, group, window, sinks):
+    """V of up to 3e5 under float16 queries: rows that see it have the sum as 32 bits
+    hold it, the others are as without it; a code that is no number (mxfp8) makes one
+    value none, in the rows that see its token."""
+    n, heads = 200, 2
+    tables = tables_for([n], bs, 16)
+    cache, k, v = make(gpu, fmt, 16, bs, heads, d, seed=4)
+    c, s = v._views()
+    byte = {"mxfp4": 127 + 15, "mxfp8": 127 + 9}[fmt]
+    tokens = [3, 33, n - new, n - new // 2 - 1, n - 1]
+    for i, t in enumerate(tokens):
+        block, inside = ref.places(tables[0], bs, [t])
+        s[block, i % heads, i % (d // 32), inside] = byte
+    if fmt == "mxfp8":
+        block, inside = ref.places(tables[0], bs, [n - 1])
+        c[block, 1, inside, d - 3] = 0x7F
+    cache = ops.QuantCache(k.raw.to(gpu), v.raw.to(gpu), kv_heads=heads, head_dim=d,
+                           block_size=bs, fmt=fmt)
+    batch = batch_for(gpu, tables, [n], [new], cache, heads=heads * group, window=window,
+                      sinks=sinks)
+    q = torch.randn(new, heads * group, d, generator=torch.Generator().manual_seed(1))
+    q = q.to(F16).to(gpu)
+    out = ops.quant_attend(cache, batch, q)
+    see = ref.visible(n, new, window, sinks)
+    any_ = see.any(0).nonzero()[:, 0].tolist()
+    place = ref.places(tables[0], bs, any_)
+    want, weight, size = ref.attend(k.get(*place), v.get(*place), q.cpu(), see[:, any_], d ** -0.5)
+    tol = ref.tolerance(want, weight, size, len(any_), d, F16)
+    got = out.cpu().double()
+    near = (got - want).abs() <= tol
+    # the result is a float16 itself: from 65520 on, half a step past the largest
+    # one, a sum that is right rounds to infinity
+    far = (got == want.sign() * math.inf) & (want.abs() + tol >= 65520)
+    assert (near | far | (got.isnan() & want.isnan())).all()
+    none = out.isnan().cpu()
+    if fmt == "mxfp8":
+        assert none[-1, group:, d - 3].all()
+        none[-1, group:, d - 3] = False
+    assert not none.any()
+
+
+@pytest.mark.parametrize("fmt,d,bs", [SHAPES[0], SHAPES[1]])
+def test_values_of_two_to_the_128_stay_with_the_rows_that_see_them(gpu, fmt, d, bs):
+    """The one power of two that bfloat16 and float32 lack."""
+    n, new = 100, 40
+    tables = tables_for([n], bs, 16)
+    cache, k, v = make(gpu, fmt, 16, bs, 2, d, seed=4)
+    c, s = v._views()
+    block, inside = ref.places(tables[0], bs, [n - 1])
+    s[block, 1, 0, inside] = 254 if fmt == "mxfp4" else 248
+    c[block, 1, inside, 0] = 0x66 if fmt == "mxfp4" else 0x78       # 4 * 2^127, 256 * 2^121
+    cache = ops.QuantCache(k.raw.to(gpu), v.raw.to(gpu), kv_heads=2, head_dim=d, block_size=bs,
+                           fmt=fmt)
+    batch = batch_for(gpu, tables, [n], [new], cache)
+    q = torch.randn(new, 2, d, generator=torch.Generator().manual_seed(1)).to(BF16).to(gpu)
+    out = ops.quant_attend(cache, batch, q)
+    assert not out[-1, 1, 0].isfinite()
+    assert out[:-1].isfinite().all() and out[-1, 0].isfinite().all()
+    check_attend(out[:-1], k, v, tables, [n - 1], [new - 1], q[:-1], bs, BF16)
