@@ -145,6 +145,25 @@ inline int64_t share_out(const std::vector<Rows>& rows, int64_t kv_heads, int ki
   return best;
 }
 
+// Slots that cuts into items of at most `each` tiles take, and the merges that join them.
+struct Parts {
+  int64_t slots, merges;
+};
+
+inline int64_t merges_of(int64_t rows, int64_t parts) {
+  return parts == 1 ? 0 : up(rows, parts <= kMergeRows ? kMergeRows : 1);
+}
+
+inline Parts parts_of(const std::vector<Rows>& rows, int64_t kv_heads, int64_t each) {
+  Parts p{0, 0};
+  for (const Rows& r : rows) {
+    const int64_t parts = up(r.tiles, each);
+    if (parts > 1) p.slots += parts * kv_heads;
+    p.merges += merges_of(r.rows, parts) * kv_heads;
+  }
+  return p;
+}
+
 inline int check(const Header& h, const Batch& b) {
   std::vector<int64_t> written;   // (block, first, end) of every block written
   int64_t columns = 0, tokens = 0, all = 0;
@@ -268,7 +287,13 @@ inline int fill(Header& h, const Batch& b, const std::vector<Rows>* rows, char* 
       return aegkv_set_error(AEGKV_ENOMEM, "the plan has no room for sequences of this many new "
                              "tokens (%s rows under a KV head)",
                              kind == kMany ? "over 64" : kind == kMore ? "17 to 64" : "up to 16");
-    const int64_t each = share_out(all, h.kv_heads, kind, room.items[kind]);
+    int64_t each = share_out(all, h.kv_heads, kind, room.items[kind]);
+    // a plan that was cut to another batch may have room for fewer parts: whole rows
+    // need none
+    for (Parts p = parts_of(all, h.kv_heads, each);
+         p.slots > room.slots[kind] || merges + p.merges > room.merges;
+         p = parts_of(all, h.kv_heads, each))
+      each *= 2;
     // the longest go first, so that the last to end are short
     std::vector<size_t> order(all.size());
     for (size_t i = 0; i < order.size(); ++i) order[i] = i;
@@ -292,9 +317,6 @@ inline int fill(Header& h, const Batch& b, const std::vector<Rows>* rows, char* 
         if (parts == 1) continue;
         const int32_t rows_each = parts <= kMergeRows ? kMergeRows : 1;
         for (int32_t first = 0; first < r.rows; first += rows_each) {
-          if (merges >= room.merges || slots > room.slots[kind])
-            return aegkv_set_error(AEGKV_ENOMEM, "the plan has no room for %lld parts of sums",
-                                   ll(slots));
           merge[merges++] = Merge{r.seq, head, r.row + first,
                                   std::min(rows_each, r.rows - first),
                                   static_cast<int32_t>(slot), static_cast<int32_t>(parts), kind,
@@ -309,7 +331,8 @@ inline int fill(Header& h, const Batch& b, const std::vector<Rows>* rows, char* 
   return 0;
 }
 
-// Room for the batch itself, or for any within the given bounds.
+// Room for the batch itself, or if bounds are given, for any within them: also where
+// this one is as large as they are, as the step is that a graph is captured on.
 inline void make_room(Header& h, const Batch& b, const std::vector<Rows>* rows, int64_t max_seqs,
                       int64_t max_columns, int64_t max_tokens) {
   Room& r = h.room;
@@ -321,7 +344,7 @@ inline void make_room(Header& h, const Batch& b, const std::vector<Rows>* rows, 
     if (fresh) new_spans += up(len, kSpan) - (len - fresh) / kSpan;
     read_spans += up(len, kSpan);
   }
-  const bool exact = max_seqs <= b.num_seqs && max_columns <= columns && max_tokens <= tokens;
+  const bool exact = max_seqs == 0 && max_columns == 0 && max_tokens == 0;
   r.seqs = std::max(max_seqs, b.num_seqs);
   max_columns = std::max(max_columns, columns);
   r.columns = max_columns + r.seqs;
@@ -344,12 +367,9 @@ inline void make_room(Header& h, const Batch& b, const std::vector<Rows>* rows, 
     if (count && exact) {
       const int64_t each = share_out(rows[kind], h.kv_heads, kind, INT32_MAX);
       r.items[kind] = items_of(rows[kind], h.kv_heads, each);
-      for (const Rows& x : rows[kind]) {
-        const int64_t parts = up(x.tiles, each);
-        if (parts == 1) continue;
-        r.slots[kind] += parts * h.kv_heads;
-        r.merges += up(x.rows, parts <= kMergeRows ? kMergeRows : 1) * h.kv_heads;
-      }
+      const Parts p = parts_of(rows[kind], h.kv_heads, each);
+      r.slots[kind] = p.slots;
+      r.merges += p.merges;
     } else if (count) {
       const int64_t most = (kind == kMany   ? r.tokens * h.group / kManyRows + r.seqs
                             : kind == kMore ? r.seqs * (kMostMore / kKindRows[kMore])

@@ -1031,7 +1031,9 @@ class CacheBatch:
     its place, also for calls captured into a graph, if it fits the room
     that max_seqs, max_columns (of all block tables) and max_tokens (new ones) asked
     for and its sequences have as many rows (new tokens times heads / kv_heads) as
-    the first batch's: up to 16, up to 64, or more.
+    the first batch's: up to 16, up to 64, or more. The room may be what the first
+    batch holds itself. Without any (all 0) a batch takes less memory, and an update
+    of the same lengths.
     """
 
     def __init__(self, block_tables, seq_lens, new_lens, *, num_blocks: int, block_size: int,

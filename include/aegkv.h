@@ -548,10 +548,12 @@ int aegkv_quant_page_bytes(int format, int32_t block_size, int32_t kv_heads, int
  *
  * `plan` takes *plan_bytes bytes, which a call with a null plan sets; the
  * caller copies them to the device (16-byte aligned) before the calls that take both.
- * max_seqs, max_columns and max_tokens (new ones) ask for room beyond this
- * batch's own. With update != 0, plan is an earlier plan of *plan_bytes bytes
+ * max_seqs, max_columns and max_tokens (new ones), if any is not 0, ask for room for
+ * every batch within them and this batch's own sizes; if all are 0, the plan is cut
+ * to this batch. With update != 0, plan is an earlier plan of *plan_bytes bytes
  * over the same blocks, heads, window and sinks, which is rewritten in place if
- * the batch fits its room (AEGKV_ENOMEM otherwise, and the plan is unchanged):
+ * the batch fits its room (AEGKV_ENOMEM otherwise, and the plan is unchanged; without room
+ * asked for, one of the same lengths fits):
  * the caller copies it to the same device memory again, ordered behind the
  * calls that use what it held, and calls captured into a graph then work on the
  * new batch when they are replayed. A plan with room takes sequences with as

@@ -284,3 +284,20 @@ def test_places_that_overlap_under_sanitizers(tmp_path):
     run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
     assert run.returncode == 0, run.stdout + run.stderr
     assert "clean" in run.stdout
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="g++ is not installed")
+def test_updates_within_the_room_are_taken_under_sanitizers(tmp_path):
+    """tests/native/batch_room_check.cpp: whatever batch a plan was made for, also one
+    that fills its room."""
+    exe = tmp_path / "batch_room_check"
+    cmd = ["g++", "-std=c++17", "-O1", "-g", "-fno-omit-frame-pointer", "-Wall",
+           "-fsanitize=address,undefined", "-fno-sanitize-recover=all", "-Wno-unused-function",
+           "-D__HIP_PLATFORM_AMD__", f"-I{REPO / 'include'}", "-I/opt/rocm/include",
+           f"-I{REPO / 'aegaeon_amd' / 'csrc'}", f"-I{REPO / 'tests' / 'native'}",
+           str(REPO / "tests" / "native" / "batch_room_check.cpp"), "-o", str(exe)]
+    res = subprocess.run(cmd, capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0, res.stderr
+    run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stdout + run.stderr
+    assert "clean" in run.stdout

@@ -1014,3 +1014,31 @@ def test_values_of_two_to_the_128_stay_with_the_rows_that_see_them(gpu, fmt, d, 
     assert not out[-1, 1, 0].isfinite()
     assert out[:-1].isfinite().all() and out[-1, 0].isfinite().all()
     check_attend(out[:-1], k, v, tables, [n - 1], [new - 1], q[:-1], bs, BF16)
+
+
+def test_a_step_captured_at_its_largest_serves_smaller_ones(gpu):
+    """The room is what the first batch holds itself; later steps have fewer
+    sequences, longer ones and other places in their blocks."""
+    heads, d, bs, blocks = 2, 128, 16, 420
+    cache, k, v = make(gpu, "mxfp4", blocks, bs, heads, d, seed=7)
+    lens = [128] * 16
+    batch = batch_for(gpu, tables_for(lens, bs, blocks), lens, [1] * 16, cache, heads=8,
+                      max_seqs=16, max_columns=128, max_tokens=16)
+    gen = torch.Generator().manual_seed(1)
+    q = torch.randn(16, 8, d, generator=gen).to(BF16).to(gpu)
+    out = torch.zeros_like(q)
+    ops.quant_attend(cache, batch, q, out=out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.quant_attend(cache, batch, q, out=out)
+    for seed, lens, new in ((1, [2048], [1]), (2, [1024, 17, 900], [1, 4, 2]), (3, [128] * 16,
+                            [1] * 16), (4, [], []), (5, [31, 0, 1500], [3, 0, 1])):
+        tables = tables_for(lens, bs, blocks, seed=seed)
+        batch.update(tables, lens, new)
+        out.fill_(3)
+        g.replay()
+        n = sum(new)
+        check_attend(out, k, v, tables, lens, new, q, bs, BF16)
+        assert (out[n:] == 3).all()
+        assert torch.equal(ops.quant_attend(cache, batch, q)[:n], out[:n])
