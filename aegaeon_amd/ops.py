@@ -1146,12 +1146,11 @@ class CacheBatch:
     def _enter(self, raw: int, stream: torch.cuda.Stream | None):
         """Order a call on the raw stream behind the upload. The stream, where
         the call is to be noted by _leave."""
-        if raw == self._stream:
-            return None
+        if raw == self._stream and _alive(self._home):
+            return None     # (a new stream may have the handle of one that is closed)
         st = stream if stream is not None else torch.cuda.current_stream(self.device)
-        with torch.cuda.stream(st):
-            if torch.cuda.is_current_stream_capturing():
-                return None     # capture begins behind a synchronize
+        if _capturing(st):
+            return None     # capture begins behind a synchronize
         if _alive(self._home):  # a closed stream was waited for
             st.wait_event(self._uploaded)
         return st
@@ -1248,8 +1247,10 @@ def _on_stream(cache: QuantCache, batch: CacheBatch, stream, fn) -> None:
     def call():
         raw = _stream_ptr(cache.device, stream)
         st = batch._enter(raw, stream)
-        _lib.check(fn(raw))
-        batch._leave(st)
+        try:
+            _lib.check(fn(raw))
+        finally:
+            batch._leave(st)    # of several launches the first may be on its way
 
     _call_on(cache.device, call)
 
@@ -1273,7 +1274,7 @@ def quant_write(cache: QuantCache, batch: CacheBatch, k: torch.Tensor, v: torch.
     and each takes its nearest code, ties to even. A group with a NaN or an
     infinity reads back as NaN.
     """
-    if stream is None:
+    if stream is None and _alive(batch._home):
         done = _lib.hostargs().quant_write(cache._packed, batch._packed, k, v, *_here(cache))
         if done is not None:
             _answer(done)
@@ -1300,7 +1301,7 @@ def quant_read(cache: QuantCache, batch: CacheBatch, *, tokens: str = "all",
     type counts); rows behind the last token are left as they were."""
     if tokens not in ("all", "new"):
         raise ValueError(f"tokens are 'all' or 'new', not {tokens!r}")
-    if stream is None:
+    if stream is None and _alive(batch._home):
         done = _lib.hostargs().quant_read(cache._packed, batch._packed, tokens == "new",
                                           _DTYPES.get(dtype) if out is None else out,
                                           *_here(cache))
@@ -1337,7 +1338,7 @@ def quant_attend(cache: QuantCache, batch: CacheBatch, q: torch.Tensor, *,
     scale: of the scores, head_dim ** -0.5 by default. `out` (q itself is fine, other
     overlaps are refused) takes the result; rows behind the batch's last token are left as they were.
     """
-    if stream is None:
+    if stream is None and _alive(batch._home):
         done = _lib.hostargs().quant_attend(cache._packed, batch._packed, q, out, scale,
                                             *_here(cache))
         if done is not None:

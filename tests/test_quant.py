@@ -204,6 +204,43 @@ def test_a_plan_s_memory_goes_back_behind_all_that_read_it(monkeypatch):
     assert dropped(monkeypatch, a, b)
 
 
+def test_calls_on_a_closed_stream_s_handle_are_noted(aegkv_lib, monkeypatch):
+    """The runtime may give a new stream the handle of one that was destroyed: calls on
+    it are not those of the batch's home, which nothing waits for any more."""
+    monkeypatch.setattr(ops, "_capturing", lambda st: False)
+    home, new = Recorded(5), Recorded(5)
+    batch = ops.CacheBatch.__new__(ops.CacheBatch)
+    batch._home = batch._pool = home
+    batch._stream, batch._used, batch._uploaded = 5, {}, "uploaded"
+    assert batch._enter(5, None) is None
+    home.closed = True
+    for fails in (False, True):     # also those that fail: something may be enqueued
+        batch._used = {}
+        cache = types.SimpleNamespace(device=torch.device("cuda", 0))
+        monkeypatch.setattr(ops, "_call_on", lambda device, fn: fn())
+        if fails:
+            with pytest.raises(ValueError):
+                ops._on_stream(cache, batch, new, lambda raw: _lib.EINVAL)
+        else:
+            ops._on_stream(cache, batch, new, lambda raw: 0)
+        assert batch._used == {5: new} and not new.waits
+    taken = []
+    native = types.SimpleNamespace(**{op: lambda *a: taken.append(1) for op in
+                                      ("quant_write", "quant_read", "quant_attend")})
+    monkeypatch.setattr(_lib, "hostargs", lambda: native)
+    batch.device = torch.device("cuda", 1)
+    batch.block_size = batch.kv_heads = batch.num_blocks = 1
+    other = types.SimpleNamespace(block_size=1, kv_heads=1, num_blocks=1,
+                                  device=torch.device("cuda", 0))
+    x = torch.zeros(1)
+    for call in (lambda: ops.quant_write(other, batch, x, x), lambda: ops.quant_read(other, batch),
+                 lambda: ops.quant_attend(other, batch, x)):
+        with pytest.raises(ValueError, match="a batch on cuda:1"):
+            call()
+    assert not taken
+    batch._home = None      # nothing to order when it goes
+
+
 def test_streams_of_another_device_are_refused(aegkv_lib):
     stream = types.SimpleNamespace(device=torch.device("cuda", 1))
     args = ([[0]], [1], [1])
