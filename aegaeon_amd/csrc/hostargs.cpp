@@ -197,7 +197,8 @@ struct QuantArgs {
     if (!t.defined() || !t.is_cuda() || t.get_device() != c.device ||
         t.layout() != at::kStrided || t.dim() != 3 || t.size(1) != heads ||
         t.size(2) != c.head_dim || !dtype_code(t.scalar_type()) || t.stride(2) != 1 ||
-        t.size(0) == 0 || (t.requires_grad() && c10::GradMode::is_enabled()))
+        t.size(0) == 0 || (t.requires_grad() && c10::GradMode::is_enabled()) ||
+        t._fw_grad(0).defined())
       return nullptr;
     return &t;
   }

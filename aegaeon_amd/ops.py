@@ -1240,6 +1240,8 @@ def _rows_arg(t: torch.Tensor, what: str, heads: int, cache: QuantCache, dtypes)
         raise ValueError(f"{what}: the last axis must be contiguous")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what} requires a gradient, which these operators do not give")
+    if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{what} carries a tangent, which these operators do not take on")
     return t.data_ptr(), t.stride(0), t.stride(1)
 
 

@@ -1042,3 +1042,30 @@ def test_a_step_captured_at_its_largest_serves_smaller_ones(gpu):
         check_attend(out, k, v, tables, lens, new, q, bs, BF16)
         assert (out[n:] == 3).all()
         assert torch.equal(ops.quant_attend(cache, batch, q)[:n], out[:n])
+
+
+def test_tangents_are_refused(gpu, monkeypatch):
+    """As gradients are: a derivative would be lost without a word."""
+    from torch.autograd import forward_ad
+
+    from aegaeon_amd import _lib
+
+    cache, _, _ = make(gpu, "mxfp4", 8, 16, 2, 128)
+    batch = batch_for(gpu, [[0, 1]], [20], [2], cache, heads=4)
+    x = torch.zeros(2, 2, 128, dtype=BF16, device=gpu)
+    q = torch.zeros(2, 4, 128, dtype=BF16, device=gpu)
+    for general in (False, True):
+        if general:
+            monkeypatch.setattr(_lib, "_hostargs", _lib._GeneralPath)
+        with forward_ad.dual_level():
+            dx = forward_ad.make_dual(x, torch.ones_like(x))
+            dq = forward_ad.make_dual(q, torch.ones_like(q))
+            for call in (lambda: ops.quant_write(cache, batch, dx, x),
+                         lambda: ops.quant_write(cache, batch, x, dx),
+                         lambda: ops.quant_attend(cache, batch, dq),
+                         lambda: ops.quant_attend(cache, batch, q, out=dq),
+                         lambda: ops.quant_read(cache, batch, tokens="new", out=(x, dx))):
+                with pytest.raises(ValueError, match="tangent"):
+                    call()
+            ops.quant_attend(cache, batch, q)
+        ops.quant_write(cache, batch, x, x)
