@@ -21,8 +21,8 @@ constexpr int kTile = 32;
 //                four waves of a workgroup take an item's tiles in turn and
 //                join at its end;
 //   kMany:       blocks of kManyRows rows, shared out to the waves.
-// 64 sequences of 2,000 tokens, 8 KV heads: 40 and 64 rows take 71 us as kMore, 83
-// and 85 as kMany; 128 rows 126 and 98.
+// 64 sequences of 2,000 tokens, 8 KV heads: 20, 40 and 64 rows take 37, 68 and 70 us as
+// kMore, 75, 85 and 87 as kMany; 128 rows 127 and 101.
 enum Kind { kFew = 0, kMore = 1, kMany = 2, kKinds = 3 };
 constexpr int kManyRows = 128;
 constexpr int kKindRows[kKinds] = {16, 32, kManyRows};

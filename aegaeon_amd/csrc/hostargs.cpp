@@ -10,7 +10,7 @@
 //
 // A decode step makes two calls a layer over a quantised cache. Their tensors
 // checked and their C arguments made in Python, they took the host 7.4 us
-// (write) and 14 (attend), 3 to 6 of which are the launches; here 4.0 and 8.1.
+// (write) and 14 (attend), 3 to 6 of which are the launches; here 3.8 and 8.3.
 // These functions too take the plain case only: None, with nothing enqueued,
 // for anything else. What the library itself answers is the answer: its status, if
 // it refused the call or failed in it, as a number. (A call made a second time

@@ -463,7 +463,10 @@ __device__ __forceinline__ Half find_half(const QuantPages& p, int64_t head_offs
   return Half{p.k + codes, p.v + codes, p.k + scales, p.v + scales};
 }
 
-// STREAM: what no other workgroup reads goes past the caches.
+// STREAM: past the caches, for what mostly one workgroup reads (64 decodes of one
+// token 58 us, through them 62). Second readers find less: the two blocks of 33 to 64
+// rows of a sequence (40 rows 69 us, through them 67; 64 rows 70 both ways) and sequences
+// that share blocks (64 decodes over a common 4,000 tokens 46 us, through them 43.5).
 template <int BYTES, bool STREAM>
 __device__ __forceinline__ void load_bytes(uint32_t* to, const char* base, uint32_t offset) {
   const char* p = base + offset;
@@ -1050,8 +1053,8 @@ __global__ __launch_bounds__(kAttendLanes, (kAttendPerSimd<D, R>)) void quant_at
 // conflicts. Two stages: while one is multiplied, the next one's bytes are on their
 // way in registers, and one barrier a stage is enough. Four prompts of 1,000 to
 // 4,096 tokens, 32 heads over 8 (158 GFLOP) take 218-230 us, 690-725 TFLOP/s; converted
-// by every wave for itself, 321. Bound by the issue of two waves a SIMD: 29 % of
-// the cycles multiply, 38 % are vector instructions (an exponential, 16
+// by every wave for itself, 321. Bound by the issue of two waves a SIMD: 30 % of
+// the cycles multiply, 39 % are vector instructions (an exponential, 16
 // cycles, for each score); reading operands earlier, waiting for loads elsewhere,
 // loads without conditions and wave priorities changed less than 3 %.
 constexpr int kStageTiles = 2, kWaveRows = 32;
