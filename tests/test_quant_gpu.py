@@ -1069,3 +1069,34 @@ def test_tangents_are_refused(gpu, monkeypatch):
                     call()
             ops.quant_attend(cache, batch, q)
         ops.quant_write(cache, batch, x, x)
+
+
+@pytest.mark.parametrize("fmt,byte", [("mxfp4", 127 + 16), ("mxfp8", 127 + 9)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_values_beyond_the_queries_type_in_rows_that_are_cut(gpu, fmt, byte, dtype):
+    """In long contexts, whose parts are joined, for single tokens and for many rows."""
+    d, bs, lens, new = 64, 16, [9000, 3000], [1, 150]
+    blocks = sum(-(-n // bs) for n in lens) + 2
+    tables = tables_for(lens, bs, blocks, seed=3)
+    cache, k, v = make(gpu, fmt, blocks, bs, 1, d, seed=5)
+    c, s = v._views()
+    for table, n, m in zip(tables, lens, new):
+        for i, t in enumerate((0, 31, n // 2, n - m, n - 1)):
+            block, inside = ref.places(table, bs, [t])
+            s[block, 0, i % 2, inside] = byte
+        if fmt == "mxfp8":      # no numbers: one that all rows see, one that only the last does
+            for t, at in ((n // 3, 5), (n - 1, 40)):
+                block, inside = ref.places(table, bs, [t])
+                c[block, 0, inside, at] = 0xFF
+    cache = ops.QuantCache(k.raw.to(gpu), v.raw.to(gpu), kv_heads=1, head_dim=d, block_size=bs,
+                           fmt=fmt)
+    batch = batch_for(gpu, tables, lens, new, cache, heads=7)
+    assert batch._workspace[d] > 0
+    q = torch.randn(sum(new), 7, d, generator=torch.Generator().manual_seed(2)).to(dtype).to(gpu)
+    out = ops.quant_attend(cache, batch, q)
+    check_attend(out, k, v, tables, lens, new, q, bs, dtype)
+    none = torch.zeros(sum(new), 7, d, dtype=torch.bool)
+    if fmt == "mxfp8":
+        none[:, :, 5] = True
+        none[[0, -1], :, 40] = True
+    assert torch.equal(out.isnan().cpu(), none)
