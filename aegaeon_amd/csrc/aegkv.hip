@@ -28,6 +28,7 @@
 #include <hip/hip_runtime.h>
 #include "aegkv.h"
 #include "batch_plan_build.h"
+#include "cache_kernels.h"
 #include "copy_walk.h"
 #include "errors.h"
 #include "staged_runs.h"
@@ -206,8 +207,6 @@ struct CopySeg {            // one backing tensor of a block copy
 static_assert(sizeof(CopySeg) == 32, "CopySeg layout");
 static_assert(sizeof(PairDesc) == 16, "PairDesc layout (descriptors are whole 16-byte words)");
 
-typedef unsigned int v4u __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(1))) v4u gv4u;  // global (VM) address space
 typedef v4u v4u_any __attribute__((aligned(1)));     // 16 bytes at any address
 typedef __attribute__((address_space(1))) v4u_any gv4u_any;
 typedef __attribute__((address_space(1))) char gchar;
@@ -2821,6 +2820,6 @@ int aegkv_host_free(void* ptr) {
 
 }  // extern "C"
 
-// ================================================ quantised cache ==
+// ================================================ paged caches ==
 
 #include "quant_calls.h"

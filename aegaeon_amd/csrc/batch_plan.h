@@ -1,5 +1,5 @@
-// The plan of one batch over a quantised paged cache: what aegkv_batch_plan
-// lays out in a caller's buffer (plan.cpp) and the kernels of quant_cache.h
+// The plan of one batch over a paged cache: what aegkv_batch_plan lays out in a
+// caller's buffer (plan.cpp) and the kernels of quant_cache.h and paged_cache.h
 // read from its copy on the device. Internal to the library.
 #ifndef AEGKV_BATCH_PLAN_H
 #define AEGKV_BATCH_PLAN_H
@@ -14,6 +14,8 @@ constexpr uint64_t kMagic = 0x314e414c50425141ull;
 // attended over in tiles of 32.
 constexpr int kSpan = 16;
 constexpr int kTile = 32;
+// Places whose weights of attention one workgroup adds up.
+constexpr int kPlaceTile = 256;
 
 // Row r of a sequence's queries under one KV head is new token r / group,
 // query head kv_head * group + r % group. Attention takes rows by kind:
@@ -34,15 +36,17 @@ struct Seq {
   int32_t table;       // first entry of its block table
   int32_t token;       // row of its first new token
   int32_t read_span;   // spans of all tokens before this sequence
-  int32_t pad;
+  int32_t place_tile;  // tiles of kPlaceTile places before this sequence
   int64_t read_token;  // tokens before this sequence
 };
 static_assert(sizeof(Seq) == 32, "Seq layout");
 
 // Up to 16 new tokens of a sequence inside one block.
 struct NewSpan {
-  int32_t block, inside, count;
+  int32_t block;
+  uint16_t inside, count;
   int32_t token;       // row of the first
+  int32_t position;    // of the first in its sequence
 };
 static_assert(sizeof(NewSpan) == 16, "NewSpan layout");
 
@@ -73,7 +77,7 @@ static_assert(sizeof(Merge) == 48, "Merge layout");
 struct Room {
   int64_t bytes;
   int64_t seqs, columns, tokens;   // sequences, table entries, new tokens
-  int64_t new_spans, read_spans;
+  int64_t new_spans, read_spans, place_tiles;
   int64_t items[kKinds];           // a workgroup each; 0: no such kernel is launched
   int64_t slots[kKinds];
   int64_t merges;
@@ -90,6 +94,7 @@ struct Header {
   int32_t new_spans, read_spans;
   int32_t items[kKinds], slots[kKinds];
   int32_t merges;
+  int32_t place_tiles;
   int32_t complete;                // every position of every sequence has its block
   int64_t read_tokens;
 };

@@ -238,6 +238,7 @@ inline int fill(Header& h, const Batch& b, const std::vector<Rows>* rows, char* 
   auto* merge = reinterpret_cast<Merge*>(base + room.at_merges);
   auto* span = reinterpret_cast<NewSpan*>(base + room.at_new_spans);
   int64_t columns = 0, tokens = 0, new_spans = 0, read_spans = 0, read_tokens = 0;
+  int64_t place_tiles = 0;
   h.complete = 1;
   for (int64_t s = 0; s < b.num_seqs; ++s) columns += up(b.lens[s], h.block_size) + 1;
   for (int64_t s = 0; s < b.num_seqs; ++s) tokens += b.fresh[s];
@@ -253,6 +254,7 @@ inline int fill(Header& h, const Batch& b, const std::vector<Rows>* rows, char* 
     seq[s].table = static_cast<int32_t>(columns);
     seq[s].token = static_cast<int32_t>(tokens);
     seq[s].read_span = static_cast<int32_t>(read_spans);
+    seq[s].place_tile = static_cast<int32_t>(place_tiles);
     seq[s].read_token = read_tokens;
     for (int64_t c = 0; c < need; ++c) {
       const int64_t id = b.ids[b.offsets[s] + c];
@@ -268,20 +270,23 @@ inline int fill(Header& h, const Batch& b, const std::vector<Rows>* rows, char* 
         return aegkv_set_error(AEGKV_ENOMEM, "the new tokens do not fit the plan's %lld spans",
                                ll(room.new_spans));
       span[new_spans++] = NewSpan{table[seq[s].table + at / h.block_size],
-                                  static_cast<int32_t>(at % h.block_size),
-                                  static_cast<int32_t>(end - at),
-                                  static_cast<int32_t>(seq[s].token + at - (len - fresh))};
+                                  static_cast<uint16_t>(at % h.block_size),
+                                  static_cast<uint16_t>(end - at),
+                                  static_cast<int32_t>(seq[s].token + at - (len - fresh)),
+                                  static_cast<int32_t>(at)};
       at = end;
     }
     read_spans += up(len, kSpan);
+    place_tiles += up(len, kPlaceTile);
     read_tokens += len;
   }
   h.num_seqs = static_cast<int32_t>(b.num_seqs);
   h.num_tokens = static_cast<int32_t>(tokens);
   h.new_spans = static_cast<int32_t>(new_spans);
   h.read_spans = static_cast<int32_t>(read_spans);
+  h.place_tiles = static_cast<int32_t>(place_tiles);
   h.read_tokens = read_tokens;
-  if (read_spans > room.read_spans)
+  if (read_spans > room.read_spans || place_tiles > room.place_tiles)
     return aegkv_set_error(AEGKV_ENOMEM, "%lld spans to read do not fit the plan", ll(read_spans));
   int64_t merges = 0;
   for (int kind = 0; kind < kKinds; ++kind) {
@@ -339,9 +344,10 @@ inline int fill(Header& h, const Batch& b, const std::vector<Rows>* rows, char* 
 inline void make_room(Header& h, const Batch& b, const std::vector<Rows>* rows, int64_t max_seqs,
                       int64_t max_columns, int64_t max_tokens) {
   Room& r = h.room;
-  int64_t columns = 0, tokens = 0, new_spans = 0, read_spans = 0;
+  int64_t columns = 0, tokens = 0, new_spans = 0, read_spans = 0, place_tiles = 0;
   for (int64_t s = 0; s < b.num_seqs; ++s) {
     const int64_t len = b.lens[s], fresh = b.fresh[s];
+    place_tiles += up(len, kPlaceTile);
     columns += up(len, h.block_size);
     tokens += fresh;
     if (fresh) new_spans += up(len, kSpan) - (len - fresh) / kSpan;
@@ -354,6 +360,9 @@ inline void make_room(Header& h, const Batch& b, const std::vector<Rows>* rows, 
   r.tokens = std::max(max_tokens, tokens);
   r.new_spans = exact ? new_spans : std::min(r.tokens, r.tokens / kSpan + 2 * r.seqs);
   r.read_spans = exact ? read_spans : max_columns * (h.block_size / kSpan);
+  // (a sequence's last tile may hold one place)
+  r.place_tiles = exact ? place_tiles
+                        : std::min(max_columns, max_columns * h.block_size / kPlaceTile + r.seqs);
   r.merges = 0;
   int64_t at = pad16(sizeof(Header));
   auto take = [&](int64_t bytes) {

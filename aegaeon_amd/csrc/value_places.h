@@ -31,8 +31,8 @@ inline bool same(const Place& a, const Place& b) {
 }
 
 // Whether two places share a byte: exactly where they differ in nothing but their
-// beginning (slices of one buffer, also interleaved ones), else by the range
-// from first to last byte.
+// beginning (slices of one buffer, also interleaved ones), by the range from first to
+// last byte of each token where those lie equally far apart, else of the whole.
 inline bool overlap(const Place& a, const Place& b) {
   if (!a.tokens || !b.tokens) return false;
   const auto end = [](const Place& p) {
@@ -40,7 +40,17 @@ inline bool overlap(const Place& a, const Place& b) {
                                             p.run);
   };
   if (a.begin >= end(b) || b.begin >= end(a)) return false;
-  if (!same(a, Place{a.begin, b.tokens, b.heads, b.run, b.token, b.head})) return true;
+  if (!same(a, Place{a.begin, b.tokens, b.heads, b.run, b.token, b.head})) {
+    if (!a.token || a.token != b.token) return true;
+    // tokens of one length (Q, K and V of a fused projection): by each token's range
+    const int64_t apart = static_cast<int64_t>(b.begin - a.begin), next = -apart / a.token;
+    for (const int64_t near : {next - 1, next, next + 1}) {
+      const int64_t gap = apart + std::clamp(near, 1 - a.tokens, b.tokens - 1) * a.token;
+      if (gap < (a.heads - 1) * a.head + a.run && -gap < (b.heads - 1) * b.head + b.run)
+        return true;
+    }
+    return false;
+  }
   // runs i tokens and j heads apart for some |i| < tokens, |j| < heads
   const int64_t apart = static_cast<int64_t>(b.begin - a.begin);
   for (int64_t j = 1 - a.heads; j < a.heads; ++j) {
