@@ -96,6 +96,11 @@ EXPORTED_SYMBOLS = (
     "aegkv_quant_read",
     "aegkv_quant_attend_workspace",
     "aegkv_quant_attend",
+    "aegkv_rotate",
+    "aegkv_paged_write",
+    "aegkv_paged_attend",
+    "aegkv_paged_weigh",
+    "aegkv_paged_evict",
 )
 
 _P = ctypes.c_void_p
@@ -106,6 +111,32 @@ _I64P = ctypes.POINTER(ctypes.c_int64)
 _I32P = ctypes.POINTER(ctypes.c_int32)
 _U64P = ctypes.POINTER(ctypes.c_uint64)
 _PP = ctypes.POINTER(ctypes.c_void_p)
+
+
+class PagedCacheArgs(ctypes.Structure):
+    """aegkv_paged_cache"""
+
+    _fields_ = [("k_pages", _P), ("v_pages", _P), ("k_block_bytes", _I64),
+                ("v_block_bytes", _I64), ("num_blocks", _I64), ("block_size", _I32),
+                ("kv_heads", _I32), ("head_dim", _I32), ("dtype", _I32), ("head_major", _I32),
+                ("reserved", _I32)]
+
+
+class Rows(ctypes.Structure):
+    """aegkv_rows"""
+
+    _fields_ = [("base", _P), ("tokens", _I64), ("token_stride", _I64), ("head_stride", _I64),
+                ("heads", _I32), ("dtype", _I32)]
+
+
+class RotaryArgs(ctypes.Structure):
+    """aegkv_rotary"""
+
+    _fields_ = [("turns", _P), ("dim", _I32), ("interleaved", _I32),
+                ("amplitude", ctypes.c_double)]
+
+
+_CACHE, _ROWS, _ROTARY = (ctypes.POINTER(t) for t in (PagedCacheArgs, Rows, RotaryArgs))
 
 # Tables and id lists of the moves are taken as plain addresses, so that the
 # packed bytes of _hostargs go through as they are (ctypes passes a bytes
@@ -164,6 +195,21 @@ _SIGNATURES = {
         _INT,
         [_P, _P, _INT, _I32, _P, _P, _P, _I64, _I64, _P, _I64, _I64, _I64, _INT,
          ctypes.c_double, _P, _I64, _P],
+    ),
+    "aegkv_rotate": (
+        _INT, [_ROTARY, _P, _I64, _INT, _I32, _ROWS, _ROWS, _ROWS, _ROWS, _P],
+    ),
+    "aegkv_paged_write": (
+        _INT, [_P, _P, _CACHE, _ROWS, _ROWS, _ROTARY, _P, _I64, _INT, _ROWS, _ROWS, _P],
+    ),
+    "aegkv_paged_attend": (
+        _INT, [_P, _P, _CACHE, _ROWS, _ROWS, _P, _I64, _I64, ctypes.c_double, _P, _I64, _P],
+    ),
+    "aegkv_paged_weigh": (
+        _INT, [_P, _P, _CACHE, _ROWS, _P, _I64, _I64, ctypes.c_double, _P, _P],
+    ),
+    "aegkv_paged_evict": (
+        _INT, [_P, _P, _CACHE, _P, _I64, _I64, _I64, _P, _P, _P, _P],
     ),
 }
 

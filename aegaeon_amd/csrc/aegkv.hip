@@ -2823,3 +2823,4 @@ int aegkv_host_free(void* ptr) {
 // ================================================ paged caches ==
 
 #include "quant_calls.h"
+#include "paged_calls.h"

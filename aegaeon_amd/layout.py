@@ -88,6 +88,14 @@ def quant_kv_tensor_specs(num_layers: int, num_blocks: int, block_size: int, kv_
             for layer in range(num_layers) for kv in ("k", "v")]
 
 
+def weight_tensor_specs(num_layers: int, num_blocks: int, block_size: int, kv_heads: int
+                        ) -> List[KVCacheTensorSpec]:
+    """The weights that a cache's tokens gather (ops.paged_weigh), as one more
+    tensor per layer beside kv_tensor_specs: float32 [num_blocks, kv_heads, block_size]."""
+    size = num_blocks * kv_heads * block_size * 4
+    return [KVCacheTensorSpec(size, (f"layers.{layer}.weights",)) for layer in range(num_layers)]
+
+
 @dataclass
 class CompositeCache:
     """Device backing tensors plus their composite layout (vllm_cache.py:43-51)."""

@@ -7,12 +7,15 @@ composite-page data plane of Worker.swap_blocks (aegaeon/worker.py:2265-2329)
 and `copy_blocks` the in-HBM block copy. Every call is one C-ABI call into
 libaegkv.so; there is no Python or CPU fallback. `QuantCache`, `CacheBatch` and
 `quant_write`, `quant_read`, `quant_attend` hold a cache in 4 or 8 bits, which the
-moves take like any other; the reference has none.
+moves take like any other; `Rotary`, `rotate`, `PagedCache` and `paged_write`,
+`paged_attend`, `paged_weigh`, `paged_evict` are what a model step does with
+an ordinary one. The reference has none of these.
 """
 
 from __future__ import annotations
 
 import ctypes
+import math
 import struct
 import sys
 import threading
@@ -1015,16 +1018,16 @@ class QuantCache:
 
 
 class CacheBatch:
-    """A batch over a quantised cache: which blocks its sequences hold, and how
-    attention over them is shared out (aegkv_batch_plan). One batch serves all
-    layers of a model step.
+    """A batch over a paged cache (QuantCache or PagedCache): which blocks its
+    sequences hold, and how attention over them is shared out (aegkv_batch_plan).
+    One batch serves all layers of a model step.
 
     block_tables: a list of block ids for each sequence, or a 2-D array with a row
     each; column c holds the positions [c * block_size, (c + 1) * block_size), -1
     marks a released column (as BlockTable.group_blocks does), and columns behind
     the sequence's last are ignored. seq_lens counts all tokens of a
-    sequence, new_lens those at its end that are new: the ones quant_write
-    writes and quant_attend takes as queries. A query at position p sees the
+    sequence, new_lens those at its end that are new: the ones that writes
+    write and attention takes as queries. A query at position p sees the
     positions j <= p with p - j < window (0: all) or j < sinks.
 
     Everything is checked here, once (ValueError). update() puts another batch in
@@ -1204,7 +1207,7 @@ def _capturing(stream: torch.cuda.Stream) -> bool:
         return torch.cuda.is_current_stream_capturing()
 
 
-def _quant_call(cache: QuantCache, batch: CacheBatch, stream: torch.cuda.Stream | None):
+def _cache_call(cache, batch: CacheBatch, stream: torch.cuda.Stream | None):
     if (batch.block_size, batch.kv_heads) != (cache.block_size, cache.kv_heads):
         raise ValueError(f"a batch of {batch.block_size}-token blocks and {batch.kv_heads} KV "
                          f"heads over a cache of {cache.block_size} and {cache.kv_heads}")
@@ -1227,7 +1230,7 @@ def _answer(done):
     return done
 
 
-def _rows_arg(t: torch.Tensor, what: str, heads: int, cache: QuantCache, dtypes):
+def _rows_arg(t: torch.Tensor, what: str, heads: int, cache, dtypes):
     """(pointer, token stride, head stride) of a [tokens, heads, head_dim] tensor."""
     if t.device != cache.device:
         raise ValueError(f"{what} on {t.device}, the cache on {cache.device}")
@@ -1245,7 +1248,7 @@ def _rows_arg(t: torch.Tensor, what: str, heads: int, cache: QuantCache, dtypes)
     return t.data_ptr(), t.stride(0), t.stride(1)
 
 
-def _on_stream(cache: QuantCache, batch: CacheBatch, stream, fn) -> None:
+def _on_stream(cache, batch: CacheBatch, stream, fn) -> None:
     def call():
         raw = _stream_ptr(cache.device, stream)
         st = batch._enter(raw, stream)
@@ -1281,7 +1284,7 @@ def quant_write(cache: QuantCache, batch: CacheBatch, k: torch.Tensor, v: torch.
         if done is not None:
             _answer(done)
             return
-    _quant_call(cache, batch, stream)
+    _cache_call(cache, batch, stream)
     kp = _rows_arg(k, "k", cache.kv_heads, cache, _DTYPES)
     vp = _rows_arg(v, "v", cache.kv_heads, cache, _DTYPES)
     if k.dtype != v.dtype or k.size(0) != v.size(0):
@@ -1309,7 +1312,7 @@ def quant_read(cache: QuantCache, batch: CacheBatch, *, tokens: str = "all",
                                           *_here(cache))
         if done is not None:
             return _answer(done)
-    _quant_call(cache, batch, stream)
+    _cache_call(cache, batch, stream)
     n = batch.read_tokens if tokens == "all" else batch.num_tokens
     if out is None:
         if dtype not in _DTYPES:
@@ -1345,7 +1348,7 @@ def quant_attend(cache: QuantCache, batch: CacheBatch, q: torch.Tensor, *,
                                             *_here(cache))
         if done is not None:
             return _answer(done)
-    _quant_call(cache, batch, stream)
+    _cache_call(cache, batch, stream)
     qp = _rows_arg(q, "q", batch.heads, cache, (torch.bfloat16, torch.float16))
     if out is None:
         out = _empty_on(stream, q.shape, dtype=q.dtype, device=q.device)
@@ -1361,3 +1364,414 @@ def quant_attend(cache: QuantCache, batch: CacheBatch, q: torch.Tensor, *,
         _DTYPES[q.dtype], d ** -0.5 if scale is None else float(scale),
         work.data_ptr() if size else None, size, raw))
     return out
+
+
+# ---- ordinary paged caches ------------------------------------------------------
+
+_HALVES = (torch.bfloat16, torch.float16)
+_turn_tables: dict = {}     # by device and contents; kept, so that no stream outlives one
+
+
+def rotary_frequencies(dim: int, *, base: float = 10000.0, scaling: str = "none",
+                       factor: float = 1.0, length: int = 0) -> tuple[np.ndarray, float]:
+    """(radians a position for each of dim / 2 pairs, amplitude) of rotary positions:
+    f_i = base ** (-2 i / dim), scaled for contexts `factor` times as long as the
+    `length` a model was trained on:
+
+    "linear"  f_i / factor
+    "base"    base * factor ** (dim / (dim - 2)) in the base's place
+    "ramp"    f_i where `length` positions hold 32 turns or more, f_i / factor where one
+              or less, between them linear in i (from the last whole i before to the
+              first behind); amplitude 0.1 ln(factor) + 1
+    "smooth"  f_i at 4 turns or more, f_i / factor at one or less, between them linear in the
+              turns
+    """
+    dim, base, factor = int(dim), float(base), float(factor)
+    if dim < 2 or dim % 2:
+        raise ValueError(f"an even number of values is rotated, not {dim}")
+    if scaling not in ("none", "linear", "base", "ramp", "smooth"):
+        raise ValueError(f"unknown scaling {scaling!r}")
+    if not (base > 1 and math.isfinite(base) and factor > 0 and math.isfinite(factor)):
+        raise ValueError(f"base {base} (over 1) and factor {factor} (positive) are no numbers "
+                         "of that kind")
+    if scaling in ("ramp", "smooth") and length <= 0:
+        raise ValueError(f"{scaling!r} needs the length that it starts from")
+    i = np.arange(dim // 2, dtype=np.float64)
+    if scaling == "base":
+        if dim == 2:
+            raise ValueError("a single pair has no base to scale")
+        base *= factor ** (dim / (dim - 2))
+    f = base ** (-2 * i / dim)
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "ramp":
+        low, high = (dim * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(base))
+                     for turns in (32, 1))
+        low, high = max(0, math.floor(low)), min(dim - 1, math.ceil(high))
+        far = np.clip((i - low) / max(high - low, 0.001), 0, 1)
+        return f / factor * far + f * (1 - far), 0.1 * math.log(factor) + 1
+    elif scaling == "smooth":
+        near = np.clip((length * f / (2 * math.pi) - 1) / 3, 0, 1)
+        f = f / factor * (1 - near) + f * near
+    return f, 1.0
+
+
+class Rotary:
+    """Rotary positions for heads of head_dim values, of which the first `dim` (default:
+    all) are rotated: pairs (i, i + dim / 2), or (2 i, 2 i + 1) where interleaved.
+    Frequencies as rotary_frequencies makes them, or a list of dim / 2 of any kind
+    with the amplitude that rotated values are multiplied by. Any stream may use it."""
+
+    def __init__(self, head_dim: int, *, dim: int | None = None, base: float = 10000.0,
+                 interleaved: bool = False, scaling: str = "none", factor: float = 1.0,
+                 length: int = 0, frequencies=None, amplitude: float | None = None,
+                 device: torch.device | None = None):
+        self.head_dim = int(head_dim)
+        self.dim = self.head_dim if dim is None else int(dim)
+        if not 2 <= self.head_dim <= 1024 or self.head_dim % 2:
+            raise ValueError(f"heads of {self.head_dim} values")
+        if not 2 <= self.dim <= self.head_dim or self.dim % 2:
+            raise ValueError(f"{self.dim} rotated values of a head of {self.head_dim}")
+        if frequencies is None:
+            f, a = rotary_frequencies(self.dim, base=base, scaling=scaling, factor=factor,
+                                      length=length)
+        else:
+            f, a = np.asarray(frequencies, dtype=np.float64).reshape(-1), 1.0
+            if f.size != self.dim // 2:
+                raise ValueError(f"{f.size} frequencies for {self.dim // 2} pairs")
+        self.frequencies, self.amplitude = f, a if amplitude is None else float(amplitude)
+        if not np.isfinite(f).all() or not math.isfinite(self.amplitude):
+            raise ValueError("frequencies and amplitude must be finite")
+        self.interleaved = bool(interleaved)
+        self.device = torch.device(device if device is not None else "cuda")
+        if self.device.type != "cuda":
+            raise ValueError(f"rotary positions live on a device (HIP), not on {self.device}")
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        turns = f / (2 * math.pi)
+        key = (self.device.index, turns.tobytes())
+        if key not in _turn_tables:
+            with torch.cuda.device(self.device):
+                if torch.cuda.is_current_stream_capturing():
+                    raise ValueError("rotary positions are not made while a stream is captured")
+                table = torch.tensor(turns, device=self.device)
+                torch.cuda.current_stream().synchronize()
+            _turn_tables[key] = table
+        self._turns = _turn_tables[key]
+        self._args = _lib.RotaryArgs(self._turns.data_ptr(), self.dim, self.interleaved,
+                                     self.amplitude)
+
+
+class PagedCache:
+    """K and V of one layer in bfloat16 or float16, as pages of a paged cache.
+
+    k_pages, v_pages: [num_blocks, block_size, kv_heads, head_dim], whose pages lie
+    together as that (layout.kv_tensor_specs), or as [kv_heads, block_size, head_dim] (a
+    transposed view); blocks may lie apart, as where K and V alternate in one
+    tensor. Blocks of 16, 32, 64 or 128 tokens, heads 64, 128 or 256 wide.
+    """
+
+    def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor):
+        for t, what in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+            if t.device.type != "cuda":
+                raise ValueError(f"{what} must be a device (HIP) tensor, got {t.device}")
+            if t.dim() != 4 or t.numel() == 0:
+                raise ValueError(f"{what} must be [num_blocks, block_size, kv_heads, head_dim], "
+                                 f"not {list(t.shape)}")
+            if t.dtype not in _HALVES:
+                raise ValueError(f"{what} of {t.dtype}: a cache holds bfloat16 or float16")
+            if t.requires_grad:
+                raise ValueError(f"{what} requires a gradient, which these operators do not give")
+        if (k_pages.shape, k_pages.dtype, k_pages.device) != (v_pages.shape, v_pages.dtype,
+                                                              v_pages.device):
+            raise ValueError("k_pages and v_pages must be equally large, of one type and on one "
+                             "device")
+        self.num_blocks, self.block_size, self.kv_heads, self.head_dim = k_pages.shape
+        if self.block_size not in (16, 32, 64, 128):
+            raise ValueError(f"a block holds 16, 32, 64 or 128 tokens, not {self.block_size}")
+        if self.head_dim not in (64, 128, 256):
+            raise ValueError(f"heads are 64, 128 or 256 values wide, not {self.head_dim}")
+        self.k_pages, self.v_pages = k_pages, v_pages
+        self.dtype, self.device = k_pages.dtype, k_pages.device
+        layouts, blocks = [], []
+        page = self.block_size * self.kv_heads * self.head_dim
+        for t, what in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+            block, token, head, value = t.stride()
+            one = self.kv_heads == 1
+            if value != 1:
+                raise ValueError(f"{what}: the last axis must be contiguous")
+            if token == self.kv_heads * self.head_dim and (one or head == self.head_dim):
+                layouts.append(False)
+            elif token == self.head_dim and head == self.block_size * self.head_dim:
+                layouts.append(True)
+            else:
+                raise ValueError(f"{what}: a page must lie together, by tokens or by heads "
+                                 f"(strides {t.stride()})")
+            if self.num_blocks == 1:
+                block = page
+            if block < page:
+                raise ValueError(f"{what}: pages of {page} values, {block} apart")
+            if t.data_ptr() % 16 or block % 8:
+                raise ValueError(f"{what}: blocks must be 16-byte aligned")
+            blocks.append(block * 2)
+        if layouts[0] != layouts[1]:
+            raise ValueError("k_pages and v_pages are laid out differently")
+        self.head_major = layouts[0]
+        self._args = _lib.PagedCacheArgs(k_pages.data_ptr(), v_pages.data_ptr(), *blocks,
+                                         self.num_blocks, self.block_size, self.kv_heads,
+                                         self.head_dim, _DTYPES[self.dtype], self.head_major, 0)
+
+
+def _paged_call(cache: PagedCache, batch: CacheBatch, stream) -> None:
+    if not isinstance(cache, PagedCache):
+        raise ValueError(f"a PagedCache, not a {type(cache).__name__}")
+    if cache.k_pages.requires_grad or cache.v_pages.requires_grad:
+        raise ValueError("the cache requires a gradient, which these operators do not give")
+    _cache_call(cache, batch, stream)
+
+
+def _rows(t: torch.Tensor, what: str, heads: int, of, dtypes) -> _lib.Rows:
+    """C argument of a [tokens, heads, head_dim] tensor; `of`: its device and width."""
+    base, token, head = _rows_arg(t, what, heads, of, dtypes)
+    return _lib.Rows(base, t.size(0), token, head, heads, _DTYPES[t.dtype])
+
+
+def _positions_arg(positions: torch.Tensor | None, device: torch.device):
+    """(pointer, count, bytes each)"""
+    if positions is None:
+        return None, 0, 8
+    if positions.device != device:
+        raise ValueError(f"positions on {positions.device}, the call on {device}")
+    if positions.dtype not in (torch.int32, torch.int64) or positions.dim() != 1:
+        raise ValueError(f"positions are one int32 or int64 a token, not {positions.dtype} "
+                         f"{list(positions.shape)}")
+    if not positions.is_contiguous():
+        raise ValueError("positions must be contiguous")
+    return positions.data_ptr(), positions.numel(), positions.element_size()
+
+
+def _check_rotary(rotary: Rotary, head_dim: int, device: torch.device) -> None:
+    if rotary.device != device:
+        raise ValueError(f"rotary positions on {rotary.device}, the call on {device}")
+    if rotary.head_dim != head_dim:
+        raise ValueError(f"rotary positions for heads of {rotary.head_dim}, not {head_dim}")
+
+
+def rotate(rotary: Rotary, positions: torch.Tensor, q: torch.Tensor,
+           k: torch.Tensor | None = None, *, out=None,
+           stream: torch.cuda.Stream | None = None):
+    """Rotate q, or q and k, by the tokens' positions (aegkv_rotate), before a
+    quantised cache takes the keys, say (paged_write rotates by itself).
+
+    q, k: [tokens, heads, head_dim] of one type (bfloat16, float16 or float32), any strides
+    on the first two axes. positions: an int32 or int64 for each token on the device; a
+    negative one turns back. Returns q, or (q, k), rotated: new tensors, or `out` (the
+    same way; q and k themselves are fine, other overlaps are refused).
+    """
+    head_dim = rotary.head_dim
+    _check_rotary(rotary, head_dim, q.device)
+    _require_stream(q.device, stream)
+    given = (q,) if k is None else (q, k)
+    if out is None:
+        out = tuple(_empty_on(stream, t.shape, dtype=t.dtype, device=t.device) for t in given)
+    elif isinstance(out, torch.Tensor):
+        out = (out,)
+    if len(out) != len(given):
+        raise ValueError(f"{len(out)} tensors for {len(given)} to rotate")
+    rows = []
+    for what, t, o in zip("qk", given, out):
+        if t.dim() != 3 or o.dim() != 3 or t.size(1) == 0:
+            raise ValueError(f"{what} must be [tokens, heads, {head_dim}], not {list(t.shape)}")
+        if t.dtype != q.dtype or t.shape != o.shape or t.size(0) != q.size(0):
+            raise ValueError(f"{what} and what it goes to: {list(t.shape)} of {t.dtype} and "
+                             f"{list(o.shape)} of {o.dtype}")
+        rows.append(_rows(t, what, t.size(1), rotary, _DTYPES))
+        rows.append(_rows(o, f"out of {what}", t.size(1), rotary, (q.dtype,)))
+    if positions is None:
+        raise ValueError("positions must be given")
+    where = _positions_arg(positions, q.device)
+    if where[1] != q.size(0):
+        raise ValueError(f"{where[1]} positions of {q.size(0)} tokens")
+    lib = _lib.load()
+    refs = [ctypes.byref(r) for r in rows] + [None] * (4 - len(rows))
+    _call_on(q.device, lambda: _lib.check(lib.aegkv_rotate(
+        ctypes.byref(rotary._args), *where, head_dim, *refs, _stream_ptr(q.device, stream))))
+    return out[0] if k is None else tuple(out)
+
+
+def paged_write(cache: PagedCache, batch: CacheBatch, k: torch.Tensor, v: torch.Tensor, *,
+                rotary: Rotary | None = None, positions: torch.Tensor | None = None,
+                q: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                stream: torch.cuda.Stream | None = None) -> torch.Tensor | None:
+    """Write the batch's new tokens into the cache (aegkv_paged_write).
+
+    k, v: [tokens, kv_heads, head_dim] of bfloat16, float16 or float32, with any
+    strides on the first two axes; row i is the batch's i-th new token, rows behind the
+    last are not read, and each value is rounded once. With rotary, k is rotated on its
+    way, and q ([tokens, heads, head_dim] of the cache's type), if given, to `out` (default: a
+    new tensor; q itself is fine), which is returned. positions: the new tokens' own (int32
+    or int64 on the device), where they are not their places in the sequences, as
+    after an eviction.
+    """
+    _paged_call(cache, batch, stream)
+    if k.dtype != v.dtype or k.size(0) != v.size(0):
+        raise ValueError(f"k and v differ: {k.size(0)} tokens of {k.dtype}, {v.size(0)} of "
+                         f"{v.dtype}")
+    if rotary is None and (q is not None or positions is not None):
+        raise ValueError("q and positions are for rotary positions, and none are given")
+    if q is None and out is not None:
+        raise ValueError("out is for q, which is not given")
+    kr = _rows(k, "k", cache.kv_heads, cache, _DTYPES)
+    vr = _rows(v, "v", cache.kv_heads, cache, _DTYPES)
+    qr = orow = turn = None
+    if rotary is not None:
+        _check_rotary(rotary, cache.head_dim, cache.device)
+        turn = ctypes.byref(rotary._args)
+    if q is not None:
+        qr = _rows(q, "q", batch.heads, cache, (cache.dtype,))
+        if out is None:
+            out = _empty_on(stream, q.shape, dtype=q.dtype, device=q.device)
+        orow = _rows(out, "out", batch.heads, cache, (cache.dtype,))
+        if out.size(0) != q.size(0):
+            raise ValueError(f"{q.size(0)} queries, {out.size(0)} rows of out")
+    where = _positions_arg(positions, cache.device)
+    lib = _lib.load()
+    ref = [None if r is None else ctypes.byref(r) for r in (qr, orow)]
+    _on_stream(cache, batch, stream, lambda raw: lib.aegkv_paged_write(
+        batch._host_ptr, batch._plan.data_ptr(), ctypes.byref(cache._args), ctypes.byref(kr),
+        ctypes.byref(vr), turn, *where, *ref, raw))
+    return out
+
+
+def _sums_arg(t: torch.Tensor, heads: int, device: torch.device):
+    """(pointer, tokens, token stride) of log-sum-exps [tokens, heads]."""
+    if t.device != device or t.dtype != torch.float32:
+        raise ValueError(f"lse must be float32 on {device}, not {t.dtype} on {t.device}")
+    if t.dim() != 2 or t.size(1) != heads or (t.numel() and heads > 1 and t.stride(1) != 1):
+        raise ValueError(f"lse must be [tokens, {heads}] with its last axis contiguous, not "
+                         f"{list(t.shape)}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError("lse requires a gradient, which these operators do not give")
+    if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError("lse carries a tangent, which these operators do not take on")
+    return t.data_ptr(), t.size(0), t.stride(0)
+
+
+def paged_attend(cache: PagedCache, batch: CacheBatch, q: torch.Tensor, *,
+                 scale: float | None = None, out: torch.Tensor | None = None,
+                 return_lse: bool = False, lse: torch.Tensor | None = None,
+                 stream: torch.cuda.Stream | None = None):
+    """Attention of the batch's new tokens over the cache (aegkv_paged_attend), for
+    single tokens, chunks and whole prompts alike, also side by side.
+
+    q: [tokens, heads, head_dim] of the cache's type, row i the query of the batch's i-th
+    new token, whose K and V are in the cache already (paged_write). scale: of the
+    scores, head_dim ** -0.5 by default. `out` (q itself is fine, other overlaps are refused)
+    takes the result; rows behind the batch's last token are left as they were. Returns out, or
+    (out, lse) with return_lse or a tensor `lse` to fill: [tokens, heads] float32, the
+    log of the sum of exp(score) over what each query sees, as paged_weigh takes it.
+    """
+    _paged_call(cache, batch, stream)
+    qr = _rows(q, "q", batch.heads, cache, (cache.dtype,))
+    if out is None:
+        out = _empty_on(stream, q.shape, dtype=q.dtype, device=q.device)
+    orow = _rows(out, "out", batch.heads, cache, (q.dtype,))
+    if out.size(0) != q.size(0):
+        raise ValueError(f"{q.size(0)} queries, {out.size(0)} rows of out")
+    if lse is None and return_lse:
+        lse = _empty_on(stream, q.shape[:2], dtype=torch.float32, device=q.device)
+    sums = (None, 0, 0)
+    if lse is not None:
+        sums = _sums_arg(lse, batch.heads, cache.device)
+        if lse.size(0) != q.size(0):
+            raise ValueError(f"{q.size(0)} queries, {lse.size(0)} rows of lse")
+    lib = _lib.load()
+    d = cache.head_dim
+    size = batch._workspace[d]
+    work = _empty_on(stream, size, dtype=torch.uint8, device=q.device) if size else None
+    _on_stream(cache, batch, stream, lambda raw: lib.aegkv_paged_attend(
+        batch._host_ptr, batch._plan.data_ptr(), ctypes.byref(cache._args), ctypes.byref(qr),
+        ctypes.byref(orow), *sums, d ** -0.5 if scale is None else float(scale),
+        work.data_ptr() if size else None, size, raw))
+    return out if lse is None else (out, lse)
+
+
+def _weights_arg(weights: torch.Tensor, cache: PagedCache) -> int:
+    shape = (cache.num_blocks, cache.kv_heads, cache.block_size)
+    if weights.device != cache.device or weights.dtype != torch.float32:
+        raise ValueError(f"weights must be float32 on {cache.device}, not {weights.dtype} on "
+                         f"{weights.device}")
+    if tuple(weights.shape) != shape or not weights.is_contiguous():
+        raise ValueError(f"weights must be contiguous [{shape[0]}, {shape[1]}, {shape[2]}], not "
+                         f"{list(weights.shape)}")
+    if weights.requires_grad:
+        raise ValueError("weights require a gradient, which these operators do not give")
+    return weights.data_ptr()
+
+
+def paged_weigh(cache: PagedCache, batch: CacheBatch, q: torch.Tensor, lse: torch.Tensor,
+                weights: torch.Tensor, *, scale: float | None = None,
+                stream: torch.cuda.Stream | None = None) -> None:
+    """Add to the weights of the cache's places the attention that the batch's new
+    tokens give them (aegkv_paged_weigh): summed over the queries, and over the query
+    heads of each KV head.
+
+    q, scale: those of paged_attend, whose log-sum-exps lse are. weights: float32 [num_blocks,
+    kv_heads, block_size], contiguous; the new tokens' places start from 0, those that no query
+    sees keep theirs. As a segment of the composite cache (layout.weight_tensor_specs)
+    they move with the blocks.
+    """
+    _paged_call(cache, batch, stream)
+    qr = _rows(q, "q", batch.heads, cache, (cache.dtype,))
+    sums = _sums_arg(lse, batch.heads, cache.device)
+    if lse.size(0) != q.size(0):
+        raise ValueError(f"{q.size(0)} queries, {lse.size(0)} rows of lse")
+    w = _weights_arg(weights, cache)
+    lib = _lib.load()
+    _on_stream(cache, batch, stream, lambda raw: lib.aegkv_paged_weigh(
+        batch._host_ptr, batch._plan.data_ptr(), ctypes.byref(cache._args), ctypes.byref(qr),
+        *sums, cache.head_dim ** -0.5 if scale is None else float(scale), w, raw))
+
+
+def paged_evict(cache: PagedCache, batch: CacheBatch, weights: torch.Tensor, keep: int, *,
+                sinks: int = 0, recent: int = 0, into: CacheBatch | None = None,
+                stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """Keep `keep` tokens of each sequence that holds more (aegkv_paged_evict).
+
+    Under each KV head stay the first `sinks` tokens, the last `recent`, and of the others
+    those of the largest weight, the earlier one of equals; K, V and weights of what
+    stays go to the sequence's first places, in their order. Every head keeps as many,
+    so a sequence's length is min(length, keep) afterwards: free the blocks behind it
+    and update the batch. Later tokens' rotary positions are no longer their places:
+    give paged_write theirs. `into`: a batch over other blocks whose sequences have room for
+    what stays, which goes there instead; the old blocks stay as they were.
+
+    Returns the places that what stays had, int32 [sequences, kv_heads, keep], -1
+    behind a shorter sequence's end.
+    """
+    _paged_call(cache, batch, stream)
+    keep = int(keep)
+    if into is not None:
+        _paged_call(cache, into, stream)
+        if into is batch:
+            raise ValueError("a batch is not evicted into itself: leave `into` out")
+    if not 1 <= keep < 1 << 31:
+        raise ValueError(f"{keep} tokens to keep")
+    w = _weights_arg(weights, cache)
+    kept = _empty_on(stream, (batch.num_seqs, cache.kv_heads, keep), dtype=torch.int32,
+                     device=cache.device)
+    lib = _lib.load()
+    other = (None, None) if into is None else (into._host_ptr, into._plan.data_ptr())
+
+    def call(raw):
+        st = None if into is None else into._enter(raw, stream)
+        try:
+            return lib.aegkv_paged_evict(
+                batch._host_ptr, batch._plan.data_ptr(), ctypes.byref(cache._args), w, keep,
+                int(sinks), int(recent), *other, kept.data_ptr() if kept.numel() else None, raw)
+        finally:
+            if into is not None:
+                into._leave(st)
+
+    _on_stream(cache, batch, stream, call)
+    return kept

@@ -4,7 +4,7 @@
  * (pinned host -> HBM) and in-HBM block copy.
  *
  * Conventions shared by every entry point
- *   - Plain pointers and sizes only. Device pointers are HIP device
+ *   - Plain pointers and sizes only (also in the structs). Device pointers are HIP device
  *     addresses on the *current* HIP device; host pool pointers must come
  *     from hipHostMalloc (aegkv_host_alloc or a pinned torch tensor).
  *   - Id arrays and metadata arrays are HOST arrays, read during the call.
@@ -22,7 +22,7 @@
  *   - The caller keeps every buffer alive until the stream has passed the
  *     enqueued work (record an event after the call and wait on it).
  *   - Calls are not for stream capture (hipGraph), except
- *     aegkv_copy_blocks_noalloc and the calls over quantised caches: the
+ *     aegkv_copy_blocks_noalloc and the calls over quantised and paged caches: the
  *     others' descriptors are copied from a host
  *     ring whose slots later calls reuse, and a replayed copy would read
  *     whatever the slot holds then. On a capturing stream they return
@@ -629,6 +629,117 @@ int aegkv_quant_attend(const void* plan, const void* device_plan, int format, in
                        int64_t out_token_stride, int64_t out_head_stride, int64_t num_tokens,
                        int dtype, double scale, void* workspace, int64_t workspace_bytes,
                        hipStream_t stream);
+
+/*
+ * Ordinary paged caches: K and V of one layer in bfloat16 or float16, with rotary
+ * positions. No counterpart in the reference, which leaves its caches' contents to the
+ * model code. The plan is the same aegkv_batch_plan; plans, arguments that may share no
+ * byte (AEGKV_EOVERLAP), streams and capture are as for quantised caches above.
+ *
+ * A page holds block_size tokens of kv_heads heads of head_dim (64, 128 or 256) values,
+ * [token][head][value], or [head][token][value] where head_major is not 0. A block's page lies
+ * together; blocks are k_block_bytes (v_block_bytes) apart, a multiple of 16 and at least a
+ * page (K and V may alternate in one tensor).
+ */
+typedef struct {
+  void* k_pages;
+  void* v_pages;
+  int64_t k_block_bytes, v_block_bytes;
+  int64_t num_blocks;
+  int32_t block_size, kv_heads, head_dim;
+  int32_t dtype;        /* AEGKV_DTYPE_BFLOAT16 or AEGKV_DTYPE_FLOAT16 */
+  int32_t head_major;
+  int32_t reserved;     /* 0 */
+} aegkv_paged_cache;
+
+/* Rows [tokens][heads][head_dim] of values; strides in elements, none negative, the last
+ * axis contiguous. */
+typedef struct {
+  void* base;
+  int64_t tokens, token_stride, head_stride;
+  int32_t heads;
+  int32_t dtype;
+} aegkv_rows;
+
+/*
+ * Rotary positions of a head's first `dim` (even) values: pair i of them, values (i, i +
+ * dim / 2), or (2 i, 2 i + 1) where interleaved is not 0, is turned by position *
+ * turns[i] whole turns and multiplied by amplitude. turns: dim / 2 doubles on the device.
+ */
+typedef struct {
+  const double* turns;
+  int32_t dim, interleaved;
+  double amplitude;
+} aegkv_rotary;
+
+/*
+ * Rotate rows by their positions: q to q_out, and k (may be null with k_out) to k_out, of one
+ * type (bfloat16, float16 or float32) and number of tokens, head_dim even and at most
+ * 1024. positions: an int32 or int64 (position_bytes) for each token, on the device, any
+ * value; a negative one turns back. Angles are made in 64 bits, values are rotated in 32
+ * and rounded once. q_out may be q itself (the same place and strides), k_out k. Can be captured.
+ */
+int aegkv_rotate(const aegkv_rotary* rotary, const void* positions, int64_t num_positions,
+                 int position_bytes, int32_t head_dim, const aegkv_rows* q, const aegkv_rows* q_out,
+                 const aegkv_rows* k, const aegkv_rows* k_out, hipStream_t stream);
+
+/*
+ * Write the batch's new tokens: k (rotated first if rotary is not null) and v, of one type
+ * (bfloat16, float16 or float32), each value rounded once to the cache's. With rotary, q of
+ * the cache's type may be rotated to q_out in the same call. positions: as above, for the batch's
+ * new tokens; null: their places in the sequences. Only the tokens' own bytes change;
+ * rows behind the last are not read, and in q_out left as they were.
+ */
+int aegkv_paged_write(const void* plan, const void* device_plan, const aegkv_paged_cache* cache,
+                      const aegkv_rows* k, const aegkv_rows* v, const aegkv_rotary* rotary,
+                      const void* positions, int64_t num_positions, int position_bytes,
+                      const aegkv_rows* q, const aegkv_rows* q_out, hipStream_t stream);
+
+/*
+ * Attention of the batch's new tokens over the cache, as aegkv_quant_attend: q and out of the
+ * cache's type. lse (may be null): [tokens][heads] floats, the rows lse_token_stride apart, take
+ * log(sum over the positions a query sees of exp(scale * q . K[j])). What a query does
+ * not see changes nothing, NaN included; an infinity or NaN of V that it sees makes that
+ * value of its result infinite or NaN.
+ *
+ * workspace: aegkv_quant_attend_workspace bytes, as there.
+ */
+int aegkv_paged_attend(const void* plan, const void* device_plan, const aegkv_paged_cache* cache,
+                       const aegkv_rows* q, const aegkv_rows* out, float* lse, int64_t lse_tokens,
+                       int64_t lse_token_stride, double scale, void* workspace,
+                       int64_t workspace_bytes, hipStream_t stream);
+
+/*
+ * Add to the weight of every place that a query of the batch sees the attention it
+ * gathers: the sum over the queries that see it, and the query heads of the KV head, of
+ * exp(scale * q . K[j] - lse). weights: [num_blocks][kv_heads][block_size] floats (a
+ * segment of the cache like K and V, which swaps and copies move). What the new tokens' places
+ * held before does not count; weights of places that no query sees are left as they were.
+ * Sums are made in 32 bits in a fixed order (no atomics).
+ */
+int aegkv_paged_weigh(const void* plan, const void* device_plan, const aegkv_paged_cache* cache,
+                      const aegkv_rows* q, const float* lse, int64_t lse_tokens,
+                      int64_t lse_token_stride, double scale, float* weights, hipStream_t stream);
+
+/*
+ * Evict tokens of sequences longer than `keep`. Under each KV head stay the first
+ * `sinks` places, the last `recent`, and of the others those of the largest weight (of
+ * equals the earlier ones; NaN counts as the least), `keep` in all; K, V and weights of what stays go, in
+ * their order, to the places 0 .. keep - 1: of the sequence's own blocks, or with into_plan of
+ * that plan's sequence of the same number, which has room for them (the sequences'
+ * own blocks are then left as they were, and shorter sequences are copied whole). kept:
+ * [sequences][kv_heads][keep] int32, takes the places that what stays had; -1 behind the
+ * end of a shorter sequence.
+ *
+ * The heads of a sequence keep different tokens but as many of them, so the new length is
+ * min(length, keep), known without asking the device. Blocks that are written
+ * may be in no other place of the tables (AEGKV_EDUP); a batch with released columns
+ * is refused, and so is capture.
+ */
+int aegkv_paged_evict(const void* plan, const void* device_plan, const aegkv_paged_cache* cache,
+                      float* weights, int64_t keep, int64_t sinks, int64_t recent,
+                      const void* into_plan, const void* into_device_plan, int32_t* kept,
+                      hipStream_t stream);
 
 #ifdef __cplusplus
 }
