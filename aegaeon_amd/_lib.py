@@ -285,6 +285,7 @@ class _GeneralPath:
         return None
 
     quant_read = quant_attend = quant_write
+    rotate = paged_write = paged_attend = paged_weigh = quant_write
 
 
 _hostargs = None

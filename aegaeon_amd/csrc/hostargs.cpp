@@ -1,5 +1,5 @@
 // aegaeon_amd._hostargs: the argument tables of a move, read from Python
-// objects in one pass, and the calls over a quantised cache.
+// objects in one pass, and the calls over quantised and paged caches.
 //
 // A copy over 72 backing tensors asks each for its device, layout, size and
 // address. Asked from Python one attribute at a time that is 50 us, several
@@ -316,6 +316,288 @@ PyObject* quant_attend(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   }
 }
 
+// What PagedCache and Rotary keep for these calls, packed by ops.py; the structs are those of
+// include/aegkv.h.
+struct PagedCacheArgs {
+  int64_t k_pages, v_pages, k_block_bytes, v_block_bytes, num_blocks;
+  int32_t block_size, kv_heads, head_dim, dtype, head_major, reserved;
+};
+struct RowsArgs {
+  void* base;
+  int64_t tokens, token_stride, head_stride;
+  int32_t heads, dtype;
+};
+struct RotaryArgs {
+  int64_t turns;
+  int32_t dim, interleaved;
+  double amplitude;
+};
+struct PagedArgs {
+  int64_t write, attend, weigh;   // addresses of the C entry points
+  PagedCacheArgs cache;
+  int64_t device;
+};
+struct TurnArgs {
+  int64_t rotate;
+  RotaryArgs rotary;
+  int64_t head_dim, device;
+};
+static_assert(sizeof(PagedArgs) == 96 && sizeof(TurnArgs) == 48, "as ops.py packs them");
+
+typedef int (*RotateFn)(const RotaryArgs*, const void*, int64_t, int, int32_t, const RowsArgs*,
+                        const RowsArgs*, const RowsArgs*, const RowsArgs*, void*);
+typedef int (*PagedWriteFn)(const void*, const void*, const PagedCacheArgs*, const RowsArgs*,
+                            const RowsArgs*, const RotaryArgs*, const void*, int64_t, int,
+                            const RowsArgs*, const RowsArgs*, void*);
+typedef int (*PagedAttendFn)(const void*, const void*, const PagedCacheArgs*, const RowsArgs*,
+                             const RowsArgs*, void*, int64_t, int64_t, double, void*, int64_t,
+                             void*);
+typedef int (*PagedWeighFn)(const void*, const void*, const PagedCacheArgs*, const RowsArgs*,
+                            const void*, int64_t, int64_t, double, void*, void*);
+
+// A tensor of a device that no gradient or tangent is asked of; null for others.
+const at::Tensor* plain_tensor(PyObject* o, int64_t device) {
+  if (!THPVariable_CheckExact(o)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.defined() || !t.is_cuda() || t.get_device() != device || t.layout() != at::kStrided ||
+      (t.requires_grad() && c10::GradMode::is_enabled()) || t._fw_grad(0).defined())
+    return nullptr;
+  return &t;
+}
+
+// [tokens, heads, head_dim] (heads 0: any number); tokens > 0.
+const at::Tensor* plain_rows(PyObject* o, int64_t device, int64_t heads, int64_t head_dim,
+                             RowsArgs* r) {
+  const at::Tensor* t = plain_tensor(o, device);
+  if (!t || t->dim() != 3 || t->size(0) == 0 || t->size(1) == 0 ||
+      (heads && t->size(1) != heads) || t->size(2) != head_dim || t->stride(2) != 1 ||
+      !dtype_code(t->scalar_type()))
+    return nullptr;
+  *r = RowsArgs{t->data_ptr(), t->size(0), t->stride(0), t->stride(1),
+                static_cast<int32_t>(t->size(1)), dtype_code(t->scalar_type())};
+  return t;
+}
+
+struct Positions {
+  const void* at = nullptr;
+  int64_t count = 0;
+  int bytes = 8;
+  bool take(PyObject* o, int64_t device) {
+    const at::Tensor* t = plain_tensor(o, device);
+    if (!t || t->dim() != 1 || !t->is_contiguous() ||
+        (t->scalar_type() != at::kInt && t->scalar_type() != at::kLong))
+      return false;
+    at = t->data_ptr();
+    count = t->numel();
+    bytes = static_cast<int>(t->element_size());
+    return true;
+  }
+};
+
+bool take_bytes(PyObject* o, void* to, Py_ssize_t size) {
+  if (!PyBytes_CheckExact(o) || PyBytes_GET_SIZE(o) != size) return false;
+  std::memcpy(to, PyBytes_AS_STRING(o), static_cast<size_t>(size));
+  return true;
+}
+
+// Cache, batch, raw stream and current device of one call.
+struct PagedCall {
+  PagedArgs c;
+  BatchArgs b;
+  void* stream;
+  bool take(PyObject* cache, PyObject* batch, PyObject* raw, PyObject* current) {
+    if (!take_bytes(cache, &c, sizeof c) || !take_bytes(batch, &b, sizeof b) ||
+        !PyLong_CheckExact(raw) || !PyLong_CheckExact(current))
+      return false;
+    const int64_t s = PyLong_AsLongLong(raw);
+    stream = at_address<void>(s);
+    return s == b.stream && PyLong_AsLongLong(current) == c.device && b.device == c.device &&
+           b.kv_heads == c.cache.kv_heads && b.block_size == c.cache.block_size &&
+           b.num_blocks <= c.cache.num_blocks && !PyErr_Occurred();
+  }
+  const at::Tensor* rows(PyObject* o, int64_t heads, RowsArgs* r) const {
+    return plain_rows(o, c.device, heads, c.cache.head_dim, r);
+  }
+  // float32 [tokens, heads] of log-sum-exps
+  const at::Tensor* sums(PyObject* o, int64_t tokens) const {
+    const at::Tensor* t = plain_tensor(o, c.device);
+    if (!t || t->scalar_type() != at::kFloat || t->dim() != 2 || t->size(0) != tokens ||
+        t->size(1) != b.heads || t->stride(1) != 1)
+      return nullptr;
+    return t;
+  }
+  double scale(PyObject* o) const {   // 0: the general path
+    if (o == Py_None)
+      return c.cache.head_dim == 64 ? 0.125
+             : c.cache.head_dim == 256 ? 0.0625 : 0.08838834764831845;
+    return PyFloat_CheckExact(o) ? PyFloat_AS_DOUBLE(o) : 0;
+  }
+};
+
+// A new tensor like t, as a Python object.
+PyObject* like(const at::Tensor& t) {
+  return THPVariable_Wrap(at::empty(t.sizes(), t.options().requires_grad(false)));
+}
+
+// rotate(rotary, positions, q, k or None, out of q or None, out of k or None, stream, device)
+// -> out of q, (out of q, out of k), a status, or None
+PyObject* rotate(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  TurnArgs t;
+  if (nargs != 8 || !take_bytes(args[0], &t, sizeof t) || !PyLong_CheckExact(args[6]) ||
+      !PyLong_CheckExact(args[7]) || PyLong_AsLongLong(args[7]) != t.device)
+    Py_RETURN_NONE;
+  try {
+    Positions where;
+    RowsArgs from[2], to[2];
+    Ref out[2] = {Ref(nullptr), Ref(nullptr)};
+    const int count = args[3] == Py_None ? 1 : 2;
+    if (!where.take(args[1], t.device)) Py_RETURN_NONE;
+    for (int i = 0; i < count; ++i) {
+      const at::Tensor* x = plain_rows(args[2 + i], t.device, 0, t.head_dim, &from[i]);
+      if (!x || from[i].tokens != where.count || from[i].dtype != from[0].dtype) Py_RETURN_NONE;
+      if (args[4 + i] == Py_None) {
+        out[i].p = like(*x);
+        if (!out[i].p) return nullptr;
+      } else {
+        Py_INCREF(args[4 + i]);
+        out[i].p = args[4 + i];
+      }
+      if (!plain_rows(out[i].p, t.device, from[i].heads, t.head_dim, &to[i]) ||
+          to[i].tokens != from[i].tokens || to[i].dtype != from[i].dtype)
+        Py_RETURN_NONE;
+    }
+    const int status = at_address<std::remove_pointer_t<RotateFn>>(t.rotate)(
+        &t.rotary, where.at, where.count, where.bytes, static_cast<int32_t>(t.head_dim), &from[0],
+        &to[0], count == 2 ? &from[1] : nullptr, count == 2 ? &to[1] : nullptr,
+        at_address<void>(PyLong_AsLongLong(args[6])));
+    if (status) return PyLong_FromLong(status);
+    if (count == 1) return out[0].release();
+    return Py_BuildValue("NN", out[0].release(), out[1].release());
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+}
+
+// paged_write(cache, batch, k, v, rotary or None, positions or None, q or None, out or None,
+// stream, device) -> out, True where there is no q, a status, or None
+PyObject* paged_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  PagedCall p;
+  if (nargs != 10 || !p.take(args[0], args[1], args[8], args[9])) Py_RETURN_NONE;
+  try {
+    RowsArgs k, v, q, to;
+    TurnArgs t;
+    Positions where;
+    if (!p.rows(args[2], p.b.kv_heads, &k) || !p.rows(args[3], p.b.kv_heads, &v) ||
+        k.dtype != v.dtype || k.tokens != v.tokens)
+      Py_RETURN_NONE;
+    const bool turn = args[4] != Py_None, query = args[6] != Py_None;
+    if (turn && (!take_bytes(args[4], &t, sizeof t) || t.device != p.c.device ||
+                 t.head_dim != p.c.cache.head_dim))
+      Py_RETURN_NONE;
+    if (args[5] != Py_None && (!turn || !where.take(args[5], p.c.device))) Py_RETURN_NONE;
+    Ref out(nullptr);
+    if (query) {
+      const at::Tensor* x = p.rows(args[6], p.b.heads, &q);
+      if (!turn || !x || q.dtype != p.c.cache.dtype) Py_RETURN_NONE;
+      if (args[7] == Py_None) {
+        out.p = like(*x);
+        if (!out.p) return nullptr;
+      } else {
+        Py_INCREF(args[7]);
+        out.p = args[7];
+      }
+      if (!p.rows(out.p, p.b.heads, &to) || to.dtype != q.dtype || to.tokens != q.tokens)
+        Py_RETURN_NONE;
+    } else if (args[7] != Py_None) {
+      Py_RETURN_NONE;
+    }
+    const int status = at_address<std::remove_pointer_t<PagedWriteFn>>(p.c.write)(
+        at_address<void>(p.b.host_plan), at_address<void>(p.b.device_plan), &p.c.cache, &k, &v,
+        turn ? &t.rotary : nullptr, where.at, where.count, where.bytes, query ? &q : nullptr,
+        query ? &to : nullptr, p.stream);
+    if (status) return PyLong_FromLong(status);
+    if (query) return out.release();
+    Py_RETURN_TRUE;
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+}
+
+// paged_attend(cache, batch, q, out or None, lse, True for a new one or None, scale or None,
+// stream, device) -> out or (out, lse), a status, or None
+PyObject* paged_attend(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  PagedCall p;
+  if (nargs != 8 || !p.take(args[0], args[1], args[6], args[7])) Py_RETURN_NONE;
+  try {
+    RowsArgs q, to;
+    const at::Tensor* x = p.rows(args[2], p.b.heads, &q);
+    const double scale = p.scale(args[5]);
+    if (!x || q.dtype != p.c.cache.dtype || scale == 0) Py_RETURN_NONE;
+    Ref out(nullptr), lse(nullptr);
+    if (args[3] == Py_None) {
+      out.p = like(*x);
+      if (!out.p) return nullptr;
+    } else {
+      Py_INCREF(args[3]);
+      out.p = args[3];
+    }
+    if (!p.rows(out.p, p.b.heads, &to) || to.dtype != q.dtype || to.tokens != q.tokens)
+      Py_RETURN_NONE;
+    const at::Tensor* sums = nullptr;
+    if (args[4] != Py_None) {
+      if (args[4] == Py_True) {
+        lse.p = THPVariable_Wrap(at::empty({q.tokens, p.b.heads},
+                                           x->options().dtype(at::kFloat).requires_grad(false)));
+        if (!lse.p) return nullptr;
+      } else {
+        Py_INCREF(args[4]);
+        lse.p = args[4];
+      }
+      sums = p.sums(lse.p, q.tokens);
+      if (!sums) Py_RETURN_NONE;
+    }
+    const int64_t bytes = p.b.workspace[p.c.cache.head_dim == 64    ? 0
+                                        : p.c.cache.head_dim == 128 ? 1 : 2];
+    at::Tensor work;   // goes back to the stream's pool, behind the call
+    if (bytes) work = at::empty({bytes}, x->options().dtype(at::kByte).requires_grad(false));
+    const int status = at_address<std::remove_pointer_t<PagedAttendFn>>(p.c.attend)(
+        at_address<void>(p.b.host_plan), at_address<void>(p.b.device_plan), &p.c.cache, &q, &to,
+        sums ? sums->data_ptr() : nullptr, sums ? sums->size(0) : 0, sums ? sums->stride(0) : 0,
+        scale, bytes ? work.data_ptr() : nullptr, bytes, p.stream);
+    if (status) return PyLong_FromLong(status);
+    if (!sums) return out.release();
+    return Py_BuildValue("NN", out.release(), lse.release());
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+}
+
+// paged_weigh(cache, batch, q, lse, weights, scale or None, stream, device) -> True, a status,
+// or None
+PyObject* paged_weigh(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  PagedCall p;
+  if (nargs != 8 || !p.take(args[0], args[1], args[6], args[7])) Py_RETURN_NONE;
+  try {
+    RowsArgs q;
+    const double scale = p.scale(args[5]);
+    if (!p.rows(args[2], p.b.heads, &q) || q.dtype != p.c.cache.dtype || scale == 0)
+      Py_RETURN_NONE;
+    const at::Tensor* sums = p.sums(args[3], q.tokens);
+    const at::Tensor* w = plain_tensor(args[4], p.c.device);
+    if (!sums || !w || w->requires_grad() || w->scalar_type() != at::kFloat || w->dim() != 3 ||
+        w->size(0) != p.c.cache.num_blocks || w->size(1) != p.c.cache.kv_heads ||
+        w->size(2) != p.c.cache.block_size || !w->is_contiguous())
+      Py_RETURN_NONE;
+    const int status = at_address<std::remove_pointer_t<PagedWeighFn>>(p.c.weigh)(
+        at_address<void>(p.b.host_plan), at_address<void>(p.b.device_plan), &p.c.cache, &q,
+        sums->data_ptr(), sums->size(0), sums->stride(0), scale, w->data_ptr(), p.stream);
+    if (status) return PyLong_FromLong(status);
+    Py_RETURN_TRUE;
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+}
+
 template <typename F>
 PyCFunction as_method(F* f) {
   return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f));
@@ -328,6 +610,10 @@ PyMethodDef methods[] = {
     {"quant_write", as_method(quant_write), METH_FASTCALL, nullptr},
     {"quant_read", as_method(quant_read), METH_FASTCALL, nullptr},
     {"quant_attend", as_method(quant_attend), METH_FASTCALL, nullptr},
+    {"rotate", as_method(rotate), METH_FASTCALL, nullptr},
+    {"paged_write", as_method(paged_write), METH_FASTCALL, nullptr},
+    {"paged_attend", as_method(paged_attend), METH_FASTCALL, nullptr},
+    {"paged_weigh", as_method(paged_weigh), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_hostargs", nullptr, -1, methods,

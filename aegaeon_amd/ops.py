@@ -1207,7 +1207,9 @@ def _capturing(stream: torch.cuda.Stream) -> bool:
         return torch.cuda.is_current_stream_capturing()
 
 
-def _cache_call(cache, batch: CacheBatch, stream: torch.cuda.Stream | None):
+def _cache_call(cache, batch: CacheBatch, stream: torch.cuda.Stream | None, kind):
+    if not isinstance(cache, kind):
+        raise ValueError(f"a {kind.__name__}, not a {type(cache).__name__}")
     if (batch.block_size, batch.kv_heads) != (cache.block_size, cache.kv_heads):
         raise ValueError(f"a batch of {batch.block_size}-token blocks and {batch.kv_heads} KV "
                          f"heads over a cache of {cache.block_size} and {cache.kv_heads}")
@@ -1218,7 +1220,7 @@ def _cache_call(cache, batch: CacheBatch, stream: torch.cuda.Stream | None):
     _require_stream(cache.device, stream)
 
 
-def _here(cache: QuantCache) -> tuple:
+def _here(cache) -> tuple:
     """(raw current stream of the cache's device, current device)."""
     return torch._C._cuda_getCurrentRawStream(cache.device.index), torch._C._cuda_getDevice()
 
@@ -1284,7 +1286,7 @@ def quant_write(cache: QuantCache, batch: CacheBatch, k: torch.Tensor, v: torch.
         if done is not None:
             _answer(done)
             return
-    _cache_call(cache, batch, stream)
+    _cache_call(cache, batch, stream, QuantCache)
     kp = _rows_arg(k, "k", cache.kv_heads, cache, _DTYPES)
     vp = _rows_arg(v, "v", cache.kv_heads, cache, _DTYPES)
     if k.dtype != v.dtype or k.size(0) != v.size(0):
@@ -1312,7 +1314,7 @@ def quant_read(cache: QuantCache, batch: CacheBatch, *, tokens: str = "all",
                                           *_here(cache))
         if done is not None:
             return _answer(done)
-    _cache_call(cache, batch, stream)
+    _cache_call(cache, batch, stream, QuantCache)
     n = batch.read_tokens if tokens == "all" else batch.num_tokens
     if out is None:
         if dtype not in _DTYPES:
@@ -1348,7 +1350,7 @@ def quant_attend(cache: QuantCache, batch: CacheBatch, q: torch.Tensor, *,
                                             *_here(cache))
         if done is not None:
             return _answer(done)
-    _cache_call(cache, batch, stream)
+    _cache_call(cache, batch, stream, QuantCache)
     qp = _rows_arg(q, "q", batch.heads, cache, (torch.bfloat16, torch.float16))
     if out is None:
         out = _empty_on(stream, q.shape, dtype=q.dtype, device=q.device)
@@ -1460,6 +1462,9 @@ class Rotary:
         self._turns = _turn_tables[key]
         self._args = _lib.RotaryArgs(self._turns.data_ptr(), self.dim, self.interleaved,
                                      self.amplitude)
+        # TurnArgs of csrc/hostargs.cpp
+        self._packed = (struct.pack("q", _lib.address("aegkv_rotate")) + bytes(self._args)
+                        + struct.pack("2q", self.head_dim, self.device.index))
 
 
 class PagedCache:
@@ -1520,14 +1525,22 @@ class PagedCache:
         self._args = _lib.PagedCacheArgs(k_pages.data_ptr(), v_pages.data_ptr(), *blocks,
                                          self.num_blocks, self.block_size, self.kv_heads,
                                          self.head_dim, _DTYPES[self.dtype], self.head_major, 0)
+        # PagedArgs of csrc/hostargs.cpp
+        self._packed = (struct.pack("3q", *(_lib.address(f"aegkv_paged_{op}")
+                                            for op in ("write", "attend", "weigh")))
+                        + bytes(self._args) + struct.pack("q", self.device.index))
+
+
+def _native(cache: PagedCache, batch: CacheBatch, stream) -> bool:
+    """Whether a call may be the plain case, which is checked and made natively."""
+    return (stream is None and _alive(batch._home) and not cache.k_pages.requires_grad
+            and not cache.v_pages.requires_grad)
 
 
 def _paged_call(cache: PagedCache, batch: CacheBatch, stream) -> None:
-    if not isinstance(cache, PagedCache):
-        raise ValueError(f"a PagedCache, not a {type(cache).__name__}")
+    _cache_call(cache, batch, stream, PagedCache)
     if cache.k_pages.requires_grad or cache.v_pages.requires_grad:
         raise ValueError("the cache requires a gradient, which these operators do not give")
-    _cache_call(cache, batch, stream)
 
 
 def _rows(t: torch.Tensor, what: str, heads: int, of, dtypes) -> _lib.Rows:
@@ -1568,6 +1581,12 @@ def rotate(rotary: Rotary, positions: torch.Tensor, q: torch.Tensor,
     negative one turns back. Returns q, or (q, k), rotated: new tensors, or `out` (the
     same way; q and k themselves are fine, other overlaps are refused).
     """
+    if stream is None:
+        to = (out, None) if k is None or out is None else out
+        if len(to) == 2:
+            done = _lib.hostargs().rotate(rotary._packed, positions, q, k, *to, *_here(rotary))
+            if done is not None:
+                return _answer(done)
     head_dim = rotary.head_dim
     _check_rotary(rotary, head_dim, q.device)
     _require_stream(q.device, stream)
@@ -1613,6 +1632,13 @@ def paged_write(cache: PagedCache, batch: CacheBatch, k: torch.Tensor, v: torch.
     or int64 on the device), where they are not their places in the sequences, as
     after an eviction.
     """
+    if _native(cache, batch, stream):
+        done = _lib.hostargs().paged_write(cache._packed, batch._packed, k, v,
+                                           None if rotary is None else rotary._packed, positions,
+                                           q, out, *_here(cache))
+        if done is not None:
+            done = _answer(done)
+            return None if done is True else done
     _paged_call(cache, batch, stream)
     if k.dtype != v.dtype or k.size(0) != v.size(0):
         raise ValueError(f"k and v differ: {k.size(0)} tokens of {k.dtype}, {v.size(0)} of "
@@ -1671,6 +1697,12 @@ def paged_attend(cache: PagedCache, batch: CacheBatch, q: torch.Tensor, *,
     (out, lse) with return_lse or a tensor `lse` to fill: [tokens, heads] float32, the
     log of the sum of exp(score) over what each query sees, as paged_weigh takes it.
     """
+    if _native(cache, batch, stream):
+        done = _lib.hostargs().paged_attend(cache._packed, batch._packed, q, out,
+                                            lse if lse is not None else return_lse or None, scale,
+                                            *_here(cache))
+        if done is not None:
+            return _answer(done)
     _paged_call(cache, batch, stream)
     qr = _rows(q, "q", batch.heads, cache, (cache.dtype,))
     if out is None:
@@ -1721,6 +1753,12 @@ def paged_weigh(cache: PagedCache, batch: CacheBatch, q: torch.Tensor, lse: torc
     sees keep theirs. As a segment of the composite cache (layout.weight_tensor_specs)
     they move with the blocks.
     """
+    if _native(cache, batch, stream):
+        done = _lib.hostargs().paged_weigh(cache._packed, batch._packed, q, lse, weights, scale,
+                                           *_here(cache))
+        if done is not None:
+            _answer(done)
+            return
     _paged_call(cache, batch, stream)
     qr = _rows(q, "q", batch.heads, cache, (cache.dtype,))
     sums = _sums_arg(lse, batch.heads, cache.device)

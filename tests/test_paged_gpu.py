@@ -746,6 +746,69 @@ def test_other_streams(gpu):
         assert torch.equal(a, b)
 
 
+def test_the_general_path_gives_the_same(gpu, monkeypatch):
+    """Plain calls are checked and made natively; the general path gives the same bits,
+    and refuses what the native one leaves to it."""
+    from aegaeon_amd import _lib
+
+    bs, heads, d, dtype, num = 32, 2, 64, F16, 20
+    outs, calls = [], []
+
+    class Counted:
+        def __getattr__(self, name):
+            fn = getattr(native, name)
+
+            def call(*args):
+                done = fn(*args)
+                calls.append((name, done is not None))
+                return done
+            return call
+
+    native = _lib.hostargs()
+    for readers in (Counted(), _lib._GeneralPath):
+        monkeypatch.setattr(_lib, "_hostargs", readers)
+        pages = [p.to(gpu) for p in make_pages(num, bs, heads, d, dtype)]
+        cache = ops.PagedCache(*pages)
+        batch = batch_for(gpu, tables_for([90, 33], bs, num), [90, 33], [3, 1], cache, heads=6)
+        g = gen(3)
+        k, v = (torch.randn(4, heads, d, generator=g).to(F32).to(gpu) for _ in range(2))
+        q = torch.randn(4, 6, d, generator=g).to(dtype).to(gpu)
+        rotary = ops.Rotary(d, dim=32, interleaved=True, device=gpu)
+        positions = torch.tensor([5, 6, 7, 8], dtype=torch.int32, device=gpu)
+        w = torch.ones(num, heads, bs, device=gpu)
+        assert ops.paged_write(cache, batch, k, v) is None
+        first = [p.clone() for p in pages]
+        ops.paged_write(cache, batch, k, v, rotary=rotary)
+        second = [p.clone() for p in pages]
+        qr = ops.paged_write(cache, batch, k, v, rotary=rotary, positions=positions, q=q)
+        out, lse = ops.paged_attend(cache, batch, qr, return_lse=True, scale=0.3)
+        given = torch.zeros_like(lse)
+        again = torch.zeros_like(out)
+        a, b = ops.paged_attend(cache, batch, qr, out=again, lse=given, scale=0.3)
+        assert a is again and b is given
+        ops.paged_weigh(cache, batch, qr, lse, w, scale=0.3)
+        qk = ops.rotate(rotary, positions, q, q[:, :2])
+        alone = ops.rotate(rotary, positions, q, out=torch.zeros_like(q))
+        outs.append((*first, *second, *pages, qr, out, lse, again, given, w, *qk, alone,
+                     ops.paged_attend(cache, batch, q)))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    assert len(calls) == 9 and all(done for _, done in calls)
+
+
+def test_calls_take_their_own_kind_of_cache(gpu):
+    pages = [p.to(gpu) for p in make_pages(4, 16, 2, 64, BF16)]
+    paged = ops.PagedCache(*pages)
+    quant = ops.QuantCache(*(torch.zeros(4, ops.quant_page_bytes("mxfp8", 16, 2, 64),
+                                         dtype=torch.uint8, device=gpu) for _ in range(2)),
+                           kv_heads=2, head_dim=64, block_size=16, fmt="mxfp8")
+    batch = batch_for(gpu, [[1]], [3], [3], paged)
+    x = torch.zeros(3, 2, 64, dtype=BF16, device=gpu)
+    with pytest.raises(ValueError, match="a PagedCache, not a QuantCache"):
+        ops.paged_attend(quant, batch, x)
+    with pytest.raises(ValueError, match="a QuantCache, not a PagedCache"):
+        ops.quant_attend(paged, batch, x)
+
+
 def test_refusals(gpu):
     bs, heads, d, dtype, num = 16, 2, 64, BF16, 10
     pages = [p.to(gpu) for p in make_pages(num, bs, heads, d, dtype)]
