@@ -82,6 +82,7 @@ struct Room {
   int64_t slots[kKinds];
   int64_t merges;
   int64_t at_seqs, at_table, at_new_spans, at_items[kKinds], at_merges;
+  int64_t at_place_tiles;          // int32: the sequence of each tile of kPlaceTile places
 };
 
 struct Header {

@@ -237,6 +237,7 @@ inline int fill(Header& h, const Batch& b, const std::vector<Rows>* rows, char* 
   auto* table = reinterpret_cast<int32_t*>(base + room.at_table);
   auto* merge = reinterpret_cast<Merge*>(base + room.at_merges);
   auto* span = reinterpret_cast<NewSpan*>(base + room.at_new_spans);
+  auto* tile_seq = reinterpret_cast<int32_t*>(base + room.at_place_tiles);
   int64_t columns = 0, tokens = 0, new_spans = 0, read_spans = 0, read_tokens = 0;
   int64_t place_tiles = 0;
   h.complete = 1;
@@ -277,7 +278,12 @@ inline int fill(Header& h, const Batch& b, const std::vector<Rows>* rows, char* 
       at = end;
     }
     read_spans += up(len, kSpan);
-    place_tiles += up(len, kPlaceTile);
+    for (int64_t at = 0; at < len; at += kPlaceTile) {
+      if (place_tiles >= room.place_tiles)
+        return aegkv_set_error(AEGKV_ENOMEM, "the sequences do not fit the plan's %lld tiles of "
+                               "places", ll(room.place_tiles));
+      tile_seq[place_tiles++] = static_cast<int32_t>(s);
+    }
     read_tokens += len;
   }
   h.num_seqs = static_cast<int32_t>(b.num_seqs);
@@ -286,7 +292,7 @@ inline int fill(Header& h, const Batch& b, const std::vector<Rows>* rows, char* 
   h.read_spans = static_cast<int32_t>(read_spans);
   h.place_tiles = static_cast<int32_t>(place_tiles);
   h.read_tokens = read_tokens;
-  if (read_spans > room.read_spans || place_tiles > room.place_tiles)
+  if (read_spans > room.read_spans)
     return aegkv_set_error(AEGKV_ENOMEM, "%lld spans to read do not fit the plan", ll(read_spans));
   int64_t merges = 0;
   for (int kind = 0; kind < kKinds; ++kind) {
@@ -344,10 +350,9 @@ inline int fill(Header& h, const Batch& b, const std::vector<Rows>* rows, char* 
 inline void make_room(Header& h, const Batch& b, const std::vector<Rows>* rows, int64_t max_seqs,
                       int64_t max_columns, int64_t max_tokens) {
   Room& r = h.room;
-  int64_t columns = 0, tokens = 0, new_spans = 0, read_spans = 0, place_tiles = 0;
+  int64_t columns = 0, tokens = 0, new_spans = 0, read_spans = 0;
   for (int64_t s = 0; s < b.num_seqs; ++s) {
     const int64_t len = b.lens[s], fresh = b.fresh[s];
-    place_tiles += up(len, kPlaceTile);
     columns += up(len, h.block_size);
     tokens += fresh;
     if (fresh) new_spans += up(len, kSpan) - (len - fresh) / kSpan;
@@ -360,9 +365,9 @@ inline void make_room(Header& h, const Batch& b, const std::vector<Rows>* rows, 
   r.tokens = std::max(max_tokens, tokens);
   r.new_spans = exact ? new_spans : std::min(r.tokens, r.tokens / kSpan + 2 * r.seqs);
   r.read_spans = exact ? read_spans : max_columns * (h.block_size / kSpan);
-  // (a sequence's last tile may hold one place)
-  r.place_tiles = exact ? place_tiles
-                        : std::min(max_columns, max_columns * h.block_size / kPlaceTile + r.seqs);
+  // (a sequence's last tile may hold one place; also where there is room for nothing
+  // else, an update may have other lengths in as many blocks)
+  r.place_tiles = std::min(max_columns, max_columns * h.block_size / kPlaceTile + r.seqs);
   r.merges = 0;
   int64_t at = pad16(sizeof(Header));
   auto take = [&](int64_t bytes) {
@@ -396,6 +401,7 @@ inline void make_room(Header& h, const Batch& b, const std::vector<Rows>* rows, 
     r.at_items[kind] = take(r.items[kind] * static_cast<int64_t>(sizeof(Item)));
   }
   r.at_merges = take(r.merges * static_cast<int64_t>(sizeof(Merge)));
+  r.at_place_tiles = take(r.place_tiles * 4);
   r.bytes = at;
 }
 

@@ -19,6 +19,24 @@ struct Pages {
   int32_t token, head;        // bytes inside a page
 };
 
+// x / by for 0 <= x: a division in 32 bits takes some thirty instructions. `part` is
+// 2^32 / by rounded down (by > 1), so the product is the quotient or one less.
+struct Divisor {
+  uint32_t by, part;
+};
+
+__host__ __device__ __forceinline__ Divisor divisor(int32_t by) {
+  return Divisor{static_cast<uint32_t>(by),
+                 by > 1 ? static_cast<uint32_t>((uint64_t(1) << 32) / static_cast<uint32_t>(by))
+                        : 0u};
+}
+
+__device__ __forceinline__ int32_t quotient(int32_t x, Divisor d) {
+  if (d.by == 1) return x;
+  const uint32_t u = static_cast<uint32_t>(x), q = __umulhi(u, d.part);
+  return static_cast<int32_t>(q + (u - q * d.by >= d.by));
+}
+
 // ---------------------------------------------------------- rotate, write --
 
 // Where the values of a kind of heads come from and go to.
@@ -31,7 +49,7 @@ struct PlaceArgs {
   const char* plan;           // null: tokens are rows, one after another
   int64_t at_new_spans;
   int64_t tokens;             // without a plan
-  int32_t chunk;              // tokens of a span without a plan
+  int32_t chunk, parts;       // tokens of a workgroup; workgroups that a plan's span is cut into
   const double* turns;        // a position's turns, for each pair
   const void* positions;      // null: the plan's
   int32_t position_bytes;
@@ -43,55 +61,153 @@ struct PlaceArgs {
   Pages pages;                // where k and v go (k.to: without a plan)
   int32_t kv_heads, block_shift;
   int32_t heads, heads_each, head_groups;   // of all kinds; of a workgroup; workgroups a span
+  Divisor each, rest;         // heads_each; the last workgroup's of a span
+  Divisor units, by_pairs;    // items of a head; pairs
 };
 
 constexpr int kPlaceLanes = 256;
-constexpr int kPlaceTokens = 16;    // of a workgroup
-constexpr int kMostAngles = kPlaceTokens * 128;
+constexpr int kPlaceTokens = 4;     // of a workgroup
+constexpr int kMostAngles = 2048;   // of a workgroup: its tokens of up to 512 pairs
 
-// N values as float32 and back, N = 1 or 8.
+// N values as float32 and back, N = 1, 4 or 8.
 template <int N, typename T>
 __device__ __forceinline__ void take(const T* p, bool whole_words, float* x) {
-  if constexpr (N == 8) load8(p, whole_words, x);
-  else x[0] = static_cast<float>(*p);
+  if constexpr (N == 8) {
+    load8(p, whole_words, x);
+  } else {
+    T t[N];
+    if (N > 1 && whole_words) {
+      typedef unsigned int words __attribute__((ext_vector_type(N * sizeof(T) / 4 ? N * sizeof(T) / 4 : 1)));
+      const words w = __builtin_nontemporal_load(reinterpret_cast<const words*>(p));
+      __builtin_memcpy(t, &w, sizeof t);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) t[i] = p[i];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = static_cast<float>(t[i]);
+  }
 }
 template <int N, typename T>
 __device__ __forceinline__ void give(T* p, bool whole_words, const float* x) {
-  if constexpr (N == 8) store8(p, whole_words, x);
-  else *p = static_cast<T>(x[0]);
+  if constexpr (N == 8) {
+    store8(p, whole_words, x);
+  } else {
+    T t[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] = static_cast<T>(x[i]);
+    if (N > 1 && whole_words) {
+      typedef unsigned int words __attribute__((ext_vector_type(N * sizeof(T) / 4 ? N * sizeof(T) / 4 : 1)));
+      words w;
+      __builtin_memcpy(&w, t, sizeof t);
+      __builtin_nontemporal_store(w, reinterpret_cast<words*>(p));
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) p[i] = t[i];
+    }
+  }
+}
+
+__device__ __forceinline__ void turn_pair(float& a, float& b, float c, float s) {
+  const float x = a * c - b * s;
+  b = b * c + a * s;
+  a = x;
 }
 
 // (a, b) -> (a c - b s, b c + a s) for each pair, c and s the cosine and sine of
 // position * turns: the angle in 64 bits, of which the whole turns are dropped before
 // it is rounded (positions of millions keep their angle), values in 32, one
-// rounding at the end. A workgroup takes up to 16 tokens of some heads: the angles,
-// 60 instructions each, are made once for all of them.
-// G: type of k and v; T: of q, of what is written and of what comes of q. N: pairs of
-// an item. A lane takes 2 N values of a head at once: N at a and N at b.
+// rounding at the end. A workgroup takes up to 4 tokens of some heads: the angles,
+// 150 instructions each, are made once for all of them, while the first values are on
+// their way.
+// G: type of k and v; T: of q, of what is written and of what comes of q. A lane takes
+// two runs of N values of a head at once, half of the rotated part (or of the others) apart:
+// both sides of N pairs, or neighbouring pairs in each run where they are interleaved, and
+// lanes side by side reach for neighbouring bytes either way. N: 8, 4 for values in
+// 32 bits (16 bytes a load), 1 for parts that are no whole runs.
 template <int N, typename G, typename T>
 __global__ __launch_bounds__(kPlaceLanes) void place_rows_kernel(PlaceArgs a) {
   __shared__ float cosine[kMostAngles], sine[kMostAngles];
-  const int32_t span = blockIdx.x / a.head_groups;
-  const int32_t first_head = (blockIdx.x - span * a.head_groups) * a.heads_each;
+  const int32_t at_span = blockIdx.x / a.head_groups;
+  const int32_t first_head = (blockIdx.x - at_span * a.head_groups) * a.heads_each;
   const int32_t heads = min(a.heads_each, a.heads - first_head);
+  const int32_t span = at_span / a.parts, part = (at_span - span * a.parts) * a.chunk;
   int64_t token;
   int32_t count, position = 0, block = 0, inside = 0;
   if (a.plan) {
     if (span >= in_plan<Header>(a.plan, 0)->new_spans) return;
     const auto* s = in_plan<NewSpan>(a.plan, a.at_new_spans) + span;
-    token = s->token;
-    count = s->count;
-    position = s->position;
+    token = int64_t(s->token) + part;
+    count = min(a.chunk, s->count - part);
+    position = s->position + part;
     block = s->block;
-    inside = s->inside;
+    inside = s->inside + part;
+    if (count <= 0) return;
   } else {
     token = int64_t(span) * a.chunk;
     count = static_cast<int32_t>(min<int64_t>(a.chunk, a.tokens - token));
   }
-  // (v's heads need no angles)
-  if (first_head < a.q.heads + a.k.heads) {
-    for (int32_t i = threadIdx.x; i < count * a.pairs; i += kPlaceLanes) {
-      const int32_t t = i / a.pairs, pair = i - t * a.pairs;
+  const int32_t turned = a.pairs / N, rotated = a.q.heads + a.k.heads;
+  const int32_t items = count * heads * static_cast<int32_t>(a.units.by);
+  const Divisor by_heads = first_head + a.heads_each <= a.heads ? a.each : a.rest;
+  char* const k_page = const_cast<char*>(a.pages.k) + (a.plan ? block * a.pages.k_block : 0);
+  char* const v_page = const_cast<char*>(a.pages.v) + (a.plan ? block * a.pages.v_block : 0);
+
+  // Item i: of token t, N values from `at` and N from `next`. (One behind the last is the
+  // last one again, and not given.)
+  struct Item {
+    int32_t t, head, unit, at, next;
+    bool turn;
+  };
+  const auto find = [&](int32_t i) {
+    Item m;
+    i = min(i, items - 1);
+    const int32_t row = quotient(i, a.units);
+    m.unit = i - row * static_cast<int32_t>(a.units.by);
+    m.t = quotient(row, by_heads);
+    m.head = first_head + row - m.t * heads;
+    m.turn = m.unit < turned && m.head < rotated;
+    const bool whole = m.head >= rotated;           // a head of v
+    const int32_t begin = whole || m.turn ? 0 : 2 * a.pairs;
+    m.at = begin + N * (m.unit - (whole || m.turn ? 0 : turned));
+    if (N == 1 && m.turn && a.interleaved) {
+      m.at = 2 * m.unit;
+      m.next = m.at + 1;
+      return m;
+    }
+    m.next = m.at + (m.turn ? a.pairs : whole ? a.head_dim / 2 : a.head_dim / 2 - a.pairs);
+    return m;
+  };
+  constexpr int kItems = 2;     // on their way together
+  float x[kItems][N], y[kItems][N];
+  const auto take_items = [&](int32_t i) {
+#pragma unroll
+    for (int u = 0; u < kItems; ++u) {
+      const Item m = find(i + u * kPlaceLanes);
+      const int64_t r = token + m.t;
+      if (m.head < a.q.heads) {
+        const T* from = reinterpret_cast<const T*>(a.q.from.base) + r * a.q.from.token +
+                        m.head * a.q.from.head;
+        take<N>(from + m.at, a.q.from.whole_words, x[u]);
+        take<N>(from + m.next, a.q.from.whole_words, y[u]);
+      } else {
+        const bool key = m.head < rotated;
+        const char* base = key ? a.k.from.base : a.v.base;
+        const bool words = key ? a.k.from.whole_words : a.v.whole_words;
+        const G* from = reinterpret_cast<const G*>(base) +
+                        r * (key ? a.k.from.token : a.v.token) +
+                        (m.head - (key ? a.q.heads : rotated)) *
+                            (key ? a.k.from.head : a.v.head);
+        take<N>(from + m.at, words, x[u]);
+        take<N>(from + m.next, words, y[u]);
+      }
+    }
+  };
+  int32_t first = threadIdx.x;
+  take_items(first);
+  if (first_head < rotated) {     // v's heads need no angles
+    for (int32_t j = threadIdx.x; j < count * a.pairs; j += kPlaceLanes) {
+      const int32_t t = quotient(j, a.by_pairs), pair = j - t * a.pairs;
       int64_t p = position + t;
       if (a.positions)
         p = a.position_bytes == 8 ? static_cast<const int64_t*>(a.positions)[token + t]
@@ -100,78 +216,53 @@ __global__ __launch_bounds__(kPlaceLanes) void place_rows_kernel(PlaceArgs a) {
       turn -= rint(turn);
       float s, c;
       sincospif(static_cast<float>(2 * turn), &s, &c);
-      cosine[i] = c * a.amplitude;
-      sine[i] = s * a.amplitude;
+      cosine[j] = c * a.amplitude;
+      sine[j] = s * a.amplitude;
     }
   }
   __syncthreads();
-  const int32_t units = a.head_dim / (2 * N), turned = a.pairs / N;
-  const int32_t items = count * heads * units;
-  const int64_t k_at = a.plan ? block * a.pages.k_block : 0;
-  const int64_t v_at = a.plan ? block * a.pages.v_block : 0;
-#pragma unroll 2
-  for (int32_t i = threadIdx.x; i < items; i += kPlaceLanes) {
-    const int32_t row = i / units, u = i - row * units;
-    const int32_t t = row / heads;
-    int32_t head = first_head + row - t * heads;
-    int32_t at = 2 * N * u, next = at + N;      // untouched values, interleaved pairs
-    const bool turn = u < turned && head < a.q.heads + a.k.heads;
-    if (turn && !a.interleaved) {
-      at = N * u;
-      next = at + a.pairs;
-    }
-    const auto work = [&](const auto* from, bool from_words, auto* to, bool to_words) {
-      float x[N], y[N];
-      take<N>(from + at, from_words, x);
-      take<N>(from + next, from_words, y);
-      if (turn) {
-        const float* c = cosine + t * a.pairs + N * u;
-        const float* s = sine + t * a.pairs + N * u;
+  for (; first < items; first += kItems * kPlaceLanes) {
+#pragma unroll
+    for (int u = 0; u < kItems; ++u) {
+      if (first + u * kPlaceLanes >= items) continue;
+      const Item m = find(first + u * kPlaceLanes);
+      if (m.turn) {
+        const float* c = cosine + m.t * a.pairs;
+        const float* s = sine + m.t * a.pairs;
         if (!a.interleaved || N == 1) {
 #pragma unroll
-          for (int j = 0; j < N; ++j) {
-            const float p = x[j] * c[j] - y[j] * s[j];
-            y[j] = y[j] * c[j] + x[j] * s[j];
-            x[j] = p;
-          }
-        } else {
-          const auto spin = [&](float* z, const float* cc, const float* ss) {
+          for (int j = 0; j < N; ++j)
+            turn_pair(x[u][j], y[u][j], c[N * m.unit + j], s[N * m.unit + j]);
+        } else if constexpr (N > 1) {
 #pragma unroll
-            for (int j = 0; j < N / 2; ++j) {
-              const float p = z[2 * j] * cc[j] - z[2 * j + 1] * ss[j];
-              z[2 * j + 1] = z[2 * j + 1] * cc[j] + z[2 * j] * ss[j];
-              z[2 * j] = p;
-            }
-          };
-          spin(x, c, s);
-          spin(y, c + N / 2, s + N / 2);
+          for (int j = 0; j < N / 2; ++j) {
+            const int pair = m.at / 2 + j, other = m.next / 2 + j;
+            turn_pair(x[u][2 * j], x[u][2 * j + 1], c[pair], s[pair]);
+            turn_pair(y[u][2 * j], y[u][2 * j + 1], c[other], s[other]);
+          }
         }
       }
-      give<N>(to + at, to_words, x);
-      give<N>(to + next, to_words, y);
-    };
-    const int64_t r = token + t;
-    if (head < a.q.heads) {
-      const Values f = a.q.from, o = a.q.to;
-      work(reinterpret_cast<const T*>(f.base) + r * f.token + head * f.head, f.whole_words,
-           reinterpret_cast<T*>(o.base) + r * o.token + head * o.head, o.whole_words);
-      continue;
+      const int64_t r = token + m.t;
+      const auto give_both = [&](auto* to, bool words) {
+        give<N>(to + m.at, words, x[u]);
+        give<N>(to + m.next, words, y[u]);
+      };
+      if (m.head < a.q.heads) {
+        give_both(reinterpret_cast<T*>(a.q.to.base) + r * a.q.to.token + m.head * a.q.to.head,
+                  a.q.to.whole_words);
+        continue;
+      }
+      const bool key = m.head < rotated;
+      const int32_t head = m.head - (key ? a.q.heads : rotated);
+      if (a.plan)
+        give_both(reinterpret_cast<T*>((key ? k_page : v_page) +
+                                       int64_t(inside + m.t) * a.pages.token +
+                                       int64_t(head) * a.pages.head), true);
+      else
+        give_both(reinterpret_cast<G*>(a.k.to.base) + r * a.k.to.token + head * a.k.to.head,
+                  a.k.to.whole_words);
     }
-    head -= a.q.heads;
-    const bool key = head < a.k.heads;
-    if (!key) head -= a.k.heads;
-    const Values f = key ? a.k.from : a.v;
-    const G* from = reinterpret_cast<const G*>(f.base) + r * f.token + head * f.head;
-    if (a.plan) {
-      char* page = const_cast<char*>(key ? a.pages.k + k_at : a.pages.v + v_at);
-      work(from, f.whole_words,
-           reinterpret_cast<T*>(page + int64_t(inside + t) * a.pages.token +
-                                int64_t(head) * a.pages.head), true);
-    } else {
-      const Values o = a.k.to;
-      work(from, f.whole_words, reinterpret_cast<G*>(o.base) + r * o.token + head * o.head,
-           o.whole_words);
-    }
+    take_items(first + kItems * kPlaceLanes);
   }
 }
 
@@ -303,11 +394,18 @@ __device__ __forceinline__ v4u query8(PagedCold args, PagedItem it, int32_t row,
   return x;
 }
 
-// Whether one of a word's two values is an infinity or no number.
+// Bits 15 and 31 of the result: whether a word's lower and upper value are infinities
+// or no numbers (an exponent of ones carries into the sign's place).
 template <typename T>
-__device__ __forceinline__ bool not_finite(uint32_t w) {
-  constexpr uint32_t kExponent = std::is_same<T, __bf16>::value ? 0x7F80u : 0x7C00u;
-  return (w & kExponent) == kExponent || ((w >> 16) & kExponent) == kExponent;
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  constexpr bool kWide = std::is_same<T, __bf16>::value;
+  return (w & (kWide ? 0x7F807F80u : 0x7C007C00u)) + (kWide ? 0x00800080u : 0x04000400u);
+}
+constexpr uint32_t kNotFinite = 0x80008000u;
+
+// All bits of the values that not_finite() found.
+__device__ __forceinline__ uint32_t whole_values(uint32_t found) {
+  return ((found >> 15) & 0x00010001u) * 0xFFFFu;
 }
 
 // Where a half tile of 16 tokens lies for one head: the same for the whole wave.
@@ -377,9 +475,10 @@ struct PagedTile {
     for (int half = 0; half < 2; ++half)
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        bool bad = false;
+        uint32_t found = 0;
 #pragma unroll
-        for (int w = 0; w < kWords; ++w) bad |= not_finite<T>(v[half][t][w]);
+        for (int w = 0; w < kWords; ++w) found |= not_finite<T>(v[half][t][w]);
+        const bool bad = (found & kNotFinite) != 0;
         const int32_t j = begin + 16 * half + 4 * g + t;
         const bool any = (j <= high) & ((low - j < a.window) | (j < a.sinks));
         odd |= (bad & any) ? 1u << (4 * half + t) : 0u;
@@ -656,24 +755,29 @@ __device__ __forceinline__ float pair_max(float x) {
 }
 
 // Prompts: 128 rows a workgroup, 32 a wave, as the above with products of 32 x 32.
-// A stage of 64 tokens' K and V lies in shared memory as rows of 16-byte chunks, each
-// row's chunks exchanged by its number so that neither product's reads meet in a bank:
-// K's operands are a token's chunk a lane, V's come four tokens of a value a lane by
-// transposing reads. Lane l (row l % 32, h = l / 32) holds the scores of tokens 8 (i / 4)
-// + 4 h + i % 4, i < 16, and they are the second product's operand as they lie.
-constexpr int kStageTokens = 64, kRowsWave = 32;
+// Tiles of 32 tokens go straight from the cache to a ring of four in shared memory, as
+// rows of 16-byte chunks, each row's chunks exchanged by its number so that neither
+// product's reads meet in a bank: K's operands are a token's chunk a lane, V's come four
+// tokens of a value a lane by transposing reads. Lane l (row l % 32, h = l / 32) holds the
+// scores of tokens 8 (i / 4) + 4 h + i % 4, i < 16, and they are the second product's
+// operand as they lie.
+constexpr int kRing = 4, kRowsWave = 32, kTileRowsWave = kTile / kPagedWaves;
 static_assert(kManyRows == kPagedWaves * kRowsWave, "rows of a workgroup");
 
 template <int D>
-struct PagedStage {
+struct PagedRing {
   static constexpr int kChunks = D / 8;    // of 16 bytes in a row
-  v4u k[kStageTokens * kChunks];
-  v4u v[kStageTokens * kChunks];
+  v4u k[kRing][kTile * kChunks];
+  v4u v[kRing][kTile * kChunks];
+  static __device__ __forceinline__ int k_turn(int token) {
+    return D == 64 ? token / 2 % 8 : token % 16;
+  }
+  static __device__ __forceinline__ int v_turn(int token) { return 2 * (token % 4); }
   static __device__ __forceinline__ int k_at(int token, int chunk) {
-    return token * kChunks + (chunk ^ (D == 64 ? token / 2 % 8 : token % 16));
+    return token * kChunks + (chunk ^ k_turn(token));
   }
   static __device__ __forceinline__ int v_at(int token, int chunk) {
-    return token * kChunks + (chunk ^ (2 * (token % 4)));
+    return token * kChunks + (chunk ^ v_turn(token));
   }
 };
 
@@ -682,15 +786,67 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 // Of 16 lanes that point at four rows of 16 values, four values a lane: lane i gets
 // value i of the four rows.
-__device__ __forceinline__ s16x4 read_turned(const char* p) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+__device__ __forceinline__ s16x4 read_turned(uint32_t at) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)static_cast<uintptr_t>(at));
+}
+
+__device__ __forceinline__ uint32_t shared_address(const v4u* p) {
+  return static_cast<uint32_t>(
+      reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const v4u*)p));
+}
+
+// 16 bytes a lane from `base` (the same for the wave) + offset to shared memory, lane
+// after lane from `to` on. The compiler does not know of it: whoever reads them waits by
+// wait_and_meet() first. (Told of it, it waits for all such loads before any read of shared
+// memory.)
+__device__ __forceinline__ void load_shared(const char* base, uint32_t offset, const v4u* to) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               :: "v"(offset), "s"(base), "s"(shared_address(to)) : "memory");
+}
+
+// All of the wave's loads have come but the last LATER, its reads of shared memory too,
+// and the other waves are here as well.
+template <int LATER>
+__device__ __forceinline__ void wait_and_meet() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(LATER) : "memory");
+}
+
+// Adds, in 32 bits and to the rows that see their tokens, the infinities and no numbers
+// that were taken out of a tile's V (they are rare).
+template <int D, typename T>
+__device__ __forceinline__ void add_odd_rows(const Sight& a, const v4u* tile, int32_t begin,
+                                             int32_t low, int32_t high, int32_t position, int n,
+                                             int h, const float (&e)[16], f32x16 (&o)[D / 32]) {
+#pragma unroll 1
+  for (int t = 0; t < kTile; ++t) {
+    const int32_t j = begin + t;
+    if (!((j <= high) & ((low - j < a.window) | (j < a.sinks)))) continue;   // none sees it
+    const bool sees = seen(a, position, j);
+    // the row's probability of token t, from the lane that has it
+    float mine = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      mine = i == 4 * (t / 8) + t % 4 ? static_cast<float>(static_cast<T>(e[i])) : mine;
+    const float weight = __shfl(mine, n + 32 * (t / 4 % 2));
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int value = 32 * d + 8 * (i / 4) + 4 * h + i % 4;
+        const T y = reinterpret_cast<const T*>(
+            &tile[PagedRing<D>::v_at(t, value / 8)])[value % 8];
+        const bool bad = not_finite<T>(__builtin_bit_cast(uint16_t, y)) & kNotFinite;
+        const float was = o[d][i];
+        o[d][i] = (bad & sees) ? __builtin_fmaf(weight, static_cast<float>(y), was) : was;
+      }
+  }
 }
 
 template <int D, typename T>
 __device__ __forceinline__ void paged_prompt_item(const Sight& a, const Pages& pages,
-                                                  PagedItem it, PagedStage<D> (&stages)[2]) {
+                                                  PagedItem it, PagedRing<D>& ring) {
   typedef typename Matrix<T>::v8 v8;
-  typedef PagedStage<D> Stage;
+  typedef PagedRing<D> Ring;
   constexpr int kSteps = D / 16, kOut = D / 32;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int lane = threadIdx.x % 64, n = lane % 32, h = lane / 32;
@@ -698,34 +854,38 @@ __device__ __forceinline__ void paged_prompt_item(const Sight& a, const Pages& p
   const auto* table = in_plan<int32_t>(args->plan, args->at_table) + it->table;
   const Tiles tiles = {it->first_tiles, it->window_tile - it->first_tiles, it->tile_end};
   const int32_t group = args->group, kv_head = it->kv_head;
+  const int32_t first = it->tile, end = it->tile_end;
 
-  // this wave's share of a stage: 16 tokens, kRows of them at a time
-  constexpr int kLanesRow = Stage::kChunks < 64 ? Stage::kChunks : 64;
-  constexpr int kRows = 64 / kLanesRow, kLoads = 16 / kRows;
-  const int own_tile = wave / 2, own_half = wave % 2;
-  const int load_row = lane / kLanesRow, load_chunk = lane % kLanesRow;
-  v4u held_k[kLoads], held_v[kLoads];
-  const auto load = [&](int32_t at) {
-    // behind the last tile the last one is read again, and not used
-    const int32_t position = tiles.at(min(at + own_tile, tiles.end - 1)) * kTile + 16 * own_half;
-    const PagedHalf half = paged_half(pages, kv_head, a.block_shift,
-                                      table[position >> a.block_shift], position);
+  // This wave's share of a tile: eight tokens of K and of V. Lane by lane the places of
+  // shared memory are given; which chunk of the row comes there follows from them.
+  constexpr int kLoads = kTileRowsWave * Ring::kChunks / 64;
+  uint32_t k_from[kLoads], v_from[kLoads];
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const uint32_t offset = (i * kRows + load_row) * pages.token + load_chunk * 16;
-      load_bytes<16, false>(reinterpret_cast<uint32_t*>(&held_k[i]), half.k, offset);
-      load_bytes<16, false>(reinterpret_cast<uint32_t*>(&held_v[i]), half.v, offset);
-    }
+  for (int i = 0; i < kLoads; ++i) {
+    const int slot = i * 64 + lane, row = slot / Ring::kChunks, at = slot % Ring::kChunks;
+    const int token = wave * kTileRowsWave + row;
+    k_from[i] = token % 16 * pages.token + (at ^ Ring::k_turn(token)) * 16;
+    v_from[i] = token % 16 * pages.token + (at ^ Ring::v_turn(token)) * 16;
+  }
+  // The block of the tile that is fetched next is looked up a tile before.
+  struct Where {
+    int32_t position, block;
   };
-  const auto lay = [&](Stage& to) {
+  const auto look_up = [&](int32_t t) {
+    // behind the last tile the last one comes again, and is not used
+    const int32_t at = tiles.at(min(t, end - 1)) * kTile + 16 * (wave / 2);
+    return Where{at, table[at >> a.block_shift]};
+  };
+  const auto fetch = [&](int32_t t, const Where& from) {
+    const PagedHalf half = paged_half(pages, kv_head, a.block_shift, from.block, from.position);
+    const int slot = (t - first) & (kRing - 1), at = wave * kTileRowsWave * Ring::kChunks;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int token = 16 * wave + i * kRows + load_row;
-      to.k[Stage::k_at(token, load_chunk)] = held_k[i];
-      to.v[Stage::v_at(token, load_chunk)] = held_v[i];
-    }
+    for (int i = 0; i < kLoads; ++i) load_shared(half.k, k_from[i], &ring.k[slot][at + i * 64]);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) load_shared(half.v, v_from[i], &ring.v[slot][at + i * 64]);
   };
-  load(it->tile);
+  const Where begin[3] = {look_up(first), look_up(first + 1), look_up(first + 2)};
+  Where ahead = look_up(first + 3);
 
   const int32_t row0 = it->row + wave * kRowsWave;
   const int32_t rows = min(max(it->rows - wave * kRowsWave, 0), kRowsWave);
@@ -739,112 +899,126 @@ __device__ __forceinline__ void paged_prompt_item(const Sight& a, const Pages& p
     const v4u x = query8<T>(args, it, row0 + n, there, 16 * s + 8 * h);
     __builtin_memcpy(&q[s], &x, 16);
   }
+#pragma unroll
+  for (int i = 0; i < 3; ++i) fetch(first + i, begin[i]);
+
   f32x16 o[kOut];
 #pragma unroll
   for (int d = 0; d < kOut; ++d) o[d] = f32x16{};
   RowSum state;
 
-  // where a lane reads V turned: token (lane % 16) / 4 of four, 4 values of 16
-  const int turn_token = lane % 16 / 4, turn_chunk = 2 * (lane / 16 % 2) + lane % 4 / 2;
-
-  const auto multiply = [&](const Stage& from, int32_t at, int tile) {
-    if (at + tile >= tiles.end) return;
-    const int32_t begin = tiles.at(at + tile) * kTile;
-    // tiles that none of the wave's rows sees
-    if ((begin > high) | ((low - (begin + kTile - 1) >= a.window) & (begin >= a.sinks))) return;
-    f32x16 x = {};
-    v8 k[kSteps];
+  // Three tiles are in work at once, so that the matrix unit has products while
+  // exponentials are made: the scores of tile t + 1, the softmax of t, the output of t - 1.
+  v8 k[kSteps], p[2];
+  uint32_t v[2][kOut][4];
+  const auto read_k = [&](int32_t t) {
+    const v4u* from = ring.k[(t - first) & (kRing - 1)];
 #pragma unroll
     for (int s = 0; s < kSteps; ++s)
-      __builtin_memcpy(&k[s], &from.k[Stage::k_at(32 * tile + n, 2 * s + h)], 16);
+      __builtin_memcpy(&k[s], &from[Ring::k_at(n, 2 * s + h)], 16);
+  };
+  // Where a lane reads V turned: token (lane % 16) / 4 of four, 4 values of 16, in the row's
+  // chunks of an even and of an odd run of 32 values; all else is added by number. V's
+  // operand: tokens 16 ks + 4 h + j and 16 ks + 8 + 4 h + j of a value.
+  uint32_t v_place[2];
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) x = Matrix<T>::mma32(k[s], q[s], x);
-    // V: tokens 16 ks + 4 h + j and 16 ks + 8 + 4 h + j of a value
-    uint32_t v[2][kOut][4];
+  for (int d = 0; d < 2; ++d)
+    v_place[d] = shared_address(ring.v[0]) + 8 * (lane % 2) +
+                 16 * Ring::v_at(4 * h + lane % 16 / 4,
+                                 4 * d + 2 * (lane / 16 % 2) + lane % 4 / 2);
+  const auto read_v = [&](int32_t t) {
+    const uint32_t slot = ((t - first) & (kRing - 1)) * sizeof ring.v[0];
+    const uint32_t place[2] = {v_place[0] + slot, v_place[1] + slot};
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
       for (int d = 0; d < kOut; ++d)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const int token = 32 * tile + 16 * ks + 8 * j + 4 * h + turn_token;
-          const s16x4 y = read_turned(
-              reinterpret_cast<const char*>(&from.v[Stage::v_at(token, 4 * d + turn_chunk)]) +
-              8 * (lane % 2));
+          const s16x4 y = read_turned(place[d % 2] + 16 * ((16 * ks + 8 * j) * Ring::kChunks +
+                                                           8 * (d / 2)));
           __builtin_memcpy(&v[ks][d][2 * j], &y, 8);
         }
+  };
+  const auto scores = [&]() {
+    f32x16 x = {};
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) x = Matrix<T>::mma32(k[s], q[s], x);
+    return x;
+  };
+  const auto outputs = [&]() {
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int d = 0; d < kOut; ++d) {
+        v8 y;
+        __builtin_memcpy(&y, v[ks][d], 16);
+        o[d] = Matrix<T>::mma32(y, p[ks], o[d]);
+      }
+  };
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) {
+    p[ks] = v8{};
+#pragma unroll
+    for (int d = 0; d < kOut; ++d)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) v[ks][d][w] = 0;
+  }
+
+  wait_and_meet<2 * 2 * kLoads>();
+  read_k(first);
+  f32x16 x = scores();
+  for (int32_t t = first; t < end; ++t) {
+    wait_and_meet<2 * kLoads>();
+    read_k(t + 1);
+    fetch(t + 3, ahead);
+    ahead = look_up(t + 4);
+    const int32_t begin = tiles.at(t) * kTile;
+    const bool whole = seen_whole(a, low, high, begin);
     float e[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) e[i] = x[i];
-    const bool whole = seen_whole(a, low, high, begin);
-    const auto some_sees = [&](int32_t j) {
-      return (j <= high) & ((low - j < a.window) | (j < a.sinks));
-    };
-    bool odd = false;
     if (!whole) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         e[i] = seen(a, position, begin + 8 * (i / 4) + 4 * h + i % 4) ? e[i] : -INFINITY;
+    }
+    outputs();
+    x = scores();
+    read_v(t);
+    // a product, two instructions and an exponential in turn
+#pragma unroll
+    for (int i = 0; i < 2 * kSteps; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x400, 1, 0);
+    }
+    softmax_part<T>(e, a.c, state, o, [](float y) { return pair_max(y); });
+    if (!whole) {
       // infinities and no numbers: a probability of 0 would make no number of them
+      uint32_t found = 0;
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
         for (int d = 0; d < kOut; ++d)
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const uint32_t bad = (not_finite<T>(v[ks][d][w] & 0xFFFFu) ? 0xFFFFu : 0u) |
-                                 (not_finite<T>(v[ks][d][w] & 0xFFFF0000u) ? 0xFFFF0000u : 0u);
-            const int32_t j = begin + 16 * ks + 8 * (w / 2) + 4 * h + 2 * (w % 2);
-            odd |= ((bad & 0xFFFFu) && some_sees(j)) || ((bad >> 16) && some_sees(j + 1));
-            v[ks][d][w] &= ~bad;
-          }
-    }
-    softmax_part<T>(e, a.c, state, o, [](float y) { return pair_max(y); });
+          for (int w = 0; w < 4; ++w) found |= not_finite<T>(v[ks][d][w]);
+      if (__any((found & kNotFinite) != 0)) {
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      const v8 p = round8<T>(e, 8 * ks);
+        for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-      for (int d = 0; d < kOut; ++d) {
-        v8 y;
-        __builtin_memcpy(&y, v[ks][d], 16);
-        o[d] = Matrix<T>::mma32(y, p, o[d]);
+          for (int d = 0; d < kOut; ++d)
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+              v[ks][d][w] &= ~whole_values(not_finite<T>(v[ks][d][w]));
+        add_odd_rows<D, T>(a, ring.v[(t - first) & (kRing - 1)], begin, low, high, position, n,
+                           h, e, o);
       }
     }
-    if (!whole && __any(odd)) {
-      // what was taken out goes to the rows that see its token
-#pragma unroll 1
-      for (int t = 0; t < kTile; ++t) {
-        const int32_t j = begin + t;
-        const bool sees = seen(a, position, j);
-        // the row's probability of token t, from the lane that has it
-        float mine = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          mine = i == 4 * (t / 8) + t % 4 ? static_cast<float>(static_cast<T>(e[i])) : mine;
-        const float weight = __shfl(mine, n + 32 * (t / 4 % 2));
-#pragma unroll
-        for (int d = 0; d < kOut; ++d)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int value = 32 * d + 8 * (i / 4) + 4 * h + i % 4;
-            const T y = reinterpret_cast<const T*>(
-                &from.v[Stage::v_at(32 * tile + t, value / 8)])[value % 8];
-            const bool bad = not_finite<T>(__builtin_bit_cast(uint16_t, y));
-            const float was = o[d][i];
-            o[d][i] = (bad & sees) ? __builtin_fmaf(weight, static_cast<float>(y), was) : was;
-          }
-      }
-    }
-  };
-
-  int turn = 0;
-  for (int32_t at = it->tile; at < tiles.end; at += 2, turn ^= 1) {
-    lay(stages[turn]);
-    load(at + 2);
-    __syncthreads();
-#pragma unroll
-    for (int tile = 0; tile < 2; ++tile) multiply(stages[turn], at, tile);
+    p[0] = round8<T>(e, 0);
+    p[1] = round8<T>(e, 8);
   }
+  outputs();
 
   const PagedCold end_args = paged_cold();
   const PagedItem ended = anew(it);
@@ -860,21 +1034,21 @@ __device__ __forceinline__ void paged_prompt_item(const Sight& a, const Pages& p
   for (int d = 0; d < kOut; ++d)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int first = 32 * d + 8 * i + 4 * h;
+      const int value = 32 * d + 8 * i + 4 * h;
       float y[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) y[j] = o[d][4 * i + j] * inv;
       if (slot >= 0) {
-        __builtin_memcpy(part + first, y, 16);
+        __builtin_memcpy(part + value, y, 16);
       } else {
-        T t[4];
+        T r[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) t[j] = static_cast<T>(y[j]);
+        for (int j = 0; j < 4; ++j) r[j] = static_cast<T>(y[j]);
         if (end_args->out.whole_words) {
-          __builtin_memcpy(__builtin_assume_aligned(to + first, 8), t, 8);
+          __builtin_memcpy(__builtin_assume_aligned(to + value, 8), r, 8);
         } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) to[first + j] = t[j];
+          for (int j = 0; j < 4; ++j) to[value + j] = r[j];
         }
       }
     }
@@ -891,12 +1065,12 @@ __device__ __forceinline__ void paged_prompt_item(const Sight& a, const Pages& p
 template <int D, typename T>
 __global__ __launch_bounds__(kPagedLanes, D == 256 ? 1 : 2) void paged_prompt_kernel(
     PagedAttendArgs args) {
-  __shared__ PagedStage<D> stages[2];
+  __shared__ PagedRing<D> ring;
   const Sight sight = args.sight;
   const Pages pages = args.pages;
   const PagedItem it = in_plan<Item>(args.plan, args.at_items) + blockIdx.x;
   if (static_cast<int32_t>(blockIdx.x) >= in_plan<Header>(args.plan, 0)->items[args.kind]) return;
-  paged_prompt_item<D, T>(sight, pages, it, stages);
+  paged_prompt_item<D, T>(sight, pages, it, ring);
 }
 
 // Rows whose tiles several items shared: their parts, scaled to the largest base of
@@ -978,16 +1152,16 @@ struct WeighArgs {
   Sight sight;
   Pages pages;
   const char* plan;
-  int64_t at_seqs, at_table;
+  int64_t at_seqs, at_table, at_place_tiles;
   Values q;
   const float* lse;
   int64_t lse_token;
   float* weights;       // [block][kv_head][token]
-  int32_t group, kv_heads;
+  Divisor group;
+  int32_t kv_heads;
 };
 
-// Places of a workgroup, and of one of its waves.
-constexpr int kWeighPlaces = kPlaceTile, kWavePlaces = kWeighPlaces / kPagedWaves;
+constexpr int kWeighPlaces = kPlaceTile;
 
 // One workgroup's work: places of one sequence under one KV head, and its queries.
 struct WeighItem {
@@ -999,80 +1173,101 @@ struct WeighItem {
   }
 };
 
-__device__ __forceinline__ bool find_places(const WeighArgs& a, WeighItem* it) {
-  const int32_t i = blockIdx.x / a.kv_heads;
+__device__ __forceinline__ bool find_places(const WeighArgs& a, int32_t index, WeighItem* it) {
+  const int32_t i = index / a.kv_heads;
   const auto* h = in_plan<Header>(a.plan, 0);
   if (i >= h->place_tiles) return false;
-  const auto* seq = in_plan<Seq>(a.plan, a.at_seqs);
-  // the last sequence that begins at or before tile i; empty sequences begin where the
-  // next one does
-  int32_t lo = 0, hi = h->num_seqs - 1;
-  while (lo < hi) {
-    const int32_t mid = (lo + hi + 1) >> 1;
-    if (seq[mid].place_tile <= i) lo = mid;
-    else hi = mid - 1;
-  }
-  const auto* s = seq + lo;
-  it->kv_head = blockIdx.x - i * a.kv_heads;
+  const auto* s = in_plan<Seq>(a.plan, a.at_seqs) +
+                  in_plan<int32_t>(a.plan, a.at_place_tiles)[i];
+  it->kv_head = index - i * a.kv_heads;
   it->first = (i - s->place_tile) * kWeighPlaces;
   it->len = s->len;
   it->base = s->len - s->fresh;
-  it->rows = s->fresh * a.group;
+  it->rows = s->fresh * static_cast<int32_t>(a.group.by);
   it->token = s->token;
   it->table = s->table;
   return it->rows > 0;
 }
 
-// Eight values of a query row from `at` on; 0 where there is none.
+// A query row's place among the values, and its log-sum-exp's.
+__device__ __forceinline__ int64_t weigh_row(const WeighArgs& a, const WeighItem& it, int32_t row,
+                                             int64_t token_stride, int64_t head_stride) {
+  const int32_t token = quotient(row, a.group);
+  return (int64_t(it.token) + token) * token_stride +
+         (int64_t(it.kv_head) * a.group.by + (row - token * static_cast<int32_t>(a.group.by))) *
+             head_stride;
+}
+
 template <typename T>
-__device__ __forceinline__ v4u weigh_query8(const WeighArgs& a, const WeighItem& it, int32_t row,
-                                            int32_t at) {
-  v4u x = {0, 0, 0, 0};
-  if (row < it.rows) {
-    const int32_t token = row / a.group;
-    const T* from = reinterpret_cast<const T*>(a.q.base) +
-                    (int64_t(it.token) + token) * a.q.token +
-                    (int64_t(it.kv_head) * a.group + (row - token * a.group)) * a.q.head + at;
-    if (a.q.whole_words) {
-      x = *(const gv4u*)from;
-    } else {
-      T t[8];
+__device__ __forceinline__ v4u read8(const T* from, bool whole_words) {
+  v4u x;
+  if (whole_words) {
+    x = *(const gv4u*)from;
+  } else {
+    T t[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) t[j] = from[j];
-      __builtin_memcpy(&x, t, 16);
-    }
+    for (int j = 0; j < 8; ++j) t[j] = from[j];
+    __builtin_memcpy(&x, t, 16);
   }
   return x;
 }
 
-// log2(e) times a row's log-sum-exp; infinity where there is no row: its share is 0.
-__device__ __forceinline__ float row_log(const WeighArgs& a, const WeighItem& it, int32_t row) {
-  if (row >= it.rows) return INFINITY;
-  const int32_t token = row / a.group;
-  return 1.4426950408889634f * a.lse[(int64_t(it.token) + token) * a.lse_token +
-                                     int64_t(it.kv_head) * a.group + (row - token * a.group)];
+// Eight values of a query row from `at` on. (Behind the last row, its own again: what comes
+// of them is dropped.)
+template <typename T>
+__device__ __forceinline__ v4u weigh_query8(const WeighArgs& a, const WeighItem& it, int32_t row,
+                                            int32_t at) {
+  const T* from = reinterpret_cast<const T*>(a.q.base) +
+                  weigh_row(a, it, min(row, it.rows - 1), a.q.token, a.q.head) + at;
+  return read8(from, a.q.whole_words);
 }
 
-__device__ __forceinline__ void add_weight(const WeighArgs& a, const WeighItem& it,
-                                           const AEGKV_CONSTANT int32_t* table, int32_t place,
-                                           float w) {
-  if (!it.reaches(a.sight, place, 1)) return;
-  const int32_t shift = a.sight.block_shift;
-  const int64_t block = table[place >> shift];
-  float* to = a.weights + (((block * a.kv_heads + it.kv_head) << shift) +
-                           (place & ((1 << shift) - 1)));
-  *to = (place < it.base ? *to : 0.f) + w;
+// log2(e) times a row's log-sum-exp; infinity where there is no row: its share is 0.
+__device__ __forceinline__ float row_log(const WeighArgs& a, const WeighItem& it, int32_t row) {
+  const float x = a.lse[weigh_row(a, it, min(row, it.rows - 1), a.lse_token, 1)];
+  return row < it.rows ? 1.4426950408889634f * x : INFINITY;
 }
+
+// A lane's place and what it has gathered before; asked for early, since what follows from it
+// depends on two loads.
+struct OwnPlace {
+  float* to;
+  float before;
+  bool seen;
+  __device__ __forceinline__ OwnPlace(const WeighArgs& a, const WeighItem& it, int32_t place) {
+    const int32_t shift = a.sight.block_shift;
+    seen = it.reaches(a.sight, place, 1);
+    place = min(place, it.len - 1);
+    const int64_t block = reinterpret_cast<const int32_t*>(a.plan + a.at_table)[it.table +
+                                                                               (place >> shift)];
+    to = a.weights + (((block * a.kv_heads + it.kv_head) << shift) +
+                      (place & ((1 << shift) - 1)));
+    before = place < it.base ? *to : 0.f;
+  }
+  __device__ __forceinline__ void add(float w) const {
+    if (seen) *to = before + w;
+  }
+};
 
 // w[place] += sum over the rows that see it of exp2(c s - log2(e) lse). A place
 // belongs to one lane at the end: no atomics, and the sum's order is fixed. Up
 // to 64 rows of a sequence: S = Q K^T by 16 x 16 x 32, a wave's 64 places in registers.
+// Bound by HBM; what takes part is asked for at once, without branches: with four
+// log-sum-exps and four places a lane, looked up one after another, 64 decodes took 150 us.
+// A wave holds 8 KiB of K: with 64 places at any width, 128-wide heads took 124.
+constexpr int weigh_parts(int head_dim) { return head_dim == 64 ? 4 : head_dim == 128 ? 2 : 1; }
+
 template <int D, typename T>
-__global__ __launch_bounds__(kPagedLanes, D <= 128 ? 3 : 2) void paged_weigh_kernel(WeighArgs a) {
+__global__ __launch_bounds__(kPagedLanes, 4) void paged_weigh_kernel(WeighArgs a) {
   typedef typename Matrix<T>::v8 v8;
-  constexpr int kSteps = D / 32, kParts = kWavePlaces / 16;
+  constexpr int kSteps = D / 32, kParts = weigh_parts(D), kWavePlaces = 16 * kParts;
+  constexpr int kShare = kWeighPlaces / (kPagedWaves * kWavePlaces);
   WeighItem it;
-  if (!find_places(a, &it) || it.rows > kMostMore) return;
+  const int32_t tile = blockIdx.x / (kShare * a.kv_heads);
+  const int32_t rest = blockIdx.x - tile * kShare * a.kv_heads, share = rest / a.kv_heads;
+  if (!find_places(a, tile * a.kv_heads + rest - share * a.kv_heads, &it) || it.rows > kMostMore)
+    return;
+  it.first += share * kPagedWaves * kWavePlaces;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int lane = threadIdx.x % 64, m = lane % 16, g = lane / 16;
   const int32_t begin = it.first + wave * kWavePlaces;
@@ -1087,9 +1282,12 @@ __global__ __launch_bounds__(kPagedLanes, D <= 128 ? 3 : 2) void paged_weigh_ker
     const PagedHalf h = paged_half(a.pages, it.kv_head, shift, table[at >> shift], at);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s)
-      load_bytes<16, true>(reinterpret_cast<uint32_t*>(&k[p][s]), h.k,
-                           m * a.pages.token + g * 16 + s * 64);
+      load_bytes<16, false>(reinterpret_cast<uint32_t*>(&k[p][s]), h.k,
+                            m * a.pages.token + g * 16 + s * 64);
   }
+  const OwnPlace own(a, it, begin + lane % kWavePlaces);
+  const bool whole = seen_whole(a.sight, it.base, last, begin) &&
+                     seen_whole(a.sight, it.base, last, begin + kWavePlaces - kTile);
   float w[kParts] = {};
 #pragma unroll 1
   for (int32_t row = 0; row < it.rows; row += 16) {
@@ -1099,12 +1297,14 @@ __global__ __launch_bounds__(kPagedLanes, D <= 128 ? 3 : 2) void paged_weigh_ker
       const v4u x = weigh_query8<T>(a, it, row + m, 32 * s + 8 * g);
       __builtin_memcpy(&q[s], &x, 16);
     }
+    const float own_log = row_log(a, it, row + m);
+    const int32_t own_position = it.base + quotient(min(row + m, it.rows - 1), a.group);
     float log[4];
     int32_t position[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      log[i] = row_log(a, it, row + 4 * g + i);
-      position[i] = it.base + min(row + 4 * g + i, it.rows - 1) / a.group;
+      log[i] = __shfl(own_log, 4 * g + i);
+      position[i] = __shfl(own_position, 4 * g + i);
     }
 #pragma unroll
     for (int p = 0; p < kParts; ++p) {
@@ -1113,45 +1313,59 @@ __global__ __launch_bounds__(kPagedLanes, D <= 128 ? 3 : 2) void paged_weigh_ker
       for (int s = 0; s < kSteps; ++s) x = Matrix<T>::mma(q[s], k[p][s], x);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
+        const bool sees = (log[i] != INFINITY) &
+                          (whole | seen(a.sight, position[i], begin + 16 * p + m));
         const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], a.sight.c, -log[i]));
-        const bool sees = (row + 4 * g + i < it.rows) &
-                          seen(a.sight, position[i], begin + 16 * p + m);
         w[p] += sees ? e : 0.f;
       }
     }
   }
+  float sum = 0.f;
 #pragma unroll
   for (int p = 0; p < kParts; ++p) {
     w[p] += __shfl_xor(w[p], 16);
     w[p] += __shfl_xor(w[p], 32);
-    if (g == p) add_weight(a, it, table, begin + 16 * p + m, w[p]);
+    sum = g == p ? w[p] : sum;
   }
+  if (g < kParts) own.add(sum);
 }
 
-// More rows: S by 32 x 32 x 16, the rows' queries in shared memory for all four
-// waves, 32 rows a stage, two stages.
+// More rows: S by 32 x 32 x 16. Two workgroups share a tile of places, 128 each; of a
+// workgroup's waves two take the one and two the other 64 places, each every other 32 rows: a
+// stage of 64 rows' queries in shared memory serves all, two stages. (One workgroup
+// with 256 places, its waves on the same rows, left a third of the chip without work.)
+constexpr int kRowsPlaces = kWeighPlaces / 2, kWavePlaces = kRowsPlaces / 2, kStageRows = 64;
+
 template <int D>
 struct WeighStage {
-  v4u q[32 * (D / 8)];
-  float log[32];
-  int32_t position[32];
+  v4u q[kStageRows * (D / 8)];
+  float log[kStageRows];
+  int32_t position[kStageRows];
 };
 
 template <int D, typename T>
 __global__ __launch_bounds__(kPagedLanes, D <= 128 ? 2 : 1) void paged_weigh_rows_kernel(
     WeighArgs a) {
   typedef typename Matrix<T>::v8 v8;
-  typedef PagedStage<D> Place;
+  typedef PagedRing<D> Places;
   constexpr int kSteps = D / 16, kParts = kWavePlaces / 32, kChunks = D / 8;
   __shared__ WeighStage<D> stages[2];
+  __shared__ float side[2][kParts][32];
   WeighItem it;
-  if (!find_places(a, &it) || it.rows <= kMostMore) return;
-  if (!it.reaches(a.sight, it.first, kWeighPlaces)) return;
+  const int32_t pair = blockIdx.x / (2 * a.kv_heads);
+  const int32_t rest = blockIdx.x - pair * 2 * a.kv_heads;
+  const int32_t half = rest >= a.kv_heads;
+  if (!find_places(a, pair * a.kv_heads + rest - half * a.kv_heads, &it) || it.rows <= kMostMore)
+    return;
+  it.first += half * kRowsPlaces;
+  if (!it.reaches(a.sight, it.first, kRowsPlaces)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int lane = threadIdx.x % 64, n = lane % 32, h = lane / 32;
-  const int32_t begin = it.first + wave * kWavePlaces;
+  const int own_places = wave % 2, own_rows = wave / 2;
+  const int32_t begin = it.first + own_places * kWavePlaces;
   const auto* table = in_plan<int32_t>(a.plan, a.at_table) + it.table;
   const int32_t last = it.len - 1, shift = a.sight.block_shift;
+  const int32_t group = static_cast<int32_t>(a.group.by);
   v8 k[kParts][kSteps];
 #pragma unroll
   for (int p = 0; p < kParts; ++p) {
@@ -1163,63 +1377,104 @@ __global__ __launch_bounds__(kPagedLanes, D <= 128 ? 2 : 1) void paged_weigh_row
   }
   // rows that see a place of the workgroup's: from the first place on, and up to where the
   // window has left the last one
-  const int32_t first_row = max(0, it.first - it.base) * a.group & ~31;
+  const int32_t first_row = (max(0, it.first - it.base) * group) & ~31;
   int32_t end_row = it.rows;
   if (it.first >= a.sight.sinks && a.sight.window != INT32_MAX) {
-    const int64_t end = (int64_t(it.first) + kWeighPlaces - 1 + a.sight.window - it.base) *
-                        a.group;
+    const int64_t end = (int64_t(it.first) + kRowsPlaces - 1 + a.sight.window - it.base) * group;
     end_row = static_cast<int32_t>(max<int64_t>(0, min<int64_t>(end_row, end)));
   }
-  constexpr int kLoads = 32 * kChunks / kPagedLanes;
+  // The rows that a lane asks for, of which the next stage's are kStageRows further on: their
+  // places go along by sums.
+  constexpr int kLoads = kStageRows * kChunks / kPagedLanes;
+  const int32_t step_tokens = quotient(kStageRows, a.group);
+  const int32_t step_heads = kStageRows - step_tokens * group;
+  struct Row {
+    int64_t at, sum;          // among the queries, among the log-sum-exps
+    int32_t row, head, token;
+  };
+  const auto row_of = [&](int32_t row) {
+    Row r;
+    r.row = row;
+    row = min(row, it.rows - 1);
+    r.token = quotient(row, a.group);
+    r.head = row - r.token * group;
+    r.at = weigh_row(a, it, row, a.q.token, a.q.head);
+    r.sum = weigh_row(a, it, row, a.lse_token, 1);
+    return r;
+  };
+  const int64_t q_step = step_tokens * a.q.token + step_heads * a.q.head;
+  const int64_t q_wrap = a.q.token - group * a.q.head;
+  const int64_t lse_step = step_tokens * a.lse_token + step_heads;
+  const int64_t lse_wrap = a.lse_token - group;
+  const auto advance = [&](Row& r) {
+    r.row += kStageRows;
+    if (r.row >= it.rows) return;     // the last row that there was again, and not used
+    const bool wraps = r.head + step_heads >= group;
+    r.head += step_heads - (wraps ? group : 0);
+    r.token += step_tokens + wraps;
+    r.at += q_step + (wraps ? q_wrap : 0);
+    r.sum += lse_step + (wraps ? lse_wrap : 0);
+  };
+  Row rows[kLoads], own = row_of(first_row + static_cast<int32_t>(threadIdx.x % kStageRows));
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i)
+    rows[i] = row_of(first_row + (i * kPagedLanes + static_cast<int32_t>(threadIdx.x)) / kChunks);
+  const int32_t own_chunk = static_cast<int32_t>(threadIdx.x) % kChunks;
   v4u held[kLoads];
   float held_log = 0.f;
-  const auto load = [&](int32_t row) {
+  const auto load = [&]() {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int at = i * kPagedLanes + threadIdx.x;
-      held[i] = weigh_query8<T>(a, it, row + at / kChunks, at % kChunks * 8);
-    }
-    if (threadIdx.x < 32) held_log = row_log(a, it, row + threadIdx.x);
+    for (int i = 0; i < kLoads; ++i)
+      held[i] = read8(reinterpret_cast<const T*>(a.q.base) + rows[i].at + own_chunk * 8,
+                      a.q.whole_words);
+    held_log = a.lse[own.sum];
   };
-  load(first_row);
+  load();
   float w[kParts] = {};
   int turn = 0;
-  for (int32_t row = first_row; row < end_row; row += 32, turn ^= 1) {
+  for (int32_t row = first_row; row < end_row; row += kStageRows, turn ^= 1) {
     WeighStage<D>& stage = stages[turn];
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int at = i * kPagedLanes + threadIdx.x;
-      stage.q[Place::k_at(at / kChunks, at % kChunks)] = held[i];
+      stage.q[Places::k_at(at / kChunks, at % kChunks)] = held[i];
     }
-    if (threadIdx.x < 32) {
-      stage.log[threadIdx.x] = held_log;
-      stage.position[threadIdx.x] =
-          it.base + min(row + static_cast<int32_t>(threadIdx.x), it.rows - 1) / a.group;
+    if (threadIdx.x < kStageRows) {
+      stage.log[threadIdx.x] = own.row < it.rows ? 1.4426950408889634f * held_log : INFINITY;
+      stage.position[threadIdx.x] = it.base + own.token;
     }
-    load(row + 32);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) advance(rows[i]);
+    advance(own);
+    load();
     __syncthreads();
-    const int32_t low = stage.position[0], high = stage.position[31];
+    const int mine = 32 * own_rows;     // of the stage's rows
+    const int32_t low = stage.position[mine], high = stage.position[mine + 31];
     v8 q[kSteps];
 #pragma unroll
     for (int s = 0; s < kSteps; ++s)
-      __builtin_memcpy(&q[s], &stage.q[Place::k_at(n, 2 * s + h)], 16);
+      __builtin_memcpy(&q[s], &stage.q[Places::k_at(mine + n, 2 * s + h)], 16);
     float log[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) log[i] = stage.log[8 * (i / 4) + 4 * h + i % 4];
+    for (int i = 0; i < 16; ++i) log[i] = stage.log[mine + 8 * (i / 4) + 4 * h + i % 4];
+    f32x16 x[kParts];
+#pragma unroll
+    for (int p = 0; p < kParts; ++p) x[p] = f32x16{};
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+      for (int p = 0; p < kParts; ++p) x[p] = Matrix<T>::mma32(q[s], k[p][s], x[p]);
 #pragma unroll
     for (int p = 0; p < kParts; ++p) {
       const int32_t place = begin + 32 * p;
-      f32x16 x = {};
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) x = Matrix<T>::mma32(q[s], k[p][s], x);
       float e[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], a.sight.c, -log[i]));
-      if (!seen_whole(a.sight, low, high, place) || row + 32 > it.rows) {
+        e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[p][i], a.sight.c, -log[i]));
+      if (!seen_whole(a.sight, low, high, place) || row + mine + 32 > it.rows) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int r = 8 * (i / 4) + 4 * h + i % 4;
+          const int r = mine + 8 * (i / 4) + 4 * h + i % 4;
           const bool sees = (row + r < it.rows) & seen(a.sight, stage.position[r], place + n);
           e[i] = sees ? e[i] : 0.f;
         }
@@ -1231,8 +1486,11 @@ __global__ __launch_bounds__(kPagedLanes, D <= 128 ? 2 : 1) void paged_weigh_row
 #pragma unroll
   for (int p = 0; p < kParts; ++p) {
     w[p] += __shfl_xor(w[p], 32);
-    if (h == p) add_weight(a, it, table, begin + 32 * p + n, w[p]);
+    if (own_rows == 1 && h == p) side[own_places][p][n] = w[p];
   }
+  __syncthreads();
+  if (own_rows == 0)
+    OwnPlace(a, it, begin + lane).add((h ? w[1] : w[0]) + side[own_places][h][n]);
 }
 
 // ---------------------------------------------------------------- eviction --
@@ -1282,10 +1540,15 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 
 // Which places stay: the first `sinks`, the last `recent`, and of those between the
 // ones of the largest weight, the earlier one of equals. The border weight is found
-// eight bits at a time from counts; then every wave goes through a run of its own, twice:
-// once to count, once to write its places where they belong.
+// eleven bits at a time from counts; then every wave goes through a run of places of its
+// own, twice: once to count, once to write its places where they belong. STEPS: 64
+// places each that a wave holds in registers from the first look on; 0: any number, read
+// anew each time.
+constexpr int kBins = 2048, kDigit = 11;
+
+template <int STEPS>
 __global__ __launch_bounds__(kSelectLanes) void paged_select_kernel(EvictArgs a) {
-  __shared__ uint32_t count[256], border, wanted;
+  __shared__ uint32_t count[kBins], border, wanted;
   __shared__ uint32_t more[kSelectWaves], same[kSelectWaves];
   const EvictSeq e = evict_seq(a, blockIdx.x);
   int32_t* kept = a.kept + e.kept;
@@ -1301,57 +1564,82 @@ __global__ __launch_bounds__(kSelectLanes) void paged_select_kernel(EvictArgs a)
     kept[keep - recent + i] = e.len - recent + i;
   const int32_t chosen = keep - sinks - recent, places = e.len - sinks - recent;
   if (chosen == 0) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+  const int32_t run = ((places + kSelectWaves - 1) / kSelectWaves + 63) & ~63;
+  const int32_t begin =
+      static_cast<int32_t>(min(int64_t(wave) * run, int64_t(places)));
+  const int32_t end = static_cast<int32_t>(min(int64_t(begin) + run, int64_t(places)));
   const auto key = [&](int32_t i) {
-    return weight_key(a.weights[weight_at(a, e.table, e.kv_head, sinks + i)]);
+    return weight_key(a.weights[weight_at(a, e.table, e.kv_head, sinks + min(i, places - 1))]);
+  };
+  // f(key, whether there is one, first place of the 64) for the wave's run
+  uint32_t held[STEPS ? STEPS : 1];
+  if constexpr (STEPS != 0) {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) held[s] = key(begin + 64 * s + lane);
+  }
+  const auto each = [&](const auto& f) {
+    if constexpr (STEPS != 0) {
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s)
+        if (begin + 64 * s < end) f(held[s], begin + 64 * s + lane < end, begin + 64 * s);
+    } else {
+      constexpr int kAtOnce = 8;
+      for (int32_t at = begin; at < end; at += 64 * kAtOnce) {
+        uint32_t x[kAtOnce];
+#pragma unroll
+        for (int s = 0; s < kAtOnce; ++s) x[s] = key(at + 64 * s + lane);
+#pragma unroll
+        for (int s = 0; s < kAtOnce; ++s)
+          if (at + 64 * s < end) f(x[s], at + 64 * s + lane < end, at + 64 * s);
+      }
+    }
   };
   uint32_t prefix = 0, need = chosen;     // of the keys that share the bits found so far
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (threadIdx.x < 256) count[threadIdx.x] = 0;
+#pragma unroll 1
+  for (int shift = 32 - kDigit; ; shift = max(0, shift - kDigit)) {
+    // the last digit, of the 32 bits' rest, is ten bits wide
+    const int known = shift == 0 ? 10 : shift + kDigit;
+    const bool first = shift == 32 - kDigit;
+    for (int i = threadIdx.x; i < kBins; i += kSelectLanes) count[i] = 0;
     __syncthreads();
-    for (int32_t i = threadIdx.x; i < places; i += kSelectLanes) {
-      const uint32_t x = key(i);
-      if (shift == 24 || x >> (shift + 8) == prefix)
-        atomicAdd(&count[x >> shift & 255], 1u);
-    }
+    each([&](uint32_t x, bool there, int32_t) {
+      if (there && (first || x >> known == prefix))
+        atomicAdd(&count[shift == 0 ? x & 1023u : x >> shift & (kBins - 1)], 1u);
+    });
     __syncthreads();
-    if (threadIdx.x < 64) {
-      // lane l holds the four bins from 252 - 4 l on: bins above it come before it
-      const int top = 252 - 4 * static_cast<int>(threadIdx.x);
-      uint32_t mine[4], all = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) all += mine[i] = count[top + i];
+    if (wave == 0) {
+      // lane l holds the 32 bins from 2016 - 32 l on: bins above it come before it
+      const int low = kBins - 32 * (lane + 1);
+      uint32_t all = 0;
+#pragma unroll 8
+      for (int i = 0; i < 32; ++i) all += count[low + (i + lane) % 32];
       uint32_t before = all;
 #pragma unroll
       for (int far = 1; far < 64; far *= 2) {
         const uint32_t x = __shfl_up(before, far);
-        before += static_cast<int>(threadIdx.x) >= far ? x : 0;
+        before += lane >= far ? x : 0;
       }
       before -= all;
-#pragma unroll
-      for (int i = 3; i >= 0; --i) {
-        if (before < need && before + mine[i] >= need) {
-          border = prefix << 8 | static_cast<uint32_t>(top + i);
-          wanted = need - before;
-        }
-        before += mine[i];
+      if (before < need && before + all >= need) {
+        int bin = low + 31;
+        while (before + count[bin] < need) before += count[bin--];
+        border = first ? static_cast<uint32_t>(bin)
+                       : prefix << (shift == 0 ? 10 : kDigit) | static_cast<uint32_t>(bin);
+        wanted = need - before;
       }
     }
     __syncthreads();
     prefix = border;
     need = wanted;
+    if (shift == 0) break;
   }
   // now `prefix` is the border weight, of which the first `need` stay
-  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-  const int32_t run = ((places + kSelectWaves - 1) / kSelectWaves + 63) & ~63;
-  const int32_t begin = min(int64_t(wave) * run, int64_t(places));
-  const int32_t end = min(int64_t(begin) + run, int64_t(places));
   uint32_t above = 0, equal = 0;
-  for (int32_t i = begin; i < end; i += 64) {
-    const uint32_t x = i + lane < end ? key(i + lane) : 0;
-    const bool there = i + lane < end;
+  each([&](uint32_t x, bool there, int32_t) {
     above += __popcll(__ballot(there && x > prefix));
     equal += __popcll(__ballot(there && x == prefix));
-  }
+  });
   if (lane == 0) {
     more[wave] = above;
     same[wave] = equal;
@@ -1364,18 +1652,16 @@ __global__ __launch_bounds__(kSelectLanes) void paged_select_kernel(EvictArgs a)
   }
   to += sinks + min(equals, need);
   const uint64_t below = (uint64_t(1) << lane) - 1;
-  for (int32_t i = begin; i < end; i += 64) {
-    const bool there = i + lane < end;
-    const uint32_t x = there ? key(i + lane) : 0;
+  each([&](uint32_t x, bool there, int32_t at) {
     const bool is_equal = there && x == prefix;
     const uint64_t same_here = __ballot(is_equal);
     const bool stays = (there && x > prefix) ||
                        (is_equal && equals + __popcll(same_here & below) < need);
     const uint64_t all = __ballot(stays);
-    if (stays) kept[to + __popcll(all & below)] = sinks + i + lane;
+    if (stays) kept[to + __popcll(all & below)] = sinks + at + lane;
     to += __popcll(all);
     equals += __popcll(same_here);
-  }
+  });
 }
 
 constexpr int kMoveLanes = 256, kMoveAtOnce = 8;
