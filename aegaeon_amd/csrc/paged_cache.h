@@ -39,74 +39,89 @@ __device__ __forceinline__ int32_t quotient(int32_t x, Divisor d) {
 
 // ---------------------------------------------------------- rotate, write --
 
-// Where the values of a kind of heads come from and go to.
-struct HeadRows {
+// A kind of heads: q, k or v. Where a plan's k and v go is a page; `to` is where else.
+struct HeadKind {
   Values from, to;
-  int32_t heads;
+  const char* pages;          // null: `to`
+  int64_t block;              // bytes from one of its blocks to the next
+  int32_t heads, turned;      // turned: rotated
+  // A workgroup takes `each` heads of up to `chunk` tokens; `groups` of them take all heads,
+  // `parts` a span of the plan's. `begin`: the first workgroup of this kind.
+  int32_t each, chunk, groups, parts;
+  int64_t begin;
 };
 
 struct PlaceArgs {
   const char* plan;           // null: tokens are rows, one after another
   int64_t at_new_spans;
   int64_t tokens;             // without a plan
-  int32_t chunk, parts;       // tokens of a workgroup; workgroups that a plan's span is cut into
   const double* turns;        // a position's turns, for each pair
   const void* positions;      // null: the plan's
   int32_t position_bytes;
   int32_t pairs, interleaved;
   float amplitude;
   int32_t head_dim;
-  HeadRows q, k;              // rotated
-  Values v;                   // written as they are
-  Pages pages;                // where k and v go (k.to: without a plan)
-  int32_t kv_heads, block_shift;
-  int32_t heads, heads_each, head_groups;   // of all kinds; of a workgroup; workgroups a span
-  Divisor each, rest;         // heads_each; the last workgroup's of a span
+  HeadKind kinds[3];          // q, k, v
+  int32_t page_token, page_head;    // bytes inside a page
   Divisor units, by_pairs;    // items of a head; pairs
 };
 
 constexpr int kPlaceLanes = 256;
-constexpr int kPlaceTokens = 4;     // of a workgroup
-constexpr int kMostAngles = 2048;   // of a workgroup: its tokens of up to 512 pairs
+constexpr int kMostAngles = 2048;   // of a workgroup: 16 tokens of 128 pairs, fewer of more
 
-// N values as float32 and back, N = 1, 4 or 8.
+typedef const AEGKV_CONSTANT char* ArgBytes;
+
+// N values (1, 4 or 8) of 16 or 32 bits as they lie in memory, up to 16 bytes.
 template <int N, typename T>
-__device__ __forceinline__ void take(const T* p, bool whole_words, float* x) {
-  if constexpr (N == 8) {
-    load8(p, whole_words, x);
-  } else {
-    T t[N];
-    if (N > 1 && whole_words) {
-      typedef unsigned int words __attribute__((ext_vector_type(N * sizeof(T) / 4 ? N * sizeof(T) / 4 : 1)));
-      const words w = __builtin_nontemporal_load(reinterpret_cast<const words*>(p));
-      __builtin_memcpy(t, &w, sizeof t);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) t[i] = p[i];
+struct Raw {
+  static constexpr int kWords = N * sizeof(T) / 4;    // 0: one value of 16 bits
+  uint32_t w[kWords ? kWords : 1];
+
+  __device__ __forceinline__ void load(const void* from, bool whole_words, bool whole_lines) {
+    if constexpr (kWords > 1) {
+      typedef unsigned int words __attribute__((ext_vector_type(kWords)));
+      if (whole_words) {
+        const auto* p = reinterpret_cast<const words*>(from);
+        const words x = whole_lines ? __builtin_nontemporal_load(p) : *p;
+        __builtin_memcpy(w, &x, sizeof w);
+        return;
+      }
     }
+    T t[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] = static_cast<const T*>(from)[i];
+    __builtin_memcpy(w, t, sizeof t);
+  }
+  __device__ __forceinline__ void store(void* to, bool whole_words, bool whole_lines) const {
+    if constexpr (kWords > 1) {
+      typedef unsigned int words __attribute__((ext_vector_type(kWords)));
+      if (whole_words) {
+        words x;
+        __builtin_memcpy(&x, w, sizeof w);
+        auto* p = reinterpret_cast<words*>(to);
+        if (whole_lines) __builtin_nontemporal_store(x, p);
+        else *p = x;
+        return;
+      }
+    }
+    T t[N];
+    __builtin_memcpy(t, w, sizeof t);
+#pragma unroll
+    for (int i = 0; i < N; ++i) static_cast<T*>(to)[i] = t[i];
+  }
+  __device__ __forceinline__ void widen(float* x) const {
+    T t[N];
+    __builtin_memcpy(t, w, sizeof t);
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = static_cast<float>(t[i]);
   }
-}
-template <int N, typename T>
-__device__ __forceinline__ void give(T* p, bool whole_words, const float* x) {
-  if constexpr (N == 8) {
-    store8(p, whole_words, x);
-  } else {
+  __device__ __forceinline__ void round(const float* x) {
     T t[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) t[i] = static_cast<T>(x[i]);
-    if (N > 1 && whole_words) {
-      typedef unsigned int words __attribute__((ext_vector_type(N * sizeof(T) / 4 ? N * sizeof(T) / 4 : 1)));
-      words w;
-      __builtin_memcpy(&w, t, sizeof t);
-      __builtin_nontemporal_store(w, reinterpret_cast<words*>(p));
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) p[i] = t[i];
-    }
+    __builtin_memcpy(w, t, sizeof t);
   }
-}
+};
 
 __device__ __forceinline__ void turn_pair(float& a, float& b, float c, float s) {
   const float x = a * c - b * s;
@@ -117,9 +132,10 @@ __device__ __forceinline__ void turn_pair(float& a, float& b, float c, float s) 
 // (a, b) -> (a c - b s, b c + a s) for each pair, c and s the cosine and sine of
 // position * turns: the angle in 64 bits, of which the whole turns are dropped before
 // it is rounded (positions of millions keep their angle), values in 32, one
-// rounding at the end. A workgroup takes up to 4 tokens of some heads: the angles,
+// rounding at the end. A workgroup takes a few tokens of some heads of a kind: the angles,
 // 150 instructions each, are made once for all of them, while the first values are on
-// their way.
+// their way. Bound by HBM, then by its instructions: 12,300 tokens of 3 x 40 heads,
+// k and v in float32, are written in 171 us (6.3 TB/s).
 // G: type of k and v; T: of q, of what is written and of what comes of q. A lane takes
 // two runs of N values of a head at once, half of the rotated part (or of the others) apart:
 // both sides of N pairs, or neighbouring pairs in each run where they are interleaved, and
@@ -128,84 +144,123 @@ __device__ __forceinline__ void turn_pair(float& a, float& b, float c, float s) 
 template <int N, typename G, typename T>
 __global__ __launch_bounds__(kPlaceLanes) void place_rows_kernel(PlaceArgs a) {
   __shared__ float cosine[kMostAngles], sine[kMostAngles];
-  const int32_t at_span = blockIdx.x / a.head_groups;
-  const int32_t first_head = (blockIdx.x - at_span * a.head_groups) * a.heads_each;
-  const int32_t heads = min(a.heads_each, a.heads - first_head);
-  const int32_t span = at_span / a.parts, part = (at_span - span * a.parts) * a.chunk;
+  const int kind = blockIdx.x < a.kinds[1].begin ? 0 : blockIdx.x < a.kinds[2].begin ? 1 : 2;
+  // read where they are: one of three, by number, would be copied to memory of the lanes'
+  const auto* own = reinterpret_cast<const AEGKV_CONSTANT PlaceArgs*>(
+                        (ArgBytes)__builtin_amdgcn_kernarg_segment_ptr())->kinds + kind;
+  const int32_t index = static_cast<int32_t>(blockIdx.x - own->begin);
+  const int32_t run = index / own->groups, first_head = (index - run * own->groups) * own->each;
+  const int32_t chunk = own->chunk, heads = min(own->each, own->heads - first_head);
+  const bool query = kind == 0, turned = own->turned;
+  const int32_t span = run / own->parts, part = (run - span * own->parts) * chunk;
   int64_t token;
   int32_t count, position = 0, block = 0, inside = 0;
   if (a.plan) {
     if (span >= in_plan<Header>(a.plan, 0)->new_spans) return;
     const auto* s = in_plan<NewSpan>(a.plan, a.at_new_spans) + span;
     token = int64_t(s->token) + part;
-    count = min(a.chunk, s->count - part);
+    count = min(chunk, s->count - part);
     position = s->position + part;
     block = s->block;
     inside = s->inside + part;
     if (count <= 0) return;
   } else {
-    token = int64_t(span) * a.chunk;
-    count = static_cast<int32_t>(min<int64_t>(a.chunk, a.tokens - token));
+    token = int64_t(span) * chunk;
+    count = static_cast<int32_t>(min<int64_t>(chunk, a.tokens - token));
   }
-  const int32_t turned = a.pairs / N, rotated = a.q.heads + a.k.heads;
-  const int32_t items = count * heads * static_cast<int32_t>(a.units.by);
-  const Divisor by_heads = first_head + a.heads_each <= a.heads ? a.each : a.rest;
-  char* const k_page = const_cast<char*>(a.pages.k) + (a.plan ? block * a.pages.k_block : 0);
-  char* const v_page = const_cast<char*>(a.pages.v) + (a.plan ? block * a.pages.v_block : 0);
+  const int32_t units = static_cast<int32_t>(a.units.by), items = count * heads * units;
+  const bool words = own->from.whole_words;
+  // Whole lines go past the caches. Where a head's runs are halves of lines, 16,000 tokens
+  // of 32 heads took 68 us that way, 50 through them.
+  const int64_t size = query ? sizeof(T) : sizeof(G);
+  const int32_t rest = turned ? a.pairs : 0;      // the part behind the rotated one
+  const auto in_lines = [&](int64_t each) {
+    return rest * each % 128 == 0 && (a.head_dim / 2 - rest) * each % 128 == 0;
+  };
+  const bool lines = in_lines(size), to_lines = in_lines(sizeof(T));
 
-  // Item i: of token t, N values from `at` and N from `next`. (One behind the last is the
-  // last one again, and not given.)
+  // From and to, of the first token and head; strides in bytes.
+  const char* const from = own->from.base + (token * own->from.token +
+                                             first_head * own->from.head) * size;
+  const int64_t from_token = own->from.token * size, from_head = own->from.head * size;
+  const bool paged = own->pages != nullptr, to_words = paged || own->to.whole_words;
+  const int64_t to_token = paged ? a.page_token : own->to.token * int64_t(sizeof(T));
+  const int64_t to_head = paged ? a.page_head : own->to.head * int64_t(sizeof(T));
+  char* const to = (paged ? const_cast<char*>(own->pages) + block * own->block
+                          : own->to.base) +
+                   (paged ? inside : token) * to_token + first_head * to_head;
+  // distances inside a workgroup are mostly 32-bit
+  const bool near = max(max(from_token, to_token) * count, max(from_head, to_head) * heads) <
+                    (int64_t(1) << 30);
+  const auto distance = [&](int32_t t, int64_t token_bytes, int32_t head, int64_t head_bytes) {
+    return near ? int64_t(static_cast<uint32_t>(t) * static_cast<uint32_t>(token_bytes) +
+                          static_cast<uint32_t>(head) * static_cast<uint32_t>(head_bytes))
+                : t * token_bytes + head * head_bytes;
+  };
+
+  // A lane's items are kPlaceLanes apart; their places go along by sums. Of a head, N values
+  // from `at` and N from `next`.
   struct Item {
-    int32_t t, head, unit, at, next;
-    bool turn;
+    int32_t t, head, unit;
   };
-  const auto find = [&](int32_t i) {
-    Item m;
-    i = min(i, items - 1);
-    const int32_t row = quotient(i, a.units);
-    m.unit = i - row * static_cast<int32_t>(a.units.by);
-    m.t = quotient(row, by_heads);
-    m.head = first_head + row - m.t * heads;
-    m.turn = m.unit < turned && m.head < rotated;
-    const bool whole = m.head >= rotated;           // a head of v
-    const int32_t begin = whole || m.turn ? 0 : 2 * a.pairs;
-    m.at = begin + N * (m.unit - (whole || m.turn ? 0 : turned));
-    if (N == 1 && m.turn && a.interleaved) {
-      m.at = 2 * m.unit;
-      m.next = m.at + 1;
-      return m;
+  const int32_t step_rows = quotient(kPlaceLanes, a.units);
+  const int32_t step_units = kPlaceLanes - step_rows * units;
+  const int32_t step_t = step_rows / heads, step_heads = step_rows - step_t * heads;
+  const auto advance = [&](Item& m) {
+    m.unit += step_units;
+    const bool row = m.unit >= units;
+    m.unit -= row ? units : 0;
+    m.head += step_heads + row;
+    const bool wraps = m.head >= heads;
+    m.head -= wraps ? heads : 0;
+    m.t += step_t + wraps;
+  };
+  const int32_t turned_units = turned ? a.pairs / N : 0;
+  const auto places = [&](const Item& m, int32_t* at, int32_t* next) {
+    const bool turn = m.unit < turned_units;
+    if (N == 1 && turn && a.interleaved) {
+      *at = 2 * m.unit;
+      *next = *at + 1;
+    } else {
+      *at = turn ? N * m.unit : rest + N * m.unit;
+      *next = *at + (turn ? a.pairs : a.head_dim / 2 - rest);
     }
-    m.next = m.at + (m.turn ? a.pairs : whole ? a.head_dim / 2 : a.head_dim / 2 - a.pairs);
-    return m;
+    return turn;
   };
+
+  // Values stay as they came until they are needed: made wider at once, each item's loads
+  // would be waited for before the next one's, and all before the angles.
   constexpr int kItems = 2;     // on their way together
-  float x[kItems][N], y[kItems][N];
-  const auto take_items = [&](int32_t i) {
-#pragma unroll
-    for (int u = 0; u < kItems; ++u) {
-      const Item m = find(i + u * kPlaceLanes);
-      const int64_t r = token + m.t;
-      if (m.head < a.q.heads) {
-        const T* from = reinterpret_cast<const T*>(a.q.from.base) + r * a.q.from.token +
-                        m.head * a.q.from.head;
-        take<N>(from + m.at, a.q.from.whole_words, x[u]);
-        take<N>(from + m.next, a.q.from.whole_words, y[u]);
-      } else {
-        const bool key = m.head < rotated;
-        const char* base = key ? a.k.from.base : a.v.base;
-        const bool words = key ? a.k.from.whole_words : a.v.whole_words;
-        const G* from = reinterpret_cast<const G*>(base) +
-                        r * (key ? a.k.from.token : a.v.token) +
-                        (m.head - (key ? a.q.heads : rotated)) *
-                            (key ? a.k.from.head : a.v.head);
-        take<N>(from + m.at, words, x[u]);
-        take<N>(from + m.next, words, y[u]);
-      }
+  constexpr bool kAlike = sizeof(T) == sizeof(G);
+  Raw<N, G> x[kItems], y[kItems];
+  Raw<N, T> xq[kItems], yq[kItems];     // (queries, where they are of another size)
+  const auto take = [&](int u, const Item& m) {
+    int32_t at, next;
+    places(m, &at, &next);
+    const char* row = from + distance(m.t, from_token, m.head, from_head);
+    if (kAlike || !query) {
+      x[u].load(reinterpret_cast<const G*>(row) + at, words, lines);
+      y[u].load(reinterpret_cast<const G*>(row) + next, words, lines);
+    } else {
+      xq[u].load(reinterpret_cast<const T*>(row) + at, words, lines);
+      yq[u].load(reinterpret_cast<const T*>(row) + next, words, lines);
     }
   };
-  int32_t first = threadIdx.x;
-  take_items(first);
-  if (first_head < rotated) {     // v's heads need no angles
+  int32_t i = threadIdx.x;
+  Item item[kItems];
+  item[0].unit = i - quotient(i, a.units) * units;
+  item[0].t = quotient(i, a.units) / heads;
+  item[0].head = quotient(i, a.units) - item[0].t * heads;
+#pragma unroll
+  for (int u = 1; u < kItems; ++u) {
+    item[u] = item[u - 1];
+    advance(item[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < kItems; ++u)
+    if (i + u * kPlaceLanes < items) take(u, item[u]);
+
+  if (turned) {
     for (int32_t j = threadIdx.x; j < count * a.pairs; j += kPlaceLanes) {
       const int32_t t = quotient(j, a.by_pairs), pair = j - t * a.pairs;
       int64_t p = position + t;
@@ -221,48 +276,59 @@ __global__ __launch_bounds__(kPlaceLanes) void place_rows_kernel(PlaceArgs a) {
     }
   }
   __syncthreads();
-  for (; first < items; first += kItems * kPlaceLanes) {
+  for (; i < items; i += kItems * kPlaceLanes) {
 #pragma unroll
     for (int u = 0; u < kItems; ++u) {
-      if (first + u * kPlaceLanes >= items) continue;
-      const Item m = find(first + u * kPlaceLanes);
-      if (m.turn) {
+      if (i + u * kPlaceLanes >= items) continue;
+      const Item& m = item[u];
+      int32_t at, next;
+      const bool turn = places(m, &at, &next);
+      float p[N], r[N];
+      if (query) {
+        Raw<N, T> px, py;
+        if constexpr (kAlike) {
+          __builtin_memcpy(px.w, x[u].w, sizeof px.w);
+          __builtin_memcpy(py.w, y[u].w, sizeof py.w);
+        } else {
+          px = xq[u];
+          py = yq[u];
+        }
+        px.widen(p);
+        py.widen(r);
+      } else {
+        x[u].widen(p);
+        y[u].widen(r);
+      }
+      if (turn) {
         const float* c = cosine + m.t * a.pairs;
         const float* s = sine + m.t * a.pairs;
         if (!a.interleaved || N == 1) {
 #pragma unroll
           for (int j = 0; j < N; ++j)
-            turn_pair(x[u][j], y[u][j], c[N * m.unit + j], s[N * m.unit + j]);
+            turn_pair(p[j], r[j], c[N * m.unit + j], s[N * m.unit + j]);
         } else if constexpr (N > 1) {
 #pragma unroll
           for (int j = 0; j < N / 2; ++j) {
-            const int pair = m.at / 2 + j, other = m.next / 2 + j;
-            turn_pair(x[u][2 * j], x[u][2 * j + 1], c[pair], s[pair]);
-            turn_pair(y[u][2 * j], y[u][2 * j + 1], c[other], s[other]);
+            const int pair = at / 2 + j, other = next / 2 + j;
+            turn_pair(p[2 * j], p[2 * j + 1], c[pair], s[pair]);
+            turn_pair(r[2 * j], r[2 * j + 1], c[other], s[other]);
           }
         }
       }
-      const int64_t r = token + m.t;
-      const auto give_both = [&](auto* to, bool words) {
-        give<N>(to + m.at, words, x[u]);
-        give<N>(to + m.next, words, y[u]);
-      };
-      if (m.head < a.q.heads) {
-        give_both(reinterpret_cast<T*>(a.q.to.base) + r * a.q.to.token + m.head * a.q.to.head,
-                  a.q.to.whole_words);
-        continue;
-      }
-      const bool key = m.head < rotated;
-      const int32_t head = m.head - (key ? a.q.heads : rotated);
-      if (a.plan)
-        give_both(reinterpret_cast<T*>((key ? k_page : v_page) +
-                                       int64_t(inside + m.t) * a.pages.token +
-                                       int64_t(head) * a.pages.head), true);
-      else
-        give_both(reinterpret_cast<G*>(a.k.to.base) + r * a.k.to.token + head * a.k.to.head,
-                  a.k.to.whole_words);
+      // all that is written is of type T; without a plan, T is G
+      T* const row = reinterpret_cast<T*>(to + distance(m.t, to_token, m.head, to_head));
+      Raw<N, T> out;
+      out.round(p);
+      out.store(row + at, to_words, to_lines);
+      out.round(r);
+      out.store(row + next, to_words, to_lines);
     }
-    take_items(first + kItems * kPlaceLanes);
+#pragma unroll
+    for (int u = 0; u < kItems; ++u) {
+#pragma unroll
+      for (int s = 0; s < kItems; ++s) advance(item[u]);
+      if (i + (kItems + u) * kPlaceLanes < items) take(u, item[u]);
+    }
   }
 }
 
@@ -1336,46 +1402,55 @@ __global__ __launch_bounds__(kPagedLanes, 4) void paged_weigh_kernel(WeighArgs a
   if (g < kParts) own.add(sum);
 }
 
-// More rows: S by 32 x 32 x 16. Two workgroups share a tile of places, 128 each; of a
-// workgroup's waves two take the one and two the other 64 places, each every other 32 rows: a
-// stage of 64 rows' queries in shared memory serves all, two stages. (One workgroup
-// with 256 places, its waves on the same rows, left a third of the chip without work.)
-constexpr int kRowsPlaces = kWeighPlaces / 2, kWavePlaces = kRowsPlaces / 2, kStageRows = 64;
+// Sum of a value over the 32 lanes of a wave's half, in all of them; by moves inside
+// the vector unit (through shared memory 160 of them took 8 us).
+template <int MOVE>
+__device__ __forceinline__ float add_moved(float x) {
+  return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), MOVE, 0xF, 0xF,
+                                                        true));
+}
+__device__ __forceinline__ float half_sum(float x) {
+  x = add_moved<0xB1>(x);     // lanes 1, 0, 3, 2 of four
+  x = add_moved<0x4E>(x);     // 2, 3, 0, 1
+  x = add_moved<0x141>(x);    // eight lanes in the other order
+  x = add_moved<0x140>(x);    // sixteen
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                  false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
 
-template <int D>
-struct WeighStage {
-  v4u q[kStageRows * (D / 8)];
-  float log[kStageRows];
-  int32_t position[kStageRows];
-};
+// More rows: S^T = K Q^T by 32 x 32 x 16. A wave holds 64 places of K, lane l's row is l %
+// 32 of 32, and each lane adds up its own rows' shares, 32 sums, until the end: a row's
+// log-sum-exp and position are its lane's, and no wave waits for another. The four waves of
+// a workgroup share its places, each takes every fourth 32 rows; queries come straight from
+// memory to shared memory of the wave's own, whole rows at a time and a step ahead.
+constexpr int kRowsPlaces = 64, kRowsParts = kRowsPlaces / 32;
 
 template <int D, typename T>
-__global__ __launch_bounds__(kPagedLanes, D <= 128 ? 2 : 1) void paged_weigh_rows_kernel(
-    WeighArgs a) {
+__global__ __launch_bounds__(kPagedLanes, D <= 64 ? 3 : D <= 128 ? 2 : 1)
+void paged_weigh_rows_kernel(WeighArgs a) {
   typedef typename Matrix<T>::v8 v8;
-  typedef PagedRing<D> Places;
-  constexpr int kSteps = D / 16, kParts = kWavePlaces / 32, kChunks = D / 8;
-  __shared__ WeighStage<D> stages[2];
-  __shared__ float side[2][kParts][32];
+  typedef PagedRing<D> Ring;
+  constexpr int kSteps = D / 16, kShare = kWeighPlaces / kRowsPlaces;
+  __shared__ v4u queue[kPagedWaves][2][32 * (D / 8)];
+  __shared__ float side[kPagedWaves][kRowsPlaces];
   WeighItem it;
-  const int32_t pair = blockIdx.x / (2 * a.kv_heads);
-  const int32_t rest = blockIdx.x - pair * 2 * a.kv_heads;
-  const int32_t half = rest >= a.kv_heads;
-  if (!find_places(a, pair * a.kv_heads + rest - half * a.kv_heads, &it) || it.rows <= kMostMore)
+  const int32_t tile = blockIdx.x / (kShare * a.kv_heads);
+  const int32_t rest = blockIdx.x - tile * kShare * a.kv_heads, share = rest / a.kv_heads;
+  if (!find_places(a, tile * a.kv_heads + rest - share * a.kv_heads, &it) ||
+      it.rows <= kMostMore)
     return;
-  it.first += half * kRowsPlaces;
+  it.first += share * kRowsPlaces;
   if (!it.reaches(a.sight, it.first, kRowsPlaces)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int lane = threadIdx.x % 64, n = lane % 32, h = lane / 32;
-  const int own_places = wave % 2, own_rows = wave / 2;
-  const int32_t begin = it.first + own_places * kWavePlaces;
   const auto* table = in_plan<int32_t>(a.plan, a.at_table) + it.table;
   const int32_t last = it.len - 1, shift = a.sight.block_shift;
   const int32_t group = static_cast<int32_t>(a.group.by);
-  v8 k[kParts][kSteps];
+  v8 k[kRowsParts][kSteps];
 #pragma unroll
-  for (int p = 0; p < kParts; ++p) {
-    const int32_t at = min(begin + 32 * p + n, last);
+  for (int p = 0; p < kRowsParts; ++p) {
+    const int32_t at = min(it.first + 32 * p + n, last);
     const char* from = paged_half(a.pages, it.kv_head, shift, table[at >> shift], at).k;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s)
@@ -1389,114 +1464,99 @@ __global__ __launch_bounds__(kPagedLanes, D <= 128 ? 2 : 1) void paged_weigh_row
     const int64_t end = (int64_t(it.first) + kRowsPlaces - 1 + a.sight.window - it.base) * group;
     end_row = static_cast<int32_t>(max<int64_t>(0, min<int64_t>(end_row, end)));
   }
-  // The rows that a lane asks for, of which the next stage's are kStageRows further on: their
-  // places go along by sums.
-  constexpr int kLoads = kStageRows * kChunks / kPagedLanes;
-  const int32_t step_tokens = quotient(kStageRows, a.group);
-  const int32_t step_heads = kStageRows - step_tokens * group;
-  struct Row {
-    int64_t at, sum;          // among the queries, among the log-sum-exps
-    int32_t row, head, token;
-  };
-  const auto row_of = [&](int32_t row) {
-    Row r;
-    r.row = row;
-    row = min(row, it.rows - 1);
-    r.token = quotient(row, a.group);
-    r.head = row - r.token * group;
-    r.at = weigh_row(a, it, row, a.q.token, a.q.head);
-    r.sum = weigh_row(a, it, row, a.lse_token, 1);
-    return r;
-  };
-  const int64_t q_step = step_tokens * a.q.token + step_heads * a.q.head;
-  const int64_t q_wrap = a.q.token - group * a.q.head;
-  const int64_t lse_step = step_tokens * a.lse_token + step_heads;
-  const int64_t lse_wrap = a.lse_token - group;
-  const auto advance = [&](Row& r) {
-    r.row += kStageRows;
-    if (r.row >= it.rows) return;     // the last row that there was again, and not used
-    const bool wraps = r.head + step_heads >= group;
-    r.head += step_heads - (wraps ? group : 0);
-    r.token += step_tokens + wraps;
-    r.at += q_step + (wraps ? q_wrap : 0);
-    r.sum += lse_step + (wraps ? lse_wrap : 0);
-  };
-  Row rows[kLoads], own = row_of(first_row + static_cast<int32_t>(threadIdx.x % kStageRows));
+  // 32 rows of queries come lane by lane as shared memory holds them (k_at). Where whole
+  // tokens make 32 rows, and rows are aligned, a lane's place is the first row's and a fixed
+  // distance; else each is looked up.
+  constexpr int kStep = 32 * kPagedWaves, kChunks = D / 8, kLoads = 32 * kChunks / 64;
+  const bool even = a.q.whole_words && 32 % group == 0 &&
+                    max(a.q.token, a.q.head) < (1 << 24);     // 32-bit distances
+  const T* const queries = reinterpret_cast<const T*>(a.q.base) + int64_t(it.token) * a.q.token +
+                           int64_t(it.kv_head) * group * a.q.head;
+  uint32_t place_of[kLoads];
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i)
-    rows[i] = row_of(first_row + (i * kPagedLanes + static_cast<int32_t>(threadIdx.x)) / kChunks);
-  const int32_t own_chunk = static_cast<int32_t>(threadIdx.x) % kChunks;
-  v4u held[kLoads];
-  float held_log = 0.f;
-  const auto load = [&]() {
+  for (int i = 0; i < kLoads; ++i) {
+    const int slot = i * 64 + lane, r = slot / kChunks, at = slot % kChunks;
+    const int32_t token = quotient(r, a.group);
+    place_of[i] = static_cast<uint32_t>(
+        (token * a.q.token + (r - token * group) * a.q.head) * 2 + (at ^ Ring::k_turn(r)) * 16);
+  }
+  const int32_t own_token = quotient(n, a.group);
+  float next_log;
+  int32_t next_token;
+  const auto load = [&](int32_t row, v4u* to) {
+    const int32_t first = __builtin_amdgcn_readfirstlane(quotient(row, a.group));
+    if (even && row + 32 <= it.rows) {
+      next_token = first + own_token;
+      const char* const from = reinterpret_cast<const char*>(queries + first * a.q.token);
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i)
-      held[i] = read8(reinterpret_cast<const T*>(a.q.base) + rows[i].at + own_chunk * 8,
-                      a.q.whole_words);
-    held_log = a.lse[own.sum];
+      for (int i = 0; i < kLoads; ++i) load_shared(from, place_of[i], to + 64 * i);
+      next_log = a.lse[(int64_t(it.token) + next_token) * a.lse_token +
+                       int64_t(it.kv_head) * group + (n - own_token * group)];
+    } else {
+      const int32_t own = min(row + n, it.rows - 1);
+      next_token = quotient(own, a.group);
+      next_log = a.lse[weigh_row(a, it, own, a.lse_token, 1)];
+#pragma unroll 1
+      for (int i = 0; i < kLoads; ++i) {
+        const int slot = i * 64 + lane, r = slot / kChunks, at = slot % kChunks;
+        to[slot] = weigh_query8<T>(a, it, row + r, 8 * (at ^ Ring::k_turn(r)));
+      }
+    }
   };
-  load();
-  float w[kParts] = {};
+  int32_t row = first_row + 32 * wave;      // of the wave's first lane
   int turn = 0;
-  for (int32_t row = first_row; row < end_row; row += kStageRows, turn ^= 1) {
-    WeighStage<D>& stage = stages[turn];
+  f32x16 w[kRowsParts];
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int at = i * kPagedLanes + threadIdx.x;
-      stage.q[Places::k_at(at / kChunks, at % kChunks)] = held[i];
-    }
-    if (threadIdx.x < kStageRows) {
-      stage.log[threadIdx.x] = own.row < it.rows ? 1.4426950408889634f * held_log : INFINITY;
-      stage.position[threadIdx.x] = it.base + own.token;
-    }
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) advance(rows[i]);
-    advance(own);
-    load();
-    __syncthreads();
-    const int mine = 32 * own_rows;     // of the stage's rows
-    const int32_t low = stage.position[mine], high = stage.position[mine + 31];
+  for (int p = 0; p < kRowsParts; ++p) w[p] = f32x16{};
+  if (row < end_row) load(row, queue[wave][0]);
+  for (; row < end_row; row += kStep, turn ^= 1) {
+    // what this wave asked for has come (it alone reads it: none to meet)
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     v8 q[kSteps];
 #pragma unroll
     for (int s = 0; s < kSteps; ++s)
-      __builtin_memcpy(&q[s], &stage.q[Places::k_at(mine + n, 2 * s + h)], 16);
-    float log[16];
+      __builtin_memcpy(&q[s], &queue[wave][turn][Ring::k_at(n, 2 * s + h)], 16);
+    const float log = row + n < it.rows ? 1.4426950408889634f * next_log : INFINITY;
+    const int32_t position = it.base + next_token;
+    if (row + kStep < end_row) load(row + kStep, queue[wave][turn ^ 1]);
+    f32x16 x[kRowsParts];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) log[i] = stage.log[mine + 8 * (i / 4) + 4 * h + i % 4];
-    f32x16 x[kParts];
+    for (int p = 0; p < kRowsParts; ++p) x[p] = f32x16{};
 #pragma unroll
-    for (int p = 0; p < kParts; ++p) x[p] = f32x16{};
+    for (int p = 0; p < kRowsParts; ++p)
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s)
+      for (int s = 0; s < kSteps; ++s) x[p] = Matrix<T>::mma32(k[p][s], q[s], x[p]);
+    const int32_t low = it.base + quotient(row, a.group);
+    const int32_t high = it.base + quotient(min(row + 31, it.rows - 1), a.group);
 #pragma unroll
-      for (int p = 0; p < kParts; ++p) x[p] = Matrix<T>::mma32(q[s], k[p][s], x[p]);
-#pragma unroll
-    for (int p = 0; p < kParts; ++p) {
-      const int32_t place = begin + 32 * p;
-      float e[16];
+    for (int p = 0; p < kRowsParts; ++p) {
+      const int32_t place = it.first + 32 * p;
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[p][i], a.sight.c, -log[i]));
-      if (!seen_whole(a.sight, low, high, place) || row + mine + 32 > it.rows) {
+        x[p][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[p][i], a.sight.c, -log));
+      if (!seen_whole(a.sight, low, high, place)) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int r = mine + 8 * (i / 4) + 4 * h + i % 4;
-          const bool sees = (row + r < it.rows) & seen(a.sight, stage.position[r], place + n);
-          e[i] = sees ? e[i] : 0.f;
-        }
+        for (int i = 0; i < 16; ++i)
+          x[p][i] = seen(a.sight, position, place + 8 * (i / 4) + 4 * h + i % 4) ? x[p][i] : 0.f;
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) w[p] += e[i];
+      for (int i = 0; i < 16; ++i) w[p][i] += x[p][i];
     }
   }
+  // over the 32 lanes of a place, then over the waves
 #pragma unroll
-  for (int p = 0; p < kParts; ++p) {
-    w[p] += __shfl_xor(w[p], 32);
-    if (own_rows == 1 && h == p) side[own_places][p][n] = w[p];
-  }
+  for (int p = 0; p < kRowsParts; ++p)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float sum = half_sum(w[p][i]);
+      if (n == 0) side[wave][32 * p + 8 * (i / 4) + 4 * h + i % 4] = sum;
+    }
   __syncthreads();
-  if (own_rows == 0)
-    OwnPlace(a, it, begin + lane).add((h ? w[1] : w[0]) + side[own_places][h][n]);
+  if (wave != 0) return;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPagedWaves; ++i) sum += side[i][lane];
+  OwnPlace(a, it, it.first + lane).add(sum);
 }
 
 // ---------------------------------------------------------------- eviction --
@@ -1544,6 +1604,15 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
+// What the waves before this one have written, added up by its lanes.
+__device__ __forceinline__ uint32_t sum_before(const uint32_t (&of)[kSelectWaves], int wave,
+                                               int lane) {
+  uint32_t x = lane < wave ? of[lane] : 0;
+#pragma unroll
+  for (int far = 1; far < kSelectWaves; far *= 2) x += __shfl_xor(x, far);
+  return __builtin_amdgcn_readfirstlane(x);
+}
+
 // Which places stay: the first `sinks`, the last `recent`, and of those between the
 // ones of the largest weight, the earlier one of equals. The border weight is found
 // eleven bits at a time from counts; then every wave goes through a run of places of its
@@ -1551,6 +1620,7 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 // places each that a wave holds in registers from the first look on; 0: any number, read
 // anew each time.
 constexpr int kBins = 2048, kDigit = 11;
+static_assert(kBins == 2 * kSelectLanes, "two bins a lane");
 
 template <int STEPS>
 __global__ __launch_bounds__(kSelectLanes) void paged_select_kernel(EvictArgs a) {
@@ -1614,26 +1684,25 @@ __global__ __launch_bounds__(kSelectLanes) void paged_select_kernel(EvictArgs a)
         atomicAdd(&count[shift == 0 ? x & 1023u : x >> shift & (kBins - 1)], 1u);
     });
     __syncthreads();
-    if (wave == 0) {
-      // lane l holds the 32 bins from 2016 - 32 l on: bins above it come before it
-      const int low = kBins - 32 * (lane + 1);
-      uint32_t all = 0;
-#pragma unroll 8
-      for (int i = 0; i < 32; ++i) all += count[low + (i + lane) % 32];
-      uint32_t before = all;
+    // a lane holds two neighbouring bins, the first lane the uppermost: bins above come
+    // before
+    const int low = kBins - 2 - 2 * static_cast<int>(threadIdx.x);
+    const uint32_t upper = count[low + 1], lower = count[low];
+    uint32_t before = upper + lower;
 #pragma unroll
-      for (int far = 1; far < 64; far *= 2) {
-        const uint32_t x = __shfl_up(before, far);
-        before += lane >= far ? x : 0;
-      }
-      before -= all;
-      if (before < need && before + all >= need) {
-        int bin = low + 31;
-        while (before + count[bin] < need) before += count[bin--];
-        border = first ? static_cast<uint32_t>(bin)
-                       : prefix << (shift == 0 ? 10 : kDigit) | static_cast<uint32_t>(bin);
-        wanted = need - before;
-      }
+    for (int far = 1; far < 64; far *= 2) {
+      const uint32_t x = __shfl_up(before, far);
+      before += lane >= far ? x : 0;
+    }
+    if (lane == 63) more[wave] = before;
+    __syncthreads();
+    before += sum_before(more, wave, lane) - upper - lower;
+    const bool in_upper = before < need && before + upper >= need;
+    if (!in_upper) before += upper;
+    if (in_upper || (before < need && before + lower >= need)) {
+      const uint32_t bin = low + in_upper;
+      border = first ? bin : prefix << (shift == 0 ? 10 : kDigit) | bin;
+      wanted = need - before;
     }
     __syncthreads();
     prefix = border;
@@ -1651,12 +1720,8 @@ __global__ __launch_bounds__(kSelectLanes) void paged_select_kernel(EvictArgs a)
     same[wave] = equal;
   }
   __syncthreads();
-  uint32_t to = 0, equals = 0;
-  for (int w = 0; w < wave; ++w) {
-    to += more[w];
-    equals += same[w];
-  }
-  to += sinks + min(equals, need);
+  uint32_t equals = sum_before(same, wave, lane);
+  uint32_t to = sum_before(more, wave, lane) + sinks + min(equals, need);
   const uint64_t below = (uint64_t(1) << lane) - 1;
   each([&](uint32_t x, bool there, int32_t at) {
     const bool is_equal = there && x == prefix;
@@ -1693,7 +1758,7 @@ __device__ __forceinline__ void move_rows(const int32_t* kept, int64_t r0, int64
     if (in_place) __syncthreads();
 #pragma unroll
     for (int u = 0; u < kMoveAtOnce; ++u)
-      if (i0 + u * rows + row < r1) *to[u] = x[u];
+      if (i0 + u * rows + row < r1) __builtin_nontemporal_store(x[u], to[u]);
   }
 }
 

@@ -158,35 +158,57 @@ int check_positions(const void* positions, int64_t given, int position_bytes, in
   return check_device_range(positions, need * position_bytes, "positions");
 }
 
-// Rows (a token of a head) that a workgroup takes about. With 512, 16 tokens and
-// 32 heads each, prompts of 12,300 tokens and 120 heads were written in 298 us instead of 247,
-// with half the tokens' angles made anew for other heads.
-constexpr int64_t kPlaceRows = 128;
+// Rows (a token of a head) that a workgroup takes about. Few tokens and many heads share
+// the angles best, and where the heads are few more tokens make up for them: with 512
+// rows, 16 tokens and 32 heads each, prompts of 12,300 tokens and 120 heads were written in 298
+// us instead of 247, and with 4 tokens of every kind, prompts of 28 heads over 4 were
+// rotated in 84 us instead of 67.
+constexpr int64_t kPlaceRows = 128, kFewTokens = 4;
 
 // Eight pairs an item where the head's parts are whole runs of eight.
 bool by_eight(const PlaceArgs& a) { return a.head_dim % 16 == 0 && a.pairs % 8 == 0; }
 
-// `runs` of up to a->chunk tokens, `tokens` in all.
-int place_grid(int64_t runs, int64_t tokens, int values, PlaceArgs* a, dim3* grid) {
-  const int64_t each = std::max<int64_t>(1, up(tokens, std::max<int64_t>(1, runs)));
-  const int64_t groups = std::max<int64_t>(1, a->heads * each / kPlaceRows);
-  a->heads_each = static_cast<int32_t>(up(a->heads, groups));
-  a->head_groups = static_cast<int32_t>(up(a->heads, a->heads_each));
-  a->each = divisor(a->heads_each);
-  a->rest = divisor(a->heads - (a->head_groups - 1) * a->heads_each);
+// The workgroups of `tokens` tokens in `spans` spans (0: one after another).
+int place_grid(int64_t spans, int64_t tokens, int values, PlaceArgs* a, dim3* grid) {
+  int64_t workgroups = 0;
+  for (HeadKind& k : a->kinds) {
+    k.begin = workgroups;
+    k.each = k.groups = k.parts = 1;
+    k.chunk = kSpan;
+    if (!k.heads) continue;
+    int64_t chunk = kFewTokens;
+    while (chunk < kSpan && chunk * k.heads < kPlaceRows) chunk *= 2;
+    if (k.turned) chunk = std::min<int64_t>(chunk, kMostAngles / a->pairs);
+    if (spans) {
+      // spans of few tokens, as a decode step's, are not cut
+      const bool whole = tokens <= spans * chunk;
+      k.parts = whole ? 1 : static_cast<int32_t>(up(kSpan, chunk));
+      if (whole) chunk = kSpan;
+    } else {
+      // fewer tokens where there are few: a thousand workgroups, for 256 CUs
+      chunk = std::min(chunk, std::max<int64_t>(1, tokens / 1024));
+    }
+    const int64_t runs = spans ? spans * k.parts : up(tokens, chunk);
+    const int64_t rows = k.heads * std::max<int64_t>(1, std::min(chunk, up(tokens, runs)));
+    const int64_t groups = std::max<int64_t>(1, rows / kPlaceRows);
+    k.chunk = static_cast<int32_t>(chunk);
+    k.each = static_cast<int32_t>(up(k.heads, groups));
+    k.groups = static_cast<int32_t>(up(k.heads, k.each));
+    workgroups += runs * k.groups;
+  }
   a->by_pairs = divisor(std::max(1, a->pairs));
   a->units = divisor(a->head_dim / (2 * values));
-  const int64_t workgroups = runs * a->head_groups;
+  const int rc = check_grid(workgroups, kPlaceLanes);
   *grid = dim3(static_cast<uint32_t>(workgroups));
-  return check_grid(workgroups, kPlaceLanes);
+  return rc;
 }
 
 template <typename G, typename T>
-int launch_place(PlaceArgs a, int64_t runs, int64_t tokens, hipStream_t stream) {
+int launch_place(PlaceArgs a, int64_t spans, int64_t tokens, hipStream_t stream) {
   constexpr int kValues = sizeof(G) == 4 ? 4 : 8;
   const bool eight = by_eight(a);
   dim3 grid;
-  const int rc = place_grid(runs, tokens, eight ? kValues : 1, &a, &grid);
+  const int rc = place_grid(spans, tokens, eight ? kValues : 1, &a, &grid);
   if (rc || grid.x == 0) return rc;
   return launch(eight ? place_rows_kernel<kValues, G, T> : place_rows_kernel<1, G, T>, grid,
                 kPlaceLanes, stream, a, "place_rows_kernel launch");
@@ -255,7 +277,6 @@ int aegkv_rotate(const aegkv_rotary* rotary, const void* positions, int64_t num_
     return fail(AEGKV_EINVAL, "heads of %d values", head_dim);
   PlaceArgs a = {};
   a.tokens = q->tokens;
-  a.parts = 1;
   a.head_dim = head_dim;
   if (a.tokens < 0 || a.tokens > kMostTokens)
     return fail(AEGKV_EINVAL, "%lld tokens", ll(a.tokens));
@@ -264,7 +285,7 @@ int aegkv_rotate(const aegkv_rotary* rotary, const void* positions, int64_t num_
   if (!rc) rc = check_positions(positions, num_positions, position_bytes, a.tokens, &a);
   if (rc) return rc;
   const int dtype = q->dtype;
-  HeadRows* const kinds[2] = {&a.q, &a.k};
+  HeadKind* const kinds[2] = {&a.kinds[0], &a.kinds[1]};
   const aegkv_rows* const from[2] = {q, k};
   const aegkv_rows* const to[2] = {q_out, k_out};
   const char* const names[4] = {"q", "k", "q_out", "k_out"};
@@ -275,6 +296,7 @@ int aegkv_rotate(const aegkv_rotary* rotary, const void* positions, int64_t num_
       return fail(AEGKV_EINVAL, "%s: %lld tokens, and %lld to write of %lld", names[i],
                   ll(from[i]->tokens), ll(to[i]->tokens), ll(a.tokens));
     kinds[i]->heads = heads;
+    kinds[i]->turned = 1;
     rc = check_rows(from[i], heads, head_dim, dtype, a.tokens, a.tokens, false, false, names[i],
                     &kinds[i]->from);
     if (!rc) rc = check_rows(to[i], heads, head_dim, dtype, a.tokens, a.tokens, false, true,
@@ -297,15 +319,9 @@ int aegkv_rotate(const aegkv_rotary* rotary, const void* positions, int64_t num_
     }
   }
   if (rc) return rc;
-  a.heads = a.q.heads + a.k.heads;
-  // fewer tokens a workgroup where there are few: a thousand of them, for 256 CUs
-  const int64_t most = std::min<int64_t>(kPlaceTokens, kMostAngles / a.pairs);
-  const int64_t groups = std::max<int64_t>(1, a.heads * most / kPlaceRows);
-  a.chunk = static_cast<int32_t>(
-      std::min<int64_t>(most, std::max<int64_t>(1, a.tokens * groups / 1024)));
   return by_type(dtype, [&](auto t) {
     typedef decltype(t) T;
-    return launch_place<T, T>(a, up(a.tokens, a.chunk), a.tokens, stream);
+    return launch_place<T, T>(a, 0, a.tokens, stream);
   });
 }
 
@@ -325,29 +341,33 @@ int aegkv_paged_write(const void* plan, const void* device_plan, const aegkv_pag
   a.plan = c.plan;
   a.at_new_spans = h.room.at_new_spans;
   a.head_dim = head_dim;
-  a.pages = c.pages;
-  a.kv_heads = h.kv_heads;
-  a.block_shift = __builtin_ctz(h.block_size);
+  a.page_token = c.pages.token;
+  a.page_head = c.pages.head;
+  HeadKind &query = a.kinds[0], &key = a.kinds[1], &value = a.kinds[2];
   const int64_t now = h.num_tokens, room = h.room.tokens, tokens = reached(c);
   rc = check_rows(k, h.kv_heads, head_dim, k->dtype, now, room, c.capturing, false, "k",
-                  &a.k.from);
+                  &key.from);
   if (!rc) rc = check_rows(v, h.kv_heads, head_dim, k->dtype, now, room, c.capturing, false, "v",
-                           &a.v);
+                           &value.from);
   if (!rc && q) rc = check_rows(q, h.heads, head_dim, cache->dtype, now, room, c.capturing, false,
-                                "q", &a.q.from);
+                                "q", &query.from);
   if (!rc && q) rc = check_rows(q_out, h.heads, head_dim, cache->dtype, now, room, c.capturing,
-                                true, "q_out", &a.q.to);
+                                true, "q_out", &query.to);
   if (!rc && rotary) rc = check_rotary(rotary, head_dim, &a);
   if (!rc && positions) rc = check_positions(positions, num_positions, position_bytes, tokens, &a);
   if (rc) return rc;
-  a.k.heads = h.kv_heads;
-  a.q.heads = q ? h.heads : 0;
-  a.heads = a.q.heads + 2 * h.kv_heads;
+  query.heads = q ? h.heads : 0;
+  key.heads = value.heads = h.kv_heads;
+  query.turned = key.turned = rotary != nullptr;
+  key.pages = c.pages.k;
+  key.block = c.pages.k_block;
+  value.pages = c.pages.v;
+  value.block = c.pages.v_block;
   const auto rows = [&](const Values& x, int32_t heads, int dtype, const char* what) {
     return rows_named(x, tokens, heads, head_dim, dtype, what);
   };
-  const Named kn = rows(a.k.from, h.kv_heads, k->dtype, "k");
-  const Named vn = rows(a.v, h.kv_heads, k->dtype, "v");
+  const Named kn = rows(key.from, h.kv_heads, k->dtype, "k");
+  const Named vn = rows(value.from, h.kv_heads, k->dtype, "v");
   const Named turns{place(a.turns, rotary ? int64_t(a.pairs) * 8 : 0), "turns"};
   const Named where{place(a.positions, positions ? tokens * a.position_bytes : 0), "positions"};
   for (const Named& written : {k_cache(c), v_cache(c)}) {
@@ -356,21 +376,17 @@ int aegkv_paged_write(const void* plan, const void* device_plan, const aegkv_pag
   }
   rc = check_apart(k_cache(c), {v_cache(c)});
   if (!rc && q) {
-    const Named qn = rows(a.q.from, h.heads, cache->dtype, "q");
-    const Named to = rows(a.q.to, h.heads, cache->dtype, "q_out");
+    const Named qn = rows(query.from, h.heads, cache->dtype, "q");
+    const Named to = rows(query.to, h.heads, cache->dtype, "q_out");
     rc = check_apart(to, {k_cache(c), v_cache(c), plan_place(c), kn, vn, turns, where});
     if (!rc && !same(to.at, qn.at)) rc = check_apart(to, {qn});
     if (!rc) rc = check_apart(qn, {k_cache(c), v_cache(c)});
   }
   if (rc) return rc;
-  // spans of single tokens, as a decode step's, are not cut
-  a.chunk = kPlaceTokens;
-  a.parts = room > 2 * h.room.new_spans ? kSpan / kPlaceTokens : 1;
-  if (a.parts == 1) a.chunk = kSpan;
+  if (!h.room.new_spans) return 0;
   return by_half_type(cache->dtype, [&](auto t) {
     return by_type(k->dtype, [&](auto given) {
-      return launch_place<decltype(given), decltype(t)>(a, h.room.new_spans * a.parts, room,
-                                                        stream);
+      return launch_place<decltype(given), decltype(t)>(a, h.room.new_spans, room, stream);
     });
   });
 }
@@ -509,7 +525,8 @@ int aegkv_paged_weigh(const void* plan, const void* device_plan, const aegkv_pag
         rc = launch(paged_weigh_kernel<kDim, T>, grid(4 / weigh_parts(kDim)), kPagedLanes, stream, a,
                     "paged_weigh_kernel launch");
       if (!rc && h.room.items[kMany])
-        rc = launch(paged_weigh_rows_kernel<kDim, T>, grid(2), kPagedLanes, stream, a,
+        rc = launch(paged_weigh_rows_kernel<kDim, T>, grid(kWeighPlaces / kRowsPlaces),
+                    kPagedLanes, stream, a,
                     "paged_weigh_rows_kernel launch");
       return rc;
     });
