@@ -97,6 +97,7 @@ struct Header {
   int32_t merges;
   int32_t place_tiles;
   int32_t complete;                // every position of every sequence has its block
+  int32_t shared, pad;             // some block is in two places of the tables
   int64_t read_tokens;
 };
 

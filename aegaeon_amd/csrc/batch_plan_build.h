@@ -230,6 +230,31 @@ inline int check(const Header& h, const Batch& b) {
   return 0;
 }
 
+// Whether some block is in two places of the sequences' columns.
+inline bool shares(const Header& h, const Batch& b, int64_t columns) {
+  if (h.num_blocks / 64 <= columns + 1024) {
+    std::vector<uint64_t> seen(static_cast<size_t>(h.num_blocks / 64 + 1));
+    for (int64_t s = 0; s < b.num_seqs; ++s) {
+      const int64_t* const ids = b.ids + b.offsets[s];
+      for (int64_t c = 0, need = up(b.lens[s], h.block_size); c < need; ++c) {
+        if (ids[c] < 0) continue;
+        uint64_t& word = seen[static_cast<size_t>(ids[c] >> 6)];
+        const uint64_t bit = uint64_t(1) << (ids[c] & 63);
+        if (word & bit) return true;
+        word |= bit;
+      }
+    }
+    return false;
+  }
+  // few columns of very many blocks
+  std::vector<int64_t> all;
+  for (int64_t s = 0; s < b.num_seqs; ++s)
+    for (int64_t c = 0; c < up(b.lens[s], h.block_size); ++c)
+      if (b.ids[b.offsets[s] + c] >= 0) all.push_back(b.ids[b.offsets[s] + c]);
+  std::sort(all.begin(), all.end());
+  return std::adjacent_find(all.begin(), all.end()) != all.end();
+}
+
 // What of the plan depends on the sequences, into a buffer with room for it.
 inline int fill(Header& h, const Batch& b, const std::vector<Rows>* rows, char* base) {
   const Room& room = h.room;
@@ -247,6 +272,7 @@ inline int fill(Header& h, const Batch& b, const std::vector<Rows>* rows, char* 
     return aegkv_set_error(AEGKV_ENOMEM, "%lld sequences, %lld columns and %lld new tokens do not "
                            "fit a plan of %lld, %lld and %lld", ll(b.num_seqs), ll(columns),
                            ll(tokens), ll(room.seqs), ll(room.columns), ll(room.tokens));
+  h.shared = shares(h, b, columns);
   columns = tokens = 0;
   for (int64_t s = 0; s < b.num_seqs; ++s) {
     const int64_t len = b.lens[s], fresh = b.fresh[s], need = up(len, h.block_size);

@@ -1248,7 +1248,8 @@ struct WeighItem {
 __device__ __forceinline__ bool find_places(const WeighArgs& a, int32_t index, WeighItem* it) {
   const int32_t i = index / a.kv_heads;
   const auto* h = in_plan<Header>(a.plan, 0);
-  if (i >= h->place_tiles) return false;
+  // (a captured call may find, after an update, a batch whose sequences share blocks)
+  if (i >= h->place_tiles || h->shared) return false;
   const auto* s = in_plan<Seq>(a.plan, a.at_seqs) +
                   in_plan<int32_t>(a.plan, a.at_place_tiles)[i];
   it->kv_head = index - i * a.kv_heads;

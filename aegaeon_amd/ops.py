@@ -1207,9 +1207,9 @@ def _capturing(stream: torch.cuda.Stream) -> bool:
         return torch.cuda.is_current_stream_capturing()
 
 
-def _cache_call(cache, batch: CacheBatch, stream: torch.cuda.Stream | None, kind):
-    if not isinstance(cache, kind):
-        raise ValueError(f"a {kind.__name__}, not a {type(cache).__name__}")
+def _cache_call(cache, batch: CacheBatch, stream: torch.cuda.Stream | None, other):
+    if isinstance(cache, other):
+        raise ValueError(f"calls of another kind of cache take a {other.__name__}")
     if (batch.block_size, batch.kv_heads) != (cache.block_size, cache.kv_heads):
         raise ValueError(f"a batch of {batch.block_size}-token blocks and {batch.kv_heads} KV "
                          f"heads over a cache of {cache.block_size} and {cache.kv_heads}")
@@ -1286,7 +1286,7 @@ def quant_write(cache: QuantCache, batch: CacheBatch, k: torch.Tensor, v: torch.
         if done is not None:
             _answer(done)
             return
-    _cache_call(cache, batch, stream, QuantCache)
+    _cache_call(cache, batch, stream, PagedCache)
     kp = _rows_arg(k, "k", cache.kv_heads, cache, _DTYPES)
     vp = _rows_arg(v, "v", cache.kv_heads, cache, _DTYPES)
     if k.dtype != v.dtype or k.size(0) != v.size(0):
@@ -1314,7 +1314,7 @@ def quant_read(cache: QuantCache, batch: CacheBatch, *, tokens: str = "all",
                                           *_here(cache))
         if done is not None:
             return _answer(done)
-    _cache_call(cache, batch, stream, QuantCache)
+    _cache_call(cache, batch, stream, PagedCache)
     n = batch.read_tokens if tokens == "all" else batch.num_tokens
     if out is None:
         if dtype not in _DTYPES:
@@ -1350,7 +1350,7 @@ def quant_attend(cache: QuantCache, batch: CacheBatch, q: torch.Tensor, *,
                                             *_here(cache))
         if done is not None:
             return _answer(done)
-    _cache_call(cache, batch, stream, QuantCache)
+    _cache_call(cache, batch, stream, PagedCache)
     qp = _rows_arg(q, "q", batch.heads, cache, (torch.bfloat16, torch.float16))
     if out is None:
         out = _empty_on(stream, q.shape, dtype=q.dtype, device=q.device)
@@ -1538,7 +1538,7 @@ def _native(cache: PagedCache, batch: CacheBatch, stream) -> bool:
 
 
 def _paged_call(cache: PagedCache, batch: CacheBatch, stream) -> None:
-    _cache_call(cache, batch, stream, PagedCache)
+    _cache_call(cache, batch, stream, QuantCache)
     if cache.k_pages.requires_grad or cache.v_pages.requires_grad:
         raise ValueError("the cache requires a gradient, which these operators do not give")
 
@@ -1583,7 +1583,7 @@ def rotate(rotary: Rotary, positions: torch.Tensor, q: torch.Tensor,
     """
     if stream is None:
         to = (out, None) if k is None or out is None else out
-        if len(to) == 2:
+        if isinstance(to, (tuple, list)) and len(to) == 2:
             done = _lib.hostargs().rotate(rotary._packed, positions, q, k, *to, *_here(rotary))
             if done is not None:
                 return _answer(done)
@@ -1750,7 +1750,7 @@ def paged_weigh(cache: PagedCache, batch: CacheBatch, q: torch.Tensor, lse: torc
 
     q, scale: those of paged_attend, whose log-sum-exps lse are. weights: float32 [num_blocks,
     kv_heads, block_size], contiguous; the new tokens' places start from 0, those that no query
-    sees keep theirs. As a segment of the composite cache (layout.weight_tensor_specs)
+    sees keep theirs. Sequences of the batch may share no blocks. As a segment of the composite cache (layout.weight_tensor_specs)
     they move with the blocks.
     """
     if _native(cache, batch, stream):

@@ -715,7 +715,8 @@ int aegkv_paged_attend(const void* plan, const void* device_plan, const aegkv_pa
  * exp(scale * q . K[j] - lse). weights: [num_blocks][kv_heads][block_size] floats (a
  * segment of the cache like K and V, which swaps and copies move). What the new tokens' places
  * held before does not count; weights of places that no query sees are left as they were.
- * Sums are made in 32 bits in a fixed order (no atomics).
+ * Sums are made in 32 bits in a fixed order (no atomics). Sequences that share blocks are
+ * refused (AEGKV_EDUP); a captured call, replayed after an update to such, does nothing.
  */
 int aegkv_paged_weigh(const void* plan, const void* device_plan, const aegkv_paged_cache* cache,
                       const aegkv_rows* q, const float* lse, int64_t lse_tokens,

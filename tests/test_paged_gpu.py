@@ -445,6 +445,37 @@ def test_weights_of_keys_that_are_no_number(gpu):
         near(w.sum(), torch.tensor(2.0 * m, dtype=torch.float64), 1e-3)
 
 
+def test_weights_of_shared_blocks_are_refused(gpu):
+    """Two sequences over common blocks would add to one place at once; a captured call that
+    finds them after an update leaves the weights as they were."""
+    bs, heads, d, num = 16, 2, 64, 12
+    cache = ops.PagedCache(*(p.to(gpu) for p in make_pages(num, bs, heads, d, BF16)))
+    weights = torch.ones(num, heads, bs, device=gpu)
+    q = torch.randn(2, heads, d, generator=gen(0)).to(BF16).to(gpu)
+    shared = batch_for(gpu, [[1, 2], [1, 3]], [20, 30], [1, 1], cache)
+    out, lse = ops.paged_attend(cache, shared, q, return_lse=True)      # (fine)
+    with pytest.raises(ValueError, match="one block"):
+        ops.paged_weigh(cache, shared, q, lse, weights)
+    room = dict(max_seqs=2, max_columns=8, max_tokens=2)
+    batch = batch_for(gpu, [[1, 2], [4, 3]], [20, 30], [1, 1], cache, **room)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.paged_weigh(cache, batch, q, lse, weights)
+    batch.update([[1, 2], [1, 3]], [20, 30], [1, 1])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (weights == 1).all()
+    batch.update([[1, 2], [4, 3]], [20, 30], [1, 1])
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert not (weights[1, :, :16] == 1).any() and (weights[5:] == 1).all()
+    # columns behind a sequence's end do not count
+    batch.update([[1, 2, 3], [4, 3]], [20, 30], [1, 1])
+    ops.paged_weigh(cache, batch, q, lse, weights)
+
+
 # ---- eviction ----------------------------------------------------------------------------
 
 
@@ -803,9 +834,9 @@ def test_calls_take_their_own_kind_of_cache(gpu):
                            kv_heads=2, head_dim=64, block_size=16, fmt="mxfp8")
     batch = batch_for(gpu, [[1]], [3], [3], paged)
     x = torch.zeros(3, 2, 64, dtype=BF16, device=gpu)
-    with pytest.raises(ValueError, match="a PagedCache, not a QuantCache"):
+    with pytest.raises(ValueError, match="another kind of cache take a QuantCache"):
         ops.paged_attend(quant, batch, x)
-    with pytest.raises(ValueError, match="a QuantCache, not a PagedCache"):
+    with pytest.raises(ValueError, match="another kind of cache take a PagedCache"):
         ops.quant_attend(paged, batch, x)
 
 
@@ -894,6 +925,7 @@ def test_refusals(gpu):
     bad("overlap", ops.rotate, rotary, positions, q, k, out=(buffer[:3 * 4 * d].view(3, 4, d),
                                                             buffer[:3 * 2 * d].view(3, 2, d)))
     bad("tensors", ops.rotate, rotary, positions, q, k, out=buffer[:3 * 4 * d].view(3, 4, d))
+    bad("tensors", ops.rotate, rotary, positions, q, q, out=torch.zeros_like(q).expand(2, 3, 4, d))
     bad("what it goes to", ops.rotate, rotary, positions, q, k.half())
     if torch.cuda.device_count() == 1:
         bad("on cpu", ops.rotate, rotary, positions.cpu(), q)
