@@ -868,12 +868,17 @@ __device__ __forceinline__ uint32_t shared_address(const v4u* p) {
 }
 
 // 16 bytes a lane from `base` (the same for the wave) + offset to shared memory, lane
-// after lane from `to` on. The compiler does not know of it: whoever reads them waits by
-// wait_and_meet() first. (Told of it, it waits for all such loads before any read of shared
-// memory.)
+// after lane from `to` on; NT: past the caches. The compiler does not know of it: whoever
+// reads them waits for them first. (Told of it, it waits for all such loads before any
+// read of shared memory.)
+template <bool NT = false>
 __device__ __forceinline__ void load_shared(const char* base, uint32_t offset, const v4u* to) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-               :: "v"(offset), "s"(base), "s"(shared_address(to)) : "memory");
+  if constexpr (NT)
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt"
+                 :: "v"(offset), "s"(base), "s"(shared_address(to)) : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :: "v"(offset), "s"(base), "s"(shared_address(to)) : "memory");
 }
 
 // All of the wave's loads have come but the last LATER, its reads of shared memory too,
@@ -1271,20 +1276,6 @@ __device__ __forceinline__ int64_t weigh_row(const WeighArgs& a, const WeighItem
              head_stride;
 }
 
-template <typename T>
-__device__ __forceinline__ v4u read8(const T* from, bool whole_words) {
-  v4u x;
-  if (whole_words) {
-    x = *(const gv4u*)from;
-  } else {
-    T t[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) t[j] = from[j];
-    __builtin_memcpy(&x, t, 16);
-  }
-  return x;
-}
-
 // Eight values of a query row from `at` on. (Behind the last row, its own again: what comes
 // of them is dropped.)
 template <typename T>
@@ -1292,7 +1283,9 @@ __device__ __forceinline__ v4u weigh_query8(const WeighArgs& a, const WeighItem&
                                             int32_t at) {
   const T* from = reinterpret_cast<const T*>(a.q.base) +
                   weigh_row(a, it, min(row, it.rows - 1), a.q.token, a.q.head) + at;
-  return read8(from, a.q.whole_words);
+  v4u x;
+  __builtin_memcpy(&x, from, 16);
+  return x;
 }
 
 // log2(e) times a row's log-sum-exp; infinity where there is no row: its share is 0.
@@ -1307,12 +1300,12 @@ struct OwnPlace {
   float* to;
   float before;
   bool seen;
-  __device__ __forceinline__ OwnPlace(const WeighArgs& a, const WeighItem& it, int32_t place) {
+  // (a place behind the sequence's last one is the last one)
+  __device__ __forceinline__ OwnPlace(const WeighArgs& a, const WeighItem& it, int32_t place,
+                                      int64_t block) {
     const int32_t shift = a.sight.block_shift;
     seen = it.reaches(a.sight, place, 1);
     place = min(place, it.len - 1);
-    const int64_t block = reinterpret_cast<const int32_t*>(a.plan + a.at_table)[it.table +
-                                                                               (place >> shift)];
     to = a.weights + (((block * a.kv_heads + it.kv_head) << shift) +
                       (place & ((1 << shift) - 1)));
     before = place < it.base ? *to : 0.f;
@@ -1324,10 +1317,12 @@ struct OwnPlace {
 
 // w[place] += sum over the rows that see it of exp2(c s - log2(e) lse). A place
 // belongs to one lane at the end: no atomics, and the sum's order is fixed. Up
-// to 64 rows of a sequence: S = Q K^T by 16 x 16 x 32, a wave's 64 places in registers.
-// Bound by HBM; what takes part is asked for at once, without branches: with four
-// log-sum-exps and four places a lane, looked up one after another, 64 decodes took 150 us.
-// A wave holds 8 KiB of K: with 64 places at any width, 128-wide heads took 124.
+// to 64 rows of a sequence: S = Q K^T by 16 x 16 x 32. Bound by HBM; what takes part is
+// asked for at once, without branches. K comes straight to shared memory of the wave's own,
+// whole rows at a time, and past the caches: into registers, a token a lane, each load
+// takes half of a line, and most waves stand at a load that is not taken yet. 64 decodes of
+// 100 to 8,000 tokens, 8 KV heads of 128, take 99 us (5.4 TB/s): 116 from registers, 110
+// through the caches. A wave holds 8 KiB of K: with 64 places 105, with 16 100.
 constexpr int weigh_parts(int head_dim) { return head_dim == 64 ? 4 : head_dim == 128 ? 2 : 1; }
 
 template <int D, typename T>
@@ -1335,6 +1330,9 @@ __global__ __launch_bounds__(kPagedLanes, 4) void paged_weigh_kernel(WeighArgs a
   typedef typename Matrix<T>::v8 v8;
   constexpr int kSteps = D / 32, kParts = weigh_parts(D), kWavePlaces = 16 * kParts;
   constexpr int kShare = kWeighPlaces / (kPagedWaves * kWavePlaces);
+  constexpr int kChunks = D / 8, kLoads = 16 * kChunks / 64;
+  typedef PagedRing<D> Ring;
+  __shared__ v4u held[kPagedWaves][kWavePlaces * kChunks];
   WeighItem it;
   const int32_t tile = blockIdx.x / (kShare * a.kv_heads);
   const int32_t rest = blockIdx.x - tile * kShare * a.kv_heads, share = rest / a.kv_heads;
@@ -1347,18 +1345,22 @@ __global__ __launch_bounds__(kPagedLanes, 4) void paged_weigh_kernel(WeighArgs a
   if (!it.reaches(a.sight, begin, kWavePlaces)) return;
   const auto* table = in_plan<int32_t>(a.plan, a.at_table) + it.table;
   const int32_t last = it.len - 1, shift = a.sight.block_shift;
-  v8 k[kParts][kSteps];
+  // (parts behind the sequence's last place read its last one again)
+  int32_t own_block = 0;
 #pragma unroll
   for (int p = 0; p < kParts; ++p) {
-    // (parts behind the sequence's last place read its last one again)
     const int32_t at = min(begin + 16 * p, last & ~15);
-    const PagedHalf h = paged_half(a.pages, it.kv_head, shift, table[at >> shift], at);
+    const int32_t block = table[at >> shift];
+    const char* const from = paged_half(a.pages, it.kv_head, shift, block, at).k;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s)
-      load_bytes<16, false>(reinterpret_cast<uint32_t*>(&k[p][s]), h.k,
-                            m * a.pages.token + g * 16 + s * 64);
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = i * (64 / kChunks) + lane / kChunks;
+      load_shared<true>(from, r * a.pages.token + (lane % kChunks ^ Ring::k_turn(r)) * 16,
+                  &held[wave][p * 16 * kChunks + i * 64]);
+    }
+    own_block = g % kParts == p ? block : own_block;
   }
-  const OwnPlace own(a, it, begin + lane % kWavePlaces);
+  const OwnPlace own(a, it, begin + lane % kWavePlaces, own_block);
   const bool whole = seen_whole(a.sight, it.base, last, begin) &&
                      seen_whole(a.sight, it.base, last, begin + kWavePlaces - kTile);
   float w[kParts] = {};
@@ -1372,6 +1374,8 @@ __global__ __launch_bounds__(kPagedLanes, 4) void paged_weigh_kernel(WeighArgs a
     }
     const float own_log = row_log(a, it, row + m);
     const int32_t own_position = it.base + quotient(min(row + m, it.rows - 1), a.group);
+    // K is here (this wave alone reads what it asked for: none to meet)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     float log[4];
     int32_t position[4];
 #pragma unroll
@@ -1383,7 +1387,11 @@ __global__ __launch_bounds__(kPagedLanes, 4) void paged_weigh_kernel(WeighArgs a
     for (int p = 0; p < kParts; ++p) {
       f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) x = Matrix<T>::mma(q[s], k[p][s], x);
+      for (int s = 0; s < kSteps; ++s) {
+        v8 k;
+        __builtin_memcpy(&k, &held[wave][p * 16 * kChunks + Ring::k_at(m, 4 * s + g)], 16);
+        x = Matrix<T>::mma(q[s], k, x);
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const bool sees = (log[i] != INFINITY) &
@@ -1557,7 +1565,8 @@ void paged_weigh_rows_kernel(WeighArgs a) {
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < kPagedWaves; ++i) sum += side[i][lane];
-  OwnPlace(a, it, it.first + lane).add(sum);
+  const int32_t place = it.first + lane;
+  OwnPlace(a, it, place, table[min(place, last) >> shift]).add(sum);
 }
 
 // ---------------------------------------------------------------- eviction --
@@ -1619,9 +1628,18 @@ __device__ __forceinline__ uint32_t sum_before(const uint32_t (&of)[kSelectWaves
 // eleven bits at a time from counts; then every wave goes through a run of places of its
 // own, twice: once to count, once to write its places where they belong. STEPS: 64
 // places each that a wave holds in registers from the first look on; 0: any number, read
-// anew each time.
+// anew each time. A workgroup has a head's places to itself, so a long sequence is bound
+// by what one compute unit does: five looks at a place, two to ten instructions each
+// (30,001 places under 4 heads 21 us, 30 with a bound tested at every place; 48 x 8 heads
+// of 1,500 to 8,000 places 16).
 constexpr int kBins = 2048, kDigit = 11;
 static_assert(kBins == 2 * kSelectLanes, "two bins a lane");
+
+// How many lanes before this one are in `mask`.
+__device__ __forceinline__ uint32_t lanes_below(uint64_t mask) {
+  return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32),
+                                   __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
+}
 
 template <int STEPS>
 __global__ __launch_bounds__(kSelectLanes) void paged_select_kernel(EvictArgs a) {
@@ -1642,14 +1660,19 @@ __global__ __launch_bounds__(kSelectLanes) void paged_select_kernel(EvictArgs a)
   const int32_t chosen = keep - sinks - recent, places = e.len - sinks - recent;
   if (chosen == 0) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
-  const int32_t run = ((places + kSelectWaves - 1) / kSelectWaves + 63) & ~63;
-  const int32_t begin =
-      static_cast<int32_t>(min(int64_t(wave) * run, int64_t(places)));
+  // places a wave goes through at a time
+  constexpr int kAtOnce = STEPS ? 1 : 8, kTurn = 64 * kAtOnce;
+  const int64_t run = (int64_t(places) - 1) / (kSelectWaves * kTurn) * kTurn + kTurn;
+  const int32_t begin = static_cast<int32_t>(min(wave * run, int64_t(places)));
   const int32_t end = static_cast<int32_t>(min(int64_t(begin) + run, int64_t(places)));
+  // a place behind the last one has the least key, and comes after all others of that key:
+  // more than `chosen` are there, so it never stays
   const auto key = [&](int32_t i) {
-    return weight_key(a.weights[weight_at(a, e.table, e.kv_head, sinks + min(i, places - 1))]);
+    const uint32_t x =
+        weight_key(a.weights[weight_at(a, e.table, e.kv_head, sinks + min(i, places - 1))]);
+    return i < places ? x : 0;
   };
-  // f(key, whether there is one, first place of the 64) for the wave's run
+  // f(key, first place of the 64) for the wave's run
   uint32_t held[STEPS ? STEPS : 1];
   if constexpr (STEPS != 0) {
 #pragma unroll
@@ -1658,17 +1681,17 @@ __global__ __launch_bounds__(kSelectLanes) void paged_select_kernel(EvictArgs a)
   const auto each = [&](const auto& f) {
     if constexpr (STEPS != 0) {
 #pragma unroll
-      for (int s = 0; s < STEPS; ++s)
-        if (begin + 64 * s < end) f(held[s], begin + 64 * s + lane < end, begin + 64 * s);
+      for (int s = 0; s < STEPS; ++s) {
+        if (begin + 64 * s >= end) break;
+        f(held[s], begin + 64 * s);
+      }
     } else {
-      constexpr int kAtOnce = 8;
       for (int32_t at = begin; at < end; at += 64 * kAtOnce) {
         uint32_t x[kAtOnce];
 #pragma unroll
         for (int s = 0; s < kAtOnce; ++s) x[s] = key(at + 64 * s + lane);
 #pragma unroll
-        for (int s = 0; s < kAtOnce; ++s)
-          if (at + 64 * s < end) f(x[s], at + 64 * s + lane < end, at + 64 * s);
+        for (int s = 0; s < kAtOnce; ++s) f(x[s], at + 64 * s);
       }
     }
   };
@@ -1680,10 +1703,16 @@ __global__ __launch_bounds__(kSelectLanes) void paged_select_kernel(EvictArgs a)
     const bool first = shift == 32 - kDigit;
     for (int i = threadIdx.x; i < kBins; i += kSelectLanes) count[i] = 0;
     __syncthreads();
-    each([&](uint32_t x, bool there, int32_t) {
-      if (there && (first || x >> known == prefix))
-        atomicAdd(&count[shift == 0 ? x & 1023u : x >> shift & (kBins - 1)], 1u);
-    });
+    const uint32_t mask = shift == 0 ? 1023u : kBins - 1;
+    if (first)
+      each([&](uint32_t x, int32_t) {
+        atomicAdd(&count[x >> shift], 1u);
+      });
+    else
+      each([&](uint32_t x, int32_t) {
+        if (x >> known == prefix)
+          atomicAdd(&count[x >> shift & mask], 1u);
+      });
     __syncthreads();
     // a lane holds two neighbouring bins, the first lane the uppermost: bins above come
     // before
@@ -1712,27 +1741,32 @@ __global__ __launch_bounds__(kSelectLanes) void paged_select_kernel(EvictArgs a)
   }
   // now `prefix` is the border weight, of which the first `need` stay
   uint32_t above = 0, equal = 0;
-  each([&](uint32_t x, bool there, int32_t) {
-    above += __popcll(__ballot(there && x > prefix));
-    equal += __popcll(__ballot(there && x == prefix));
+  each([&](uint32_t x, int32_t) {
+    above += x > prefix;
+    equal += x == prefix;
   });
+#pragma unroll
+  for (int far = 1; far < 64; far *= 2) {
+    above += __shfl_xor(above, far);
+    equal += __shfl_xor(equal, far);
+  }
   if (lane == 0) {
     more[wave] = above;
     same[wave] = equal;
   }
   __syncthreads();
   uint32_t equals = sum_before(same, wave, lane);
-  uint32_t to = sum_before(more, wave, lane) + sinks + min(equals, need);
-  const uint64_t below = (uint64_t(1) << lane) - 1;
-  each([&](uint32_t x, bool there, int32_t at) {
-    const bool is_equal = there && x == prefix;
-    const uint64_t same_here = __ballot(is_equal);
-    const bool stays = (there && x > prefix) ||
-                       (is_equal && equals + __popcll(same_here & below) < need);
+  int32_t* to = kept + sum_before(more, wave, lane) + sinks + min(equals, need);
+  each([&](uint32_t x, int32_t at) {
+    bool stays = x > prefix;
+    const uint64_t same_here = __ballot(x == prefix);
+    if (same_here) {
+      stays |= (x == prefix) & (equals + lanes_below(same_here) < need);
+      equals += __popcll(same_here);
+    }
     const uint64_t all = __ballot(stays);
-    if (stays) kept[to + __popcll(all & below)] = sinks + at + lane;
+    if (stays) to[lanes_below(all)] = sinks + at + lane;
     to += __popcll(all);
-    equals += __popcll(same_here);
   });
 }
 

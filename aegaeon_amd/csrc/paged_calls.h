@@ -232,7 +232,12 @@ int by_width(int head_dim, const F& f) {
 // in no other place of either batch's tables.
 int check_targets(const Header& h, const char* host, const Header* into, const char* into_host,
                   int64_t keep) {
-  std::vector<uint8_t> use(static_cast<size_t>(h.num_blocks), 0);   // 1: read, 2: written
+  std::vector<uint8_t> use;   // 1: read, 2: written
+  try {
+    use.resize(static_cast<size_t>(h.num_blocks));
+  } catch (const std::exception& e) {
+    return fail(AEGKV_ENOMEM, "the tables' blocks: %s", e.what());
+  }
   const auto walk = [&](const Header& of, const char* plan, int64_t s, int64_t columns,
                         uint8_t mark) {
     const auto* seq = seqs(plan, of.room) + s;
