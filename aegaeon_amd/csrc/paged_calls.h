@@ -628,8 +628,9 @@ int aegkv_paged_evict(const void* plan, const void* device_plan, const aegkv_pag
   for (int64_t s = 0; s < h.num_seqs; ++s)
     longest = std::max<int64_t>(longest, seqs(plan, h.room)[s].len);
   a.groups = static_cast<int32_t>(std::max<int64_t>(1, up(std::min(keep, longest), a.rows_each)));
+  const int move_lanes = into_plan ? kMoveLanes : kMostMoveLanes;
   rc = check_grid(count, kSelectLanes);
-  if (!rc) rc = check_grid(count * a.groups, kMoveLanes);
+  if (!rc) rc = check_grid(3 * count * a.groups, move_lanes);
   if (rc) return rc;
   const auto select = longest <= 8 * kSelectLanes    ? paged_select_kernel<8>
                       : longest <= 32 * kSelectLanes ? paged_select_kernel<32>
@@ -637,7 +638,7 @@ int aegkv_paged_evict(const void* plan, const void* device_plan, const aegkv_pag
   rc = launch(select, dim3(static_cast<uint32_t>(count)), kSelectLanes, stream, a,
               "paged_select_kernel launch");
   if (rc) return rc;
-  return launch(paged_move_kernel, dim3(static_cast<uint32_t>(count * a.groups), 3), kMoveLanes,
+  return launch(paged_move_kernel, dim3(static_cast<uint32_t>(3 * count * a.groups)), move_lanes,
                 stream, a, "paged_move_kernel launch");
 }
 
