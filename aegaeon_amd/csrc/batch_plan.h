@@ -36,10 +36,15 @@ struct Seq {
   int32_t table;       // first entry of its block table
   int32_t token;       // row of its first new token
   int32_t read_span;   // spans of all tokens before this sequence
-  int32_t place_tile;  // tiles of kPlaceTile places before this sequence
+  int32_t pad;
   int64_t read_token;  // tokens before this sequence
 };
 static_assert(sizeof(Seq) == 32, "Seq layout");
+
+// kPlaceTile places of a sequence, of which some query sees one.
+struct PlaceTile {
+  int32_t seq, first;
+};
 
 // Up to 16 new tokens of a sequence inside one block.
 struct NewSpan {
@@ -82,7 +87,7 @@ struct Room {
   int64_t slots[kKinds];
   int64_t merges;
   int64_t at_seqs, at_table, at_new_spans, at_items[kKinds], at_merges;
-  int64_t at_place_tiles;          // int32: the sequence of each tile of kPlaceTile places
+  int64_t at_place_tiles;
 };
 
 struct Header {
@@ -95,9 +100,9 @@ struct Header {
   int32_t new_spans, read_spans;
   int32_t items[kKinds], slots[kKinds];
   int32_t merges;
-  int32_t place_tiles;
+  int32_t many_tiles, place_tiles; // tiles of kMany's sequences, which come first; all
   int32_t complete;                // every position of every sequence has its block
-  int32_t shared, pad;             // some block is in two places of the tables
+  int32_t shared;                  // some block is in two places of the tables
   int64_t read_tokens;
 };
 

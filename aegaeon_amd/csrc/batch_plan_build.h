@@ -262,7 +262,7 @@ inline int fill(Header& h, const Batch& b, const std::vector<Rows>* rows, char* 
   auto* table = reinterpret_cast<int32_t*>(base + room.at_table);
   auto* merge = reinterpret_cast<Merge*>(base + room.at_merges);
   auto* span = reinterpret_cast<NewSpan*>(base + room.at_new_spans);
-  auto* tile_seq = reinterpret_cast<int32_t*>(base + room.at_place_tiles);
+  auto* tile = reinterpret_cast<PlaceTile*>(base + room.at_place_tiles);
   int64_t columns = 0, tokens = 0, new_spans = 0, read_spans = 0, read_tokens = 0;
   int64_t place_tiles = 0;
   h.complete = 1;
@@ -281,7 +281,7 @@ inline int fill(Header& h, const Batch& b, const std::vector<Rows>* rows, char* 
     seq[s].table = static_cast<int32_t>(columns);
     seq[s].token = static_cast<int32_t>(tokens);
     seq[s].read_span = static_cast<int32_t>(read_spans);
-    seq[s].place_tile = static_cast<int32_t>(place_tiles);
+    seq[s].pad = 0;
     seq[s].read_token = read_tokens;
     for (int64_t c = 0; c < need; ++c) {
       const int64_t id = b.ids[b.offsets[s] + c];
@@ -304,18 +304,27 @@ inline int fill(Header& h, const Batch& b, const std::vector<Rows>* rows, char* 
       at = end;
     }
     read_spans += up(len, kSpan);
-    for (int64_t at = 0; at < len; at += kPlaceTile) {
-      if (place_tiles >= room.place_tiles)
-        return aegkv_set_error(AEGKV_ENOMEM, "the sequences do not fit the plan's %lld tiles of "
-                               "places", ll(room.place_tiles));
-      tile_seq[place_tiles++] = static_cast<int32_t>(s);
-    }
     read_tokens += len;
   }
   h.num_seqs = static_cast<int32_t>(b.num_seqs);
   h.num_tokens = static_cast<int32_t>(tokens);
   h.new_spans = static_cast<int32_t>(new_spans);
   h.read_spans = static_cast<int32_t>(read_spans);
+  const int64_t window = h.window ? h.window : INT32_MAX;
+  for (const bool many : {true, false}) {
+    for (int64_t s = 0; s < b.num_seqs; ++s) {
+      const int64_t len = b.lens[s], fresh = b.fresh[s], base = len - fresh;
+      if (fresh == 0 || (fresh * h.group > kMostMore) != many) continue;
+      for (int64_t at = 0; at < len; at += kPlaceTile) {
+        if (base - (at + kPlaceTile - 1) >= window && at >= h.sinks) continue;
+        if (place_tiles >= room.place_tiles)
+          return aegkv_set_error(AEGKV_ENOMEM, "the sequences do not fit the plan's %lld tiles of "
+                                 "places", ll(room.place_tiles));
+        tile[place_tiles++] = PlaceTile{static_cast<int32_t>(s), static_cast<int32_t>(at)};
+      }
+    }
+    if (many) h.many_tiles = static_cast<int32_t>(place_tiles);
+  }
   h.place_tiles = static_cast<int32_t>(place_tiles);
   h.read_tokens = read_tokens;
   if (read_spans > room.read_spans)
@@ -427,7 +436,7 @@ inline void make_room(Header& h, const Batch& b, const std::vector<Rows>* rows, 
     r.at_items[kind] = take(r.items[kind] * static_cast<int64_t>(sizeof(Item)));
   }
   r.at_merges = take(r.merges * static_cast<int64_t>(sizeof(Merge)));
-  r.at_place_tiles = take(r.place_tiles * 4);
+  r.at_place_tiles = take(r.place_tiles * static_cast<int64_t>(sizeof(PlaceTile)));
   r.bytes = at;
 }
 

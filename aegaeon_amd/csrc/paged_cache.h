@@ -832,7 +832,12 @@ __device__ __forceinline__ float pair_max(float x) {
 // product's reads meet in a bank: K's operands are a token's chunk a lane, V's come four
 // tokens of a value a lane by transposing reads. Lane l (row l % 32, h = l / 32) holds the
 // scores of tokens 8 (i / 4) + 4 h + i % 4, i < 16, and they are the second product's
-// operand as they lie.
+// operand as they lie. Three tiles are in work at once: the second product of one beside
+// the scores of the next and the exponents between them. Bound by what two waves a SIMD
+// issue: matrix units are busy 48 % of a long prompt's time, the vector unit 50. Four
+// prompts of 1,000 to 4,096 tokens, 8 KV heads of 32, 128 wide, take 190 us (825 TFLOP/s), one
+// of 32,768 runs at 1,050, 64-wide heads at 690, 256-wide ones at 730; with registers
+// instead of the ring they took 208, a tile after another without its order of issue 193.
 constexpr int kRing = 4, kRowsWave = 32, kTileRowsWave = kTile / kPagedWaves;
 static_assert(kManyRows == kPagedWaves * kRowsWave, "rows of a workgroup");
 
@@ -1154,6 +1159,7 @@ __global__ __launch_bounds__(kPagedLanes, D == 256 ? 1 : 2) void paged_prompt_ke
 // all, over the sum of their sums. A workgroup's lanes are groups of D / 4,
 // four values a lane. Of up to kMergeRows parts each group takes rows of its own;
 // more (few rows over a long axis) are shared out to the groups, one row a workgroup.
+// 4 to 6 us, of which 3 are a launch and the reads that follow one another.
 template <int D, typename T>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttendArgs a) {
   constexpr int kLanes = D / 4, kSides = 256 / kLanes;
@@ -1235,7 +1241,7 @@ struct WeighArgs {
   int64_t lse_token;
   float* weights;       // [block][kv_head][token]
   Divisor group;
-  int32_t kv_heads;
+  int32_t kv_heads, first_tile;
 };
 
 constexpr int kWeighPlaces = kPlaceTile;
@@ -1250,21 +1256,26 @@ struct WeighItem {
   }
 };
 
+// MANY: of the sequences of more than kMostMore rows, whose tiles come first. A captured
+// call has a workgroup for each tile that there is room for, and may find, after an
+// update, a batch whose sequences share blocks.
+template <bool MANY>
 __device__ __forceinline__ bool find_places(const WeighArgs& a, int32_t index, WeighItem* it) {
-  const int32_t i = index / a.kv_heads;
+  const int32_t i = index / a.kv_heads, at = i + a.first_tile;
   const auto* h = in_plan<Header>(a.plan, 0);
-  // (a captured call may find, after an update, a batch whose sequences share blocks)
-  if (i >= h->place_tiles || h->shared) return false;
-  const auto* s = in_plan<Seq>(a.plan, a.at_seqs) +
-                  in_plan<int32_t>(a.plan, a.at_place_tiles)[i];
+  if (h->shared || at >= (MANY ? h->many_tiles : h->place_tiles) ||
+      (!MANY && at < h->many_tiles))
+    return false;
+  const auto* tile = in_plan<PlaceTile>(a.plan, a.at_place_tiles) + at;
+  const auto* s = in_plan<Seq>(a.plan, a.at_seqs) + tile->seq;
   it->kv_head = index - i * a.kv_heads;
-  it->first = (i - s->place_tile) * kWeighPlaces;
+  it->first = tile->first;
   it->len = s->len;
   it->base = s->len - s->fresh;
   it->rows = s->fresh * static_cast<int32_t>(a.group.by);
   it->token = s->token;
   it->table = s->table;
-  return it->rows > 0;
+  return true;
 }
 
 // A query row's place among the values, and its log-sum-exp's.
@@ -1294,8 +1305,7 @@ __device__ __forceinline__ float row_log(const WeighArgs& a, const WeighItem& it
   return row < it.rows ? 1.4426950408889634f * x : INFINITY;
 }
 
-// A lane's place and what it has gathered before; asked for early, since what follows from it
-// depends on two loads.
+// A lane's place and what it has gathered before; asked for before its scores are made.
 struct OwnPlace {
   float* to;
   float before;
@@ -1336,8 +1346,7 @@ __global__ __launch_bounds__(kPagedLanes, 4) void paged_weigh_kernel(WeighArgs a
   WeighItem it;
   const int32_t tile = blockIdx.x / (kShare * a.kv_heads);
   const int32_t rest = blockIdx.x - tile * kShare * a.kv_heads, share = rest / a.kv_heads;
-  if (!find_places(a, tile * a.kv_heads + rest - share * a.kv_heads, &it) || it.rows > kMostMore)
-    return;
+  if (!find_places<false>(a, tile * a.kv_heads + rest - share * a.kv_heads, &it)) return;
   it.first += share * kPagedWaves * kWavePlaces;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int lane = threadIdx.x % 64, m = lane % 16, g = lane / 16;
@@ -1432,7 +1441,12 @@ __device__ __forceinline__ float half_sum(float x) {
 // 32 of 32, and each lane adds up its own rows' shares, 32 sums, until the end: a row's
 // log-sum-exp and position are its lane's, and no wave waits for another. The four waves of
 // a workgroup share its places, each takes every fourth 32 rows; queries come straight from
-// memory to shared memory of the wave's own, whole rows at a time and a step ahead.
+// memory to shared memory of the wave's own, whole rows at a time and a step ahead. Bound by
+// the vector unit (a score takes an exponential, a quarter of its rate, a product and a sum:
+// 1.5 times its matrix products at 128 wide, 3 times at 64), busy 53 % of the time, and by
+// the ends of few workgroups. The four prompts above, 128 wide: 128 us (617 TFLOP/s); three
+// chunks of 512 under 64-wide heads and a window of 4,096: 102. With four waves in step the
+// prompts took 252; with exponentials beside the next part's products 135.
 constexpr int kRowsPlaces = 64, kRowsParts = kRowsPlaces / 32;
 
 template <int D, typename T>
@@ -1446,9 +1460,7 @@ void paged_weigh_rows_kernel(WeighArgs a) {
   WeighItem it;
   const int32_t tile = blockIdx.x / (kShare * a.kv_heads);
   const int32_t rest = blockIdx.x - tile * kShare * a.kv_heads, share = rest / a.kv_heads;
-  if (!find_places(a, tile * a.kv_heads + rest - share * a.kv_heads, &it) ||
-      it.rows <= kMostMore)
-    return;
+  if (!find_places<true>(a, tile * a.kv_heads + rest - share * a.kv_heads, &it)) return;
   it.first += share * kRowsPlaces;
   if (!it.reaches(a.sight, it.first, kRowsPlaces)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);

@@ -520,22 +520,29 @@ int aegkv_paged_weigh(const void* plan, const void* device_plan, const aegkv_pag
   a.weights = weights;
   a.group = divisor(h.group);
   a.kv_heads = h.kv_heads;
-  const int64_t groups = h.room.place_tiles * h.kv_heads;
-  rc = check_grid(4 * groups, kPagedLanes);
-  if (rc || groups == 0) return rc;
-  const auto grid = [&](int shares) { return dim3(static_cast<uint32_t>(shares * groups)); };
+  // a captured call's batch may hold any tiles that there is room for, under the same rows
+  const bool few_rows = h.room.items[kFew] || h.room.items[kMore];
+  const int64_t many = !h.room.items[kMany] ? 0 : c.capturing ? h.room.place_tiles : h.many_tiles;
+  const int64_t few = !few_rows     ? 0
+                      : c.capturing ? h.room.place_tiles
+                                    : h.place_tiles - h.many_tiles;
+  rc = check_grid(4 * std::max(many, few) * h.kv_heads, kPagedLanes);
+  if (rc) return rc;
+  const auto grid = [&](int shares, int64_t tiles) {
+    return dim3(static_cast<uint32_t>(shares * tiles * h.kv_heads));
+  };
   return by_width(head_dim, [&](auto d) {
     return by_half_type(dtype, [&](auto t) {
       constexpr int kDim = decltype(d)::value;
       typedef decltype(t) T;
       int rc = 0;
-      if (h.room.items[kFew] || h.room.items[kMore])
-        rc = launch(paged_weigh_kernel<kDim, T>, grid(4 / weigh_parts(kDim)), kPagedLanes, stream, a,
-                    "paged_weigh_kernel launch");
-      if (!rc && h.room.items[kMany])
-        rc = launch(paged_weigh_rows_kernel<kDim, T>, grid(kWeighPlaces / kRowsPlaces),
-                    kPagedLanes, stream, a,
-                    "paged_weigh_rows_kernel launch");
+      if (many)
+        rc = launch(paged_weigh_rows_kernel<kDim, T>, grid(kWeighPlaces / kRowsPlaces, many),
+                    kPagedLanes, stream, a, "paged_weigh_rows_kernel launch");
+      a.first_tile = c.capturing ? 0 : h.many_tiles;
+      if (!rc && few)
+        rc = launch(paged_weigh_kernel<kDim, T>, grid(4 / weigh_parts(kDim), few), kPagedLanes,
+                    stream, a, "paged_weigh_kernel launch");
       return rc;
     });
   });
