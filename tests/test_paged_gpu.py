@@ -476,6 +476,36 @@ def test_weights_of_shared_blocks_are_refused(gpu):
     ops.paged_weigh(cache, batch, q, lse, weights)
 
 
+@pytest.mark.parametrize("window,sinks", [(0, 0), (300, 5)])
+def test_captured_weights_follow_prompts_and_single_tokens(gpu, window, sinks):
+    """One captured call, whose sequences' new tokens change from update to update: the same
+    sums as calls with batches of their own."""
+    bs, heads, group, d, num = 16, 2, 4, 64, 200
+    cache = ops.PagedCache(*(p.to(gpu) for p in make_pages(num, bs, heads, d, F16)))
+    lens = [1100, 900, 257]
+    tables = tables_for(lens, bs, num)
+    batch = batch_for(gpu, tables, lens, [70, 1, 1], cache, heads=heads * group, window=window,
+                      sinks=sinks, max_seqs=3, max_columns=200, max_tokens=150)
+    q = torch.randn(150, heads * group, d, generator=gen(0)).to(F16).to(gpu)
+    lse = (torch.randn(150, heads * group, generator=gen(1)) + 5).to(gpu)
+    weights = torch.zeros(num, heads, bs, device=gpu)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.paged_weigh(cache, batch, q, lse, weights)
+    want = weights.clone()
+    for new in ([70, 1, 1], [1, 1, 1], [1, 70, 70], [3, 0, 100], [70, 70, 1], [0, 0, 0], [1, 2, 17]):
+        batch.update(tables, lens, new)
+        graph.replay()
+        eager = batch_for(gpu, tables, lens, new, cache, heads=heads * group, window=window,
+                          sinks=sinks)
+        n = sum(new)
+        ops.paged_weigh(cache, eager, q[:n], lse[:n], want)
+        torch.cuda.synchronize()
+        assert torch.equal(weights, want), new
+        assert not any(new) or float(want.sum()) > 0
+
+
 # ---- eviction ----------------------------------------------------------------------------
 
 
