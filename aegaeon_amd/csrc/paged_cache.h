@@ -135,7 +135,7 @@ __device__ __forceinline__ void turn_pair(float& a, float& b, float c, float s) 
 // rounding at the end. A workgroup takes a few tokens of some heads of a kind: the angles,
 // 150 instructions each, are made once for all of them, while the first values are on
 // their way. Bound by HBM, then by its instructions: 12,300 tokens of 3 x 40 heads,
-// in float32, are written in 212 us (5.1 TB/s), 16,000 of 32 heads rotated in 50 (5.2).
+// in float32, are written in 212 us (5.1 TB/s), 16,000 of 32 heads rotated in 47 (5.6).
 // G: type of k and v; T: of q, of what is written and of what comes of q. A lane takes
 // two runs of N values of a head at once, half of the rotated part (or of the others) apart:
 // both sides of N pairs, or neighbouring pairs in each run where they are interleaved, and
@@ -230,7 +230,9 @@ __global__ __launch_bounds__(kPlaceLanes) void place_rows_kernel(PlaceArgs a) {
 
   // Values stay as they came until they are needed: made wider at once, each item's loads
   // would be waited for before the next one's, and all before the angles.
-  constexpr int kItems = 2;     // on their way together
+  // Items on their way together: of 16-bit values, 16,000 tokens of 32 heads take 50 us by
+  // two and 47 by three or four; of 32 bits, prompts take 213 by one to three, 217 by four.
+  constexpr int kItems = N == 8 ? 3 : 2;
   constexpr bool kAlike = sizeof(T) == sizeof(G);
   Raw<N, G> x[kItems], y[kItems];
   Raw<N, T> xq[kItems], yq[kItems];     // (queries, where they are of another size)
