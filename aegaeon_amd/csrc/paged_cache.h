@@ -371,11 +371,12 @@ struct RowSum {
   float sum = 0.f;
 };
 
-// log2 of what sums are taken against: exactly what the exponents had added.
+// log2 of what sums are taken against: exactly what the exponents had added. A row
+// without a score has nothing to compare: its base is below any that scores make.
 template <typename T>
 __device__ __forceinline__ float row_base(const RowSum& s, float c) {
-  return fabsf(s.lift) > Matrix<T>::kLimit && s.top != -INFINITY ? s.top * c - Matrix<T>::kLift
-                                                                 : -s.lift;
+  if (s.top == -INFINITY) return s.top;
+  return fabsf(s.lift) > Matrix<T>::kLimit ? s.top * c - Matrix<T>::kLift : -s.lift;
 }
 
 // N scores of a row (x, -inf where hidden) into probabilities in place; `most_of` is the
