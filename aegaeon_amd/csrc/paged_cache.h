@@ -876,17 +876,17 @@ __device__ __forceinline__ uint32_t shared_address(const v4u* p) {
 }
 
 // 16 bytes a lane from `base` (the same for the wave) + offset to shared memory, lane
-// after lane from `to` on; NT: past the caches. The compiler does not know of it: whoever
-// reads them waits for them first. (Told of it, it waits for all such loads before any
-// read of shared memory.)
+// after lane from `to` on, which the instruction takes from m0; NT: past the caches. The
+// compiler does not know that shared memory changes: whoever reads it waits for the loads
+// first. (Told of it, it waits for all such loads before any read of shared memory.)
 template <bool NT = false>
 __device__ __forceinline__ void load_shared(const char* base, uint32_t offset, const v4u* to) {
   if constexpr (NT)
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt"
-                 :: "v"(offset), "s"(base), "s"(shared_address(to)) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt"
+                 :: "v"(offset), "s"(base), "{m0}"(shared_address(to)) : "memory");
   else
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-                 :: "v"(offset), "s"(base), "s"(shared_address(to)) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :: "v"(offset), "s"(base), "{m0}"(shared_address(to)) : "memory");
 }
 
 // All of the wave's loads have come but the last LATER, its reads of shared memory too,
