@@ -1374,6 +1374,12 @@ _HALVES = (torch.bfloat16, torch.float16)
 _turn_tables: dict = {}     # by device and contents; kept, so that no stream outlives one
 
 
+def _turn_table(key: tuple, make) -> torch.Tensor:
+    table = _turn_tables.get(key)
+    # of threads that make equal ones at once all take the first that is kept
+    return table if table is not None else _turn_tables.setdefault(key, make())
+
+
 def rotary_frequencies(dim: int, *, base: float = 10000.0, scaling: str = "none",
                        factor: float = 1.0, length: int = 0) -> tuple[np.ndarray, float]:
     """(radians a position for each of dim / 2 pairs, amplitude) of rotary positions:
@@ -1451,20 +1457,21 @@ class Rotary:
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
         turns = f / (2 * math.pi)
-        key = (self.device.index, turns.tobytes())
-        if key not in _turn_tables:
-            with torch.cuda.device(self.device):
-                if torch.cuda.is_current_stream_capturing():
-                    raise ValueError("rotary positions are not made while a stream is captured")
-                table = torch.tensor(turns, device=self.device)
-                torch.cuda.current_stream().synchronize()
-            _turn_tables[key] = table
-        self._turns = _turn_tables[key]
+        self._turns = _turn_table((self.device.index, turns.tobytes()),
+                                  lambda: self._upload(turns))
         self._args = _lib.RotaryArgs(self._turns.data_ptr(), self.dim, self.interleaved,
                                      self.amplitude)
         # TurnArgs of csrc/hostargs.cpp
         self._packed = (struct.pack("q", _lib.address("aegkv_rotate")) + bytes(self._args)
                         + struct.pack("2q", self.head_dim, self.device.index))
+
+    def _upload(self, turns: np.ndarray) -> torch.Tensor:
+        with torch.cuda.device(self.device):
+            if torch.cuda.is_current_stream_capturing():
+                raise ValueError("rotary positions are not made while a stream is captured")
+            table = torch.tensor(turns, device=self.device)
+            torch.cuda.current_stream().synchronize()
+        return table
 
 
 class PagedCache:
