@@ -1390,7 +1390,7 @@ def rotary_frequencies(dim: int, *, base: float = 10000.0, scaling: str = "none"
     "base"    base * factor ** (dim / (dim - 2)) in the base's place
     "ramp"    f_i where `length` positions hold 32 turns or more, f_i / factor where one
               or less, between them linear in i (from the last whole i before to the
-              first behind); amplitude 0.1 ln(factor) + 1
+              first behind); amplitude 0.1 ln(factor) + 1, and 1 for factors below 1
     "smooth"  f_i at 4 turns or more, f_i / factor at one or less, between them linear in the
               turns
     """
@@ -1417,7 +1417,7 @@ def rotary_frequencies(dim: int, *, base: float = 10000.0, scaling: str = "none"
                      for turns in (32, 1))
         low, high = max(0, math.floor(low)), min(dim - 1, math.ceil(high))
         far = np.clip((i - low) / max(high - low, 0.001), 0, 1)
-        return f / factor * far + f * (1 - far), 0.1 * math.log(factor) + 1
+        return f / factor * far + f * (1 - far), 0.1 * math.log(max(factor, 1.0)) + 1
     elif scaling == "smooth":
         near = np.clip((length * f / (2 * math.pi) - 1) / 3, 0, 1)
         f = f / factor * (1 - near) + f * near
