@@ -1492,8 +1492,7 @@ class PagedCache:
                                  f"not {list(t.shape)}")
             if t.dtype not in _HALVES:
                 raise ValueError(f"{what} of {t.dtype}: a cache holds bfloat16 or float16")
-            if t.requires_grad:
-                raise ValueError(f"{what} requires a gradient, which these operators do not give")
+            _require_plain(t, what)
         if (k_pages.shape, k_pages.dtype, k_pages.device) != (v_pages.shape, v_pages.dtype,
                                                               v_pages.device):
             raise ValueError("k_pages and v_pages must be equally large, of one type and on one "
@@ -1539,15 +1538,25 @@ class PagedCache:
 
 
 def _native(cache: PagedCache, batch: CacheBatch, stream) -> bool:
-    """Whether a call may be the plain case, which is checked and made natively."""
+    """Whether a call may be the plain case, which is checked and made natively. (Where
+    tangents may be carried, the general path looks at the cache's, too.)"""
     return (stream is None and _alive(batch._home) and not cache.k_pages.requires_grad
-            and not cache.v_pages.requires_grad)
+            and not cache.v_pages.requires_grad
+            and getattr(torch.autograd.forward_ad, "_current_level", 0) < 0)
+
+
+def _require_plain(t: torch.Tensor, what: str) -> None:
+    """What a call changes carries neither, whatever the mode."""
+    if t.requires_grad:
+        raise ValueError(f"{what} require a gradient, which these operators do not give")
+    if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{what} carry a tangent, which these operators do not take on")
 
 
 def _paged_call(cache: PagedCache, batch: CacheBatch, stream) -> None:
     _cache_call(cache, batch, stream, QuantCache)
-    if cache.k_pages.requires_grad or cache.v_pages.requires_grad:
-        raise ValueError("the cache requires a gradient, which these operators do not give")
+    for pages in (cache.k_pages, cache.v_pages):
+        _require_plain(pages, "the cache's pages")
 
 
 def _rows(t: torch.Tensor, what: str, heads: int, of, dtypes) -> _lib.Rows:
@@ -1743,8 +1752,7 @@ def _weights_arg(weights: torch.Tensor, cache: PagedCache) -> int:
     if tuple(weights.shape) != shape or not weights.is_contiguous():
         raise ValueError(f"weights must be contiguous [{shape[0]}, {shape[1]}, {shape[2]}], not "
                          f"{list(weights.shape)}")
-    if weights.requires_grad:
-        raise ValueError("weights require a gradient, which these operators do not give")
+    _require_plain(weights, "weights")
     return weights.data_ptr()
 
 
