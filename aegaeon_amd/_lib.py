@@ -92,6 +92,7 @@ EXPORTED_SYMBOLS = (
     "aegkv_stream_release",
     "aegkv_quant_page_bytes",
     "aegkv_batch_plan",
+    "aegkv_batch_shared",
     "aegkv_quant_write",
     "aegkv_quant_read",
     "aegkv_quant_attend_workspace",
@@ -177,6 +178,7 @@ _SIGNATURES = {
     "aegkv_stream_destroy": (_INT, [_P]),
     "aegkv_stream_release": (_INT, [_P]),
     "aegkv_quant_page_bytes": (_INT, [_INT, _I32, _I32, _I32, _I64P]),
+    "aegkv_batch_shared": (_INT, [_P, _I32P]),
     "aegkv_batch_plan": (
         _INT,
         [_I64, _I64P, _I64P, _I64P, _I64P, _I64, _I32, _I32, _I32, _I64, _I64, _I64, _I64, _I64,

@@ -102,7 +102,7 @@ struct Header {
   int32_t merges;
   int32_t many_tiles, place_tiles; // tiles of kMany's sequences, which come first; all
   int32_t complete;                // every position of every sequence has its block
-  int32_t shared;                  // some block is in two places of the tables
+  int32_t shared;                  // some block is in two places that queries see
   int64_t read_tokens;
 };
 

@@ -230,27 +230,44 @@ inline int check(const Header& h, const Batch& b) {
   return 0;
 }
 
-// Whether some block is in two places of the sequences' columns.
+// Columns of a sequence that its queries see: [0, firsts) and [rest, end), whole blocks.
+struct SeenColumns {
+  int64_t firsts, rest, end;
+};
+
+inline SeenColumns seen_columns(const Header& h, int64_t len, int64_t fresh) {
+  if (!fresh) return SeenColumns{0, 0, 0};
+  const int64_t begin = window_begin(h, len - fresh);
+  const int64_t rest = begin / h.block_size;
+  const int64_t firsts = h.window ? std::min<int64_t>(h.sinks, begin) : 0;
+  return SeenColumns{std::min(up(firsts, h.block_size), rest), rest, up(len, h.block_size)};
+}
+
+// Whether some block is in two places that queries see: sequences without new tokens, and
+// columns before a window, gather no weights.
 inline bool shares(const Header& h, const Batch& b, int64_t columns) {
-  if (h.num_blocks / 64 <= columns + 1024) {
-    std::vector<uint64_t> seen(static_cast<size_t>(h.num_blocks / 64 + 1));
+  const auto each = [&](const auto& f) {
     for (int64_t s = 0; s < b.num_seqs; ++s) {
       const int64_t* const ids = b.ids + b.offsets[s];
-      for (int64_t c = 0, need = up(b.lens[s], h.block_size); c < need; ++c) {
-        if (ids[c] < 0) continue;
-        uint64_t& word = seen[static_cast<size_t>(ids[c] >> 6)];
-        const uint64_t bit = uint64_t(1) << (ids[c] & 63);
-        if (word & bit) return true;
-        word |= bit;
-      }
+      const SeenColumns seen = seen_columns(h, b.lens[s], b.fresh[s]);
+      for (int64_t c = 0; c < seen.firsts; ++c) f(ids[c]);
+      for (int64_t c = seen.rest; c < seen.end; ++c) f(ids[c]);
     }
-    return false;
+  };
+  if (h.num_blocks / 64 <= columns + 1024) {
+    std::vector<uint64_t> seen(static_cast<size_t>(h.num_blocks / 64 + 1));
+    uint64_t twice = 0;
+    each([&](int64_t id) {
+      uint64_t& word = seen[static_cast<size_t>(id >> 6)];
+      const uint64_t bit = uint64_t(1) << (id & 63);
+      twice |= word & bit;
+      word |= bit;
+    });
+    return twice != 0;
   }
   // few columns of very many blocks
   std::vector<int64_t> all;
-  for (int64_t s = 0; s < b.num_seqs; ++s)
-    for (int64_t c = 0; c < up(b.lens[s], h.block_size); ++c)
-      if (b.ids[b.offsets[s] + c] >= 0) all.push_back(b.ids[b.offsets[s] + c]);
+  each([&](int64_t id) { all.push_back(id); });
   std::sort(all.begin(), all.end());
   return std::adjacent_find(all.begin(), all.end()) != all.end();
 }

@@ -1261,7 +1261,7 @@ struct WeighItem {
 
 // MANY: of the sequences of more than kMostMore rows, whose tiles come first. A captured
 // call has a workgroup for each tile that there is room for, and may find, after an
-// update, a batch whose sequences share blocks.
+// update, a batch whose queries see one block in two places.
 template <bool MANY>
 __device__ __forceinline__ bool find_places(const WeighArgs& a, int32_t index, WeighItem* it) {
   const int32_t i = index / a.kv_heads, at = i + a.first_tile;

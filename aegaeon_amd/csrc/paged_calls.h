@@ -485,8 +485,8 @@ int aegkv_paged_weigh(const void* plan, const void* device_plan, const aegkv_pag
   if (rc) return rc;
   const Header& h = c.h;
   if (h.shared && !c.capturing)
-    return fail(AEGKV_EDUP, "two places of the batch's tables are one block, which would "
-                "gather two sequences' weights at once");
+    return fail(AEGKV_EDUP, "two places of the batch's tables that queries see are one block, "
+                "which would gather two sequences' weights at once");
   const int32_t head_dim = cache->head_dim;
   const int dtype = cache->dtype;
   WeighArgs a = {};

@@ -184,4 +184,15 @@ int aegkv_batch_plan(int64_t num_seqs, const int64_t* column_offsets, const int6
   }
 }
 
+int aegkv_batch_shared(const void* plan, int32_t* shared) {
+  using namespace aegkv_batch;
+  aegkv_clear_error();
+  if (!plan || !shared) return plan_fail(AEGKV_EINVAL, "plan and shared must not be null");
+  Header h;
+  std::memcpy(&h, plan, sizeof h);
+  if (h.magic != kMagic) return plan_fail(AEGKV_EINVAL, "this is no plan of aegkv_batch_plan");
+  *shared = h.shared;
+  return 0;
+}
+
 }  // extern "C"

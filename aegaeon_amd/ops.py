@@ -1103,6 +1103,16 @@ class CacheBatch:
         self.num_seqs, self.num_tokens = int(lens.size), int(new.sum())
         self.read_tokens = int(lens.sum())
 
+    @property
+    def shared(self) -> bool:
+        """Whether two places of the tables that queries see are one block (a prefix that
+        sequences with new tokens have in common, say). Such a batch is attended over
+        as any other, but paged_weigh refuses it, and where an update brought it under a
+        captured paged_weigh, a replay adds no weights at all: look here before."""
+        shared = ctypes.c_int32()
+        _lib.check(_lib.load().aegkv_batch_shared(self._host_ptr, ctypes.byref(shared)))
+        return bool(shared.value)
+
     def _pinned(self) -> torch.Tensor:
         return torch.empty(self._host.size, dtype=torch.uint8, pin_memory=True)
 
@@ -1765,8 +1775,8 @@ def paged_weigh(cache: PagedCache, batch: CacheBatch, q: torch.Tensor, lse: torc
 
     q, scale: those of paged_attend, whose log-sum-exps lse are. weights: float32 [num_blocks,
     kv_heads, block_size], contiguous; the new tokens' places start from 0, those that no query
-    sees keep theirs. Sequences of the batch may share no blocks. As a segment of the composite cache (layout.weight_tensor_specs)
-    they move with the blocks.
+    sees keep theirs. No block may be in two places that queries see (CacheBatch.shared). As a
+    segment of the composite cache (layout.weight_tensor_specs) they move with the blocks.
     """
     if _native(cache, batch, stream):
         done = _lib.hostargs().paged_weigh(cache._packed, batch._packed, q, lse, weights, scale,

@@ -567,6 +567,13 @@ int aegkv_batch_plan(int64_t num_seqs, const int64_t* column_offsets, const int6
                      int update, void* plan, int64_t* plan_bytes);
 
 /*
+ * *shared: whether two places of a plan's tables that queries see are one block (host-only).
+ * Attention reads such a batch as any other; aegkv_paged_weigh does not take it. What
+ * no query sees does not count: sequences without new tokens, columns before a window.
+ */
+int aegkv_batch_shared(const void* plan, int32_t* shared);
+
+/*
  * Write the batch's new tokens into the cache. k and v: [num_tokens][kv_heads]
  * [head_dim] values of `dtype`, strides in elements (none negative; the last
  * axis is contiguous), row i the batch's i-th new token; rows behind the last
@@ -715,8 +722,9 @@ int aegkv_paged_attend(const void* plan, const void* device_plan, const aegkv_pa
  * exp(scale * q . K[j] - lse). weights: [num_blocks][kv_heads][block_size] floats (a
  * segment of the cache like K and V, which swaps and copies move). What the new tokens' places
  * held before does not count; weights of places that no query sees are left as they were.
- * Sums are made in 32 bits in a fixed order (no atomics). Sequences that share blocks are
- * refused (AEGKV_EDUP); a captured call, replayed after an update to such, does nothing.
+ * Sums are made in 32 bits in a fixed order (no atomics). A batch whose queries see a block in
+ * two places is refused (AEGKV_EDUP; aegkv_batch_shared); a captured call, replayed after an
+ * update to such a batch, adds nothing for any of its sequences.
  */
 int aegkv_paged_weigh(const void* plan, const void* device_plan, const aegkv_paged_cache* cache,
                       const aegkv_rows* q, const float* lse, int64_t lse_tokens,
