@@ -167,6 +167,19 @@ inline Parts parts_of(const std::vector<Rows>& rows, int64_t kv_heads, int64_t e
   return p;
 }
 
+// Columns of a sequence that its queries see: [0, firsts) and [rest, end), whole blocks.
+struct SeenColumns {
+  int64_t firsts, rest, end;
+};
+
+inline SeenColumns seen_columns(const Header& h, int64_t len, int64_t fresh) {
+  if (!fresh) return SeenColumns{0, 0, 0};
+  const int64_t begin = window_begin(h, len - fresh);
+  const int64_t rest = begin / h.block_size;
+  const int64_t firsts = h.window ? std::min<int64_t>(h.sinks, begin) : 0;
+  return SeenColumns{std::min(up(firsts, h.block_size), rest), rest, up(len, h.block_size)};
+}
+
 inline int check(const Header& h, const Batch& b) {
   std::vector<int64_t> written;   // (block, first, end) of every block written
   int64_t columns = 0, tokens = 0, all = 0;
@@ -185,25 +198,34 @@ inline int check(const Header& h, const Batch& b) {
     if (hi - lo < need)
       return aegkv_set_error(AEGKV_ERANGE, "sequence %lld: %lld tokens in %lld blocks of %d", ll(s),
                              ll(len), ll(hi - lo), h.block_size);
-    for (int64_t c = lo; c < hi; ++c)
-      if (b.ids[c] < -1 || b.ids[c] >= h.num_blocks)
-        return aegkv_set_error(AEGKV_ERANGE, "sequence %lld: block id %lld outside [0, %lld)",
-                               ll(s), ll(b.ids[c]), ll(h.num_blocks));
+    // (each look at the columns is without branches: a decode step pays them all)
+    const int64_t* const ids = b.ids + lo;
+    uint64_t outside = 0;       // its sign: that of id + 1 and num_blocks - 1 - id
+    for (int64_t c = 0; c < hi - lo; ++c) {
+      const uint64_t id = static_cast<uint64_t>(ids[c]);
+      outside |= (id + 1) | (static_cast<uint64_t>(h.num_blocks) - 1 - id);
+    }
+    if (static_cast<int64_t>(outside) < 0)
+      for (int64_t c = 0; c < hi - lo; ++c)
+        if (ids[c] < -1 || ids[c] >= h.num_blocks)
+          return aegkv_set_error(AEGKV_ERANGE, "sequence %lld: block id %lld outside [0, %lld)",
+                                 ll(s), ll(ids[c]), ll(h.num_blocks));
     if (fresh) {
-      const int64_t begin = window_begin(h, len - fresh);
-      const int64_t firsts = h.window ? std::min<int64_t>(h.sinks, begin) : 0;
-      for (int64_t c = 0; c < need; ++c) {
+      const SeenColumns seen = seen_columns(h, len, fresh);
+      int64_t released = 0;     // negative: some
+      for (int64_t c = 0; c < seen.firsts; ++c) released |= ids[c];
+      for (int64_t c = seen.rest; c < seen.end; ++c) released |= ids[c];
+      if (released < 0)
+        for (int64_t c = 0; c < need; ++c)
+          if (ids[c] < 0 && (c < seen.firsts || c >= seen.rest))
+            return aegkv_set_error(AEGKV_ERANGE,
+                                   "sequence %lld: column %lld is released but its tokens are "
+                                   "seen", ll(s), ll(c));
+      for (int64_t c = (len - fresh) / h.block_size; c < need; ++c) {
         const int64_t at = c * h.block_size;
-        const bool seen = at < firsts || at + h.block_size > begin;
-        if (seen && b.ids[lo + c] < 0)
-          return aegkv_set_error(AEGKV_ERANGE,
-                                 "sequence %lld: column %lld is released but its tokens are seen",
-                                 ll(s), ll(c));
-        if (at + h.block_size > len - fresh) {
-          written.push_back(b.ids[lo + c]);
-          written.push_back(std::max<int64_t>(0, len - fresh - at));
-          written.push_back(std::min<int64_t>(h.block_size, len - at));
-        }
+        written.push_back(ids[c]);
+        written.push_back(std::max<int64_t>(0, len - fresh - at));
+        written.push_back(std::min<int64_t>(h.block_size, len - at));
       }
     }
     columns += need + 1;
@@ -228,19 +250,6 @@ inline int check(const Header& h, const Batch& b) {
                              ll(c[0]));
   }
   return 0;
-}
-
-// Columns of a sequence that its queries see: [0, firsts) and [rest, end), whole blocks.
-struct SeenColumns {
-  int64_t firsts, rest, end;
-};
-
-inline SeenColumns seen_columns(const Header& h, int64_t len, int64_t fresh) {
-  if (!fresh) return SeenColumns{0, 0, 0};
-  const int64_t begin = window_begin(h, len - fresh);
-  const int64_t rest = begin / h.block_size;
-  const int64_t firsts = h.window ? std::min<int64_t>(h.sinks, begin) : 0;
-  return SeenColumns{std::min(up(firsts, h.block_size), rest), rest, up(len, h.block_size)};
 }
 
 // Whether some block is in two places that queries see: sequences without new tokens, and
@@ -300,11 +309,15 @@ inline int fill(Header& h, const Batch& b, const std::vector<Rows>* rows, char* 
     seq[s].read_span = static_cast<int32_t>(read_spans);
     seq[s].pad = 0;
     seq[s].read_token = read_tokens;
+    const int64_t* const ids = b.ids + b.offsets[s];
+    int32_t* const to = table + columns;
+    int64_t released = 0;       // negative: some
     for (int64_t c = 0; c < need; ++c) {
-      const int64_t id = b.ids[b.offsets[s] + c];
-      if (id < 0) h.complete = 0;
-      table[columns + c] = static_cast<int32_t>(std::max<int64_t>(id, 0));
+      released |= ids[c];
+      const int32_t id = static_cast<int32_t>(ids[c]);
+      to[c] = id & ~(id >> 31);     // 0 for -1
     }
+    if (released < 0) h.complete = 0;
     table[columns + need] = 0;   // the tile behind the last block may look here
     columns += need + 1;
     tokens += fresh;
