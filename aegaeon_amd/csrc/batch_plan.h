@@ -23,8 +23,11 @@ constexpr int kPlaceTile = 256;
 //                four waves of a workgroup take an item's tiles in turn and
 //                join at its end;
 //   kMany:       blocks of kManyRows rows, shared out to the waves.
-// 64 sequences of 2,000 tokens, 8 KV heads: 20, 40 and 64 rows take 37, 68 and 70 us as
-// kMore, 75, 85 and 87 as kMany; 128 rows 127 and 101.
+// Over a cache in 4 bits, 64 sequences of 2,000 tokens, 8 KV heads: 20, 40 and 64 rows take
+// 37, 68 and 70 us as kMore, 75, 85 and 87 as kMany; 128 rows 127 and 101. A 16-bit cache has
+// four times the bytes, which each block of 32 rows reads: there 40 and 64 rows take 136 and
+// 138 us as kMore, and would take 107 and 108 as kMany (128 wide). A plan knows no cache, and
+// goes by the quantised ones'.
 enum Kind { kFew = 0, kMore = 1, kMany = 2, kKinds = 3 };
 constexpr int kManyRows = 128;
 constexpr int kKindRows[kKinds] = {16, 32, kManyRows};

@@ -17,7 +17,8 @@ namespace aegkv_batch {
 // Positions are 32-bit in the kernels, with room for a tile behind the last.
 constexpr int64_t kMostTokens = (int64_t(1) << 31) - 1024;
 
-// Cutting rows over workgroups. Whole rows, the longest first, where the chip is
+// Cutting rows over workgroups. All times are of 4-bit caches; a 16-bit cache takes the same
+// cuts, and has not been measured with others. Whole rows, the longest first, where the chip is
 // evenly full of them (48 sequences of 40 heads: 119 us cut at every 1/1024 of the
 // tiles, 104 whole); else the cut whose estimated time is least. Equal shares of the
 // flattened tiles, a workgroup going from one sequence's end to the next one's

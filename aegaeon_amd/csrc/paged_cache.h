@@ -134,8 +134,10 @@ __device__ __forceinline__ void turn_pair(float& a, float& b, float c, float s) 
 // it is rounded (positions of millions keep their angle), values in 32, one
 // rounding at the end. A workgroup takes a few tokens of some heads of a kind: the angles,
 // 150 instructions each, are made once for all of them, while the first values are on
-// their way. Bound by HBM, then by its instructions: 12,300 tokens of 3 x 40 heads,
-// in float32, are written in 212 us (5.1 TB/s), 16,000 of 32 heads rotated in 47 (5.6).
+// their way. Bound by HBM, then by its instructions: 12,300 tokens of 3 x 40 heads are
+// written in 213 us from float32 (5.1 TB/s) and in 156 from 16 bits (5.2); 16,000 tokens of
+// 32 heads are rotated in 47 to 55 us (4.8-5.6 TB/s: the less, the less of them the cache
+// behind the L2 still holds), in float32 in 105 (5.0).
 // G: type of k and v; T: of q, of what is written and of what comes of q. A lane takes
 // two runs of N values of a head at once, half of the rotated part (or of the others) apart:
 // both sides of N pairs, or neighbouring pairs in each run where they are interleaved, and
@@ -171,7 +173,7 @@ __global__ __launch_bounds__(kPlaceLanes) void place_rows_kernel(PlaceArgs a) {
   const int32_t units = static_cast<int32_t>(a.units.by), items = count * heads * units;
   const bool words = own->from.whole_words;
   // Whole lines go past the caches. Where a head's runs are halves of lines, 16,000 tokens
-  // of 32 heads took 68 us that way, 50 through them.
+  // of 32 heads took 68 us that way, 50 through them (three sets of rows in turn).
   const int64_t size = query ? sizeof(T) : sizeof(G);
   const int32_t rest = turned ? a.pairs : 0;      // the part behind the rotated one
   const auto in_lines = [&](int64_t each) {
@@ -230,8 +232,9 @@ __global__ __launch_bounds__(kPlaceLanes) void place_rows_kernel(PlaceArgs a) {
 
   // Values stay as they came until they are needed: made wider at once, each item's loads
   // would be waited for before the next one's, and all before the angles.
-  // Items on their way together: of 16-bit values, 16,000 tokens of 32 heads take 50 us by
-  // two and 47 by three or four; of 32 bits, prompts take 213 by one to three, 217 by four.
+  // Items on their way together: of 16-bit values, 16,000 tokens of 32 heads (three sets in
+  // turn) take 50 us by two and 47 by three or four; of 32 bits, prompts take 213 by one to
+  // three, 217 by four.
   constexpr int kItems = N == 8 ? 3 : 2;
   constexpr bool kAlike = sizeof(T) == sizeof(G);
   Raw<N, G> x[kItems], y[kItems];
@@ -417,6 +420,13 @@ __device__ __forceinline__ void softmax_part(float (&x)[N], float c, RowSum& s, 
   s.sum += sum;
 }
 
+// Probabilities as the second product's operand. The matrix units take 16 bits, so each is
+// rounded once (the row's sum, and with it the log-sum-exp, is of the unrounded ones): a
+// result is off by at most half a step of the sum of probability times |V|, as much again as
+// its own rounding. 64 decodes in bfloat16 are 0.0021 off, of the size of their results; with
+// a second product over what the rounding leaves 0.0017, what rounding the exact results gives,
+// but then 64 decodes take 222 us instead of 177, two long contexts 104 instead of 82, and
+// four prompts 249 instead of 195.
 template <typename T, int N>
 __device__ __forceinline__ typename Matrix<T>::v8 round8(const float (&x)[N], int from) {
   typename Matrix<T>::v8 p;
@@ -508,7 +518,7 @@ struct PagedJoin {
 // tokens that the lane's probabilities belong to, so that these are the second
 // product's operand as they are; eight tokens of a value come side by side by
 // byte permutes. K comes through the caches, 64 bytes of a row at a time (two contexts
-// of 100,000 tokens 73 us, past them 80), V, whole rows, past them.
+// of 100,000 tokens, 4 KV heads of 28: 73 us, past them 80), V, whole rows, past them.
 template <int D>
 struct PagedTile {
   static constexpr int kRun = D / 16, kWords = kRun / 2;
@@ -838,9 +848,10 @@ __device__ __forceinline__ float pair_max(float x) {
 // operand as they lie. Three tiles are in work at once: the second product of one beside
 // the scores of the next and the exponents between them. Bound by what two waves a SIMD
 // issue: matrix units are busy 48 % of a long prompt's time, the vector unit 50. Four
-// prompts of 1,000 to 4,096 tokens, 8 KV heads of 32, 128 wide, take 190 us (825 TFLOP/s), one
-// of 32,768 runs at 1,050, 64-wide heads at 690, 256-wide ones at 730; with registers
-// instead of the ring they took 208, a tile after another without its order of issue 193.
+// prompts of 1,000 to 4,096 tokens, 8 KV heads of 32, take 195 to 205 us 128 wide (770 to 810
+// TFLOP/s), 121 64 wide (650) and 430 256 wide (735, one wave a SIMD: a CU holds one ring),
+// and one of 32,768 runs at 1,055, 890 and 965. With registers instead of the ring the four
+// took 208, a tile after another without its order of issue 193, where this took 188.
 constexpr int kRing = 4, kRowsWave = 32, kTileRowsWave = kTile / kPagedWaves;
 static_assert(kManyRows == kPagedWaves * kRowsWave, "rows of a workgroup");
 
@@ -1447,9 +1458,10 @@ __device__ __forceinline__ float half_sum(float x) {
 // memory to shared memory of the wave's own, whole rows at a time and a step ahead. Bound by
 // the vector unit (a score takes an exponential, a quarter of its rate, a product and a sum:
 // 1.5 times its matrix products at 128 wide, 3 times at 64), busy 53 % of the time, and by
-// the ends of few workgroups. The four prompts above, 128 wide: 128 us (617 TFLOP/s); three
-// chunks of 512 under 64-wide heads and a window of 4,096: 102. With four waves in step the
-// prompts took 252; with exponentials beside the next part's products 135.
+// the ends of few workgroups. The four prompts above, 128 wide: 128 to 135 us (585 to 617
+// TFLOP/s); three chunks of 512 under 64-wide heads and a window of 4,096: 102. With four
+// waves in step the prompts took 252; with exponentials beside the next part's products 135
+// where they took 128.
 constexpr int kRowsPlaces = 64, kRowsParts = kRowsPlaces / 32;
 
 template <int D, typename T>
@@ -1797,8 +1809,8 @@ constexpr int kMoveLanes = 256, kMostMoveLanes = 1024, kMoveAtOnce = 8;
 // TB/s). K, V and the weights of the same rows are neighbours, and their places come from
 // the caches: with all of K first 168. A workgroup that moves K and V of a row at once
 // takes longer (201 of both). In their own blocks one workgroup has all of a head's rows:
-// of 1,024 lanes, since it waits for each turn (30,001 tokens to 4,096, 4 heads: 52 us of
-// both kernels, 71 with 256 lanes).
+// of 1,024 lanes, since it waits for each turn (30,001 tokens to 4,096, 4 heads: 52 to 56 us
+// of both kernels, 71 with 256 lanes).
 template <typename W, typename F>
 __device__ __forceinline__ void move_rows(const int32_t* kept, int64_t r0, int64_t r1,
                                           int words, bool in_place, const F& place) {

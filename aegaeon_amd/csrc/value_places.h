@@ -1,4 +1,4 @@
-// Where the values of a call over a quantised cache lie, and whether two of them
+// Where the values of a call over a paged cache lie, and whether two of them
 // share a byte. Host-only; internal to the library.
 #ifndef AEGKV_VALUE_PLACES_H
 #define AEGKV_VALUE_PLACES_H

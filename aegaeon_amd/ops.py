@@ -1353,7 +1353,8 @@ def quant_attend(cache: QuantCache, batch: CacheBatch, q: torch.Tensor, *,
     q: [tokens, heads, head_dim] of bfloat16 or float16, row i the query of the
     batch's i-th new token, whose K and V are in the cache already (quant_write).
     scale: of the scores, head_dim ** -0.5 by default. `out` (q itself is fine, other
-    overlaps are refused) takes the result; rows behind the batch's last token are left as they were.
+    overlaps are refused) takes the result; rows behind the batch's last token are left as
+    they were.
     """
     if stream is None and _alive(batch._home):
         done = _lib.hostargs().quant_attend(cache._packed, batch._packed, q, out, scale,
@@ -1605,7 +1606,9 @@ def rotate(rotary: Rotary, positions: torch.Tensor, q: torch.Tensor,
     q, k: [tokens, heads, head_dim] of one type (bfloat16, float16 or float32), any strides
     on the first two axes. positions: an int32 or int64 for each token on the device; a
     negative one turns back. Returns q, or (q, k), rotated: new tensors, or `out` (the
-    same way; q and k themselves are fine, other overlaps are refused).
+    same way; q and k themselves are fine, other overlaps are refused). On a `stream` other
+    than the current one, the caller orders the inputs before the call and keeps them until
+    it has run, as for every call here.
     """
     if stream is None:
         to = (out, None) if k is None or out is None else out
@@ -1806,7 +1809,8 @@ def paged_evict(cache: PagedCache, batch: CacheBatch, weights: torch.Tensor, kee
     stays go to the sequence's first places, in their order. Every head keeps as many,
     so a sequence's length is min(length, keep) afterwards: free the blocks behind it
     and update the batch. Later tokens' rotary positions are no longer their places:
-    give paged_write theirs. `into`: a batch over other blocks whose sequences have room for
+    give paged_write theirs; a batch's window goes on by places, so it reaches back over
+    what stayed. `into`: a batch over other blocks whose sequences have room for
     what stays, which goes there instead; the old blocks stay as they were.
 
     Returns the places that what stays had, int32 [sequences, kv_heads, keep], -1

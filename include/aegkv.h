@@ -733,12 +733,12 @@ int aegkv_paged_weigh(const void* plan, const void* device_plan, const aegkv_pag
 /*
  * Evict tokens of sequences longer than `keep`. Under each KV head stay the first
  * `sinks` places, the last `recent`, and of the others those of the largest weight (of
- * equals the earlier ones; NaN counts as the least), `keep` in all; K, V and weights of what stays go, in
- * their order, to the places 0 .. keep - 1: of the sequence's own blocks, or with into_plan of
- * that plan's sequence of the same number, which has room for them (the sequences'
- * own blocks are then left as they were, and shorter sequences are copied whole). kept:
- * [sequences][kv_heads][keep] int32, takes the places that what stays had; -1 behind the
- * end of a shorter sequence.
+ * equals the earlier ones; NaN counts as the least), `keep` in all; K, V and weights of
+ * what stays go, in their order, to the places 0 .. keep - 1: of the sequence's own blocks, or
+ * with into_plan of that plan's sequence of the same number, which has room for them (the
+ * sequences' own blocks are then left as they were, and shorter sequences are copied whole).
+ * kept: [sequences][kv_heads][keep] int32, takes the places that what stays had; -1 behind the
+ * end of a shorter sequence. Windows of later plans count the places of what stayed.
  *
  * The heads of a sequence keep different tokens but as many of them, so the new length is
  * min(length, keep), known without asking the device. Blocks that are written
